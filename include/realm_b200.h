@@ -53,7 +53,8 @@ extern "C" {
 #define RB_PTR_HOST 0u
 #define RB_PTR_DEVICE 1u
 /* With RB_PTR_DEVICE: enqueue on the context stream and return without waiting
- * (rb_weight_matmul, rb_attention_forward); device-side failures surface at the
+ * (rb_weight_matmul, rb_attention_forward, rb_plan_append, rb_plan_attention,
+ * rb_sample_filtered); device-side failures surface at the
  * next rb_sync. Without RB_PTR_DEVICE the flag is ignored. */
 #define RB_ASYNC 2u
 
@@ -75,6 +76,12 @@ typedef struct rb_config {
 
 /* ---- context ---- */
 int32_t rb_ctx_create(const rb_config* cfg, rb_ctx** out);
+/* rb_ctx_create on a stream of the caller's (a cudaStream_t of cfg->device; NULL:
+ * the legacy default stream), which has to outlive the context. All work of the
+ * context is enqueued there, so calls are ordered with the caller's own work on
+ * it without events. On the legacy default stream, which cannot be captured,
+ * use_graphs is ignored. */
+int32_t rb_ctx_create_on_stream(const rb_config* cfg, void* stream, rb_ctx** out);
 int32_t rb_ctx_destroy(rb_ctx* ctx);
 int32_t rb_last_error(char* buf, size_t len);
 /* Waits for all work on the context's stream (bounded: RB_ERR_TIMEOUT after ~60 s). */
@@ -174,6 +181,9 @@ int32_t rb_kv_pool_destroy(rb_ctx* ctx, int32_t pool);
 /* Permutes the order in which free pages are handed out (deterministic in seed). */
 int32_t rb_kv_pool_shuffle(rb_ctx* ctx, int32_t pool, uint64_t seed);
 int32_t rb_kv_pool_free_pages(rb_ctx* ctx, int32_t pool);
+/* The pool's device memory, [page][layer][k | v][kv head][16 tokens][head_dim] in its
+ * dtype, and its size in bytes. */
+int32_t rb_kv_pool_data(rb_ctx* ctx, int32_t pool, void** data, uint64_t* bytes);
 /* KVCache::new (kv_cache.rs:24-34) for one tenant. */
 int32_t rb_kv_create(rb_ctx* ctx, int32_t pool, uint32_t tenant);
 int32_t rb_kv_destroy(rb_ctx* ctx, int32_t pool, uint32_t tenant);
@@ -201,6 +211,81 @@ int32_t rb_kv_gather(rb_ctx* ctx, int32_t pool, uint32_t tenant, uint32_t layer,
 int32_t rb_attention_forward(rb_ctx* ctx, int32_t pool, uint32_t layer, uint32_t n_rows, const uint32_t* tenants,
                              const uint32_t* positions, const float* q, const float* k_new, const float* v_new,
                              float* out, uint32_t n_heads, float scale, uint32_t flags);
+
+/* ---- row plans ----
+ * Operators of models that the reference does not have: per-head norms of queries
+ * and keys, rotation of part of a head or of adjacent pairs, attention with capped
+ * scores, a bias that falls with distance, and document, prefix and window masks.
+ * They work on the rows of one step over a KV pool, any number of them. A plan
+ * holds the rows and what the kernels need to know about them; it is made once for
+ * a step and used by every layer. */
+typedef struct rb_plan_desc {
+  uint32_t n_heads;          /* query heads: a multiple of the pool's kv heads, at most 64 per kv head */
+  uint32_t n_rows;
+  const uint32_t* tenants;   /* [n_rows] */
+  const uint32_t* positions; /* [n_rows], or NULL: each tenant's next positions (after its length at layer 0) */
+  const uint32_t* begin;     /* [n_rows] first key that a row sees, or NULL: 0 (a document's first token) */
+  const uint32_t* end;       /* [n_rows] one past the last, or NULL: position + 1 (a prefix that every row
+                              * sees: max(position + 1, prefix length)); end <= begin: the row sees no key */
+  uint32_t window;           /* 0: none; else a row at position t sees no key below t - window + 1 */
+} rb_plan_desc;
+/* Makes a plan (host arrays, copied). Pages for every position and key of its rows
+ * are taken from the pool here, all or none (RB_ERR_KV_POOL_EXHAUSTED). Fails with
+ * RB_ERR_NOT_FOUND (tenant), RB_ERR_KV_OVERFLOW (position or end past max_seq),
+ * RB_ERR_UNSUPPORTED (heads). Returns RB_OK. */
+int32_t rb_plan_create(rb_ctx* ctx, int32_t pool, const rb_plan_desc* desc, int32_t* plan);
+/* Waits for the context's stream, then frees the plan. Cached tokens stay. */
+int32_t rb_plan_destroy(rb_ctx* ctx, int32_t plan);
+
+/* Layouts of the rows that go in: element (row, head, i) of q lies at
+ * q[row * ldq + head * head_dim + i], and so on; ld* count elements, and at least
+ * heads * head_dim of them, so q, k and v may be slices of one projection's output. */
+#define RB_ROPE_HALF 0     /* pairs (i, i + rotary / 2) */
+#define RB_ROPE_ADJACENT 1 /* pairs (2i, 2i + 1), crates/realm-models/src/attention.rs:171-240 */
+typedef struct rb_append_desc {
+  int32_t dtype;       /* of q, k, v and q_out: RB_F32 or RB_F16 */
+  int32_t rope_style;  /* RB_ROPE_HALF or RB_ROPE_ADJACENT */
+  const void* q;       /* NULL: keys and values only */
+  const void* k;
+  const void* v;
+  void* q_out;         /* may be q itself, with ldo == ldq */
+  uint64_t ldq, ldk, ldv, ldo;
+  const float* q_norm; /* [head_dim] weights of the queries' norms, or NULL: no norm */
+  const float* k_norm;
+  float eps;
+  uint32_t rotary;     /* elements of each head that are rotated: 0, or a multiple of 8 up to head_dim */
+  const float* rope;   /* [rope_len][rotary]: the cosines of a position's rotary / 2 angles, then their sines */
+  uint32_t rope_len;   /* > every position of the plan */
+} rb_append_desc;
+/* q and k of the plan's rows are normalised head by head,
+ * x_i w_i / sqrt(mean x^2 + eps), then rotated, all in fp32; q goes to q_out, k and
+ * v to `layer` of the cache, each rounded once. A tenant's rows must continue its
+ * cache: ascending positions without gaps, the first at most its length at `layer`
+ * (below it: cached tokens are overwritten). Returns n_rows. */
+int32_t rb_plan_append(rb_ctx* ctx, int32_t plan, uint32_t layer, const rb_append_desc* desc, uint32_t flags);
+
+typedef struct rb_attention_desc {
+  int32_t dtype;       /* of q and out: RB_F32 or RB_F16 */
+  float scale;
+  float softcap;       /* 0: none; else x -> softcap * tanh(x / softcap) */
+  const void* q;
+  void* out;
+  uint64_t ldq, ldo;
+  const float* slopes; /* [n_heads] or NULL: slopes[h] * |position - key| is taken off the (capped) score */
+} rb_attention_desc;
+/* Attention of the plan's rows over `layer` of the cache: out = softmax(s) . v over
+ * the keys that a row sees, s = cap(scale * q . k) - slope * distance; 0 for a row
+ * that sees none. What lies in keys that a row does not see never reaches it.
+ * Every key of the plan has to be cached (RB_ERR_OUT_OF_BOUNDS). fp32 rows are
+ * computed to fp32 accuracy on either cache type, fp16 rows with probabilities
+ * rounded to fp16 on fp16 caches. Returns n_rows. */
+int32_t rb_plan_attention(rb_ctx* ctx, int32_t plan, uint32_t layer, const rb_attention_desc* desc, uint32_t flags);
+/* Test hook, host only: the work lists for rows [n_rows][4] (position, first key,
+ * one past the last, tenant) as rb_plan_create makes them. Writes at most cap units
+ * of 10 values (kernel 0 small / 1 tile, CTA, row0, v0, nv, kv head, tenant, k0, k1,
+ * slot) and returns their number. */
+int32_t rb_plan_partition(uint32_t n_rows, const int32_t* rows, uint32_t n_heads, uint32_t n_kv, uint32_t num_sms,
+                          int32_t f16_cache, int32_t* units, uint32_t cap);
 
 /* ---- model ---- */
 typedef struct rb_model_config {
@@ -407,6 +492,31 @@ typedef struct rb_sampling {
 int32_t rb_sample_logits(rb_ctx* ctx, const float* logits, uint32_t ld, uint32_t n_rows, uint32_t vocab,
                          const rb_sampling* params, const uint32_t* prev_tokens, const uint32_t* prev_offsets,
                          const float* uniforms, uint32_t* out_tokens, uint32_t flags);
+/* Filtered sampling: any vocabulary up to 262144, fp32 or fp16 logits, with min-p.
+ * With x the row after its repetition penalty (as above), m = max x and t the
+ * temperature, a token weighs w = exp(x / t - m / t) in fp32, kept in fixed point
+ * with 40 fractional bits, so that all sums are exact and the result depends on no
+ * order. Tokens rank by weight, ties by the lowest index. Kept are the first top_k
+ * ranks with w >= min_p, and of these the ranks with less than top_p of their
+ * weight before them; the draw takes the first kept index whose running sum
+ * exceeds uniform * total. A temperature below 1e-7 takes the first rank. A logit
+ * that is not a number counts as -infinity. */
+typedef struct rb_sampling_filter {
+  float temperature;
+  uint32_t top_k;           /* used when 0 < top_k < vocab */
+  float top_p;              /* used when 0 < top_p < 1 */
+  float min_p;              /* 0: off; above 1 counts as 1 */
+  float repetition_penalty; /* 1: off */
+} rb_sampling_filter;
+/* One token per row of logits [n_rows][ld] (dtype RB_F32 or RB_F16). params, prev_*,
+ * uniforms and pointer spaces as rb_sample_logits; probs: NULL, or [n_rows] the
+ * tokens' probabilities among those kept. A row without a finite or +infinite
+ * logit gets token 0xffffffff; unless RB_ASYNC, the call then returns
+ * RB_ERR_INVALID ("Failed to create weighted index"). Returns n_rows. */
+int32_t rb_sample_filtered(rb_ctx* ctx, int32_t dtype, const void* logits, uint64_t ld, uint32_t n_rows,
+                           uint32_t vocab, const rb_sampling_filter* params, const uint32_t* prev_tokens,
+                           const uint32_t* prev_offsets, const float* uniforms, uint32_t* out_tokens, float* probs,
+                           uint32_t flags);
 /* The counter-based uniform draw in [0, 1) (a multiple of 2^-23) of (seed, counter):
  * SplitMix64 of seed + counter * 0x9E3779B97F4A7C15, top 23 bits. */
 float rb_sampling_uniform(uint64_t seed, uint64_t counter);

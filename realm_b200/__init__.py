@@ -72,6 +72,7 @@ def _sig(name, args, res=C.c_int32):
 
 
 _sig("rb_ctx_create", [C.POINTER(_Config), C.POINTER(_vp)])
+_sig("rb_ctx_create_on_stream", [C.POINTER(_Config), _vp, C.POINTER(_vp)])
 _sig("rb_ctx_destroy", [_vp])
 _sig("rb_last_error", [C.c_char_p, _sz])
 _sig("rb_sync", [_vp])
@@ -95,6 +96,7 @@ _sig("rb_kv_pool_create", [_vp, _u32, _u32, _u32, _i32, _u32, _u32, _u32, _I32P]
 _sig("rb_kv_pool_destroy", [_vp, _i32])
 _sig("rb_kv_pool_shuffle", [_vp, _i32, _u64])
 _sig("rb_kv_pool_free_pages", [_vp, _i32])
+_sig("rb_kv_pool_data", [_vp, _i32, C.POINTER(_vp), C.POINTER(_u64)])
 _sig("rb_kv_create", [_vp, _i32, _u32])
 _sig("rb_kv_destroy", [_vp, _i32, _u32])
 _sig("rb_kv_clear", [_vp, _i32, _u32])
@@ -191,12 +193,17 @@ def _u32arr(a):
 
 
 class Context:
-    """One GPU (rb_ctx). Calls are serialised on the context's stream."""
+    """One GPU (rb_ctx). Calls are serialised on the context's stream: its own, or
+    the caller's cudaStream_t `stream` (e.g. torch.cuda.current_stream().cuda_stream)."""
 
-    def __init__(self, device: int = 0, max_rows: int = 64, pdl: bool = True, graphs: bool = True):
+    def __init__(self, device: int = 0, max_rows: int = 64, pdl: bool = True, graphs: bool = True,
+                 stream: Optional[int] = None):
         cfg = _Config(device, max_rows, int(pdl), int(graphs))
         h = _vp()
-        _check(_lib.rb_ctx_create(C.byref(cfg), C.byref(h)))
+        if stream is None:
+            _check(_lib.rb_ctx_create(C.byref(cfg), C.byref(h)))
+        else:
+            _check(_lib.rb_ctx_create_on_stream(C.byref(cfg), stream, C.byref(h)))
         self._h = h
         self.device = device
         _ORDER_CTX[0] = self
@@ -351,12 +358,42 @@ class KVPool:
         self.ctx = ctx
         self.n_layers, self.n_kv, self.hd, self.kv_dtype = n_layers, n_kv_heads, head_dim, kv_dtype
         self.max_seq = max_seq
+        self._owned = handle is None  # a model's pool goes with its model
         if handle is None:
             h = C.c_int32()
             _check(_lib.rb_kv_pool_create(ctx.handle, n_layers, n_kv_heads, head_dim, kv_dtype, n_pages,
                                           max_tenants, max_seq, C.byref(h)))
             handle = h.value
         self.handle = handle
+
+    def close(self):
+        """Frees the pool's memory and its plans."""
+        if not self._owned:
+            raise ValueError("the pool belongs to a model")
+        if self.handle >= 0 and self.ctx.handle:
+            _check(_lib.rb_kv_pool_destroy(self.ctx.handle, self.handle))
+        self.handle = -1
+
+    def pages(self):
+        """The pool's memory as a CUDA tensor [page][layer][k | v][kv head][16][head_dim] (a view)."""
+        import torch
+        p, n = _vp(), _u64()
+        _check(_lib.rb_kv_pool_data(self.ctx.handle, self.handle, C.byref(p), C.byref(n)))
+        esz = 2 if self.kv_dtype == F16 else 4
+        shape = (n.value // (esz * self.n_layers * 2 * self.n_kv * 16 * self.hd), self.n_layers, 2, self.n_kv, 16,
+                 self.hd)
+
+        class _View:
+            __cuda_array_interface__ = {"shape": shape, "typestr": "<f2" if esz == 2 else "<f4",
+                                        "data": (p.value, False), "version": 3}
+
+        return torch.as_tensor(_View(), device=torch.device("cuda", self.ctx.device))
+
+    def plan(self, tenants, n_heads: int, positions=None, begin=None, end=None, window: int = 0) -> "RowPlan":
+        """The rows of one step: row r is tenants[r] at positions[r] (None: the tenants' next
+        positions) and sees the keys [begin[r], end[r]) (None: 0 and position + 1), within the
+        last `window` up to its own position where window > 0."""
+        return RowPlan(self, tenants, n_heads, positions, begin, end, window)
 
     def shuffle(self, seed: int):
         _check(_lib.rb_kv_pool_shuffle(self.ctx.handle, self.handle, seed))
@@ -578,3 +615,4 @@ from .batching import (BatchedRequest, BatchStats, ContinuousBatcher, Scheduler,
                        prepare_batch)
 from .gguf import GGUFFile, TensorDesc  # noqa: E402
 from .sampling import LogitsProcessor, SamplingParams, sample_logits, sampling_uniform  # noqa: E402
+from .rows import RowPlan, SamplingFilter, pack_filters, rope_table, sample_filtered  # noqa: E402

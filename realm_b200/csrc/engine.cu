@@ -18,8 +18,10 @@
 #include "../../include/realm_b200.h"
 #include "attention.cuh"
 #include "common.cuh"
+#include "filter.cuh"
 #include "gemv.cuh"
 #include "quant.cuh"
+#include "rows.cuh"
 #include "sample.cuh"
 #include "xfrag.cuh"
 
@@ -272,6 +274,18 @@ struct Model {
   std::map<int, int> graph_launches;
 };
 
+// The rows of a step (rb_plan_create) and the attention kernels' work lists.
+struct RowPlanTenant {
+  int tenant, first, count, max_key;  // positions [first, first + count) when ascending; keys below max_key
+  bool ascending;
+};
+struct RowSet {
+  int pool = -1, n_heads = 0, n_rows = 0, max_pos = 0;
+  std::vector<RowPlanTenant> tenants;
+  int n_cta = 0, n_tile = 0, n_joins = 0;
+  DevBuf rows, small, cta, tile, joins, part_o, part_ml;
+};
+
 struct Ctx {
   int device = 0, num_sms = 148, max_rows = 64;
   bool pdl = true, graphs = true;
@@ -288,6 +302,8 @@ struct Ctx {
   std::vector<std::unique_ptr<Weight>> weights;
   std::vector<std::unique_ptr<KvPool>> pools;
   std::vector<std::unique_ptr<Model>> models;
+  std::vector<std::unique_ptr<RowSet>> plans;
+  bool own_stream = true;
   float last_ms = 0.f;
   int last_launches = 0;
   int gemv_dbg = 0;  // measurement hook (RB_GEMV_DBG): bit 0 skips the GEMV math, bit 1 phase stamps
@@ -976,7 +992,7 @@ int32_t rb_last_error(char* buf, size_t len) {
   return (int32_t)n;
 }
 
-int32_t rb_ctx_create(const rb_config* cfg, rb_ctx** out) {
+static int32_t ctx_create(const rb_config* cfg, bool own_stream, cudaStream_t stream, rb_ctx** out) {
   if (!out) return fail(RB_ERR_INVALID, "out is NULL");
   rb_config def{0, 64, 1, 1};
   if (!cfg) cfg = &def;
@@ -1006,7 +1022,13 @@ int32_t rb_ctx_create(const rb_config* cfg, rb_ctx** out) {
   if (const char* d = getenv("RB_ATTN_GROUP")) c->attn_group = atoi(d) != 0;
   if (const char* d = getenv("RB_ATTN_WHOLE")) c->attn_whole = atoi(d);
   if (const char* d = getenv("RB_MERGE_V")) c->merge_v = atoi(d) != 0;
-  RB_CUDA(cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking));
+  c->own_stream = own_stream;
+  if (own_stream) {
+    RB_CUDA(cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking));
+  } else {
+    c->stream = stream;
+    if (!stream || stream == cudaStreamLegacy) c->graphs = false;
+  }
   RB_CUDA(cudaEventCreate(&c->ev0));
   RB_CUDA(cudaEventCreate(&c->ev1));
   RB_CUDA(cudaEventCreateWithFlags(&c->pinned_ev, cudaEventDisableTiming));
@@ -1026,6 +1048,11 @@ int32_t rb_ctx_create(const rb_config* cfg, rb_ctx** out) {
   return RB_OK;
 }
 
+int32_t rb_ctx_create(const rb_config* cfg, rb_ctx** out) { return ctx_create(cfg, true, nullptr, out); }
+int32_t rb_ctx_create_on_stream(const rb_config* cfg, void* stream, rb_ctx** out) {
+  return ctx_create(cfg, false, (cudaStream_t)stream, out);
+}
+
 int32_t rb_ctx_destroy(rb_ctx* c) {
   if (!c) return fail(RB_ERR_BAD_HANDLE, "null context");
   cudaSetDevice(c->device);
@@ -1034,13 +1061,14 @@ int32_t rb_ctx_destroy(rb_ctx* c) {
     if (m)
       for (auto& g : m->graphs) cudaGraphExecDestroy(g.second);
   c->models.clear();
+  c->plans.clear();
   c->pools.clear();
   c->weights.clear();
   if (c->pinned) cudaFreeHost(c->pinned);
   cudaEventDestroy(c->ev0);
   cudaEventDestroy(c->ev1);
   cudaEventDestroy(c->pinned_ev);
-  cudaStreamDestroy(c->stream);
+  if (c->own_stream) cudaStreamDestroy(c->stream);
   delete c;
   return RB_OK;
 }
@@ -1344,6 +1372,8 @@ int32_t rb_kv_pool_create(rb_ctx* c, uint32_t n_layers, uint32_t n_kv, uint32_t 
 int32_t rb_kv_pool_destroy(rb_ctx* c, int32_t pool) {
   if (!get_pool(c, pool)) return fail(RB_ERR_BAD_HANDLE, "pool %d", pool);
   cudaStreamSynchronize(c->stream);
+  for (auto& p : c->plans)
+    if (p && p->pool == pool) p.reset();
   c->pools[pool].reset();
   return RB_OK;
 }
@@ -1360,6 +1390,15 @@ int32_t rb_kv_pool_free_pages(rb_ctx* c, int32_t pool) {
   KvPool* P = get_pool(c, pool);
   if (!P) return fail(RB_ERR_BAD_HANDLE, "pool %d", pool);
   return (int32_t)P->free_list.size();
+}
+
+int32_t rb_kv_pool_data(rb_ctx* c, int32_t pool, void** data, uint64_t* bytes) {
+  KvPool* P = get_pool(c, pool);
+  if (!P) return fail(RB_ERR_BAD_HANDLE, "pool %d", pool);
+  if (!data || !bytes) return fail(RB_ERR_INVALID, "null output");
+  *data = P->pool.p;
+  *bytes = P->pool.n;
+  return RB_OK;
 }
 
 int32_t rb_kv_create(rb_ctx* c, int32_t pool, uint32_t t) {
@@ -2125,3 +2164,351 @@ extern "C" int32_t rb_weight_matmul_noalloc(rb_ctx* c, int32_t h, const float* i
   if (int rc = sync_ctx(c)) return rc;
   return (int32_t)(batch * w.n);
 }
+
+// ---------------------------------------------------------------------------
+// row plans (rb_plan_*) and filtered sampling
+// ---------------------------------------------------------------------------
+namespace {
+
+RowSet* get_plan(rb_ctx* c, int32_t plan) {
+  if (!c || plan < 0 || plan >= (int)c->plans.size() || !c->plans[plan]) return nullptr;
+  return c->plans[plan].get();
+}
+
+template <class T>
+int upload_vec(Ctx* c, DevBuf& d, const std::vector<T>& v) {
+  if (v.empty()) return RB_OK;
+  RB_CUDA(d.alloc(v.size() * sizeof(T)));
+  RB_CUDA(cudaMemcpyAsync(d.p, v.data(), v.size() * sizeof(T), cudaMemcpyHostToDevice, c->stream));
+  return RB_OK;
+}
+
+int row_dtype(int32_t dtype) {
+  if (dtype != RB_F32 && dtype != RB_F16) return fail(RB_ERR_UNSUPPORTED, "row dtype %d", dtype);
+  return RB_OK;
+}
+
+// A buffer of `rows` rows of `width` elements, `ld` apart: checked, and staged on
+// the device when it is host memory.
+int stage_rows(Ctx* c, const char* name, const void* p, uint64_t ld, size_t rows, size_t width, size_t esz,
+               uint32_t flags, Staged& out) {
+  if (!p) return fail(RB_ERR_INVALID, "%s NULL", name);
+  if (ld < width) return fail(RB_ERR_INVALID, "ld %llu of %s below its row of %zu", (unsigned long long)ld, name, width);
+  if ((uintptr_t)p % esz) return fail(RB_ERR_INVALID, "%s is not aligned to its elements", name);
+  return stage(c, p, ((rows - 1) * ld + width) * esz, flags, out);
+}
+
+// Takes pages so that tenants[i].second positions fit, all or none, and copies the
+// new page-table entries to the device.
+int reserve_pages(Ctx* c, KvPool& P, const std::vector<std::pair<int, int>>& want) {
+  std::vector<std::pair<int, int>> taken;  // tenant, pages it had
+  for (auto [t, upto] : want) {
+    KvTenant& T = P.tenants[t];
+    taken.push_back({t, (int)T.pages.size()});
+    while ((int)T.pages.size() * kRowPage < upto) {
+      if (P.free_list.empty()) {
+        for (auto it = taken.rbegin(); it != taken.rend(); ++it) {
+          std::vector<int>& pg = P.tenants[it->first].pages;
+          while ((int)pg.size() > it->second) {
+            P.free_list.push_back(pg.back());
+            pg.pop_back();
+          }
+        }
+        return fail(RB_ERR_KV_POOL_EXHAUSTED, "KV page pool exhausted");
+      }
+      T.pages.push_back(P.free_list.back());
+      P.free_list.pop_back();
+    }
+  }
+  for (auto [t, had] : taken) {
+    const std::vector<int>& pg = P.tenants[t].pages;
+    const int n = (int)pg.size() - had;
+    if (n <= 0) continue;
+    int32_t* h = &P.h_ptab[(size_t)t * P.max_pages_per_tenant + had];
+    std::copy(pg.begin() + had, pg.end(), h);
+    RB_CUDA(cudaMemcpyAsync(P.ptab.as<int32_t>() + (size_t)t * P.max_pages_per_tenant + had, h, (size_t)n * 4,
+                            cudaMemcpyHostToDevice, c->stream));
+  }
+  return RB_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t rb_plan_partition(uint32_t n_rows, const int32_t* rows, uint32_t n_heads, uint32_t n_kv, uint32_t num_sms,
+                          int32_t f16_cache, int32_t* units, uint32_t cap) {
+  if (!rows || !n_rows || !n_kv || !n_heads || n_heads % n_kv || !num_sms || (cap && !units))
+    return fail(RB_ERR_INVALID, "bad partition arguments");
+  std::vector<RowInfo> r(n_rows);
+  for (uint32_t i = 0; i < n_rows; ++i) r[i] = {rows[4 * i], rows[4 * i + 1], rows[4 * i + 2], rows[4 * i + 3]};
+  RowWork w;
+  rows_partition(r, (int)n_heads, (int)n_kv, (int)num_sms, f16_cache != 0, w);
+  uint32_t n = 0;
+  auto put = [&](int kind, int cta, const AttnUnit& u) {
+    if (n < cap) {
+      const int32_t v[10] = {kind, cta, u.row0, u.v0, u.nv, u.kvh, u.tenant, u.k0, u.k1, u.slot};
+      std::copy(v, v + 10, units + (size_t)n * 10);
+    }
+    ++n;
+  };
+  for (size_t b = 0; b + 1 < w.small_cta.size(); ++b)
+    for (int i = w.small_cta[b]; i < w.small_cta[b + 1]; ++i) put(0, (int)b, w.small[i]);
+  for (size_t i = 0; i < w.tile.size(); ++i) put(1, (int)i, w.tile[i]);
+  return (int32_t)n;
+}
+
+int32_t rb_plan_create(rb_ctx* c, int32_t pool, const rb_plan_desc* d, int32_t* plan) {
+  KvPool* P = get_pool(c, pool);
+  if (!P) return fail(RB_ERR_BAD_HANDLE, "pool %d", pool);
+  if (!d || !plan || !d->tenants) return fail(RB_ERR_INVALID, "null argument");
+  if (d->n_rows == 0 || d->n_rows > (1u << 24)) return fail(RB_ERR_INVALID, "n_rows %u not in [1, 2^24]", d->n_rows);
+  if (d->n_heads == 0 || d->n_heads % P->n_kv || d->n_heads / P->n_kv > (uint32_t)kMaxRep)
+    return fail(RB_ERR_UNSUPPORTED, "n_heads %u for %d kv heads", d->n_heads, P->n_kv);
+  RB_CUDA(cudaSetDevice(c->device));
+  auto S = std::make_unique<RowSet>();
+  S->pool = pool;
+  S->n_heads = (int)d->n_heads;
+  S->n_rows = (int)d->n_rows;
+  std::vector<RowInfo> rows(d->n_rows);
+  std::vector<int> of(P->max_tenants, -1);
+  for (uint32_t r = 0; r < d->n_rows; ++r) {
+    const uint32_t t = d->tenants[r];
+    if (t >= (uint32_t)P->max_tenants || !P->tenants[t].live) return fail(RB_ERR_NOT_FOUND, "tenant %u not created", t);
+    if (of[t] < 0) {
+      of[t] = (int)S->tenants.size();
+      const int first = d->positions ? (int)std::min<uint32_t>(d->positions[r], 1u << 30) : P->tenants[t].len[0];
+      S->tenants.push_back({(int)t, first, 0, 0, true});
+    }
+    RowPlanTenant& T = S->tenants[of[t]];
+    const uint32_t next = (uint32_t)(T.first + T.count);
+    const uint32_t pos = d->positions ? d->positions[r] : next;
+    if (pos >= (uint32_t)P->max_seq) return fail(RB_ERR_KV_OVERFLOW, "KV cache overflow: %u + 1 > %d", pos, P->max_seq);
+    const uint32_t begin = d->begin ? d->begin[r] : 0, end = d->end ? d->end[r] : pos + 1;
+    if (end > (uint32_t)P->max_seq) return fail(RB_ERR_KV_OVERFLOW, "row %u: end %u > %d", r, end, P->max_seq);
+    T.ascending = T.ascending && pos == next;
+    ++T.count;
+    uint32_t lo = begin;
+    if (d->window && pos >= d->window) lo = std::max(lo, pos - d->window + 1);
+    rows[r] = lo < end ? RowInfo{(int)pos, (int)lo, (int)end, (int)t} : RowInfo{(int)pos, 0, 0, (int)t};
+    T.max_key = std::max(T.max_key, rows[r].hi);
+    S->max_pos = std::max(S->max_pos, (int)pos);
+  }
+  std::vector<std::pair<int, int>> want;
+  for (const RowPlanTenant& T : S->tenants)
+    want.push_back({T.tenant, std::max(T.max_key, T.ascending ? T.first + T.count : 0)});
+  RowWork w;
+  rows_partition(rows, S->n_heads, P->n_kv, c->num_sms, false, w);
+  S->n_cta = (int)w.small_cta.size() ? (int)w.small_cta.size() - 1 : 0;
+  S->n_tile = (int)w.tile.size();
+  S->n_joins = (int)w.joins.size();
+  if (int rc = upload_vec(c, S->rows, rows)) return rc;
+  if (int rc = upload_vec(c, S->small, w.small)) return rc;
+  if (int rc = upload_vec(c, S->cta, w.small_cta)) return rc;
+  if (int rc = upload_vec(c, S->tile, w.tile)) return rc;
+  if (int rc = upload_vec(c, S->joins, w.joins)) return rc;
+  if (w.n_slots) {
+    if (S->part_o.alloc((size_t)w.n_slots * P->hd * 4) != cudaSuccess ||
+        S->part_ml.alloc((size_t)w.n_slots * 8) != cudaSuccess)
+      return fail(RB_ERR_OOM, "partial results of %d vectors", w.n_slots);
+  }
+  if (int rc = reserve_pages(c, *P, want)) return rc;
+  // the lists are copied from this call's own memory
+  RB_CUDA(cudaStreamSynchronize(c->stream));
+  size_t h = 0;
+  while (h < c->plans.size() && c->plans[h]) ++h;
+  if (h == c->plans.size()) c->plans.emplace_back();
+  c->plans[h] = std::move(S);
+  *plan = (int32_t)h;
+  return RB_OK;
+}
+
+int32_t rb_plan_destroy(rb_ctx* c, int32_t plan) {
+  if (!get_plan(c, plan)) return fail(RB_ERR_BAD_HANDLE, "plan %d", plan);
+  cudaStreamSynchronize(c->stream);
+  c->plans[plan].reset();
+  return RB_OK;
+}
+
+int32_t rb_plan_append(rb_ctx* c, int32_t plan, uint32_t layer, const rb_append_desc* d, uint32_t flags) {
+  RowSet* S = get_plan(c, plan);
+  if (!S) return fail(RB_ERR_BAD_HANDLE, "plan %d", plan);
+  KvPool& P = *c->pools[S->pool];
+  if (!d) return fail(RB_ERR_INVALID, "null descriptor");
+  if (layer >= (uint32_t)P.n_layers) return fail(RB_ERR_NOT_FOUND, "layer %u", layer);
+  if (int rc = row_dtype(d->dtype)) return rc;
+  if (d->rope_style != RB_ROPE_HALF && d->rope_style != RB_ROPE_ADJACENT)
+    return fail(RB_ERR_UNSUPPORTED, "rope style %d", d->rope_style);
+  if (d->rotary % 8 || d->rotary > (uint32_t)P.hd)
+    return fail(RB_ERR_UNSUPPORTED, "rotary %u not a multiple of 8 up to %d", d->rotary, P.hd);
+  if (d->rotary && (!d->rope || d->rope_len <= (uint32_t)S->max_pos))
+    return fail(RB_ERR_INVALID, "rotation table of %u positions, %d needed", d->rope ? d->rope_len : 0, S->max_pos + 1);
+  for (const RowPlanTenant& T : S->tenants) {
+    const KvTenant& K = P.tenants[T.tenant];
+    if (!K.live) return fail(RB_ERR_NOT_FOUND, "tenant %d not created", T.tenant);
+    if (!T.ascending) return fail(RB_ERR_INVALID, "tenant %d: positions of the plan do not follow one another", T.tenant);
+    if (T.first > K.len[layer])
+      return fail(RB_ERR_INVALID, "tenant %d: position %d past cache length %d", T.tenant, T.first, K.len[layer]);
+    if ((int)K.pages.size() * kRowPage < T.first + T.count)
+      return fail(RB_ERR_OUT_OF_BOUNDS, "tenant %d was cleared after the plan was made", T.tenant);
+  }
+  RB_CUDA(cudaSetDevice(c->device));
+  const size_t esz = d->dtype == RB_F16 ? 2 : 4, n = (size_t)S->n_rows;
+  const size_t wq = (size_t)S->n_heads * P.hd, wk = (size_t)P.n_kv * P.hd;
+  Staged sq, sk, sv, nq, nk, sr, so;
+  if (d->q) {
+    if (int rc = stage_rows(c, "q", d->q, d->ldq, n, wq, esz, flags, sq)) return rc;
+    if (d->q_out == d->q && d->ldo != d->ldq) return fail(RB_ERR_INVALID, "q_out is q with another ld");
+    if (int rc = stage_rows(c, "q_out", d->q_out, d->ldo, n, wq, esz, flags, so)) return rc;
+  }
+  if (int rc = stage_rows(c, "k", d->k, d->ldk, n, wk, esz, flags, sk)) return rc;
+  if (int rc = stage_rows(c, "v", d->v, d->ldv, n, wk, esz, flags, sv)) return rc;
+  if (d->q_norm)
+    if (int rc = stage(c, d->q_norm, (size_t)P.hd * 4, flags, nq)) return rc;
+  if (d->k_norm)
+    if (int rc = stage(c, d->k_norm, (size_t)P.hd * 4, flags, nk)) return rc;
+  if (d->rotary)
+    if (int rc = stage(c, d->rope, (size_t)(S->max_pos + 1) * d->rotary * 4, flags, sr)) return rc;
+  RowAppendArgs a;
+  a.q = sq.dptr;
+  a.k = sk.dptr;
+  a.v = sv.dptr;
+  a.q_out = const_cast<void*>(so.dptr);
+  a.ldq = (int64_t)d->ldq;
+  a.ldk = (int64_t)d->ldk;
+  a.ldv = (int64_t)d->ldv;
+  a.ldo = (int64_t)d->ldo;
+  a.in16 = d->dtype == RB_F16;
+  a.n_rows = S->n_rows;
+  a.n_heads = S->n_heads;
+  a.layer = (int)layer;
+  a.q_norm = (const float*)nq.dptr;
+  a.k_norm = (const float*)nk.dptr;
+  a.eps = d->eps;
+  a.rope = (const float*)sr.dptr;
+  a.rotary = (int)d->rotary;
+  a.adjacent = d->rope_style == RB_ROPE_ADJACENT;
+  a.rows = S->rows.as<RowInfo>();
+  a.kv = P.view();
+  RB_CUDA(rows_append_launch(a, c->num_sms, c->stream));
+  for (const RowPlanTenant& T : S->tenants) {
+    int& len = P.tenants[T.tenant].len[layer];
+    len = std::max(len, T.first + T.count);
+  }
+  if (d->q && !(flags & RB_PTR_DEVICE))
+    RB_CUDA(cudaMemcpy2DAsync(d->q_out, d->ldo * esz, a.q_out, d->ldo * esz, wq * esz, n, cudaMemcpyDeviceToHost,
+                              c->stream));
+  if (!((flags & RB_PTR_DEVICE) && (flags & RB_ASYNC)))
+    if (int rc = sync_ctx(c)) return rc;
+  return S->n_rows;
+}
+
+int32_t rb_plan_attention(rb_ctx* c, int32_t plan, uint32_t layer, const rb_attention_desc* d, uint32_t flags) {
+  RowSet* S = get_plan(c, plan);
+  if (!S) return fail(RB_ERR_BAD_HANDLE, "plan %d", plan);
+  KvPool& P = *c->pools[S->pool];
+  if (!d) return fail(RB_ERR_INVALID, "null descriptor");
+  if (layer >= (uint32_t)P.n_layers) return fail(RB_ERR_NOT_FOUND, "layer %u", layer);
+  if (int rc = row_dtype(d->dtype)) return rc;
+  if (!(d->softcap >= 0.f) || !std::isfinite(d->softcap) || !std::isfinite(d->scale))
+    return fail(RB_ERR_INVALID, "softcap %g, scale %g", d->softcap, d->scale);
+  for (const RowPlanTenant& T : S->tenants) {
+    const KvTenant& K = P.tenants[T.tenant];
+    if (!K.live) return fail(RB_ERR_NOT_FOUND, "tenant %d not created", T.tenant);
+    if (T.max_key > K.len[layer])
+      return fail(RB_ERR_OUT_OF_BOUNDS, "tenant %d: key %d outside cache [0,%d)", T.tenant, T.max_key - 1, K.len[layer]);
+  }
+  RB_CUDA(cudaSetDevice(c->device));
+  const size_t esz = d->dtype == RB_F16 ? 2 : 4, n = (size_t)S->n_rows, w = (size_t)S->n_heads * P.hd;
+  Staged sq, so, ss;
+  if (int rc = stage_rows(c, "q", d->q, d->ldq, n, w, esz, flags, sq)) return rc;
+  if (int rc = stage_rows(c, "out", d->out, d->ldo, n, w, esz, flags, so)) return rc;
+  if (d->slopes)
+    if (int rc = stage(c, d->slopes, (size_t)S->n_heads * 4, flags, ss)) return rc;
+  RowAttnArgs a;
+  if (P.f16) a.tmap = P.tmap;
+  a.q = sq.dptr;
+  a.out = const_cast<void*>(so.dptr);
+  a.ldq = (int64_t)d->ldq;
+  a.ldo = (int64_t)d->ldo;
+  a.q16 = d->dtype == RB_F16;
+  a.layer = (int)layer;
+  a.n_heads = S->n_heads;
+  a.n_rep = S->n_heads / P.n_kv;
+  a.scale = d->scale;
+  a.cap = d->softcap;
+  a.slopes = (const float*)ss.dptr;
+  a.kv = P.view();
+  a.rows = S->rows.as<RowInfo>();
+  a.part_o = S->part_o.as<float>();
+  a.part_ml = S->part_ml.as<float2>();
+  a.err = c->err.as<uint32_t>();
+  a.units = S->small.as<AttnUnit>();
+  a.cta = S->cta.as<int32_t>();
+  a.n_cta = S->n_cta;
+  RB_CUDA(rows_small_launch(a, c->stream));
+  a.joins = S->joins.as<JoinItem>();
+  a.n_joins = S->n_joins;
+  RB_CUDA(rows_join_launch(a, c->stream));
+  if (!(flags & RB_PTR_DEVICE))
+    RB_CUDA(cudaMemcpy2DAsync(d->out, d->ldo * esz, a.out, d->ldo * esz, w * esz, n, cudaMemcpyDeviceToHost, c->stream));
+  if (!((flags & RB_PTR_DEVICE) && (flags & RB_ASYNC)))
+    if (int rc = sync_ctx(c)) return rc;
+  return S->n_rows;
+}
+
+int32_t rb_sample_filtered(rb_ctx* c, int32_t dtype, const void* logits, uint64_t ld, uint32_t n_rows,
+                           uint32_t vocab, const rb_sampling_filter* params, const uint32_t* prev,
+                           const uint32_t* prev_off, const float* uniforms, uint32_t* out, float* probs,
+                           uint32_t flags) {
+  if (!c) return fail(RB_ERR_BAD_HANDLE, "null context");
+  if (int rc = row_dtype(dtype)) return rc;
+  if (!logits || !params || !uniforms || !out) return fail(RB_ERR_INVALID, "logits/params/uniforms/out NULL");
+  if ((prev == nullptr) != (prev_off == nullptr)) return fail(RB_ERR_INVALID, "prev_tokens and prev_offsets go together");
+  if (vocab == 0 || vocab > (uint32_t)kFilterMaxVocab || ld < vocab)
+    return fail(RB_ERR_UNSUPPORTED, "vocab %u not in [1, %d] or ld %llu < vocab", vocab, kFilterMaxVocab,
+                (unsigned long long)ld);
+  if (n_rows == 0) return 0;
+  if (n_rows > (1u << 24)) return fail(RB_ERR_INVALID, "n_rows %u > 2^24", n_rows);
+  RB_CUDA(cudaSetDevice(c->device));
+  const bool dev = flags & RB_PTR_DEVICE;
+  const size_t esz = dtype == RB_F16 ? 2 : 4;
+  Staged sl, sp, sprev, soff, su;
+  if (int rc = stage_rows(c, "logits", logits, ld, n_rows, vocab, esz, flags, sl)) return rc;
+  if (int rc = stage(c, params, (size_t)n_rows * sizeof(rb_sampling_filter), flags, sp)) return rc;
+  if (prev_off) {
+    if (int rc = stage(c, prev_off, (size_t)(n_rows + 1) * 4, flags, soff)) return rc;
+    if (int rc = stage(c, prev, dev ? 0 : (size_t)prev_off[n_rows] * 4, flags, sprev)) return rc;
+  }
+  if (int rc = stage(c, uniforms, (size_t)n_rows * 4, flags, su)) return rc;
+  DevBuf dout;
+  FilterArgs a;
+  a.logits = sl.dptr;
+  a.ld = (int64_t)ld;
+  a.x16 = dtype == RB_F16;
+  a.n_rows = (int)n_rows;
+  a.vocab = (int)vocab;
+  a.params = (const rb_sampling_filter*)sp.dptr;
+  a.prev = (const uint32_t*)sprev.dptr;
+  a.prev_off = prev_off ? (const uint32_t*)soff.dptr : nullptr;
+  a.uniforms = (const float*)su.dptr;
+  a.tokens = out;
+  a.probs = probs;
+  if (!dev) {
+    RB_CUDA(dout.alloc((size_t)n_rows * 8));
+    a.tokens = dout.as<uint32_t>();
+    a.probs = probs ? dout.as<float>() + n_rows : nullptr;
+  }
+  RB_CUDA(filter_launch(a, c->num_sms, c->stream));
+  if (dev && (flags & RB_ASYNC)) return (int32_t)n_rows;
+  std::vector<uint32_t> h(n_rows);
+  RB_CUDA(cudaMemcpyAsync(h.data(), a.tokens, (size_t)n_rows * 4, cudaMemcpyDeviceToHost, c->stream));
+  if (!dev && probs) RB_CUDA(cudaMemcpyAsync(probs, a.probs, (size_t)n_rows * 4, cudaMemcpyDeviceToHost, c->stream));
+  if (int rc = sync_ctx(c)) return rc;
+  for (uint32_t r = 0; r < n_rows; ++r)
+    if (h[r] == 0xffffffffu) return fail(RB_ERR_INVALID, "row %u: Failed to create weighted index", r);
+  if (!dev) std::copy(h.begin(), h.end(), out);
+  return (int32_t)n_rows;
+}
+
+}  // extern "C"

@@ -1,0 +1,101 @@
+// Rows of a step around the paged cache: the plan's work lists (rows_plan.cpp),
+// the append with per-head norms and rotation (rows_append.cu) and masked
+// attention (rows_attn.cu, rows_tile.cu).
+#pragma once
+#include <stdint.h>
+
+#include <vector>
+
+namespace rb {
+
+constexpr int kRowPage = 16;      // tokens per cache page
+constexpr int kSmallVecs = 8;     // query vectors per item of the small kernels
+constexpr int kTileVecs = 256;    // query vectors per item of the tile kernel (two tiles of 128)
+constexpr int kTileKeys = 128;    // keys per block of the tile kernel
+constexpr int kMaxRep = 64;       // query heads per kv head
+
+// One row as the kernels see it: the keys [lo, hi) of its tenant (hi <= lo: none).
+struct RowInfo {
+  int32_t pos, lo, hi, tenant;
+};
+
+// A piece of one item. An item is up to kSmallVecs (kTileVecs) query vectors of
+// one kv head over consecutive rows of one tenant: vector i is head
+// kvh * n_rep + (v0 + i) % n_rep of row row0 + (v0 + i) / n_rep. A unit covers the
+// item's keys [k0, k1) (k0 a multiple of the page size). slot < 0: the unit is the
+// whole item and writes the output; else its vectors' partial results go to
+// slot .. slot + nv.
+struct AttnUnit {
+  int32_t row0, v0, nv, kvh, tenant, k0, k1, slot;
+};
+
+// An item cut into n_parts units: part p of vector i lies at slot0 + p * nv + i.
+struct JoinItem {
+  int32_t row0, v0, nv, kvh, slot0, n_parts;
+};
+
+// Work lists of one plan. CTA b of the small (tile) kernel runs the units
+// [cta[b], cta[b + 1]) of its list.
+struct RowWork {
+  std::vector<AttnUnit> small, tile;
+  std::vector<int32_t> small_cta;
+  std::vector<JoinItem> joins;
+  int32_t n_slots = 0;      // partial result vectors
+  int32_t max_join_parts = 0;
+};
+
+// rows: the plan's rows in call order; use_tile: whether long runs go to the tile
+// kernel (fp16 caches). Pure host code.
+void rows_partition(const std::vector<RowInfo>& rows, int n_heads, int n_kv, int num_sms, bool use_tile, RowWork& out);
+
+}  // namespace rb
+
+#ifdef __CUDACC__
+#include "attention.cuh"
+
+namespace rb {
+
+struct RowAttnArgs {
+  CUtensorMap tmap;  // fp16 caches (kv_tensor_map)
+  const void* q = nullptr;
+  void* out = nullptr;
+  int64_t ldq = 0, ldo = 0;  // elements between rows
+  int32_t q16 = 0;           // 1: q and out are fp16, 0: fp32
+  int32_t layer = 0, n_heads = 0, n_rep = 1;
+  float scale = 1.f, cap = 0.f;
+  const float* slopes = nullptr;  // [n_heads] or null
+  KvView kv;
+  const RowInfo* rows = nullptr;
+  const AttnUnit* units = nullptr;
+  const int32_t* cta = nullptr;  // small kernels
+  int32_t n_cta = 0, n_units = 0;
+  const JoinItem* joins = nullptr;
+  int32_t n_joins = 0;
+  float* part_o = nullptr;   // [n_slots][hd]
+  float2* part_ml = nullptr; // [n_slots] (maximum in base-2 units, sum)
+  uint32_t* err = nullptr;
+};
+
+struct RowAppendArgs {
+  const void *q = nullptr, *k = nullptr, *v = nullptr;  // q may be null
+  void* q_out = nullptr;
+  int64_t ldq = 0, ldk = 0, ldv = 0, ldo = 0;
+  int32_t in16 = 0;
+  int32_t n_rows = 0, n_heads = 0, layer = 0;
+  const float *q_norm = nullptr, *k_norm = nullptr;
+  float eps = 0.f;
+  const float* rope = nullptr;  // [rope_len][rotary]: cosines, then sines
+  int32_t rotary = 0, adjacent = 0;
+  const RowInfo* rows = nullptr;
+  KvView kv;
+};
+
+cudaError_t rows_append_launch(const RowAppendArgs& a, int num_sms, cudaStream_t s);
+// the small kernel over a.units / a.cta
+cudaError_t rows_small_launch(const RowAttnArgs& a, cudaStream_t s);
+// the tile kernel over a.units (one CTA each)
+cudaError_t rows_tile_launch(const RowAttnArgs& a, cudaStream_t s);
+cudaError_t rows_join_launch(const RowAttnArgs& a, cudaStream_t s);
+
+}  // namespace rb
+#endif
