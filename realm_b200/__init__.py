@@ -206,6 +206,7 @@ class Context:
             _check(_lib.rb_ctx_create_on_stream(C.byref(cfg), stream, C.byref(h)))
         self._h = h
         self.device = device
+        self._stream_id = self.stream or 0
         _ORDER_CTX[0] = self
 
     def close(self):
@@ -350,6 +351,25 @@ class Weight:
             self.handle = -1
 
 
+class _PoolMemory:
+    """Frees a closed pool once no KVPool and no tensor uses it."""
+
+    def __init__(self, ctx: Context, handle: int):
+        self.ctx, self.handle, self.closed = ctx, handle, False
+
+    def __del__(self):
+        if self.closed and self.ctx._h and _lib is not None:
+            _lib.rb_kv_pool_destroy(self.ctx.handle, self.handle)
+
+
+class _PoolView:
+    """A pool's memory for torch, which keeps this object, and so the memory."""
+
+    def __init__(self, memory, shape, typestr, ptr):
+        self._memory = memory
+        self.__cuda_array_interface__ = {"shape": shape, "typestr": typestr, "data": (ptr, False), "version": 3}
+
+
 class KVPool:
     """Paged KV pool (16-token pages for all layers of one geometry)."""
 
@@ -365,14 +385,15 @@ class KVPool:
                                           max_tenants, max_seq, C.byref(h)))
             handle = h.value
         self.handle = handle
+        self._memory = _PoolMemory(ctx, handle) if self._owned else None
 
     def close(self):
-        """Frees the pool's memory and its plans."""
+        """Ends the use of the pool and its plans; its memory is freed once no tensor of pages() is left."""
         if not self._owned:
             raise ValueError("the pool belongs to a model")
-        if self.handle >= 0 and self.ctx.handle:
-            _check(_lib.rb_kv_pool_destroy(self.ctx.handle, self.handle))
-        self.handle = -1
+        if self._memory is not None:
+            self._memory.closed = True
+        self.handle, self._memory = -1, None
 
     def pages(self):
         """The pool's memory as a CUDA tensor [page][layer][k | v][kv head][16][head_dim] (a view)."""
@@ -382,12 +403,8 @@ class KVPool:
         esz = 2 if self.kv_dtype == F16 else 4
         shape = (n.value // (esz * self.n_layers * 2 * self.n_kv * 16 * self.hd), self.n_layers, 2, self.n_kv, 16,
                  self.hd)
-
-        class _View:
-            __cuda_array_interface__ = {"shape": shape, "typestr": "<f2" if esz == 2 else "<f4",
-                                        "data": (p.value, False), "version": 3}
-
-        return torch.as_tensor(_View(), device=torch.device("cuda", self.ctx.device))
+        return torch.as_tensor(_PoolView(self._memory, shape, "<f2" if esz == 2 else "<f4", p.value),
+                               device=torch.device("cuda", self.ctx.device))
 
     def plan(self, tenants, n_heads: int, positions=None, begin=None, end=None, window: int = 0) -> "RowPlan":
         """The rows of one step: row r is tenants[r] at positions[r] (None: the tenants' next

@@ -14,7 +14,7 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "librealm_b200.so")
 SOURCES = ["gemv.cu", "attention.cu", "engine.cu", "sample.cu", "scheduler.cpp", "gguf.cpp", "rows_plan.cpp",
-           "rows_append.cu", "rows_attn.cu", "filter.cu"]
+           "rows_append.cu", "rows_attn.cu", "rows_tile.cu", "filter.cu"]
 HEADERS = ["common.cuh", "quant.cuh", "gemv.cuh", "attention.cuh", "xfrag.cuh", "sample.cuh", "rows.cuh", "filter.cuh"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo",

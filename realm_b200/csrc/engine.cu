@@ -2198,35 +2198,32 @@ int stage_rows(Ctx* c, const char* name, const void* p, uint64_t ld, size_t rows
   return stage(c, p, ((rows - 1) * ld + width) * esz, flags, out);
 }
 
-// Takes pages so that tenants[i].second positions fit, all or none, and copies the
-// new page-table entries to the device.
+// Takes pages so that want[i].second tokens of tenant want[i].first fit, in the
+// order of `want`, all or none, and copies the new page-table entries to the device.
 int reserve_pages(Ctx* c, KvPool& P, const std::vector<std::pair<int, int>>& want) {
-  std::vector<std::pair<int, int>> taken;  // tenant, pages it had
+  std::vector<int> taken;         // tenant of every page taken, in order
+  std::map<int, int> had;         // pages a tenant had before its first
   for (auto [t, upto] : want) {
     KvTenant& T = P.tenants[t];
-    taken.push_back({t, (int)T.pages.size()});
     while ((int)T.pages.size() * kRowPage < upto) {
       if (P.free_list.empty()) {
         for (auto it = taken.rbegin(); it != taken.rend(); ++it) {
-          std::vector<int>& pg = P.tenants[it->first].pages;
-          while ((int)pg.size() > it->second) {
-            P.free_list.push_back(pg.back());
-            pg.pop_back();
-          }
+          P.free_list.push_back(P.tenants[*it].pages.back());
+          P.tenants[*it].pages.pop_back();
         }
         return fail(RB_ERR_KV_POOL_EXHAUSTED, "KV page pool exhausted");
       }
+      had.emplace(t, (int)T.pages.size());
       T.pages.push_back(P.free_list.back());
       P.free_list.pop_back();
+      taken.push_back(t);
     }
   }
-  for (auto [t, had] : taken) {
+  for (auto [t, n0] : had) {
     const std::vector<int>& pg = P.tenants[t].pages;
-    const int n = (int)pg.size() - had;
-    if (n <= 0) continue;
-    int32_t* h = &P.h_ptab[(size_t)t * P.max_pages_per_tenant + had];
-    std::copy(pg.begin() + had, pg.end(), h);
-    RB_CUDA(cudaMemcpyAsync(P.ptab.as<int32_t>() + (size_t)t * P.max_pages_per_tenant + had, h, (size_t)n * 4,
+    int32_t* h = &P.h_ptab[(size_t)t * P.max_pages_per_tenant + n0];
+    std::copy(pg.begin() + n0, pg.end(), h);
+    RB_CUDA(cudaMemcpyAsync(P.ptab.as<int32_t>() + (size_t)t * P.max_pages_per_tenant + n0, h, (pg.size() - n0) * 4,
                             cudaMemcpyHostToDevice, c->stream));
   }
   return RB_OK;
@@ -2294,11 +2291,11 @@ int32_t rb_plan_create(rb_ctx* c, int32_t pool, const rb_plan_desc* d, int32_t* 
     T.max_key = std::max(T.max_key, rows[r].hi);
     S->max_pos = std::max(S->max_pos, (int)pos);
   }
-  std::vector<std::pair<int, int>> want;
-  for (const RowPlanTenant& T : S->tenants)
-    want.push_back({T.tenant, std::max(T.max_key, T.ascending ? T.first + T.count : 0)});
+  std::vector<std::pair<int, int>> want;  // rows to be appended need a page for their own position as well
+  for (const RowInfo& r : rows)
+    want.push_back({r.tenant, std::max(r.hi, S->tenants[of[r.tenant]].ascending ? r.pos + 1 : 0)});
   RowWork w;
-  rows_partition(rows, S->n_heads, P->n_kv, c->num_sms, false, w);
+  rows_partition(rows, S->n_heads, P->n_kv, c->num_sms, P->f16 != 0, w);
   S->n_cta = (int)w.small_cta.size() ? (int)w.small_cta.size() - 1 : 0;
   S->n_tile = (int)w.tile.size();
   S->n_joins = (int)w.joins.size();
@@ -2447,6 +2444,9 @@ int32_t rb_plan_attention(rb_ctx* c, int32_t plan, uint32_t layer, const rb_atte
   a.cta = S->cta.as<int32_t>();
   a.n_cta = S->n_cta;
   RB_CUDA(rows_small_launch(a, c->stream));
+  a.units = S->tile.as<AttnUnit>();
+  a.n_units = S->n_tile;
+  RB_CUDA(rows_tile_launch(a, c->stream));
   a.joins = S->joins.as<JoinItem>();
   a.n_joins = S->n_joins;
   RB_CUDA(rows_join_launch(a, c->stream));

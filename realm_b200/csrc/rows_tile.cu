@@ -1,0 +1,584 @@
+// Masked attention of long runs of rows (prompts, chunks) over fp16 caches on
+// tcgen05: the function of rows_attn.cu for up to 256 query vectors of one kv head
+// and tenant, as two tiles of 128 that share every block of 128 keys.
+//
+// Per tile and block: S = Q K^T (tcgen05.mma, both operands in shared memory, S in
+// TMEM), softmax in registers with one thread a row (tcgen05.ld), P back to TMEM
+// over S, O += P V with P as the TMEM operand and V as it lies in the page
+// ([key][element]: the MN-major operand). The tiles take turns: while one's scores
+// are in the softmax warps the tensor core works on the other's.
+//
+// fp32 rows: q and p as fp16 hi + lo parts, two products each (22 bits); q is
+// brought to a power of two near 2^8 first. p counts from 2^kBias and the running
+// maximum is raised only when a score passes it by 2^kSlack, so p stays below
+// 2^15, fp16's range, and O is rarely rescaled.
+//
+// Warps: 0-3 softmax of tile 0, 4-7 of tile 1, 8 issues the products, 9 the loads.
+#include "common.cuh"
+#include "rows.cuh"
+
+namespace rb {
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kBias = 6.f, kSlack = 8.f;
+constexpr int kTileThreads = 320;
+
+// ---- tcgen05 ----
+// shared-memory operand with 128-byte swizzle; sbo: bytes between groups of 8 rows,
+// lbo: between panels of 64 columns (MN-major only)
+__device__ __forceinline__ uint64_t desc128(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) |
+         ((uint64_t)((sbo >> 4) & 0x3FFFu) << 32) | (1ull << 46) | (2ull << 61);
+}
+__host__ __device__ constexpr uint32_t idesc16(int m, int n, int b_mn_major) {
+  return (1u << 4) | ((uint32_t)b_mn_major << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t ad, uint64_t bd, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(ad), "l"(bd), "r"(id), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t at, uint64_t bd, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(at), "l"(bd), "r"(id), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// 32 columns of this thread's TMEM lane; the registers are valid after wait_ld()
+__device__ __forceinline__ void ld32(uint32_t ta, float* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+        "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]),
+        "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]),
+        "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+      : "r"(ta)
+      : "memory");
+}
+__device__ __forceinline__ void st32(uint32_t ta, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(ta),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ float ld1(uint32_t ta) {
+  float r;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=f"(r) : "r"(ta) : "memory");
+  wait_ld();
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b) { return h2_as_u32(__floats2half2_rn(a, b)); }
+__device__ __forceinline__ uint32_t pack2_lo(float a, float b, uint32_t hi) {
+  const float2 f = __half22float2(u32_as_h2(hi));
+  return pack2(a - f.x, b - f.y);
+}
+// barrier of the n softmax threads in use, with the "or" of their values
+__device__ __forceinline__ bool any_softmax(int n, bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, "
+      "q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)v), "r"(n)
+      : "memory");
+  return r != 0;
+}
+// the sign bits of the two halves of w that are infinite or not a number
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) { return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u; }
+
+template <int HD, int HL>
+struct TileCfg {
+  static constexpr int PANEL = 128 * 128;             // 128 rows x 64 fp16
+  static constexpr int QT = HD / 64 * PANEL;          // one tile of q (one part)
+  static constexpr int SLOT = HD / 64 * PANEL;        // a block of K or V
+  static constexpr int NS = HD == 128 ? (HL ? 3 : 5) : 6;
+  static constexpr int SMEM = 1024 + 2 * (1 + HL) * QT + NS * SLOT;
+};
+
+template <int HD, int HL, int CAP, int BIAS>
+__global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid_constant__ RowAttnArgs a) {
+  using C = TileCfg<HD, HL>;
+  constexpr int NS = C::NS, B = kTileKeys;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = smem + 2 * (1 + HL) * C::QT;
+  __shared__ uint64_t q_bar[2], s_bar[2], p_bar[2], o_bar[2], full[NS], freeb[NS], drain;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int primed[2];    // O holds something before the first product
+  __shared__ int span[2][2];  // keys that every row of a tile sees
+  __shared__ int seen[2];     // keys that some row of the unit sees
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const AttnUnit u = a.units[blockIdx.x];
+  const int nt = u.nv > 128 ? 2 : 1, nb = (u.k1 - u.k0 + B - 1) / B;
+
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (tid == 0) {
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&q_bar[t], 128);
+      mbar_init(&s_bar[t], 1);
+      mbar_init(&p_bar[t], 128);
+      mbar_init(&o_bar[t], 1);
+      primed[t] = 0;
+      span[t][0] = 0;
+      span[t][1] = 0x7fffffff;
+    }
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&freeb[i], 1);
+    }
+    mbar_init(&drain, 1);
+    seen[0] = 0x7fffffff;
+    seen[1] = 0;
+    fence_barrier_init();
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = tmem_slot;
+  const int tile = warp >> 2;  // softmax warps
+  RowInfo r{0, 0, 0x7fffffff, 0};
+  int head = 0, row = 0;
+  const bool active = warp < 8 && tid < u.nv;
+  if (active) {
+    const int v = u.v0 + tid;
+    row = u.row0 + v / a.n_rep;
+    head = u.kvh * a.n_rep + v % a.n_rep;
+    r = a.rows[row];
+    atomicMax(&span[tile][0], r.lo);
+    atomicMin(&span[tile][1], r.hi);
+    if (r.hi > r.lo) {
+      atomicMin(&seen[0], r.lo);
+      atomicMax(&seen[1], r.hi);
+    }
+  }
+  __syncthreads();
+
+  if (warp == 9) {
+    // ---- loads: blocks K0, V0, K1, V1, ... through the ring ----
+    bool ok = true;
+    int it = 0;
+    const int page_end = (u.k1 + 15) >> 4;
+    const int32_t* pt = a.kv.ptab + (size_t)u.tenant * a.kv.ptab_stride;
+    for (int j = 0; j < nb && ok; ++j) {
+      const int p0 = (u.k0 >> 4) + j * (B / 16), np = min(B / 16, page_end - p0);
+      const int mine = lane & 7, page = mine < np ? pt[p0 + mine] : 0;
+      for (int w = 0; w < 2; ++w, ++it) {
+        const int s = it % NS;
+        if (it >= NS) {
+          if (lane == 0) ok = mbar_wait(&freeb[s], (uint32_t)((it / NS - 1) & 1), a.err, DEV_TIMEOUT_EMPTY);
+          ok = __shfl_sync(0xffffffffu, ok, 0);
+        }
+        if (!ok) break;  // the whole warp
+        if (lane == 0) mbar_arrive_expect_tx(&full[s], (uint32_t)(np * 16 * HD * 2));
+        __syncwarp();
+        if (mine < np && (lane >> 3) < HD / 64) {
+          const int y = (((page * a.kv.n_layers + a.layer) * 2 + w) * a.kv.n_kv + u.kvh) * 16;
+          asm volatile(
+              "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+              "[%4];" ::"r"(smem_u32(ring + s * C::SLOT + (lane >> 3) * C::PANEL + mine * 2048)),
+              "l"(reinterpret_cast<uint64_t>(&a.tmap)), "r"((lane >> 3) * 64), "r"(y), "r"(smem_u32(&full[s]))
+              : "memory");
+        }
+      }
+    }
+    // copies in flight land before the CTA's shared memory goes away
+    for (int i = max(0, it - NS); i < it; ++i) mbar_wait(&full[i % NS], (uint32_t)((i / NS) & 1), nullptr, 0);
+  } else if (warp == 8) {
+    // ---- products ----
+    if (lane == 0 && nb > 0) {
+      bool ok = true;
+      constexpr uint32_t ids = idesc16(128, B, 0), ido = idesc16(128, HD, 1);
+      const uint32_t qa = smem_u32(smem), ra = smem_u32(ring);
+      auto scores = [&](int t, int slot) {
+#pragma unroll
+        for (int part = 0; part < 1 + HL; ++part)
+#pragma unroll
+          for (int ks = 0; ks < HD / 16; ++ks) {
+            const uint32_t off = (ks >> 2) * C::PANEL + (ks & 3) * 32;
+            mma_ss(tmem + t * B, desc128(qa + (t * (1 + HL) + part) * C::QT + off, 16, 1024),
+                   desc128(ra + slot * C::SLOT + off, 16, 1024), ids, part || ks);
+          }
+      };
+      auto wait = [&](uint64_t* bar, int phase, uint32_t code) {
+        ok = ok && mbar_wait(bar, (uint32_t)(phase & 1), a.err, code);
+        tc_after();
+      };
+      for (int t = 0; t < nt; ++t) wait(&q_bar[t], 0, DEV_TIMEOUT_SMEM);
+      wait(&full[0], 0, DEV_TIMEOUT_FULL);
+      if (ok) {
+        for (int t = 0; t < nt; ++t) {
+          scores(t, 0);
+          tc_commit(&s_bar[t]);
+        }
+        tc_commit(&freeb[0]);
+      }
+      for (int j = 0; j < nb && ok; ++j) {
+        const int iv = 2 * j + 1, ik = 2 * j + 2, vs = iv % NS, ks_ = ik % NS;
+        wait(&full[vs], iv / NS, DEV_TIMEOUT_FULL);
+        for (int t = 0; t < nt && ok; ++t) {
+          wait(&p_bar[t], j, DEV_TIMEOUT_DRAIN);
+          if (!ok) break;
+          const uint32_t more = j || *(volatile int*)&primed[t];
+#pragma unroll
+          for (int part = 0; part < 1 + HL; ++part)
+#pragma unroll
+            for (int ks = 0; ks < B / 16; ++ks)
+              mma_ts(tmem + 2 * B + t * HD, tmem + t * B + part * (B / 2) + ks * 8,
+                     desc128(ra + vs * C::SLOT + ks * 2048, C::PANEL, 1024), ido, more || part || ks);
+          if (t == nt - 1) tc_commit(&freeb[vs]);
+          if (j + 1 < nb) {
+            if (t == 0) wait(&full[ks_], ik / NS, DEV_TIMEOUT_FULL);
+            if (!ok) break;
+            scores(t, ks_);
+            tc_commit(&s_bar[t]);
+            if (t == nt - 1) tc_commit(&freeb[ks_]);
+          } else {
+            tc_commit(&o_bar[t]);
+          }
+        }
+      }
+      tc_commit(&drain);  // own products complete before the accumulators are freed
+      mbar_wait(&drain, 0, a.err, DEV_TIMEOUT_DRAIN);
+    }
+    __syncwarp();
+  } else if (tile < nt) {
+    // ---- softmax: thread = row of its tile ----
+    const int tr = tid & 127;
+    const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t ts = lane_base + tile * B, to = lane_base + 2 * B + tile * HD;
+    bool alive = true;
+    float sv = fabsf(a.scale);
+    {  // q into shared memory, K-major with 128-byte swizzle; a negative scale turns q
+      const float sign = a.scale < 0.f ? -1.f : 1.f;
+      uint8_t* qd = smem + tile * (1 + HL) * C::QT + tr * 128;
+      const size_t at = (size_t)row * a.ldq + (size_t)head * HD;
+      const int rx = tr & 7;
+      if (HL) {
+        const float* q = reinterpret_cast<const float*>(a.q) + at;
+        const bool vec = ((reinterpret_cast<uintptr_t>(a.q) | (size_t)a.ldq * 4) & 15) == 0;
+        float top = 0.f;
+        if (active)
+          for (int d = 0; d < HD; d += 4) {
+            if (vec) {
+              const float4 x = *reinterpret_cast<const float4*>(q + d);
+              top = fmaxf(fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
+            } else {
+              for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(q[d + e]));
+            }
+          }
+        float mul = 1.f;
+        const int e = (int)(__float_as_uint(top) >> 23);
+        if (e > 8 && e < 255) mul = __uint_as_float((uint32_t)min(254, 127 + 8 + 127 - e) << 23);
+        sv = sv / mul;
+        mul *= sign;
+        for (int ch = 0; ch < HD / 8; ++ch) {
+          float x[8];
+          if (active && vec) {
+            *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(q + ch * 8);
+            *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(q + ch * 8 + 4);
+          } else {
+            for (int i = 0; i < 8; ++i) x[i] = active ? q[ch * 8 + i] : 0.f;
+          }
+          uint4 hi, lo;
+          uint32_t* h = &hi.x;
+          uint32_t* l = &lo.x;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            x[2 * i] *= mul;
+            x[2 * i + 1] *= mul;
+            h[i] = pack2(x[2 * i], x[2 * i + 1]);
+            l[i] = pack2_lo(x[2 * i], x[2 * i + 1], h[i]);
+          }
+          uint8_t* dst = qd + (ch >> 3) * C::PANEL + (((ch & 7) ^ rx) << 4);
+          *reinterpret_cast<uint4*>(dst) = hi;
+          *reinterpret_cast<uint4*>(dst + HL * C::QT) = lo;
+        }
+      } else {
+        const __half* q = reinterpret_cast<const __half*>(a.q) + at;
+        const bool vec = ((reinterpret_cast<uintptr_t>(a.q) | (size_t)a.ldq * 2) & 15) == 0;
+        const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+        for (int ch = 0; ch < HD / 8; ++ch) {
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (active) {
+            if (vec) {
+              x = *reinterpret_cast<const uint4*>(q + ch * 8);
+            } else {
+              uint16_t* h = reinterpret_cast<uint16_t*>(&x);
+              for (int i = 0; i < 8; ++i) h[i] = __half_as_ushort(q[ch * 8 + i]);
+            }
+          }
+          x.x ^= flip;
+          x.y ^= flip;
+          x.z ^= flip;
+          x.w ^= flip;
+          *reinterpret_cast<uint4*>(qd + (ch >> 3) * C::PANEL + (((ch & 7) ^ rx) << 4)) = x;
+        }
+      }
+      proxy_fence();
+      mbar_arrive(&q_bar[tile]);
+    }
+    const int all0 = span[tile][0], all1 = span[tile][1], in0 = seen[0], in1 = seen[1];
+    const int both0 = max(span[0][0], span[1][0]), both1 = min(span[0][1], span[1][1]);
+    const float slope = BIAS && active ? a.slopes[head] * kLog2e : 0.f;
+    const float cap2 = a.cap * kLog2e, kcap = CAP ? 2.f * kLog2e * sv / a.cap : 0.f;
+    const float mult = (CAP || BIAS) ? 1.f : fmaxf(sv * kLog2e, 1e-30f);  // scores to base-2 units (-inf stays)
+    const float sv2 = sv * kLog2e;
+    float m = -INFINITY, l = 0.f;
+    for (int j = 0; j < nb; ++j) {
+      const int kb = u.k0 + j * B;
+      if (alive) alive = mbar_wait(&s_bar[tile], (uint32_t)(j & 1), a.err, DEV_TIMEOUT_FULL);
+      tc_after();
+      float x[B];
+#pragma unroll
+      for (int i = 0; i < B / 32; ++i) ld32(ts + 32 * i, x + 32 * i);
+      wait_ld();
+      const bool partial = kb < all0 || kb + B > all1;  // the same for the whole tile
+      if (CAP) {
+        // cap tanh(y / cap) = cap - 2 cap / (1 + e^(2 y / cap))
+#pragma unroll
+        for (int i = 0; i < B; ++i) x[i] = fmaf(-2.f * cap2, rcp(1.f + ex2(x[i] * kcap)), cap2);
+      }
+      if (BIAS) {
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+          x[i] = fmaf(-slope, fabsf((float)(r.pos - kb - i)), CAP ? x[i] : x[i] * sv2);
+      }
+      if (partial) {
+        const uint32_t base = (uint32_t)(kb - r.lo), n = (uint32_t)max(0, r.hi - r.lo);
+#pragma unroll
+        for (int i = 0; i < B; ++i) x[i] = base + i < n ? x[i] : -INFINITY;
+      }
+      float mx4[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+      for (int i = 4; i < B; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], x[i]);
+      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * mult;
+      // each row raises its maximum by its own scores alone
+      const bool up = mx > (m == -INFINITY ? m : m + kSlack);
+      float alpha = 1.f;
+      if (up) {
+        alpha = ex2(m - mx);
+        l *= alpha;
+        m = mx;
+      }
+      if (__any_sync(0xffffffffu, up) && j > 0) {
+        // the scores of this block were issued after the last block's P V: O is at rest
+#pragma unroll 1
+        for (int d = 0; d < HD; d += 32) {
+          float o[32];
+          ld32(to + d, o);
+          wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] *= alpha;
+          st32(to + d, reinterpret_cast<uint32_t*>(o));
+        }
+      }
+      const float off = kBias - (m == -INFINITY ? 0.f : m);
+      float s4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < B / 64; ++i) {
+        uint32_t hi[32], lo[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const float p0 = ex2(fmaf(x[64 * i + 2 * e], mult, off)), p1 = ex2(fmaf(x[64 * i + 2 * e + 1], mult, off));
+          s4[(2 * e) & 3] += p0;
+          s4[(2 * e + 1) & 3] += p1;
+          hi[e] = pack2(p0, p1);
+          if (HL) lo[e] = pack2_lo(p0, p1, hi[e]);
+        }
+        st32(ts + 32 * i, hi);
+        if (HL) st32(ts + B / 2 + 32 * i, lo);
+      }
+      l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+      if (kb < both0 || kb + B > both1) {
+        // A block that some row of the unit does not see whole. Values of keys that no
+        // row sees become 0, and so do those of pages that were not loaded. Values that
+        // are not finite enter O here, each row adding those of its own keys, and are 0
+        // for the product: 0 times one of them would reach the rows that do not see it.
+        const int vs = (2 * j + 1) % NS;
+        if (alive) alive = mbar_wait(&full[vs], (uint32_t)(((2 * j + 1) / NS) & 1), a.err, DEV_TIMEOUT_FULL);
+        uint8_t* vrow = ring + vs * C::SLOT + tr * 128;
+        const bool in = kb + tr >= in0 && kb + tr < in1;
+        const int c0 = tile * (HD / 8 / nt), c1 = c0 + HD / 8 / nt;  // the tiles share the chunks
+        uint32_t bad = 0;
+        for (int ch = c0; ch < c1; ++ch) {
+          uint4* p = reinterpret_cast<uint4*>(vrow + (ch >> 3) * C::PANEL + ((ch & 7) << 4));
+          if (in) {
+            const uint4 q = *p;
+            bad |= not_finite(q.x) | not_finite(q.y) | not_finite(q.z) | not_finite(q.w);
+          } else {
+            *p = make_uint4(0, 0, 0, 0);
+          }
+        }
+        proxy_fence();
+        if (any_softmax(128 * nt, bad != 0)) {
+          wait_st();
+#pragma unroll 1
+          for (int d = 0; d < HD; d += 32) {
+            float o[32];
+            ld32(to + d, o);
+            wait_ld();
+            if (j == 0)
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = 0.f;
+#pragma unroll 1
+            for (int k = 0; k < B; ++k) {
+              float p = 0.f;
+#pragma unroll
+              for (int part = 0; part < 1 + HL; ++part) {
+                const uint32_t w = __float_as_uint(ld1(ts + part * (B / 2) + (k >> 1)));
+                p += half_bits_to_float((k & 1) ? w >> 16 : w);
+              }
+              const uint8_t* vk = ring + vs * C::SLOT + k * 128 + (d >> 6) * C::PANEL;
+              if (p != 0.f)
+#pragma unroll
+                for (int ch = 0; ch < 4; ++ch) {
+                  const uint4 q = *reinterpret_cast<const uint4*>(vk + (((((d >> 3) + ch) & 7) ^ (k & 7)) << 4));
+                  const uint32_t* w = &q.x;
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    const uint32_t nf = not_finite(w[e]);
+                    const float2 f = __half22float2(u32_as_h2(w[e]));
+                    if (nf & 0x8000u) o[ch * 8 + 2 * e] = fmaf(p, f.x, o[ch * 8 + 2 * e]);
+                    if (nf & 0x80000000u) o[ch * 8 + 2 * e + 1] = fmaf(p, f.y, o[ch * 8 + 2 * e + 1]);
+                  }
+                }
+              __syncwarp();
+            }
+            st32(to + d, reinterpret_cast<uint32_t*>(o));
+          }
+          any_softmax(128 * nt, false);  // all rows have taken theirs
+          for (int ch = c0; ch < c1; ++ch) {
+            uint4* p = reinterpret_cast<uint4*>(vrow + (ch >> 3) * C::PANEL + ((ch & 7) << 4));
+            uint32_t* w = reinterpret_cast<uint32_t*>(p);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t nf = not_finite(w[e]);
+              w[e] &= ((nf & 0x8000u) ? 0u : 0xffffu) | ((nf & 0x80000000u) ? 0u : 0xffff0000u);
+            }
+          }
+          proxy_fence();
+          any_softmax(128 * nt, false);
+          if (tr == 0 && j == 0) *(volatile int*)&primed[tile] = 1;
+        }
+      }
+      wait_st();
+      tc_before();
+      mbar_arrive(&p_bar[tile]);
+    }
+    if (nb > 0) {
+      if (alive) alive = mbar_wait(&o_bar[tile], 0, a.err, DEV_TIMEOUT_DRAIN);
+      tc_after();
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int slot = u.slot + tid;
+    if (u.slot >= 0 && active) a.part_ml[slot] = make_float2(m, l);
+    const size_t at = (size_t)row * a.ldo + (size_t)head * HD;
+    const bool vec = ((reinterpret_cast<uintptr_t>(a.out) | (size_t)a.ldo * (HL ? 4 : 2)) & 15) == 0;
+#pragma unroll 1
+    for (int d = 0; d < HD; d += 32) {
+      float o[32];
+      ld32(to + d, o);
+      wait_ld();
+      if (nb == 0 || l == 0.f)
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = 0.f;
+      if (!active) continue;
+      if (u.slot >= 0) {
+        float4* dst = reinterpret_cast<float4*>(a.part_o + (size_t)slot * HD + d);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+      } else if (HL) {
+        float* dst = reinterpret_cast<float*>(a.out) + at + d;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] *= inv;
+        if (vec) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            reinterpret_cast<float4*>(dst)[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) dst[i] = o[i];
+        }
+      } else {
+        __half* dst = reinterpret_cast<__half*>(a.out) + at + d;
+        uint32_t h[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) h[i] = pack2(o[2 * i] * inv, o[2 * i + 1] * inv);
+        if (vec) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            reinterpret_cast<uint4*>(dst)[i] = make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            dst[i] = __ushort_as_half((unsigned short)((i & 1) ? h[i >> 1] >> 16 : h[i >> 1]));
+        }
+      }
+    }
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  if (warp == 8)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+template <int HD, int HL, int CAP, int BIAS>
+cudaError_t launch(const RowAttnArgs& a, cudaStream_t s) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  constexpr int smem = TileCfg<HD, HL>::SMEM;
+  if (cudaError_t e = ensure_smem_attr(rows_tile_kernel<HD, HL, CAP, BIAS>, smem, dev)) return e;
+  rows_tile_kernel<HD, HL, CAP, BIAS><<<a.n_units, kTileThreads, smem, s>>>(a);
+  return cudaGetLastError();
+}
+template <int HD, int HL>
+cudaError_t launch_score(const RowAttnArgs& a, cudaStream_t s) {
+  if (a.cap > 0.f) return a.slopes ? launch<HD, HL, 1, 1>(a, s) : launch<HD, HL, 1, 0>(a, s);
+  return a.slopes ? launch<HD, HL, 0, 1>(a, s) : launch<HD, HL, 0, 0>(a, s);
+}
+
+}  // namespace
+
+cudaError_t rows_tile_launch(const RowAttnArgs& a, cudaStream_t s) {
+  if (a.n_units < 1) return cudaSuccess;
+  if (!a.kv.f16) return cudaErrorInvalidValue;
+  if (a.kv.hd == 128) return a.q16 ? launch_score<128, 0>(a, s) : launch_score<128, 1>(a, s);
+  return a.q16 ? launch_score<64, 0>(a, s) : launch_score<64, 1>(a, s);
+}
+
+}  // namespace rb

@@ -20,7 +20,7 @@ from typing import Optional, Sequence
 
 import numpy as np
 
-from . import F16, F32, PTR_DEVICE, PTR_HOST, _check, _lib, _sig
+from . import F16, F32, PTR_DEVICE, PTR_HOST, _check, _lib, _sig  # noqa: E402
 from .sampling import _prev_arrays
 
 _vp, _u32, _u64, _i32, _f = C.c_void_p, C.c_uint32, C.c_uint64, C.c_int32, C.c_float
@@ -80,55 +80,84 @@ def _rows3(a, n, heads, hd, name):
     else:
         shape, ptr = a.shape, a.ctypes.data
         stride = [s // a.itemsize for s in a.strides]
-    if len(shape) == 2:
-        ok = shape[0] == n and shape[1] == heads * hd and (stride[1] == 1)
+    if len(shape) == 3:
+        ok = shape[0] == n and shape[1] == heads and shape[2] == hd and stride[2] == 1 and \
+            (stride[1] == hd or heads == 1)
     else:
-        ok = len(shape) == 3 and shape[0] == n and shape[1] == heads and shape[2] == hd and stride[2] == 1 and \
-            (heads == 1 or stride[1] == hd)
-    if not ok or (n > 1 and stride[0] < heads * hd):
+        ok = len(shape) == 2 and shape[0] == n and shape[1] == heads * hd and stride[1] == 1
+    if n == 1:
+        ld = heads * hd
+    else:
+        ld = stride[0]
+        ok = ok and ld >= heads * hd
+    if not ok:
         raise ValueError(f"{name}: [{n}][{heads}][{hd}] with contiguous heads wanted, got {tuple(shape)} / {tuple(stride)}")
-    return ptr, stride[0] if n > 1 else heads * hd
+    return ptr, ld
 
 
 _DTYPES = {"torch.float32": F32, "torch.float16": F16, "float32": F32, "float16": F16}
+_SEEN = {}  # dtype objects met so far
 
 
 def _dtype(arrays, ctx):
-    """(dtype id, flags) of arrays that share a type and a memory space; tensors have to be on the context's device."""
-    first = arrays[0]
-    dev = _is_tensor(first)
+    """(dtype id, flags) of arrays that share a type and a memory space."""
+    dtype = arrays[0].dtype
     for a in arrays:
-        if a.dtype != first.dtype:
-            raise ValueError(f"mixed types {first.dtype} and {a.dtype}")
-    _space(arrays, ctx)
-    dt = _DTYPES.get(str(first.dtype))
+        if a.dtype != dtype:
+            raise ValueError(f"mixed types {dtype} and {a.dtype}")
+    dt = _SEEN.get(dtype)
     if dt is None:
-        raise ValueError(f"unsupported type {first.dtype}")
-    return dt, PTR_DEVICE | ASYNC if dev else PTR_HOST
+        dt = _DTYPES.get(str(dtype))
+        if dt is None:
+            raise ValueError(f"unsupported type {dtype}")
+        _SEEN[dtype] = dt
+    return dt, _space(arrays, ctx)
 
 
 def _space(arrays, ctx):
+    """Flags of arrays that are all host arrays, or all tensors on the context's device."""
     dev = _is_tensor(arrays[0])
     for a in arrays:
-        if a is not None and (_is_tensor(a) != dev or (dev and (not a.is_cuda or a.device.index != ctx.device))):
+        if a is not None and (_is_tensor(a) != dev or (dev and a.get_device() != ctx.device)):
             raise ValueError("host arrays, or tensors on the context's device, wanted: not a mix")
+    return PTR_DEVICE | ASYNC if dev else PTR_HOST
+
+
+_raw_stream = None
+
+
+def _current_stream(device: int) -> int:
+    """The cudaStream_t of torch's current stream."""
+    global _raw_stream
+    if _raw_stream is None:
+        import torch
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+            (lambda d: torch.cuda.current_stream(d).cuda_stream)
+    return _raw_stream(device)
 
 
 class _Order:
-    """Orders a device call on the context's stream after torch's current stream, and what comes after it there."""
+    """Orders a device call on a context's own stream after torch's current one, and what follows there after it."""
 
-    def __init__(self, ctx, flags):
-        self.ext = None
-        if flags & PTR_DEVICE:
-            import torch
-            self.cur = torch.cuda.current_stream(ctx.device)
-            if self.cur.cuda_stream != (ctx.stream or 0):
-                self.ext = torch.cuda.ExternalStream(ctx.stream, device=self.cur.device)
-                self.ext.wait_stream(self.cur)
+    def __init__(self, ctx):
+        import torch
+        self.cur = torch.cuda.current_stream(ctx.device)
+        self.ext = torch.cuda.ExternalStream(ctx.stream, device=self.cur.device)
+        self.ext.wait_stream(self.cur)
 
     def done(self):
-        if self.ext is not None:
-            self.cur.wait_stream(self.ext)
+        self.cur.wait_stream(self.ext)
+
+
+def _call(ctx, flags, fn, *args):
+    if not flags & PTR_DEVICE or _current_stream(ctx.device) == ctx._stream_id:
+        rc = fn(*args, flags)
+    else:
+        order = _Order(ctx)
+        rc = fn(*args, flags)
+        order.done()
+    if rc < 0:
+        _check(rc)
 
 
 class RowPlan:
@@ -147,6 +176,7 @@ class RowPlan:
         _check(_lib.rb_plan_create(self.ctx.handle, pool.handle, C.byref(d), C.byref(h)))
         self.handle = h.value
         self._append, self._attention = _AppendDesc(), _AttentionDesc()
+        self._append_ref, self._attention_ref = C.byref(self._append), C.byref(self._attention)
 
     def append(self, layer: int, k, v, q=None, q_out=None, q_norm=None, k_norm=None, eps: float = 1e-6, rope=None,
                adjacent: bool = False):
@@ -159,8 +189,9 @@ class RowPlan:
                 q_out = torch.empty((n, H, hd), dtype=q.dtype, device=q.device)
             else:
                 q_out = np.empty((n, H, hd), q.dtype)
-        dt, flags = _dtype([k, v] if q is None else [k, v, q, q_out], self.ctx)
-        _space([k, q_norm, k_norm, rope], self.ctx)
+        dt, flags = _dtype((k, v) if q is None else (k, v, q, q_out), self.ctx)
+        if q_norm is not None or k_norm is not None or rope is not None:
+            _space((k, q_norm, k_norm, rope), self.ctx)
         d = self._append
         d.dtype, d.rope_style, d.eps = dt, int(bool(adjacent)), eps
         d.k, d.ldk = _rows3(k, n, kv, hd, "k")
@@ -173,9 +204,7 @@ class RowPlan:
         else:
             d.rope_len, d.rotary = rope.shape
             d.rope = _vec(rope, "float32", d.rope_len * d.rotary, "rope")
-        order = _Order(self.ctx, flags)
-        _check(_lib.rb_plan_append(self.ctx.handle, self.handle, layer, C.byref(d), flags))
-        order.done()
+        _call(self.ctx, flags, _lib.rb_plan_append, self.ctx._h, self.handle, layer, self._append_ref)
         return q_out
 
     def attention(self, layer: int, q, scale: float, softcap: float = 0.0, slopes=None, out=None):
@@ -187,16 +216,15 @@ class RowPlan:
                 out = torch.empty((n, H, hd), dtype=q.dtype, device=q.device)
             else:
                 out = np.empty((n, H, hd), q.dtype)
-        dt, flags = _dtype([q, out], self.ctx)
-        _space([q, slopes], self.ctx)
+        dt, flags = _dtype((q, out), self.ctx)
+        if slopes is not None:
+            _space((q, slopes), self.ctx)
         d = self._attention
         d.dtype, d.scale, d.softcap = dt, scale, softcap
         d.q, d.ldq = _rows3(q, n, H, hd, "q")
         d.out, d.ldo = _rows3(out, n, H, hd, "out")
         d.slopes = _vec(slopes, "float32", H, "slopes")
-        order = _Order(self.ctx, flags)
-        _check(_lib.rb_plan_attention(self.ctx.handle, self.handle, layer, C.byref(d), flags))
-        order.done()
+        _call(self.ctx, flags, _lib.rb_plan_attention, self.ctx._h, self.handle, layer, self._attention_ref)
         return out
 
     def close(self):
@@ -277,15 +305,13 @@ def sample_filtered(ctx, logits, filters, uniforms, prev=None, out=None, probs=N
         out = torch.empty(n, dtype=torch.int32, device=logits.device)
     prev = prev or (None, None)
     _space([logits, filters, uniforms, out, probs, *prev], ctx)
-    order = _Order(ctx, flags)
-    _check(_lib.rb_sample_filtered(
-        ctx.handle, dt, logits.data_ptr(), logits.stride(0) if n > 1 else v, n, v,
+    _call(
+        ctx, flags, _lib.rb_sample_filtered, ctx._h, dt, logits.data_ptr(), logits.stride(0) if n > 1 else v, n, v,
         _vec(filters, "uint8", n * C.sizeof(_Filter), "filters"),
         None if prev[0] is None else _vec(prev[0], "int32", prev[0].numel(), "prev tokens"),
         None if prev[1] is None else _vec(prev[1], "int32", n + 1, "prev offsets"),
         _vec(uniforms, "float32", n, "uniforms"), _vec(out, "int32", n, "out"),
-        _vec(probs, "float32", n, "probs"), flags))
-    order.done()
+        _vec(probs, "float32", n, "probs"))
     return out
 
 
