@@ -282,8 +282,8 @@ struct RowPlanTenant {
 struct RowSet {
   int pool = -1, n_heads = 0, n_rows = 0, max_pos = 0;
   std::vector<RowPlanTenant> tenants;
-  int n_cta = 0, n_tile = 0, n_joins = 0;
-  DevBuf rows, small, cta, tile, joins, part_o, part_ml;
+  int n_cta = 0, n_tile = 0, n_joins = 0, n_small_joins = 0, max_nv = 0;
+  DevBuf rows, small, cta, tile, joins, counters, part_o, part_ml;
 };
 
 struct Ctx {
@@ -2299,11 +2299,14 @@ int32_t rb_plan_create(rb_ctx* c, int32_t pool, const rb_plan_desc* d, int32_t* 
   S->n_cta = (int)w.small_cta.size() ? (int)w.small_cta.size() - 1 : 0;
   S->n_tile = (int)w.tile.size();
   S->n_joins = (int)w.joins.size();
+  S->n_small_joins = w.n_small_joins;
+  S->max_nv = w.max_nv;
   if (int rc = upload_vec(c, S->rows, rows)) return rc;
   if (int rc = upload_vec(c, S->small, w.small)) return rc;
   if (int rc = upload_vec(c, S->cta, w.small_cta)) return rc;
   if (int rc = upload_vec(c, S->tile, w.tile)) return rc;
   if (int rc = upload_vec(c, S->joins, w.joins)) return rc;
+  if (int rc = upload_vec(c, S->counters, std::vector<int32_t>(w.n_small_joins, 0))) return rc;
   if (w.n_slots) {
     if (S->part_o.alloc((size_t)w.n_slots * P->hd * 4) != cudaSuccess ||
         S->part_ml.alloc((size_t)w.n_slots * 8) != cudaSuccess)
@@ -2443,12 +2446,15 @@ int32_t rb_plan_attention(rb_ctx* c, int32_t plan, uint32_t layer, const rb_atte
   a.units = S->small.as<AttnUnit>();
   a.cta = S->cta.as<int32_t>();
   a.n_cta = S->n_cta;
+  a.max_nv = S->max_nv;
+  a.joins = S->joins.as<JoinItem>();
+  a.n_joins = S->n_joins;
+  a.n_small_joins = S->n_small_joins;
+  a.counters = S->counters.as<int32_t>();
   RB_CUDA(rows_small_launch(a, c->stream));
   a.units = S->tile.as<AttnUnit>();
   a.n_units = S->n_tile;
   RB_CUDA(rows_tile_launch(a, c->stream));
-  a.joins = S->joins.as<JoinItem>();
-  a.n_joins = S->n_joins;
   RB_CUDA(rows_join_launch(a, c->stream));
   if (!(flags & RB_PTR_DEVICE))
     RB_CUDA(cudaMemcpy2DAsync(d->out, d->ldo * esz, a.out, d->ldo * esz, w * esz, n, cudaMemcpyDeviceToHost, c->stream));

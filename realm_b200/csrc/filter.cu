@@ -11,10 +11,20 @@
 // and the draw takes the first index whose running sum of kept W exceeds
 // floor(u sum W). t < 1e-7 takes the first rank.
 //
-// A cluster of CTAs holds one row in shared memory, each CTA a contiguous share
-// cut into one chunk per thread. Thresholds come from a radix walk over the bits
-// of w in three digits of ten bits, each one histogram (counts and sums) that the
-// cluster adds up through distributed shared memory.
+// A cluster of CTAs holds one row in registers: each CTA a contiguous share of its
+// 16-byte vectors, thread t the vectors t, t + 1024, ... of the share. Thresholds come
+// from a radix walk over the bits of w: first its binade (W has 40 bits, so 41 of
+// them), then the 23 bits of its mantissa in digits of 8, 8 and 7, until a bin is kept
+// whole; each step is a histogram of counts and sums that the cluster adds up through
+// distributed shared memory. Within a binade W is v << s with a v of 24 bits, so a sum
+// is that of v's low 10 and high 14 bits, in 32-bit words: 64-bit shared-memory atomics
+// are loops. The binades of a row are few, so their histogram has a copy per lane (no
+// two lanes of a warp meet); mantissas are spread, and there only the elements of the
+// chosen binade count.
+//
+// Bound by instructions (about 50 an element) and, for few rows, by the chain of
+// barriers: 96 rows of 151937 took 315 us with the rows in shared memory and 64-bit
+// atomics, 208 us with the 32-bit histograms.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -27,28 +37,37 @@ namespace rb {
 namespace {
 
 constexpr int kFT = 1024, kFW = kFT / 32;
-constexpr int kBins = 1024;       // ten bits of w a pass: w <= 1 has 30 significant bits
+constexpr int kBinades = 48;      // 41 in use: binade b holds exponents 127 - b
+constexpr int kBins = 256;
 constexpr int kMaxCluster = 8;
-constexpr double kFix = 1099511627776.0;  // 2^40
+constexpr int kMaxElems = 40;     // of a thread: one vector more than 262144 / 8 / 1024, for rows off 16 bytes
 using u64 = unsigned long long;
 
 struct FilterShared {
-  uint32_t cnt[2][kBins];
-  u64 sum[2][kBins];
+  uint32_t ba[kBinades * 32], bb[kBinades * 32];  // per lane: count << 21 | sum of low parts; sum of high parts
+  uint32_t cnt[2][kBins], lo[2][kBins], hi[2][kBins];
   u64 xch[2][kMaxCluster];  // one value of every CTA of the cluster
-  u64 red[kFW];
-  uint32_t redc[kFW];
-  u64 out_a, out_b;
-  uint32_t out_bin, out_cnt;
+  u64 red[kFW], red2[kFW];
+  u64 part[kMaxElems / 4][kFW];  // kept weight by vector round and warp
+  u64 above_c, above_s, in_s, base;
+  uint32_t bin, in_bin, round, warp;
 };
+// one lane's copy takes at most kMaxElems elements of each warp: 11 bits of count, 21 of low parts
+static_assert(kFW * kMaxElems < 2048 && kFilterMaxVocab + 8 <= kMaxCluster * kFT * kMaxElems, "");
 
-__device__ __forceinline__ u64 fix(float w) { return (u64)((double)w * kFix); }
-
-__device__ __forceinline__ u64 warp_sum(u64 v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+// W and its parts: W = v << s
+__device__ __forceinline__ uint32_t part_of(float w, int& binade) {
+  const uint32_t b = __float_as_uint(w), m = (b & 0x7fffffu) | 0x800000u;
+  binade = 127 - (int)(b >> 23);
+  return binade > 40 ? 0u : binade > 17 ? m >> (binade - 17) : m;
 }
+__device__ __forceinline__ int shift_of(int binade) { return binade > 17 ? 0 : 17 - binade; }
+__device__ __forceinline__ u64 fix(float w) {
+  int b;
+  const uint32_t v = part_of(w, b);
+  return (u64)v << shift_of(b);
+}
+
 __device__ __forceinline__ u64 warp_max(u64 v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -57,191 +76,249 @@ __device__ __forceinline__ u64 warp_max(u64 v) {
   }
   return v;
 }
-
-template <bool MAX>
-__device__ u64 block_reduce(u64 v, FilterShared& s) {
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  v = MAX ? warp_max(v) : warp_sum(v);
-  __syncthreads();
-  if (lane == 0) s.red[w] = v;
-  __syncthreads();
-  v = s.red[lane];
-  return MAX ? warp_max(v) : warp_sum(v);
+__device__ __forceinline__ u64 warp_scan(u64 v) {  // inclusive
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += y;
+  }
+  return v;
 }
 
 // exclusive prefix in thread order, and the block's total
-__device__ u64 block_scan(u64 v, FilterShared& s, u64& total) {
+__device__ u64 block_scan(u64 v, u64* red, u64& total) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  u64 x = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const u64 y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
+  const u64 x = warp_scan(v);
   __syncthreads();
-  if (lane == 31) s.red[w] = x;
+  if (lane == 31) red[w] = x;
   __syncthreads();
-  const u64 t = s.red[lane];
-  u64 incl = t;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const u64 y = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += y;
-  }
+  const u64 t = red[lane], incl = warp_scan(t);
   total = __shfl_sync(0xffffffffu, incl, 31);
   return __shfl_sync(0xffffffffu, incl - t, w) + x - v;
 }
+// sum over the warp of values below 2^43
+__device__ __forceinline__ u64 warp_sum43(u64 v) {
+  const uint32_t lo = __reduce_add_sync(0xffffffffu, (uint32_t)v & 0x3fffffu),
+                 hi = __reduce_add_sync(0xffffffffu, (uint32_t)(v >> 22));
+  return ((u64)hi << 22) + lo;
+}
 
-// Every CTA's value to every CTA; slot alternates, so that one barrier a call does.
+// Buffers alternate with `turn`, which every barrier of the cluster raises: one
+// barrier per exchange does.
+template <int N>
 struct Cluster {
   cg::cluster_group g;
   FilterShared& s;
-  int n, rank, turn = 0;
-  __device__ Cluster(FilterShared& sh) : g(cg::this_cluster()), s(sh), n(g.num_blocks()), rank(g.block_rank()) {}
+  int rank, turn = 0;
+  __device__ Cluster(FilterShared& sh) : g(cg::this_cluster()), s(sh), rank(N > 1 ? (int)g.block_rank() : 0) {}
+  __device__ void sync() {
+    if (N > 1) g.sync();
+    else __syncthreads();
+    ++turn;
+  }
+  // every CTA's value (the same in all its threads) to every CTA
   __device__ const u64* share(u64 v) {
     u64* mine = s.xch[turn & 1];
-    if ((int)threadIdx.x < n) g.map_shared_rank(mine, threadIdx.x)[rank] = v;
-    ++turn;
-    g.sync();
+    if (threadIdx.x < N) *g.map_shared_rank(&mine[rank], threadIdx.x) = v;
+    sync();
     return mine;
   }
+  // the sum of everybody's copies of a histogram word
+  __device__ u64 gather(const uint32_t* p) {
+    if (N == 1) return *p;
+    uint32_t x[N];
+#pragma unroll
+    for (int r = 0; r < N; ++r) x[r] = *g.map_shared_rank(p, r);
+    u64 t = 0;
+#pragma unroll
+    for (int r = 0; r < N; ++r) t += x[r];
+    return t;
+  }
 };
 
-__host__ __device__ inline int share_len(int V, int n) { return (V + n - 1) / n; }
-__host__ __device__ inline int chunk_len(int S) { return (S + kFT - 1) / kFT; }
-// an odd stride between the threads' chunks: a warp that walks its chunks in step meets 32 banks
-__host__ __device__ inline int chunk_stride(int C) { return C | 1; }
-
-// The walk over the digits. Among elements with bits <= cap (cap_eq of those equal
-// to it, by index; only their number matters here) finds the largest threshold T
-//   by count: so that `want` elements rank at or before T's last kept tie,
-//   by sum:   so that the sum ranked before a kept element is below `want`.
-// Returns T, the ties to keep, and the count and sum strictly above T.
+// What is kept: weights with more than `bits`, and the first `ties` of those with
+// just these bits, of which there are `equal`.
 struct Cut {
-  uint32_t bits, ties;
-  u64 above;  // sum of W above bits
+  uint32_t bits, ties, equal;
 };
 
+// One step's choice: thread t < n holds the count c and sum w of a bin, the bins in
+// falling order of weight. The last bin that holds an element ranked before `want`
+// (by count, or by the sum before it) is taken; acc_*: what lies above its range.
 template <bool COUNT>
-__device__ Cut radix_cut(const float* sc, int n, const Cut& top, u64 want, Cluster& cl) {
+__device__ void choose(uint32_t c, u64 w, int n, u64 want, u64& acc_c, u64& acc_s, FilterShared& s) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = n >> 5;
+  u64 ic = 0, is = 0;
+  if (warp < nw) {
+    ic = warp_scan(c);
+    is = warp_scan(w);
+    if (lane == 31) {
+      s.red[warp] = ic;
+      s.red2[warp] = is;
+    }
+  }
+  __syncthreads();
+  if (warp < nw) {
+    u64 bc = acc_c, bs = acc_s;
+    for (int q = 0; q < warp; ++q) {
+      bc += s.red[q];
+      bs += s.red2[q];
+    }
+    const u64 ac = bc + ic - c, as = bs + is - w;
+    const bool has = c > 0 && (COUNT ? ac < want : as < want);
+    const unsigned any = __ballot_sync(0xffffffffu, has);
+    const u64 ec = bc + __shfl_sync(0xffffffffu, ic, 31), es = bs + __shfl_sync(0xffffffffu, is, 31);
+    bool last = any != 0;
+    if (last && (COUNT ? ec < want : es < want)) {  // a later warp with a bin of its own has the say
+      u64 rest = 0;
+      for (int q = warp + 1; q < nw; ++q) rest += s.red[q];
+      last = rest == 0;
+    }
+    if (last && lane == 31 - __clz(any)) {
+      s.bin = tid;
+      s.in_bin = c;
+      s.in_s = w;
+      s.above_c = ac;
+      s.above_s = as;
+    }
+  }
+  __syncthreads();
+  acc_c = s.above_c;
+  acc_s = s.above_s;
+}
+
+// The cut of one rule. bc, bw: this thread's binade (thread t < kBinades holds binade
+// t). total: the sum of what it keeps.
+template <bool COUNT, int NEL, int N>
+__device__ Cut radix_cut(const float (&x)[NEL], uint32_t bc, u64 bw, u64 want, Cluster<N>& cl, u64& total) {
   FilterShared& s = cl.s;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  uint32_t pre = 0;
-  u64 acc_s = 0, acc_c = 0;
-  for (int pass = 2; pass >= 0; --pass) {
+  const int tid = threadIdx.x;
+  u64 acc_c = 0, acc_s = 0;
+  choose<COUNT>(bc, bw, 64, want, acc_c, acc_s, s);
+  const int binade = (int)s.bin, shift = shift_of(binade);
+  uint32_t pre = (uint32_t)(127 - binade) << 23;
+  int sh = 23;
+  // a bin with one element, or (by count) without one too many, is kept whole
+  auto whole = [&]() { return s.in_bin == 1 || (COUNT && acc_c + s.in_bin <= want); };
+  while (sh > 0 && !whole()) {
+    const int width = sh == 7 ? 7 : 8;
+    const uint32_t hmask = 0xffffffffu << sh;
+    sh -= width;
     const int turn = cl.turn & 1;
-    s.cnt[turn][tid] = 0;
-    s.sum[turn][tid] = 0;
+    uint32_t *cnt = s.cnt[turn], *lo = s.lo[turn], *hi = s.hi[turn];
+    if (tid < kBins) cnt[tid] = lo[tid] = hi[tid] = 0;
     __syncthreads();
-    const int sh = 10 * pass;
-    const uint32_t hmask = pass == 2 ? 0u : 0xffffffffu << (sh + 10);
-    for (int i = 0; i < n; ++i) {
-      const uint32_t b = __float_as_uint(sc[i]);
-      if (b && (b & hmask) == pre) {
-        atomicAdd(&s.cnt[turn][(b >> sh) & 1023u], 1u);
-        atomicAdd(&s.sum[turn][(b >> sh) & 1023u], fix(sc[i]));
+#pragma unroll
+    for (int i = 0; i < NEL; ++i) {
+      const uint32_t b = __float_as_uint(x[i]);
+      if ((b & hmask) == pre) {
+        int e;
+        const uint32_t v = part_of(x[i], e), bin = (b >> sh) & ((1u << width) - 1);
+        atomicAdd(&cnt[bin], 1u);
+        atomicAdd(&lo[bin], v & 1023u);
+        atomicAdd(&hi[bin], v >> 10);
       }
     }
-    cl.g.sync();
+    cl.sync();
+    // thread t owns bin 2^width - 1 - t
     uint32_t c = 0;
     u64 w = 0;
-    // thread t owns bin 1023 - t: prefixes in thread order run from the largest weight down
-    const int bin = kBins - 1 - tid;
-    for (int r = 0; r < cl.n; ++r) {
-      c += cl.g.map_shared_rank(&s.cnt[turn][0], r)[bin];
-      w += cl.g.map_shared_rank(&s.sum[turn][0], r)[bin];
+    const int bin = (1 << width) - 1 - tid;
+    if (bin >= 0) {
+      c = (uint32_t)cl.gather(&cnt[bin]);
+      w = cl.gather(&lo[bin]) + (cl.gather(&hi[bin]) << 10);
     }
-    u64 tot_s, tot_c;
-    const u64 above_c = block_scan(c, s, tot_c) + acc_c;
-    const u64 above_s = block_scan(w, s, tot_s) + acc_s;
-    // the last bin, going down, that still holds a kept element
-    const bool has = c > 0 && (COUNT ? above_c < want : above_s < want);
-    const unsigned any = __ballot_sync(0xffffffffu, has);
-    __syncthreads();
-    if (lane == 0) s.redc[warp] = any;
-    __syncthreads();
-    int pick = 0;
-    for (int q = 0; q < kFW; ++q)
-      if (s.redc[q]) pick = q * 32 + 31 - __clz(s.redc[q]);
-    if (tid == pick) {
-      s.out_bin = (uint32_t)bin;
-      s.out_a = above_c;
-      s.out_b = above_s;
-      s.out_cnt = c;
-    }
-    __syncthreads();
-    pre |= s.out_bin << sh;
-    acc_c = s.out_a;
-    acc_s = s.out_b;
-    ++cl.turn;
+    choose<COUNT>(c, w << shift, 1 << width, want, acc_c, acc_s, s);
+    pre |= ((1u << width) - 1 - s.bin) << sh;
   }
-  Cut r;
-  r.bits = pre;
-  r.above = acc_s;
-  const uint32_t eq = s.out_cnt;
-  if (COUNT) {
-    const u64 left = want > acc_c ? want - acc_c : 0;
-    r.ties = left < eq ? (uint32_t)left : eq;
-  } else {
-    const u64 tq = fix(__uint_as_float(pre));
-    u64 ties = eq;
-    if (tq) {
-      const u64 k = want > acc_s ? (want - acc_s + tq - 1) / tq : 0;  // j-th tie kept while above + j tq < want
-      ties = k < eq ? k : eq;
-    }
-    r.ties = (uint32_t)ties;
+  if (whole()) {
+    total = acc_s + s.in_s;
+    return Cut{pre, 0xffffffffu, 0xffffffffu};
   }
-  if (r.bits == top.bits && r.ties > top.ties) r.ties = top.ties;
+  const u64 tq = fix(__uint_as_float(pre));
+  // by sum: the j-th tie is kept while above + j tq < want
+  const u64 ties = COUNT ? want - acc_c : (want - acc_s + tq - 1) / tq;
+  Cut r{pre, ties < s.in_bin ? (uint32_t)ties : s.in_bin, s.in_bin};
+  total = acc_s + r.ties * tq;
   return r;
 }
 
-template <class T>
+template <class T, int NV, int N>
 __global__ void __launch_bounds__(kFT) filter_kernel(const __grid_constant__ FilterArgs a) {
-  extern __shared__ float sv[];
+  constexpr int E = 16 / sizeof(T), NEL = NV * E;
   __shared__ FilterShared s;
-  Cluster cl(s);
-  const int tid = threadIdx.x;
-  cl.g.sync();  // every CTA of the cluster runs before its shared memory is written
-  const int row = blockIdx.x / cl.n;
+  Cluster<N> cl(s);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (N > 1) cg::this_cluster().barrier_arrive();
+  const int row = blockIdx.x / N;
   rb_sampling_filter p = a.params[row];
   p.min_p = fminf(p.min_p, 1.f);  // the first rank always stays
-  const int V = a.vocab, S = share_len(V, cl.n), C = chunk_len(S), CS = chunk_stride(C);
-  const int base = cl.rank * S, len = max(0, min(S, V - base));
-  const T* lg = reinterpret_cast<const T*>(a.logits) + (size_t)row * a.ld + base;
-  for (int i = tid; i < len; i += kFT) {
-    float x;
-    if constexpr (sizeof(T) == 2) x = __half2float(lg[i]);
-    else x = lg[i];
-    sv[(i / C) * CS + i % C] = x != x ? -INFINITY : x;
+  const int V = a.vocab;
+  const T* lg = reinterpret_cast<const T*>(a.logits) + (size_t)row * a.ld;
+  // the row's 16-byte vectors, the first one up to E - 1 elements before the row
+  const int mis = (int)((reinterpret_cast<uintptr_t>(lg) & 15) / sizeof(T));
+  const int vecs = (V + mis + E - 1) / E, share = (vecs + N - 1) / N;
+  const int v0 = cl.rank * share, v1 = min(vecs, v0 + share);
+  auto index = [&](int r) { return (v0 + r * kFT + tid) * E - mis; };  // of vector round r's first element
+  float x[NEL];
+#pragma unroll
+  for (int r = 0; r < NV; ++r) {
+    const int i = index(r);
+    const bool in = v0 + r * kFT + tid < v1;
+    if (in && i >= 0 && i + E <= V) {
+      const uint4 q = __ldcs(reinterpret_cast<const uint4*>(lg + i));
+      const T* y = reinterpret_cast<const T*>(&q);
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[r * E + e] = (float)y[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[r * E + e] = in && i + e >= 0 && i + e < V ? (float)lg[i + e] : -INFINITY;
+    }
   }
-  __syncthreads();
+  for (int i = tid; i < kBinades * 32; i += kFT) s.ba[i] = s.bb[i] = 0;
+  const float t = p.temperature;
+  const bool greedy = !(t >= 1e-7f);
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < NEL; ++i)
+    if (x[i] != x[i]) x[i] = -INFINITY;
   if (a.prev_off && p.repetition_penalty != 1.0f) {
     // one thread applies all occurrences of a token, in order
     const uint32_t j1 = a.prev_off[row + 1];
     for (uint32_t j = a.prev_off[row]; j < j1; ++j) {
-      const long long t = (long long)a.prev[j] - base;
-      if (t >= 0 && t < len && (int)(t % kFT) == tid) {
-        float& x = sv[(t / C) * CS + t % C];
-        x = x > 0.f ? __fdiv_rn(x, p.repetition_penalty) : __fmul_rn(x, p.repetition_penalty);
+      const uint32_t tok = a.prev[j];
+      const int at = tok < (uint32_t)V ? (int)tok + mis : -1, local = at / E - v0;
+      if (at >= 0 && local >= 0 && at / E < v1 && local % kFT == tid) {
+        const int k = local / kFT * E + at % E;
+#pragma unroll
+        for (int i = 0; i < NEL; ++i)
+          if (i == k) x[i] = x[i] > 0.f ? __fdiv_rn(x[i], p.repetition_penalty) : __fmul_rn(x[i], p.repetition_penalty);
       }
     }
-    __syncthreads();
   }
-  const int i0 = min(tid * C, len), n = min(C, len - i0);
-  float* sc = sv + tid * CS;
-  const float t = p.temperature;
-  const bool greedy = !(t >= 1e-7f);
-  u64 best = 0;  // order key of the value, then the lowest index
-  for (int i = 0; i < n; ++i) {
-    const float x = greedy ? sc[i] : __fdiv_rn(sc[i], t);
-    sc[i] = x;
-    const u64 k = ((u64)float_order_key(x) << 32) | (0xffffffffu - (uint32_t)(base + i0 + i));
-    best = k > best ? k : best;
+  if (!greedy && t != 1.f)
+#pragma unroll
+    for (int i = 0; i < NEL; ++i) x[i] = __fdiv_rn(x[i], t);
+#pragma unroll
+  for (int i = 0; i < NEL; ++i) top = fmaxf(top, x[i]);
+  u64 best = (u64)float_order_key(top) << 32;
+  if (greedy) {  // and the lowest index that has it
+    uint32_t at = 0xffffffffu;
+#pragma unroll
+    for (int i = NEL - 1; i >= 0; --i)
+      if (x[i] == top && top != -INFINITY) at = (uint32_t)(index(i / E) + i % E);
+    best |= 0xffffffffu - at;
   }
-  best = block_reduce<true>(best, s);
-  {
+  best = warp_max(best);
+  if (lane == 0) s.red[warp] = best;
+  __syncthreads();
+  best = warp_max(s.red[lane]);
+  if (N > 1) {
+    cg::this_cluster().barrier_wait();  // every CTA of the cluster runs before its shared memory is written
     const u64* all = cl.share(best);
-    for (int r = 0; r < cl.n; ++r) best = all[r] > best ? all[r] : best;
+#pragma unroll
+    for (int r = 0; r < N; ++r) best = all[r] > best ? all[r] : best;
   }
   const uint32_t mk = (uint32_t)(best >> 32);
   const float m = __uint_as_float((mk & 0x80000000u) ? mk & 0x7fffffffu : ~mk);
@@ -251,104 +328,194 @@ __global__ void __launch_bounds__(kFT) filter_kernel(const __grid_constant__ Fil
       a.tokens[row] = none ? 0xffffffffu : 0xffffffffu - (uint32_t)best;
       if (a.probs) a.probs[row] = none ? 0.f : 1.f;
     }
-    cl.g.sync();
     return;
   }
-  u64 mass = 0;
-  for (int i = 0; i < n; ++i) {
-    float w = sc[i] == m ? 1.f : expf(sc[i] - m);
-    if (!(w >= p.min_p)) w = 0.f;
-    sc[i] = w;
-    mass += fix(w);
-  }
-  mass = block_reduce<false>(mass, s);
-  u64 total = 0;
-  {
-    const u64* all = cl.share(mass);
-    for (int r = 0; r < cl.n; ++r) total += all[r];
-  }
-  Cut cut{0u, 0xffffffffu, 0};  // keeps everything
-  if (p.top_k > 0 && p.top_k < (uint32_t)V) {
-    cut = radix_cut<true>(sc, n, cut, p.top_k, cl);
-    total = cut.above + (u64)cut.ties * fix(__uint_as_float(cut.bits));
-  }
-  if (p.top_p > 0.f && p.top_p < 1.f) {
-    u64 want = (u64)((double)total * (double)p.top_p);
-    if (want < 1) want = 1;
-    Cut c = radix_cut<false>(sc, n, cut, want, cl);
-    if (c.bits >= cut.bits) cut = c;
-    total = cut.above + (u64)cut.ties * fix(__uint_as_float(cut.bits));
-  }
-  // kept weights: bits above the cut, and its ties with the lowest indices
-  u64 eq = 0;
-  for (int i = 0; i < n; ++i) eq += __float_as_uint(sc[i]) == cut.bits;
-  u64 cta_eq;
-  u64 tie = block_scan(eq, s, cta_eq);
-  {
-    const u64* all = cl.share(cta_eq);
-    for (int r = 0; r < cl.rank; ++r) tie += all[r];
-  }
-  u64 mine = 0;
-  {
-    u64 k = tie;
-    for (int i = 0; i < n; ++i) {
-      const uint32_t b = __float_as_uint(sc[i]);
-      if (b < cut.bits || (b == cut.bits && k++ >= cut.ties)) sc[i] = 0.f;
-      else mine += fix(sc[i]);
+  const bool use_k = p.top_k > 0 && p.top_k < (uint32_t)V, use_p = p.top_p > 0.f && p.top_p < 1.f;
+  const bool hist = use_k || use_p;
+#pragma unroll
+  for (int i = 0; i < NEL; ++i) {
+    float w = x[i] == m ? 1.f : expf(x[i] - m);
+    int b;
+    const uint32_t v = part_of(w, b);
+    const bool in = w >= p.min_p && v != 0;  // v 0: below the fixed point, never drawn
+    x[i] = in ? w : 0.f;
+    if (hist && in) {
+      atomicAdd(&s.ba[b * 32 + lane], 1u << 21 | (v & 1023u));
+      atomicAdd(&s.bb[b * 32 + lane], v >> 10);
     }
   }
-  u64 cta_mass;
-  u64 run = block_scan(mine, s, cta_mass);
-  {
-    const u64* all = cl.share(cta_mass);
+  if (hist) {
+    Cut cut{0u, 0xffffffffu, 0xffffffffu};
+    // the row's binades: sums over the lanes' copies, then over the cluster
+    const int turn = cl.turn & 1;
+    __syncthreads();
+    for (int b = warp; b < kBinades; b += kFW) {
+      const uint32_t y = s.ba[b * 32 + lane], z = s.bb[b * 32 + lane];
+      const uint32_t c = __reduce_add_sync(0xffffffffu, y >> 21), l = __reduce_add_sync(0xffffffffu, y & 0x1fffffu),
+                     h = __reduce_add_sync(0xffffffffu, z);
+      if (lane == 0) {
+        s.cnt[turn][b] = c;
+        s.lo[turn][b] = l;
+        s.hi[turn][b] = h;
+      }
+    }
+    cl.sync();
+    uint32_t bc = 0;
+    u64 bw = 0;
+    if (tid < kBinades) {
+      bc = (uint32_t)cl.gather(&s.cnt[turn][tid]);
+      bw = (cl.gather(&s.lo[turn][tid]) + (cl.gather(&s.hi[turn][tid]) << 10)) << shift_of(tid);
+    }
+    u64 total = 0;
+    if (use_k) {
+      cut = radix_cut<true, NEL, N>(x, bc, bw, p.top_k, cl, total);
+    } else {
+      if (tid < 64) {  // two warps hold the binades
+        const u64 y = warp_scan(bw);
+        if (lane == 31) s.red[warp] = y;
+      }
+      __syncthreads();
+      total = s.red[0] + s.red[1];
+      __syncthreads();
+    }
+    if (use_p) {
+      u64 want = (u64)((double)total * (double)p.top_p);
+      if (want < 1) want = 1;
+      const Cut c = radix_cut<false, NEL, N>(x, bc, bw, want, cl, total);
+      // never below the first cut; at the same weight, the fewer ties
+      if (c.bits > cut.bits || (c.bits == cut.bits && c.ties < cut.ties)) cut = c;
+    }
+    // kept: bits above the cut, and its ties with the lowest indices
+#pragma unroll
+    for (int i = 0; i < NEL; ++i)
+      if (__float_as_uint(x[i]) < cut.bits) x[i] = 0.f;
+    if (cut.ties < cut.equal) {  // the same in every thread of the cluster
+      u64 mine = 0, cta;
+#pragma unroll
+      for (int i = 0; i < NEL; ++i) mine += __float_as_uint(x[i]) == cut.bits;
+      block_scan(mine, s.red, cta);
+      u64 before = 0;
+      if (N > 1) {
+        const u64* all = cl.share(cta);
+        for (int r = 0; r < cl.rank; ++r) before += all[r];
+      }
+#pragma unroll
+      for (int r = 0; r < NV; ++r) {
+        u64 eq = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) eq += __float_as_uint(x[r * E + e]) == cut.bits;
+        u64 round;
+        u64 rank = before + block_scan(eq, s.red, round);
+        before += round;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (__float_as_uint(x[r * E + e]) == cut.bits && rank++ >= cut.ties) x[r * E + e] = 0.f;
+      }
+    }
+  }
+  // the draw: rounds of vectors, then warps, then lanes are in the order of the indices
+#pragma unroll
+  for (int r = 0; r < NV; ++r) {
+    u64 w = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (x[r * E + e] != 0.f) w += fix(x[r * E + e]);
+    w = warp_sum43(w);
+    if (lane == 0) s.part[r][warp] = w;
+  }
+  __syncthreads();
+  u64 mass = 0;
+#pragma unroll
+  for (int r = 0; r < NV; ++r) mass += s.part[r][lane];
+  u64 total = __shfl_sync(0xffffffffu, warp_scan(mass), 31), run = 0;
+  mass = total;
+  if (N > 1) {
+    const u64* all = cl.share(total);
     total = 0;
-    for (int r = 0; r < cl.n; ++r) {
+#pragma unroll
+    for (int r = 0; r < N; ++r) {
       if (r < cl.rank) run += all[r];
       total += all[r];
     }
   }
   const u64 target = (u64)((double)a.uniforms[row] * (double)total);
-  // exactly one thread's kept weights reach past the target (target < total)
-  if (run <= target && target < run + mine) {
-    for (int i = 0; i < n; ++i) {
-      const u64 w = fix(sc[i]);
-      if (run + w > target) {
-        a.tokens[row] = (uint32_t)(base + i0 + i);
-        if (a.probs) a.probs[row] = (float)((double)w / (double)total);
-        break;
+  if (target < run || target >= run + mass) return;  // the whole CTA
+  // exactly one CTA's, warp's and lane's kept weights reach past the target (target < total)
+  if (warp == 0) {
+    u64 at = run;
+#pragma unroll 1
+    for (int r = 0; r < NV; ++r) {
+      const u64 w = s.part[r][lane], incl = at + warp_scan(w);
+      if (incl - w <= target && target < incl) {
+        s.round = r;
+        s.warp = lane;
+        s.base = incl - w;
       }
-      run += w;
+      at = __shfl_sync(0xffffffffu, incl, 31);
     }
   }
-  cl.g.sync();  // no CTA leaves while another reads its shared memory
+  __syncthreads();
+  if (warp != (int)s.warp) return;
+  const int round = (int)s.round;
+  u64 w = 0;
+#pragma unroll
+  for (int i = 0; i < NEL; ++i)
+    if (i / E == round) w += fix(x[i]);
+  u64 at = s.base + warp_scan(w) - w;
+  if (at <= target && target < at + w) {
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < NEL; ++i)
+      if (i / E == round && !found) {
+        const u64 f = fix(x[i]);
+        if (at + f > target) {
+          a.tokens[row] = (uint32_t)(index(i / E) + i % E);
+          if (a.probs) a.probs[row] = (float)((double)f / (double)total);
+          found = true;
+        }
+        at += f;
+      }
+  }
 }
 
-template <class T>
-cudaError_t launch_t(const FilterArgs& a, int n, cudaStream_t s) {
-  const size_t smem = (size_t)kFT * chunk_stride(chunk_len(share_len(a.vocab, n))) * 4;
-  int dev = 0;
-  cudaGetDevice(&dev);
-  const int most = kFT * chunk_stride(chunk_len(share_len(kFilterMaxVocab, kMaxCluster))) * 4;
-  if (cudaError_t e = ensure_smem_attr(filter_kernel<T>, most, dev)) return e;
+template <class T, int NV, int N>
+cudaError_t launch(const FilterArgs& a, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.n_rows * n));
+  cfg.gridDim = dim3((unsigned)(a.n_rows * N));
   cfg.blockDim = dim3(kFT);
-  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute at;
   at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim.x = n;
+  at.val.clusterDim.x = N;
   at.val.clusterDim.y = at.val.clusterDim.z = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, filter_kernel<T>, a);
+  return cudaLaunchKernelEx(&cfg, filter_kernel<T, NV, N>, a);
+}
+
+template <class T>
+cudaError_t launch_type(const FilterArgs& a, cudaStream_t s) {
+  constexpr int E = 16 / sizeof(T);
+  // vectors of a row, wherever it starts, and of a thread in a cluster of n
+  const int vecs = (a.vocab + E - 1 + E - 1) / E;
+  auto rounds = [&](int n) { return ((vecs + n - 1) / n + kFT - 1) / kFT; };
+  const int r8 = rounds(8);
+  if (r8 <= 1) return launch<T, 1, 8>(a, s);
+  if (r8 <= 2) return launch<T, 2, 8>(a, s);
+  if (r8 <= 3) return launch<T, 3, 8>(a, s);
+  if constexpr (E == 4) {
+    if (r8 <= 5) return launch<T, 5, 8>(a, s);
+    return launch<T, 9, 8>(a, s);
+  } else {
+    return r8 <= 4 ? launch<T, 4, 8>(a, s) : launch<T, 5, 8>(a, s);
+  }
 }
 
 }  // namespace
 
 cudaError_t filter_launch(const FilterArgs& a, int num_sms, cudaStream_t s) {
   (void)num_sms;
-  return a.x16 ? launch_t<__half>(a, kMaxCluster, s) : launch_t<float>(a, kMaxCluster, s);
+  return a.x16 ? launch_type<__half>(a, s) : launch_type<float>(a, s);
 }
 
 }  // namespace rb

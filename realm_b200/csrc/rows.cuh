@@ -26,7 +26,7 @@ struct RowInfo {
 // whole item and writes the output; else its vectors' partial results go to
 // slot .. slot + nv.
 struct AttnUnit {
-  int32_t row0, v0, nv, kvh, tenant, k0, k1, slot;
+  int32_t row0, v0, nv, kvh, tenant, k0, k1, slot, join;  // join: its entry of the item list, or -1
 };
 
 // An item cut into n_parts units: part p of vector i lies at slot0 + p * nv + i.
@@ -39,9 +39,10 @@ struct JoinItem {
 struct RowWork {
   std::vector<AttnUnit> small, tile;
   std::vector<int32_t> small_cta;
-  std::vector<JoinItem> joins;
+  std::vector<JoinItem> joins;       // the small kernels' items first: their last CTA joins them
+  int32_t n_small_joins = 0;
   int32_t n_slots = 0;      // partial result vectors
-  int32_t max_join_parts = 0;
+  int32_t max_nv = 0;       // vectors of the largest small item
 };
 
 // rows: the plan's rows in call order; use_tile: whether long runs go to the tile
@@ -68,9 +69,10 @@ struct RowAttnArgs {
   const RowInfo* rows = nullptr;
   const AttnUnit* units = nullptr;
   const int32_t* cta = nullptr;  // small kernels
-  int32_t n_cta = 0, n_units = 0;
+  int32_t n_cta = 0, n_units = 0, max_nv = 0;  // max_nv: vectors of the largest small item
   const JoinItem* joins = nullptr;
-  int32_t n_joins = 0;
+  int32_t n_small_joins = 0, n_joins = 0;
+  int32_t* counters = nullptr;  // [n_small_joins], zero between launches
   float* part_o = nullptr;   // [n_slots][hd]
   float2* part_ml = nullptr; // [n_slots] (maximum in base-2 units, sum)
   uint32_t* err = nullptr;
@@ -95,6 +97,7 @@ cudaError_t rows_append_launch(const RowAppendArgs& a, int num_sms, cudaStream_t
 cudaError_t rows_small_launch(const RowAttnArgs& a, cudaStream_t s);
 // the tile kernel over a.units (one CTA each)
 cudaError_t rows_tile_launch(const RowAttnArgs& a, cudaStream_t s);
+// joins the tile kernel's items
 cudaError_t rows_join_launch(const RowAttnArgs& a, cudaStream_t s);
 
 }  // namespace rb

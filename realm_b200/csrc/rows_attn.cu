@@ -26,18 +26,138 @@ struct VecInfo {
   float slope;
 };
 
-// Scalar kernel: any cache type; K and V read straight from the pages.
-template <int HD, class T>
-__global__ void __launch_bounds__(kRowWarps * 32) rows_scalar_kernel(const __grid_constant__ RowAttnArgs a) {
-  constexpr int NV = kSmallVecs, DPL = HD / 32;
+// The last CTA that deposits a part of unit u's item joins all of them, in the order
+// of the keys whichever CTA that is, so the result depends on no order of arrival.
+// Every thread's parts are stored before. Ends with a barrier of the CTA.
+template <int HD, class TO>
+__device__ void join_last(const RowAttnArgs& a, const AttnUnit& u) {
+  __shared__ int last;
+  const JoinItem it = a.joins[u.join];
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    last = atom_add_acq_rel(&a.counters[u.join], 1) == it.n_parts - 1;
+    if (last) a.counters[u.join] = 0;
+  }
+  __syncthreads();
+  if (last) {
+    // a thread has four elements of one vector; the parts' loads do not wait for one another
+    for (int i = threadIdx.x; i < it.nv * (HD / 4); i += blockDim.x) {
+      const int v = i / (HD / 4), d = i % (HD / 4) * 4;
+      const float2* pml = a.part_ml + it.slot0 + v;
+      const float4* po = reinterpret_cast<const float4*>(a.part_o + (size_t)(it.slot0 + v) * HD + d);
+      float M = -INFINITY, L = 0.f;
+      float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int p0 = 0; p0 < it.n_parts; p0 += 8) {
+        float2 ml[8];
+        float4 o[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const bool in = p0 + q < it.n_parts;
+          ml[q] = in ? __ldcg(pml + (size_t)(p0 + q) * it.nv) : make_float2(-INFINITY, 0.f);
+          o[q] = in ? __ldcg(po + (size_t)(p0 + q) * it.nv * (HD / 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        float m8 = M;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) m8 = fmaxf(m8, ml[q].x);
+        const float f0 = m8 == -INFINITY ? 1.f : exp2f(M - m8);
+        L *= f0;
+        O.x *= f0;
+        O.y *= f0;
+        O.z *= f0;
+        O.w *= f0;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const float f = m8 == -INFINITY ? 1.f : exp2f(ml[q].x - m8);
+          L += ml[q].y * f;
+          O.x += o[q].x * f;
+          O.y += o[q].y * f;
+          O.z += o[q].z * f;
+          O.w += o[q].w * f;
+        }
+        M = m8;
+      }
+      const float r = L == 0.f ? 0.f : 1.f / L;
+      const float e[4] = {O.x * r, O.y * r, O.z * r, O.w * r};
+      const size_t at = (size_t)(it.row0 + (it.v0 + v) / a.n_rep) * a.ldo +
+                        (size_t)(it.kvh * a.n_rep + (it.v0 + v) % a.n_rep) * HD + d;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if constexpr (sizeof(TO) == 2) reinterpret_cast<__half*>(a.out)[at + q] = __float2half_rn(e[q]);
+        else reinterpret_cast<float*>(a.out)[at + q] = e[q];
+      }
+    }
+  }
+  __syncthreads();
+}
+
+// fp32 caches: K and V in fp32 on the CUDA cores. Each warp streams every fourth page
+// of its CTA's share through a ring of its own (bulk copies). Scores: lane (j, hh)
+// has key j and half of its elements, starting at chunk j, so that eight lanes meet
+// all banks; P V: a lane owns HD / 32 elements. NVT: the vectors an item of this
+// launch may have, so that a query head without others on its kv head (1) does not
+// pay for eight.
+template <int HD>
+struct F32Cfg {
+  static constexpr int BLK = 16 * HD * 4;
+  static constexpr int STAGE = 2 * BLK;
+  static constexpr int NST = HD == 128 ? 1 : 3;   // 64 / 96 KB a CTA
+  static constexpr int SMEM = 128 + kRowWarps * NST * STAGE + kRowWarps * NST * 8;
+};
+
+template <int HD, int NV, class TQ>
+__global__ void __launch_bounds__(kRowWarps * 32) rows_f32_kernel(const __grid_constant__ RowAttnArgs a) {
+  using C = F32Cfg<HD>;
+  constexpr int DPL = HD / 32, NST = C::NST, NCH = HD / 8;  // 16-byte chunks in half a key
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 127) & ~uintptr_t(127));
   __shared__ __align__(16) float qs[NV][HD];
   __shared__ VecInfo vi[NV];
   __shared__ float pb[kRowWarps][NV][16];
   __shared__ float mo[kRowWarps][NV][HD];
   __shared__ float mm[kRowWarps][NV], ml[kRowWarps][NV];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, j = lane & 15, hh = lane >> 4;
-  const T* pool = reinterpret_cast<const T*>(a.kv.pool);
-  for (int ui = a.cta[blockIdx.x]; ui < a.cta[blockIdx.x + 1]; ++ui) {
+  const float* pool = reinterpret_cast<const float*>(a.kv.pool);
+  uint8_t* ring = smem + warp * NST * C::STAGE;
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + kRowWarps * NST * C::STAGE) + warp * NST;
+  if (lane == 0) {
+    for (int i = 0; i < NST; ++i) mbar_init(&bar[i], 1);
+    fence_barrier_init();
+  }
+  __syncwarp();
+  const int u_begin = a.cta[blockIdx.x], u_end = a.cta[blockIdx.x + 1];
+  int pu = u_begin, pk = 0, pk1 = 0, pten = 0, pkvh = 0;
+  auto open = [&]() {
+    for (; pu < u_end; ++pu) {
+      const AttnUnit u = a.units[pu];
+      pk = u.k0 + 16 * warp;
+      pk1 = u.k1;
+      pten = u.tenant;
+      pkvh = u.kvh;
+      if (pk < pk1) return;
+    }
+  };
+  open();
+  int issued = 0, used = 0;
+  auto issue = [&](int limit) {
+    while (issued < limit && pu < u_end) {
+      if (lane == 0) {
+        const int page = a.kv.ptab[(size_t)pten * a.kv.ptab_stride + (pk >> 4)], s = issued % NST;
+        const float* kb = pool + ((((size_t)page * a.kv.n_layers + a.layer) * 2) * a.kv.n_kv + pkvh) * 16 * HD;
+        mbar_arrive_expect_tx(&bar[s], C::STAGE);
+        bulk_g2s(ring + s * C::STAGE, kb, C::BLK, &bar[s]);
+        bulk_g2s(ring + s * C::STAGE + C::BLK, kb + (size_t)a.kv.n_kv * 16 * HD, C::BLK, &bar[s]);
+      }
+      ++issued;
+      pk += 16 * kRowWarps;
+      if (pk >= pk1) {
+        ++pu;
+        open();
+      }
+    }
+  };
+  issue(NST);
+  bool alive = true;
+  for (int ui = u_begin; ui < u_end; ++ui) {
     const AttnUnit u = a.units[ui];
     __syncthreads();
     for (int i = threadIdx.x; i < NV * HD; i += blockDim.x) {
@@ -45,8 +165,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) rows_scalar_kernel(const __gri
       float x = 0.f;
       if (v < u.nv) {
         const int row = u.row0 + (u.v0 + v) / a.n_rep, head = u.kvh * a.n_rep + (u.v0 + v) % a.n_rep;
-        const size_t at = (size_t)row * a.ldq + (size_t)head * HD + d;
-        x = a.q16 ? ld_f32<__half>(a.q, at) : ld_f32<float>(a.q, at);
+        x = ld_f32<TQ>(a.q, (size_t)row * a.ldq + (size_t)head * HD + d);
       }
       qs[v][d] = x;
     }
@@ -73,20 +192,22 @@ __global__ void __launch_bounds__(kRowWarps * 32) rows_scalar_kernel(const __gri
       for (int d = 0; d < DPL; ++d) o[v][d] = 0.f;
     }
     for (int k = u.k0 + 16 * warp; k < u.k1; k += 16 * kRowWarps) {
-      const int page = a.kv.ptab[(size_t)u.tenant * a.kv.ptab_stride + (k >> 4)];
-      const T* kb = pool + ((((size_t)page * a.kv.n_layers + a.layer) * 2) * a.kv.n_kv + u.kvh) * 16 * HD;
-      const T* vb = kb + (size_t)a.kv.n_kv * 16 * HD;
+      issue(used + NST);
+      const int s = used % NST;
+      if (alive) alive = mbar_wait(&bar[s], (used / NST) & 1, a.err, DEV_TIMEOUT_FULL);
+      const float* kb = reinterpret_cast<const float*>(ring + s * C::STAGE);
+      const float* vb = kb + 16 * HD;
       float dot[NV];
 #pragma unroll
       for (int v = 0; v < NV; ++v) dot[v] = 0.f;
-      for (int d = hh * (HD / 2); d < (hh + 1) * (HD / 2); d += 4) {
-        float kf[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) kf[e] = ld_f32<T>(kb, j * HD + d + e);
+#pragma unroll 8
+      for (int ch = 0; ch < NCH; ++ch) {
+        const int d = hh * (HD / 2) + ((ch + j) & (NCH - 1)) * 4;
+        const float4 kf = *reinterpret_cast<const float4*>(kb + j * HD + d);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
           const float4 q = *reinterpret_cast<const float4*>(&qs[v][d]);
-          dot[v] = fmaf(q.x, kf[0], fmaf(q.y, kf[1], fmaf(q.z, kf[2], fmaf(q.w, kf[3], dot[v]))));
+          dot[v] = fmaf(q.x, kf.x, fmaf(q.y, kf.y, fmaf(q.z, kf.z, fmaf(q.w, kf.w, dot[v]))));
         }
       }
       const int key = k + j;
@@ -96,27 +217,31 @@ __global__ void __launch_bounds__(kRowWarps * 32) rows_scalar_kernel(const __gri
         if (a.cap > 0.f) x = a.cap * tanhf(x / a.cap);
         x = (x - vi[v].slope * fabsf((float)(vi[v].pos - key))) * kLog2e;
         const bool in = key >= vi[v].lo && key < vi[v].hi;
-        float mx = in ? x : -INFINITY;
+        // the maximum is raised only when some score passes it; the sums stay per lane
+        if (__any_sync(0xffffffffu, in && x > m[v])) {
+          float mx = in ? x : -INFINITY;
 #pragma unroll
-        for (int s = 8; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
-        const float mn = fmaxf(m[v], mx);
-        const float alpha = mn == -INFINITY ? 1.f : exp2f(m[v] - mn);
-        const float p = in ? exp2f(x - (mn == -INFINITY ? 0.f : mn)) : 0.f;
-        float sum = p;
+          for (int w = 8; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+          mx = fmaxf(m[v], mx);
+          const float alpha = mx == -INFINITY ? 1.f : exp2f(m[v] - mx);
+          l[v] *= alpha;
+          m[v] = mx;
 #pragma unroll
-        for (int s = 8; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-        l[v] = l[v] * alpha + sum;
-        m[v] = mn;
-        if (hh == 0) pb[warp][v][j] = p;
-#pragma unroll
-        for (int d = 0; d < DPL; ++d) o[v][d] *= alpha;
+          for (int d = 0; d < DPL; ++d) o[v][d] *= alpha;
+        }
+        const float p = in ? exp2f(x - (m[v] == -INFINITY ? 0.f : m[v])) : 0.f;
+        if (hh == 0) {
+          l[v] += p;
+          pb[warp][v][j] = p;
+        }
       }
       __syncwarp();
       const int nk = min(16, u.k1 - k);
+#pragma unroll 4
       for (int t = 0; t < nk; ++t) {
         float vf[DPL];
-#pragma unroll
-        for (int d = 0; d < DPL; ++d) vf[d] = ld_f32<T>(vb, t * HD + lane * DPL + d);
+        if constexpr (DPL == 4) *reinterpret_cast<float4*>(vf) = *reinterpret_cast<const float4*>(vb + t * HD + lane * DPL);
+        else *reinterpret_cast<float2*>(vf) = *reinterpret_cast<const float2*>(vb + t * HD + lane * DPL);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
           const float p = pb[warp][v][t];
@@ -126,9 +251,12 @@ __global__ void __launch_bounds__(kRowWarps * 32) rows_scalar_kernel(const __gri
         }
       }
       __syncwarp();
+      ++used;
     }
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
+#pragma unroll
+      for (int w = 8; w > 0; w >>= 1) l[v] += __shfl_xor_sync(0xffffffffu, l[v], w);
 #pragma unroll
       for (int d = 0; d < DPL; ++d) mo[warp][v][lane * DPL + d] = o[v][d];
       if (lane == 0) {
@@ -139,31 +267,26 @@ __global__ void __launch_bounds__(kRowWarps * 32) rows_scalar_kernel(const __gri
     __syncthreads();
     for (int i = threadIdx.x; i < u.nv * HD; i += blockDim.x) {
       const int v = i / HD, d = i % HD;
-      float M = -INFINITY;
+      float M = -INFINITY, L = 0.f, O = 0.f;
 #pragma unroll
       for (int w = 0; w < kRowWarps; ++w) M = fmaxf(M, mm[w][v]);
-      float L = 0.f, O = 0.f;
-      if (M != -INFINITY)
 #pragma unroll
-        for (int w = 0; w < kRowWarps; ++w) {
-          const float f = exp2f(mm[w][v] - M);
-          L += ml[w][v] * f;
-          O += mo[w][v][d] * f;
-        }
-      else
-#pragma unroll
-        for (int w = 0; w < kRowWarps; ++w) L += ml[w][v];  // a score that is not a number leaves M unset
+      for (int w = 0; w < kRowWarps; ++w) {
+        const float f = M == -INFINITY ? 1.f : exp2f(mm[w][v] - M);
+        L += ml[w][v] * f;
+        O += mo[w][v][d] * f;
+      }
       if (u.slot >= 0) {
         a.part_o[(size_t)(u.slot + v) * HD + d] = O;
         if (d == 0) a.part_ml[u.slot + v] = make_float2(M, L);
       } else {
-        const float r = L == 0.f ? 0.f : M == -INFINITY ? L : O / L;
-        const int row = u.row0 + (u.v0 + v) / a.n_rep;
-        const size_t at = (size_t)row * a.ldo + (size_t)vi[v].head * HD + d;
-        if (a.q16) reinterpret_cast<__half*>(a.out)[at] = __float2half_rn(r);
+        const float r = L == 0.f ? 0.f : O / L;
+        const size_t at = (size_t)(u.row0 + (u.v0 + v) / a.n_rep) * a.ldo + (size_t)vi[v].head * HD + d;
+        if constexpr (sizeof(TQ) == 2) reinterpret_cast<__half*>(a.out)[at] = __float2half_rn(r);
         else reinterpret_cast<float*>(a.out)[at] = r;
       }
     }
+    if (u.slot >= 0) join_last<HD, TQ>(a, u);
   }
 }
 
@@ -552,13 +675,17 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) rows_mma_kernel(const __gri
         else reinterpret_cast<__half*>(a.out)[at] = __float2half_rn(r);
       }
     }
+    if (u.slot >= 0) {
+      if (HL) join_last<HD, float>(a, u);
+      else join_last<HD, __half>(a, u);
+    }
   }
 }
 
-// Joins the parts of an item: one CTA per (item, vector), parts in order.
+// Joins the parts of a tile item: a CTA for every 32nd vector, parts in order.
 template <int HD>
 __global__ void __launch_bounds__(HD) rows_join_kernel(const __grid_constant__ RowAttnArgs a) {
-  const JoinItem it = a.joins[blockIdx.x];
+  const JoinItem it = a.joins[a.n_small_joins + blockIdx.x];
   const int d = threadIdx.x;
   for (int v = blockIdx.y; v < it.nv; v += gridDim.y) {
     float M = -INFINITY;
@@ -590,21 +717,41 @@ static cudaError_t launch_mma(const RowAttnArgs& a, cudaStream_t s) {
   return cudaGetLastError();
 }
 
+template <int HD, int NV>
+static cudaError_t launch_f32(const RowAttnArgs& a, cudaStream_t s) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  constexpr int smem = F32Cfg<HD>::SMEM;
+  if (a.q16) {
+    if (cudaError_t e = ensure_smem_attr(rows_f32_kernel<HD, NV, __half>, smem, dev)) return e;
+    rows_f32_kernel<HD, NV, __half><<<a.n_cta, kRowWarps * 32, smem, s>>>(a);
+  } else {
+    if (cudaError_t e = ensure_smem_attr(rows_f32_kernel<HD, NV, float>, smem, dev)) return e;
+    rows_f32_kernel<HD, NV, float><<<a.n_cta, kRowWarps * 32, smem, s>>>(a);
+  }
+  return cudaGetLastError();
+}
+template <int HD>
+static cudaError_t launch_f32_vecs(const RowAttnArgs& a, cudaStream_t s) {
+  if (a.max_nv <= 1) return launch_f32<HD, 1>(a, s);
+  if (a.max_nv <= 2) return launch_f32<HD, 2>(a, s);
+  if (a.max_nv <= 4) return launch_f32<HD, 4>(a, s);
+  return launch_f32<HD, 8>(a, s);
+}
+
 cudaError_t rows_small_launch(const RowAttnArgs& a, cudaStream_t s) {
   if (a.n_cta < 1) return cudaSuccess;
-  const dim3 g(a.n_cta), b(kRowWarps * 32);
   if (a.kv.f16) {
     if (a.kv.hd == 128) return a.q16 ? launch_mma<128, 0>(a, s) : launch_mma<128, 1>(a, s);
     return a.q16 ? launch_mma<64, 0>(a, s) : launch_mma<64, 1>(a, s);
   }
-  if (a.kv.hd == 128) rows_scalar_kernel<128, float><<<g, b, 0, s>>>(a);
-  else rows_scalar_kernel<64, float><<<g, b, 0, s>>>(a);
-  return cudaGetLastError();
+  return a.kv.hd == 128 ? launch_f32_vecs<128>(a, s) : launch_f32_vecs<64>(a, s);
 }
 
 cudaError_t rows_join_launch(const RowAttnArgs& a, cudaStream_t s) {
-  if (a.n_joins < 1) return cudaSuccess;
-  const dim3 g(a.n_joins, kSmallVecs);
+  const int n = a.n_joins - a.n_small_joins;
+  if (n < 1) return cudaSuccess;
+  const dim3 g(n, 32);
   if (a.kv.hd == 128) rows_join_kernel<128><<<g, 128, 0, s>>>(a);
   else rows_join_kernel<64><<<g, 64, 0, s>>>(a);
   return cudaGetLastError();

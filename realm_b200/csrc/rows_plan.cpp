@@ -63,7 +63,8 @@ void rows_partition(const std::vector<RowInfo>& rows, int n_heads, int n_kv, int
     out.small_cta.assign(1, 0);
     long long at = 0, cta = 0;  // pages handed out so far, CTA being filled
     auto cta_end = [&](long long c) { return pages * (c + 1) / G; };
-    for (const Item& it : small)
+    for (const Item& it : small) {
+      out.max_nv = std::max(out.max_nv, it.nv);
       for (int h = 0; h < n_kv; ++h) {
         const int np = blocks_of(it, kRowPage);
         const size_t first = out.small.size();
@@ -75,7 +76,7 @@ void rows_partition(const std::vector<RowInfo>& rows, int n_heads, int n_kv, int
           }
           const int take = (int)std::min<long long>(np - p, cta + 1 < G ? cta_end(cta) - at : np - p);
           AttnUnit u{it.row0, it.v0, it.nv, h, it.tenant, it.k0 + p * kRowPage,
-                     std::min(it.k1, it.k0 + (p + take) * kRowPage), -1};
+                     std::min(it.k1, it.k0 + (p + take) * kRowPage), -1, -1};
           out.small.push_back(u);
           p += take;
           at += take;
@@ -84,14 +85,16 @@ void rows_partition(const std::vector<RowInfo>& rows, int n_heads, int n_kv, int
         if (parts > 1) {
           out.joins.push_back({it.row0, it.v0, it.nv, h, out.n_slots, parts});
           for (size_t i = first; i < out.small.size(); ++i) {
+            out.small[i].join = (int)out.joins.size() - 1;
             out.small[i].slot = out.n_slots;
             out.n_slots += it.nv;
           }
-          out.max_join_parts = std::max(out.max_join_parts, parts);
         }
       }
+    }
     while ((long long)out.small_cta.size() <= G) out.small_cta.push_back((int)out.small.size());
   }
+  out.n_small_joins = (int)out.joins.size();
 
   // tile items: one CTA per unit, the longest first. Where the items are fewer
   // than the SMs, their keys are cut so that the units fill them.
@@ -106,12 +109,11 @@ void rows_partition(const std::vector<RowInfo>& rows, int n_heads, int n_kv, int
       for (int h = 0; h < n_kv; ++h) {
         if (parts > 1) {
           out.joins.push_back({it.row0, it.v0, it.nv, h, out.n_slots, parts});
-          out.max_join_parts = std::max(out.max_join_parts, parts);
         }
         for (int p = 0; p < parts; ++p) {
           const int b0 = (int)((long long)nb * p / parts), b1 = (int)((long long)nb * (p + 1) / parts);
           AttnUnit u{it.row0, it.v0, it.nv, h, it.tenant, it.k0 + b0 * kTileKeys,
-                     std::min(it.k1, it.k0 + b1 * kTileKeys), -1};
+                     std::min(it.k1, it.k0 + b1 * kTileKeys), -1, -1};
           if (parts > 1) {
             u.slot = out.n_slots;
             out.n_slots += it.nv;

@@ -60,17 +60,25 @@ def _is_tensor(a) -> bool:
     return hasattr(a, "data_ptr")
 
 
+_TORCH = {}  # torch's dtypes by name
+
+
+def _torch_dtype(name):
+    import torch
+    _TORCH[name] = getattr(torch, name)
+    return _TORCH[name]
+
+
 def _vec(a, dtype, n, name):
     """Pointer of a contiguous vector of n elements, or None."""
     if a is None:
         return None
     if _is_tensor(a):
-        if str(a.dtype) != "torch." + dtype or a.numel() != n or not a.is_contiguous():
-            raise ValueError(f"{name}: {n} contiguous {dtype} values wanted")
-        return a.data_ptr()
-    if a.dtype != dtype or a.size != n or not a.flags.c_contiguous:
-        raise ValueError(f"{name}: {n} contiguous {dtype} values wanted")
-    return a.ctypes.data
+        if a.dtype is (_TORCH.get(dtype) or _torch_dtype(dtype)) and a.numel() == n and a.is_contiguous():
+            return a.data_ptr()
+    elif a.dtype == dtype and a.size == n and a.flags.c_contiguous:
+        return a.ctypes.data
+    raise ValueError(f"{name}: {n} contiguous {dtype} values wanted")
 
 
 def _rows3(a, n, heads, hd, name):
