@@ -13,7 +13,8 @@
 // maximum is raised only when a score passes it by 2^kSlack, so p stays below
 // 2^15, fp16's range, and O is rarely rescaled.
 //
-// Warps: 0-3 softmax of tile 0, 4-7 of tile 1, 8 issues the products, 9 the loads.
+// Warps: 0-3 softmax of tile 0, 4-7 of tile 1, 8 issues the products, 9 the loads
+// (10 and 11 fill the third warpgroup, which gives registers to the others).
 #include "common.cuh"
 #include "rows.cuh"
 
@@ -23,7 +24,9 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kBias = 6.f, kSlack = 8.f;
-constexpr int kTileThreads = 320;
+constexpr int kTileThreads = 384;
+// registers a thread: 384 x 168 at launch; the softmax warps take 224, the others keep 56
+// (256 x 224 + 128 x 56 = 384 x 168)
 
 // ---- tcgen05 ----
 // shared-memory operand with 128-byte swizzle; sbo: bytes between groups of 8 rows,
@@ -81,6 +84,14 @@ __device__ __forceinline__ void st32(uint32_t ta, const uint32_t* r) {
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ void st16(uint32_t ta, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(ta),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 __device__ __forceinline__ float ld1(uint32_t ta) {
   float r;
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=f"(r) : "r"(ta) : "memory");
@@ -102,6 +113,57 @@ __device__ __forceinline__ uint32_t pack2_lo(float a, float b, uint32_t hi) {
   const float2 f = __half22float2(u32_as_h2(hi));
   return pack2(a - f.x, b - f.y);
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+// two fp32 values in one register pair, and the packed operations on them
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 pair(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(f2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// tanh(y) = y P(y^2) for |y| <= limit, fitted for the least largest relative
+// error: 6e-7 with four terms (fp16 rows, whose probabilities are rounded to 2^-12),
+// 4e-9 with six.
+template <int HL>
+struct Tanh;
+template <>
+struct Tanh<0> {
+  static constexpr int N = 4;
+  static constexpr float limit = 0.5f;
+  static __device__ __forceinline__ float c(int i) {
+    constexpr float k[4] = {0.999999456f, -0.333263179f, 0.131902966f, -0.0444022264f};
+    return k[i];
+  }
+};
+template <>
+struct Tanh<1> {
+  static constexpr int N = 6;
+  static constexpr float limit = 0.625f;
+  static __device__ __forceinline__ float c(int i) {
+    constexpr float k[6] = {0.999999996f, -0.333332605f, 0.133311275f, -0.053721068f, 0.0205909884f, -0.00565998907f};
+    return k[i];
+  }
+};
 // barrier of the n softmax threads in use, with the "or" of their values
 __device__ __forceinline__ bool any_softmax(int n, bool v) {
   uint32_t r;
@@ -187,7 +249,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
   }
   __syncthreads();
 
-  if (warp == 9) {
+  if (warp >= 10) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+  } else if (warp == 9) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     // ---- loads: blocks K0, V0, K1, V1, ... through the ring ----
     bool ok = true;
     int it = 0;
@@ -218,20 +283,28 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
     // copies in flight land before the CTA's shared memory goes away
     for (int i = max(0, it - NS); i < it; ++i) mbar_wait(&full[i % NS], (uint32_t)((i / NS) & 1), nullptr, 0);
   } else if (warp == 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     // ---- products ----
     if (lane == 0 && nb > 0) {
       bool ok = true;
       constexpr uint32_t ids = idesc16(128, B, 0), ido = idesc16(128, HD, 1);
       const uint32_t qa = smem_u32(smem), ra = smem_u32(ring);
+      // the compiler may not carry every operand's descriptor through the loop in registers
+      auto fresh = [](uint64_t d) {
+        asm volatile("" : "+l"(d));
+        return d;
+      };
       auto scores = [&](int t, int slot) {
+        const uint64_t kd = fresh(desc128(ra + slot * C::SLOT, 16, 1024));
 #pragma unroll
-        for (int part = 0; part < 1 + HL; ++part)
+        for (int part = 0; part < 1 + HL; ++part) {
+          const uint64_t qd = fresh(desc128(qa + (t * (1 + HL) + part) * C::QT, 16, 1024));
 #pragma unroll
           for (int ks = 0; ks < HD / 16; ++ks) {
-            const uint32_t off = (ks >> 2) * C::PANEL + (ks & 3) * 32;
-            mma_ss(tmem + t * B, desc128(qa + (t * (1 + HL) + part) * C::QT + off, 16, 1024),
-                   desc128(ra + slot * C::SLOT + off, 16, 1024), ids, part || ks);
+            const uint32_t off = ((ks >> 2) * C::PANEL + (ks & 3) * 32) >> 4;
+            mma_ss(tmem + t * B, qd + off, kd + off, ids, part || ks);
           }
+        }
       };
       auto wait = [&](uint64_t* bar, int phase, uint32_t code) {
         ok = ok && mbar_wait(bar, (uint32_t)(phase & 1), a.err, code);
@@ -253,12 +326,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
           wait(&p_bar[t], j, DEV_TIMEOUT_DRAIN);
           if (!ok) break;
           const uint32_t more = j || *(volatile int*)&primed[t];
+          const uint64_t vd = fresh(desc128(ra + vs * C::SLOT, C::PANEL, 1024));
 #pragma unroll
           for (int part = 0; part < 1 + HL; ++part)
 #pragma unroll
             for (int ks = 0; ks < B / 16; ++ks)
-              mma_ts(tmem + 2 * B + t * HD, tmem + t * B + part * (B / 2) + ks * 8,
-                     desc128(ra + vs * C::SLOT + ks * 2048, C::PANEL, 1024), ido, more || part || ks);
+              mma_ts(tmem + 2 * B + t * HD, tmem + t * B + part * (B / 2) + ks * 8, vd + ks * (2048 >> 4), ido,
+                     more || part || ks);
           if (t == nt - 1) tc_commit(&freeb[vs]);
           if (j + 1 < nb) {
             if (t == 0) wait(&full[ks_], ik / NS, DEV_TIMEOUT_FULL);
@@ -275,7 +349,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
       mbar_wait(&drain, 0, a.err, DEV_TIMEOUT_DRAIN);
     }
     __syncwarp();
-  } else if (tile < nt) {
+  } else if (warp < 8 && tile < nt) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     // ---- softmax: thread = row of its tile ----
     const int tr = tid & 127;
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
@@ -354,7 +429,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
     const int all0 = span[tile][0], all1 = span[tile][1], in0 = seen[0], in1 = seen[1];
     const int both0 = max(span[0][0], span[1][0]), both1 = min(span[0][1], span[1][1]);
     const float slope = BIAS && active ? a.slopes[head] * kLog2e : 0.f;
-    const float cap2 = a.cap * kLog2e, kcap = CAP ? 2.f * kLog2e * sv / a.cap : 0.f;
+    const float cap2 = a.cap * kLog2e, kcap = CAP ? sv / a.cap : 0.f;
     const float mult = (CAP || BIAS) ? 1.f : fmaxf(sv * kLog2e, 1e-30f);  // scores to base-2 units (-inf stays)
     const float sv2 = sv * kLog2e;
     float m = -INFINITY, l = 0.f;
@@ -368,14 +443,43 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
       wait_ld();
       const bool partial = kb < all0 || kb + B > all1;  // the same for the whole tile
       if (CAP) {
-        // cap tanh(y / cap) = cap - 2 cap / (1 + e^(2 y / cap))
+        float top = 0.f;
 #pragma unroll
-        for (int i = 0; i < B; ++i) x[i] = fmaf(-2.f * cap2, rcp(1.f + ex2(x[i] * kcap)), cap2);
+        for (int i = 0; i < B; i += 2) top = max3(top, fabsf(x[i]), fabsf(x[i + 1]));
+        using P = Tanh<HL>;
+        if (__all_sync(0xffffffffu, top * kcap <= P::limit)) {
+          const f2 k2 = pair(kcap, kcap);
+          f2 c[P::N];
+#pragma unroll
+          for (int q = 0; q < P::N; ++q) c[q] = pair(cap2 * P::c(q), cap2 * P::c(q));
+#pragma unroll
+          for (int i = 0; i < B; i += 2) {
+            const f2 y = mul2(pair(x[i], x[i + 1]), k2), z = mul2(y, y);
+            f2 t = c[P::N - 1];
+#pragma unroll
+            for (int q = P::N - 2; q >= 0; --q) t = fma2(t, z, c[q]);
+            unpair(mul2(t, y), x[i], x[i + 1]);
+          }
+        } else {
+          // cap tanh(y) = cap - 2 cap / (1 + e^(2 y))
+          const float k = 2.f * kLog2e * kcap;
+#pragma unroll
+          for (int i = 0; i < B; ++i) x[i] = fmaf(-2.f * cap2, rcp(1.f + ex2(x[i] * k)), cap2);
+        }
       }
       if (BIAS) {
+        if (__all_sync(0xffffffffu, kb + B - 1 <= r.pos)) {  // no key after its row: the distance is linear
+          const f2 sl = pair(slope, slope), s2 = pair(CAP ? 1.f : sv2, CAP ? 1.f : sv2);
+          const float b0 = slope * (float)(kb - r.pos);
+          const f2 b2 = pair(b0, b0);
 #pragma unroll
-        for (int i = 0; i < B; ++i)
-          x[i] = fmaf(-slope, fabsf((float)(r.pos - kb - i)), CAP ? x[i] : x[i] * sv2);
+          for (int i = 0; i < B; i += 2)
+            unpair(fma2(pair(x[i], x[i + 1]), s2, fma2(pair((float)i, (float)(i + 1)), sl, b2)), x[i], x[i + 1]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < B; ++i)
+            x[i] = fmaf(-slope, fabsf((float)(r.pos - kb - i)), CAP ? x[i] : x[i] * sv2);
+        }
       }
       if (partial) {
         const uint32_t base = (uint32_t)(kb - r.lo), n = (uint32_t)max(0, r.hi - r.lo);
@@ -384,8 +488,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
       }
       float mx4[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-      for (int i = 4; i < B; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], x[i]);
-      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * mult;
+      for (int i = 4; i < B; i += 8)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (i + 2 * q + 1 < B) mx4[q] = max3(mx4[q], x[i + 2 * q], x[i + 2 * q + 1]);
+      const float mx = max3(fmaxf(mx4[0], mx4[1]), mx4[2], mx4[3]) * mult;
       // each row raises its maximum by its own scores alone
       const bool up = mx > (m == -INFINITY ? m : m + kSlack);
       float alpha = 1.f;
@@ -407,22 +514,29 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
         }
       }
       const float off = kBias - (m == -INFINITY ? 0.f : m);
-      float s4[4] = {0.f, 0.f, 0.f, 0.f};
+      const f2 mult2 = pair(mult, mult), off2 = pair(off, off);
+      f2 s2[2] = {0ull, 0ull};
 #pragma unroll
-      for (int i = 0; i < B / 64; ++i) {
-        uint32_t hi[32], lo[32];
+      for (int i = 0; i < B / 32; ++i) {
+        uint32_t hi[16], lo[16];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float p0 = ex2(fmaf(x[64 * i + 2 * e], mult, off)), p1 = ex2(fmaf(x[64 * i + 2 * e + 1], mult, off));
-          s4[(2 * e) & 3] += p0;
-          s4[(2 * e + 1) & 3] += p1;
+        for (int e = 0; e < 16; ++e) {
+          float p0, p1;
+          unpair(fma2(pair(x[32 * i + 2 * e], x[32 * i + 2 * e + 1]), mult2, off2), p0, p1);
+          p0 = ex2(p0);
+          p1 = ex2(p1);
+          s2[e & 1] = add2(s2[e & 1], pair(p0, p1));
           hi[e] = pack2(p0, p1);
           if (HL) lo[e] = pack2_lo(p0, p1, hi[e]);
         }
-        st32(ts + 32 * i, hi);
-        if (HL) st32(ts + B / 2 + 32 * i, lo);
+        st16(ts + 16 * i, hi);
+        if (HL) st16(ts + B / 2 + 16 * i, lo);
       }
-      l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+      {
+        float p0, p1;
+        unpair(add2(s2[0], s2[1]), p0, p1);
+        l += p0 + p1;
+      }
       if (kb < both0 || kb + B > both1) {
         // A block that some row of the unit does not see whole. Values of keys that no
         // row sees become 0, and so do those of pages that were not loaded. Values that
