@@ -283,7 +283,7 @@ struct RowSet {
   int pool = -1, n_heads = 0, n_rows = 0, max_pos = 0;
   std::vector<RowPlanTenant> tenants;
   int n_cta = 0, n_tile = 0, n_joins = 0, n_small_joins = 0, max_nv = 0;
-  DevBuf rows, small, cta, tile, joins, counters, part_o, part_ml;
+  DevBuf rows, small, cta, tile, spans, joins, counters, part_o, part_ml;
 };
 
 struct Ctx {
@@ -2305,6 +2305,7 @@ int32_t rb_plan_create(rb_ctx* c, int32_t pool, const rb_plan_desc* d, int32_t* 
   if (int rc = upload_vec(c, S->small, w.small)) return rc;
   if (int rc = upload_vec(c, S->cta, w.small_cta)) return rc;
   if (int rc = upload_vec(c, S->tile, w.tile)) return rc;
+  if (int rc = upload_vec(c, S->spans, w.spans)) return rc;
   if (int rc = upload_vec(c, S->joins, w.joins)) return rc;
   if (int rc = upload_vec(c, S->counters, std::vector<int32_t>(w.n_small_joins, 0))) return rc;
   if (w.n_slots) {
@@ -2454,6 +2455,7 @@ int32_t rb_plan_attention(rb_ctx* c, int32_t plan, uint32_t layer, const rb_atte
   RB_CUDA(rows_small_launch(a, c->stream));
   a.units = S->tile.as<AttnUnit>();
   a.n_units = S->n_tile;
+  a.spans = S->spans.as<TileSpan>();
   RB_CUDA(rows_tile_launch(a, c->stream));
   RB_CUDA(rows_join_launch(a, c->stream));
   if (!(flags & RB_PTR_DEVICE))

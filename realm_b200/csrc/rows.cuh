@@ -34,10 +34,17 @@ struct JoinItem {
   int32_t row0, v0, nv, kvh, slot0, n_parts;
 };
 
+// What the rows of a tile unit see: keys that every row of tile t sees [all0, all1),
+// and that some row of the unit sees [in0, in1).
+struct TileSpan {
+  int32_t all0[2], all1[2], in0, in1;
+};
+
 // Work lists of one plan. CTA b of the small (tile) kernel runs the units
 // [cta[b], cta[b + 1]) of its list.
 struct RowWork {
   std::vector<AttnUnit> small, tile;
+  std::vector<TileSpan> spans;       // of the tile units
   std::vector<int32_t> small_cta;
   std::vector<JoinItem> joins;       // the small kernels' items first: their last CTA joins them
   int32_t n_small_joins = 0;
@@ -70,6 +77,7 @@ struct RowAttnArgs {
   const AttnUnit* units = nullptr;
   const int32_t* cta = nullptr;  // small kernels
   int32_t n_cta = 0, n_units = 0, max_nv = 0;  // max_nv: vectors of the largest small item
+  const TileSpan* spans = nullptr;  // tile kernel
   const JoinItem* joins = nullptr;
   int32_t n_small_joins = 0, n_joins = 0;
   int32_t* counters = nullptr;  // [n_small_joins], zero between launches

@@ -96,16 +96,16 @@ void rows_partition(const std::vector<RowInfo>& rows, int n_heads, int n_kv, int
   }
   out.n_small_joins = (int)out.joins.size();
 
-  // tile items: one CTA per unit, the longest first. Where the items are fewer
-  // than the SMs, their keys are cut so that the units fill them.
+  // tile items: one CTA per unit, the longest first. Items of more blocks than half an
+  // SM's even share are cut, so that the last ones to run do not leave SMs idle, but
+  // not below four blocks: a unit's start and end cost about as much as those.
   if (!tile.empty()) {
     long long blocks = 0;
     for (const Item& it : tile) blocks += (long long)n_kv * std::max(1, blocks_of(it, kTileKeys));
-    const long long seg = std::max<long long>(4, (blocks + num_sms - 1) / num_sms);
-    const bool cut = (long long)tile.size() * n_kv < num_sms;
+    const long long seg = std::max<long long>(4, (blocks + 2 * num_sms - 1) / (2 * num_sms));
     for (const Item& it : tile) {
       const int nb = blocks_of(it, kTileKeys);
-      const int parts = cut && nb > seg ? (int)((nb + seg - 1) / seg) : 1;
+      const int parts = nb > seg ? (int)((nb + seg - 1) / seg) : 1;
       for (int h = 0; h < n_kv; ++h) {
         if (parts > 1) {
           out.joins.push_back({it.row0, it.v0, it.nv, h, out.n_slots, parts});
@@ -124,6 +124,24 @@ void rows_partition(const std::vector<RowInfo>& rows, int n_heads, int n_kv, int
     }
     std::stable_sort(out.tile.begin(), out.tile.end(),
                      [](const AttnUnit& a, const AttnUnit& b) { return a.k1 - a.k0 > b.k1 - b.k0; });
+    for (const AttnUnit& u : out.tile) {
+      TileSpan s{{0, 0}, {0x7fffffff, 0x7fffffff}, 0, 0};
+      bool any = false;
+      for (int t = 0; t < 2; ++t) {
+        const int v0 = u.v0 + t * (kTileVecs / 2), v1 = u.v0 + std::min(u.nv, (t + 1) * (kTileVecs / 2));
+        if (v0 >= v1) continue;
+        for (int r = u.row0 + v0 / n_rep; r <= u.row0 + (v1 - 1) / n_rep; ++r) {
+          s.all0[t] = std::max(s.all0[t], rows[r].lo);
+          s.all1[t] = std::min(s.all1[t], rows[r].hi);
+          if (rows[r].hi > rows[r].lo) {
+            s.in0 = any ? std::min(s.in0, rows[r].lo) : rows[r].lo;
+            s.in1 = std::max(s.in1, rows[r].hi);
+            any = true;
+          }
+        }
+      }
+      out.spans.push_back(s);
+    }
   }
 }
 

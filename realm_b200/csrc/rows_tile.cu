@@ -3,8 +3,7 @@
 // and tenant, as two tiles of 128 that share every block of 128 keys.
 //
 // Per tile and block: S = Q K^T (tcgen05.mma, both operands in shared memory, S in
-// TMEM), softmax in registers with two threads a row (tcgen05.ld, 64 keys each: four
-// warps a scheduler hide one another's latencies), P back to TMEM over S, O += P V with P as the TMEM operand and V as it lies in the page
+// TMEM), softmax in registers with one thread a row (tcgen05.ld), P back to TMEM, O += P V with P as the TMEM operand and V as it lies in the page
 // ([key][element]: the MN-major operand). The tiles take turns: while one's scores
 // are in the softmax warps the tensor core works on the other's.
 //
@@ -13,9 +12,8 @@
 // maximum is raised only when a score passes it by 2^kSlack, so p stays below
 // 2^15, fp16's range, and O is rarely rescaled.
 //
-// Warps: 0-7 softmax of tile 0 (0-3 the first 64 keys of a block, 4-7 the others), 8-15
-// of tile 1, 16 issues the products, 17 the loads (18 and 19 fill the last warpgroup,
-// which gives registers to the others).
+// Warps: 0-3 softmax of tile 0, 4-7 of tile 1, 8 issues the products, 9 the loads (10
+// and 11 fill the last warpgroup, which gives registers to the others).
 #include "common.cuh"
 #include "rows.cuh"
 
@@ -25,14 +23,10 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kBias = 6.f, kSlack = 8.f;
-#ifndef TPR_
-#define TPR_ 1
-#endif
-constexpr int kTpr = TPR_;                    // softmax threads a row
-constexpr int kSoftWarps = 8 * kTpr;
+constexpr int kSoftWarps = 8;
 constexpr int kTileThreads = (kSoftWarps + 4) * 32;
 // registers a thread at launch, of a softmax warp and of the others: the split uses what the launch gave
-constexpr int kRegSoft = kTpr == 1 ? 224 : 104, kRegRest = kTpr == 1 ? 56 : 64;
+constexpr int kRegSoft = 224, kRegRest = 56;  // 256 x 224 + 128 x 56 = 384 x 168
 
 // ---- tcgen05 ----
 // shared-memory operand with 128-byte swizzle; sbo: bytes between groups of 8 rows,
@@ -162,22 +156,21 @@ __device__ __forceinline__ f2 add2(f2 a, f2 b) {
   asm volatile("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-// tanh(y) = y P(y^2) for |y| <= limit, fitted for the least largest relative
-// error: 6e-7 with four terms (fp16 rows, whose probabilities are rounded to 2^-12),
-// 4e-9 with six.
+// tanh(y) = y P(y^2) for |y| <= limit, fitted for the least largest relative error. In
+// the fused form (together with the exponential): 1e-06 with three terms (fp16 rows, whose
+// probabilities are rounded to 2^-12), 1e-08 with five. An odd number of terms has a
+// positive last one, so that a masked score, -inf, stays -inf.
 template <int HL>
-struct Tanh;
-template <>
-struct Tanh<0> {
-  static constexpr int N = 4;
-  static constexpr float limit = 0.5f;
+struct Fused {
+  static constexpr int N = HL ? 5 : 3;
+  static constexpr float limit = HL ? 0.5f : 0.3f;
   static __device__ __forceinline__ float c(int i) {
-    constexpr float k[4] = {0.999999456f, -0.333263179f, 0.131902966f, -0.0444022264f};
-    return k[i];
+    constexpr float k[5] = {0.999999987f, -0.333330694f, 0.133247793f, -0.0529860753f, 0.0171350067f}, k3[3] = {0.999998839f, -0.333100216f, 0.12633946f};
+    return HL ? k[i] : k3[i < 3 ? i : 0];
   }
 };
-template <>
-struct Tanh<1> {
+// The wider form, 4e-09.
+struct Wide {
   static constexpr int N = 6;
   static constexpr float limit = 0.625f;
   static __device__ __forceinline__ float c(int i) {
@@ -185,14 +178,14 @@ struct Tanh<1> {
     return k[i];
   }
 };
-// barrier of the n softmax threads in use, with the "or" of their values
-__device__ __forceinline__ bool any_softmax(int n, bool v) {
+// named barrier `id` of n threads, with the "or" of their values
+__device__ __forceinline__ bool any_softmax(int id, int n, bool v) {
   uint32_t r;
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, "
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %3, %2, p;\n\tselp.u32 %0, 1, 0, "
       "q;\n\t}"
       : "=r"(r)
-      : "r"((uint32_t)v), "r"(n)
+      : "r"((uint32_t)v), "r"(n), "r"(id)
       : "memory");
   return r != 0;
 }
@@ -228,7 +221,7 @@ struct TileCfg {
 template <int HD, int HL, int CAP, int BIAS>
 __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid_constant__ RowAttnArgs a) {
   using C = TileCfg<HD, HL>;
-  constexpr int NS = C::NS, B = kTileKeys, H = B / kTpr, NSOFT = 128 * kTpr;  // softmax threads a tile
+  constexpr int NS = C::NS, B = kTileKeys;
   extern __shared__ __align__(1024) uint8_t smem[];  // the swizzle follows the address bits
   if (smem_u32(smem) & 1023) {
     report_error(a.err, DEV_TIMEOUT_SMEM);
@@ -238,13 +231,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
   __shared__ uint64_t q_bar[2], s_bar[2], p_bar[2], o_bar[2], s_free, full[NS], freeb[NS], drain;
   __shared__ uint32_t tmem_slot;
   __shared__ int primed[2];    // O holds something before the first product
-  __shared__ int span[2][2];  // keys that every row of a tile sees
-  __shared__ int seen[2];     // keys that some row of the unit sees
-  // Between the two threads of a row, by block parity: one may be a block ahead of the
-  // other, except where S waits for both (p over S).
-  __shared__ float xch[C::SEP ? 2 : 1][2][kTpr][128];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const AttnUnit u = a.units[blockIdx.x];
+  const TileSpan sp = a.spans[blockIdx.x];
   const int nt = u.nv > 128 ? 2 : 1, nb = (u.k1 - u.k0 + B - 1) / B;
 
   if (warp == kSoftWarps) {
@@ -254,30 +243,26 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
   }
   if (tid == 0) {
     for (int t = 0; t < 2; ++t) {
-      mbar_init(&q_bar[t], NSOFT);
+      mbar_init(&q_bar[t], 128);
       mbar_init(&s_bar[t], 1);
-      mbar_init(&p_bar[t], NSOFT);
+      mbar_init(&p_bar[t], 128);
       mbar_init(&o_bar[t], 1);
       primed[t] = 0;
-      span[t][0] = 0;
-      span[t][1] = 0x7fffffff;
     }
     for (int i = 0; i < NS; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&freeb[i], 1);
     }
     mbar_init(&drain, 1);
-    mbar_init(&s_free, NSOFT);
-    seen[0] = 0x7fffffff;
-    seen[1] = 0;
+    mbar_init(&s_free, 128);
     fence_barrier_init();
   }
   tc_before();
   __syncthreads();
   tc_after();
   const uint32_t tmem = tmem_slot;
-  // softmax warps: this thread has row tr of its tile and half of a block's keys
-  const int tile = warp / (4 * kTpr), half = kTpr == 1 ? 0 : (warp >> 2) & 1, tr = (warp & 3) * 32 + lane, vec_id = tile * 128 + tr;
+  // softmax warps: this thread has row tr of its tile
+  const int tile = warp >> 2, tr = (warp & 3) * 32 + lane, vec_id = tile * 128 + tr;
   RowInfo r{0, 0, 0x7fffffff, 0};
   int head = 0, row = 0;
   const bool active = warp < kSoftWarps && vec_id < u.nv;
@@ -286,14 +271,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
     row = u.row0 + v / a.n_rep;
     head = u.kvh * a.n_rep + v % a.n_rep;
     r = a.rows[row];
-    atomicMax(&span[tile][0], r.lo);
-    atomicMin(&span[tile][1], r.hi);
-    if (r.hi > r.lo) {
-      atomicMin(&seen[0], r.lo);
-      atomicMax(&seen[1], r.hi);
-    }
   }
-  __syncthreads();
 
   if (warp >= kSoftWarps + 2) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegRest));
@@ -395,95 +373,110 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
   } else if (tile < nt) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegSoft));
     // ---- softmax ----
-    const int d_begin = half * (HD / kTpr), d_end = d_begin + HD / kTpr;  // this thread's part of O
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t ts = lane_base + C::S0 + tile * C::SW + half * H, to = lane_base + tile * HD,
+    const uint32_t ts = lane_base + C::S0 + tile * C::SW, to = lane_base + tile * HD,
                    tp = lane_base + C::P0 + tile * C::PW;
     bool alive = true;
     float sv = fabsf(a.scale);
-    {  // q into shared memory, K-major with 128-byte swizzle; a negative scale turns q
+    // This warp's 32 rows move between global memory and shared memory 16 bytes a lane,
+    // whole rows at a time: a lane per row would touch 32 lines with every access.
+    // Chunk ch (16 bytes) of row tr in part `part` of the tile's q, K-major with swizzle:
+    uint8_t* const q_tile = smem + tile * (1 + HL) * C::QT;
+    auto chunk_at = [&](int row_, int part, int ch) {
+      return reinterpret_cast<uint4*>(q_tile + part * C::QT + (ch >> 3) * C::PANEL + row_ * 128 +
+                                      (((ch & 7) ^ (row_ & 7)) << 4));
+    };
+    const int w0 = (warp & 3) * 32;  // the warp's first row
+    constexpr int ESZ = HL ? 4 : 2, NCH = HD * ESZ / 16, LPR = NCH, RPI = 32 / LPR;  // lanes a row, rows an access
+    const int sub = lane / LPR, ch = lane % LPR;
+    {  // q; a negative scale turns it
+      const unsigned long long mine =
+          active ? (unsigned long long)a.q + ((size_t)row * a.ldq + (size_t)head * HD) * ESZ : 0ull;
+      const bool vec = ((reinterpret_cast<uintptr_t>(a.q) | (size_t)a.ldq * ESZ) & 15) == 0;
       const float sign = a.scale < 0.f ? -1.f : 1.f;
-      uint8_t* qd = smem + tile * (1 + HL) * C::QT + tr * 128;
-      const size_t at = (size_t)row * a.ldq + (size_t)head * HD;
-      const int rx = tr & 7;
-      if (HL) {
-        const float* q = reinterpret_cast<const float*>(a.q) + at;
-        const bool vec = ((reinterpret_cast<uintptr_t>(a.q) | (size_t)a.ldq * 4) & 15) == 0;
-        float top = 0.f;
-        if (active)
-          for (int d = 0; d < HD; d += 4) {
-            if (vec) {
-              const float4 x = *reinterpret_cast<const float4*>(q + d);
-              top = fmaxf(fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
-            } else {
-              for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(q[d + e]));
-            }
-          }
-        float mul = 1.f;
-        const int e = (int)(__float_as_uint(top) >> 23);
-        if (e > 8 && e < 255) mul = __uint_as_float((uint32_t)min(254, 127 + 8 + 127 - e) << 23);
-        sv = sv / mul;
-        mul *= sign;
-        for (int ch = d_begin / 8; ch < d_end / 8; ++ch) {
-          float x[8];
-          if (active && vec) {
-            *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(q + ch * 8);
-            *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(q + ch * 8 + 4);
-          } else {
-            for (int i = 0; i < 8; ++i) x[i] = active ? q[ch * 8 + i] : 0.f;
-          }
-          uint4 hi, lo;
-          uint32_t* h = &hi.x;
-          uint32_t* l = &lo.x;
+      const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+      float my_mul = 1.f;
+#pragma unroll 1
+      for (int i0 = 0; i0 < 32; i0 += 8 * RPI) {
+        uint4 raw[8];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            x[2 * i] *= mul;
-            x[2 * i + 1] *= mul;
-            h[i] = pack2(x[2 * i], x[2 * i + 1]);
-            l[i] = pack2_lo(x[2 * i], x[2 * i + 1], h[i]);
-          }
-          uint8_t* dst = qd + (ch >> 3) * C::PANEL + (((ch & 7) ^ rx) << 4);
-          *reinterpret_cast<uint4*>(dst) = hi;
-          *reinterpret_cast<uint4*>(dst + HL * C::QT) = lo;
-        }
-      } else {
-        const __half* q = reinterpret_cast<const __half*>(a.q) + at;
-        const bool vec = ((reinterpret_cast<uintptr_t>(a.q) | (size_t)a.ldq * 2) & 15) == 0;
-        const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
-        for (int ch = d_begin / 8; ch < d_end / 8; ++ch) {
-          uint4 x = make_uint4(0, 0, 0, 0);
-          if (active) {
+        for (int i = 0; i < 8; ++i) {
+          const unsigned long long p = __shfl_sync(0xffffffffu, mine, i0 + i * RPI + sub);
+          raw[i] = make_uint4(0, 0, 0, 0);
+          if (p) {
             if (vec) {
-              x = *reinterpret_cast<const uint4*>(q + ch * 8);
+              raw[i] = reinterpret_cast<const uint4*>(p)[ch];
+            } else if (HL) {
+              const uint32_t* q = reinterpret_cast<const uint32_t*>(p) + 4 * ch;
+              raw[i] = make_uint4(q[0], q[1], q[2], q[3]);
             } else {
-              uint16_t* h = reinterpret_cast<uint16_t*>(&x);
-              for (int i = 0; i < 8; ++i) h[i] = __half_as_ushort(q[ch * 8 + i]);
+              const uint16_t* q = reinterpret_cast<const uint16_t*>(p) + 8 * ch;
+              raw[i] = make_uint4(q[0] | (uint32_t)q[1] << 16, q[2] | (uint32_t)q[3] << 16,
+                                  q[4] | (uint32_t)q[5] << 16, q[6] | (uint32_t)q[7] << 16);
             }
           }
-          x.x ^= flip;
-          x.y ^= flip;
-          x.z ^= flip;
-          x.w ^= flip;
-          *reinterpret_cast<uint4*>(qd + (ch >> 3) * C::PANEL + (((ch & 7) ^ rx) << 4)) = x;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int rr = i0 + i * RPI + sub;  // of the warp's rows
+          if (HL) {
+            float x[4] = {__uint_as_float(raw[i].x), __uint_as_float(raw[i].y), __uint_as_float(raw[i].z),
+                          __uint_as_float(raw[i].w)};
+            float top = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+#pragma unroll
+            for (int o = LPR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            float mul = 1.f;  // 2^(8 - exponent of top), for normal finite tops
+            const int e = (int)(__float_as_uint(top) >> 23);
+            if (e > 8 && e < 255) mul = __uint_as_float((uint32_t)min(254, 127 + 8 + 127 - e) << 23);
+#pragma unroll
+            for (int q = 0; q < RPI; ++q) {
+              const float m = __shfl_sync(0xffffffffu, mul, q * LPR);
+              if (lane == i0 + i * RPI + q) my_mul = m;
+            }
+            mul *= sign;
+            uint2 hi, lo;
+            hi.x = pack2(x[0] * mul, x[1] * mul);
+            hi.y = pack2(x[2] * mul, x[3] * mul);
+            lo.x = pack2_lo(x[0] * mul, x[1] * mul, hi.x);
+            lo.y = pack2_lo(x[2] * mul, x[3] * mul, hi.y);
+            reinterpret_cast<uint2*>(chunk_at(w0 + rr, 0, ch >> 1))[ch & 1] = hi;
+            reinterpret_cast<uint2*>(chunk_at(w0 + rr, HL, ch >> 1))[ch & 1] = lo;
+          } else {
+            raw[i].x ^= flip;
+            raw[i].y ^= flip;
+            raw[i].z ^= flip;
+            raw[i].w ^= flip;
+            *chunk_at(w0 + rr, 0, ch) = raw[i];
+          }
         }
       }
+      if (HL) sv /= my_mul;
       proxy_fence();
       mbar_arrive(&q_bar[tile]);
     }
-    const int all0 = span[tile][0], all1 = span[tile][1], in0 = seen[0], in1 = seen[1];
-    const int both0 = max(span[0][0], span[1][0]), both1 = min(span[0][1], span[1][1]);
+    const int all0 = sp.all0[tile], all1 = sp.all1[tile], in0 = sp.in0, in1 = sp.in1;
+    const int both0 = max(sp.all0[0], sp.all0[1]), both1 = min(sp.all1[0], sp.all1[1]);
     const float slope = BIAS && active ? a.slopes[head] * kLog2e : 0.f;
     const float cap2 = a.cap * kLog2e, kcap = CAP ? sv / a.cap : 0.f;
     const float mult = (CAP || BIAS) ? 1.f : fmaxf(sv * kLog2e, 1e-30f);  // scores to base-2 units (-inf stays)
     const float sv2 = sv * kLog2e;
+    // coefficients of the fused form, for fp16 rows in powers of the raw score (kept normal)
+    float coef[Fused<HL>::N];
+    float kp = HL ? cap2 : cap2 * kcap;
+#pragma unroll
+    for (int q = 0; q < Fused<HL>::N; ++q) {
+      coef[q] = kp * Fused<HL>::c(q);
+      if (!HL) kp *= kcap * kcap;
+    }
+    const bool fuse_ok = HL || (kcap > 1e-6f && kcap < 1e4f && cap2 < 1e6f);
     float m = -INFINITY, l = 0.f;
     for (int j = 0; j < nb; ++j) {
-      const int kb = u.k0 + j * B, kh = kb + half * H;  // the block's first key, and this thread's
+      const int kb = u.k0 + j * B;
       if (alive) alive = mbar_wait(&s_bar[tile], (uint32_t)(j & 1), a.err, DEV_TIMEOUT_FULL);
       tc_after();
-      float x[H];
+      float x[B];
 #pragma unroll
-      for (int i = 0; i < H / 32; ++i) ld32(ts + 32 * i, x + 32 * i);
+      for (int i = 0; i < B / 32; ++i) ld32(ts + 32 * i, x + 32 * i);
       wait_ld();
       if (C::SEP) {
         tc_before();
@@ -491,64 +484,72 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
       }
       const bool partial = kb < all0 || kb + B > all1;  // the same for the whole tile
       bool fused = false;  // the cap is applied together with the exponential
-      float raw_top = 0.f;
       if (CAP) {
-        // the largest magnitude, from both ends: the maximum is wanted anyway
-        float lo4[4] = {0.f, 0.f, 0.f, 0.f}, hi4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        // the largest magnitude of the warp's scores, unseen keys' included
+        float lo4[4] = {0.f, 0.f, 0.f, 0.f}, hi4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < H; i += 8)
+        for (int i = 0; i < B; i += 8)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            lo4[q] = min3(lo4[q], x[i + 2 * q], x[i + 2 * q + 1]);
-            hi4[q] = max3(hi4[q], x[i + 2 * q], x[i + 2 * q + 1]);
-          }
-        const float lo = min3(fminf(lo4[0], lo4[1]), lo4[2], lo4[3]);
-        raw_top = max3(fmaxf(hi4[0], hi4[1]), hi4[2], hi4[3]);
-        fused = !BIAS && !partial && __all_sync(0xffffffffu, fmaxf(raw_top, -lo) * kcap <= Tanh<HL>::limit);
+          for (int q = 0; q < 4; ++q) lo4[q] = min3(lo4[q], x[i + 2 * q], x[i + 2 * q + 1]);
+#pragma unroll
+        for (int i = 0; i < B; i += 8)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) hi4[q] = max3(hi4[q], x[i + 2 * q], x[i + 2 * q + 1]);
+        const float top = fmaxf(max3(fmaxf(hi4[0], hi4[1]), hi4[2], hi4[3]),
+                                -min3(fminf(lo4[0], lo4[1]), lo4[2], lo4[3]));
+        fused = !BIAS && fuse_ok && __all_sync(0xffffffffu, top * kcap <= Fused<HL>::limit);
         if (!fused) {
-          // cap tanh(y) = cap - 2 cap / (1 + e^(2 y))
-          const float k = 2.f * kLog2e * kcap;
+          if (__all_sync(0xffffffffu, top * kcap <= Wide::limit)) {
+            const f2 k2 = pair(kcap, kcap);
 #pragma unroll
-          for (int i = 0; i < H; ++i) x[i] = fmaf(-2.f * cap2, rcp(1.f + ex2(x[i] * k)), cap2);
+            for (int i = 0; i < B; i += 2) {
+              const f2 y = mul2(pair(x[i], x[i + 1]), k2), z = mul2(y, y);
+              f2 t = pair(cap2 * Wide::c(Wide::N - 1), cap2 * Wide::c(Wide::N - 1));
+#pragma unroll
+              for (int q = Wide::N - 2; q >= 0; --q) t = fma2(t, z, pair(cap2 * Wide::c(q), cap2 * Wide::c(q)));
+              unpair(mul2(t, y), x[i], x[i + 1]);
+            }
+          } else {
+            // cap tanh(y) = cap - 2 cap / (1 + e^(2 y))
+            const float k = 2.f * kLog2e * kcap;
+#pragma unroll
+            for (int i = 0; i < B; ++i) x[i] = fmaf(-2.f * cap2, rcp(1.f + ex2(x[i] * k)), cap2);
+          }
         }
       }
       if (BIAS) {
-        if (__all_sync(0xffffffffu, kh + H - 1 <= r.pos)) {  // no key after its row: the distance is linear
+        if (__all_sync(0xffffffffu, kb + B - 1 <= r.pos)) {  // no key after its row: the distance is linear
           const f2 sl = pair(slope, slope), s2 = pair(CAP ? 1.f : sv2, CAP ? 1.f : sv2);
-          const float b0 = slope * (float)(kh - r.pos);
+          const float b0 = slope * (float)(kb - r.pos);
           const f2 b2 = pair(b0, b0);
 #pragma unroll
-          for (int i = 0; i < H; i += 2)
+          for (int i = 0; i < B; i += 2)
             unpair(fma2(pair(x[i], x[i + 1]), s2, fma2(pair((float)i, (float)(i + 1)), sl, b2)), x[i], x[i + 1]);
         } else {
 #pragma unroll
-          for (int i = 0; i < H; ++i)
-            x[i] = fmaf(-slope, fabsf((float)(r.pos - kh - i)), CAP ? x[i] : x[i] * sv2);
+          for (int i = 0; i < B; ++i)
+            x[i] = fmaf(-slope, fabsf((float)(r.pos - kb - i)), CAP ? x[i] : x[i] * sv2);
         }
       }
       if (partial) {
-        const uint32_t base = (uint32_t)(kh - r.lo), n = (uint32_t)max(0, r.hi - r.lo);
+        const int lo = r.lo - kb, hi = max(r.hi, r.lo) - kb;
+        if (__any_sync(0xffffffffu, hi < B)) {
 #pragma unroll
-        for (int i = 0; i < H; ++i) x[i] = base + i < n ? x[i] : -INFINITY;
-      }
-      float mx;
-      if (CAP && fused) {
-        // the cap keeps the order: it is applied to the maximum alone
-        mx = fmaf(-2.f * cap2, rcp(1.f + ex2(raw_top * (2.f * kLog2e * kcap))), cap2);
-      } else {
-        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          for (int i = 0; i < B; ++i) x[i] = i < hi ? x[i] : -INFINITY;
+        }
+        if (__any_sync(0xffffffffu, lo > 0)) {
 #pragma unroll
-        for (int i = 0; i < H; i += 8)
+          for (int i = 0; i < B; ++i) x[i] = i >= lo ? x[i] : -INFINITY;
+        }
+      }
+      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int q = 0; q < 4; ++q) mx4[q] = max3(mx4[q], x[i + 2 * q], x[i + 2 * q + 1]);
-        mx = max3(fmaxf(mx4[0], mx4[1]), mx4[2], mx4[3]) * mult;
-      }
-      if (kTpr == 2) {  // the row's other thread
-        float(*xb)[128] = xch[C::SEP ? j & 1 : 0][tile];
-        xb[half][tr] = mx;
-        asm volatile("bar.sync %0, 64;" ::"r"(2 + tile * 4 + (warp & 3)) : "memory");
-        mx = fmaxf(mx, xb[half ^ 1][tr]);
-      }
+      for (int i = 0; i < B; i += 8)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) mx4[q] = max3(mx4[q], x[i + 2 * q], x[i + 2 * q + 1]);
+      float mx = max3(fmaxf(mx4[0], mx4[1]), mx4[2], mx4[3]) * mult;
+      // the cap keeps the order: where it is fused, it is applied to the maximum alone
+      if (CAP && fused && mx != -INFINITY) mx = fmaf(-2.f * cap2, rcp(1.f + ex2(mx * (2.f * kLog2e * kcap))), cap2);
       // each row raises its maximum by its own scores alone
       const bool up = mx > (m == -INFINITY ? m : m + kSlack);
       float alpha = 1.f;
@@ -563,7 +564,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
       }
       if (__any_sync(0xffffffffu, up) && j > 0) {
 #pragma unroll 1
-        for (int d = d_begin; d < d_end; d += 32) {
+        for (int d = 0; d < HD; d += 32) {
           float o[32];
           ld32(to + d, o);
           wait_ld();
@@ -575,17 +576,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
       const float off = kBias - (m == -INFINITY ? 0.f : m);
       const f2 mult2 = pair(mult, mult), off2 = pair(off, off);
       f2 s2[2] = {0ull, 0ull};
-      // Groups of 2 G keys, every step for the whole group before the next one: the
+      // Groups of 16 keys, every step for the whole group before the next one: the
       // steps of a key wait for one another, the keys do not.
       auto exps = [&](auto capped) {
         constexpr bool FUSED = decltype(capped)::value;
-        using P = Tanh<HL>;
+        using P = Fused<HL>;
         f2 pc[P::N];
 #pragma unroll
-        for (int q = 0; q < P::N; ++q) pc[q] = pair(cap2 * P::c(q), cap2 * P::c(q));
-        constexpr int G = kTpr == 1 ? 8 : 4;  // pairs
+        for (int q = 0; q < P::N; ++q) pc[q] = pair(coef[q], coef[q]);
+        constexpr int G = 8;  // pairs
 #pragma unroll
-        for (int i = 0; i < H / 32; ++i) {
+        for (int i = 0; i < B / 32; ++i) {
           uint32_t hi[16], lo[16];
 #pragma unroll
           for (int h = 0; h < 16 / G; ++h) {
@@ -594,10 +595,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
 #pragma unroll
             for (int g = 0; g < G; ++g) y[g] = pair(x[32 * i + 2 * G * h + 2 * g], x[32 * i + 2 * G * h + 2 * g + 1]);
             if (FUSED) {
-              const f2 k2 = pair(kcap, kcap);
               f2 z[G], t[G];
+              if (HL) {  // rows have scales of their own, too far apart for powers of them
+                const f2 k2 = pair(kcap, kcap);
 #pragma unroll
-              for (int g = 0; g < G; ++g) y[g] = mul2(y[g], k2);
+                for (int g = 0; g < G; ++g) y[g] = mul2(y[g], k2);
+              }
 #pragma unroll
               for (int g = 0; g < G; ++g) z[g] = mul2(y[g], y[g]);
 #pragma unroll
@@ -627,8 +630,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
 #pragma unroll
               for (int g = 0; g < G; ++g) lo[G * h + g] = pack2_lo(e[2 * g], e[2 * g + 1], hi[G * h + g]);
           }
-          st16(tp + C::pcol(half * (H / 16) + 2 * i, 0), hi);
-          if (HL) st16(tp + C::pcol(half * (H / 16) + 2 * i, 1), lo);
+          st16(tp + C::pcol(2 * i, 0), hi);
+          if (HL) st16(tp + C::pcol(2 * i, 1), lo);
         }
       };
       if (CAP && fused) exps(Flag<true>());
@@ -647,10 +650,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
         if (alive) alive = mbar_wait(&full[vs], (uint32_t)(((2 * j + 1) / NS) & 1), a.err, DEV_TIMEOUT_FULL);
         uint8_t* vrow = ring + vs * C::SLOT + tr * 128;
         const bool in = kb + tr >= in0 && kb + tr < in1;
-        const int nc = HD / 8 / kTpr / nt, c0 = (tile * kTpr + half) * nc, c1 = c0 + nc;  // the threads of a key share its chunks
+        // Each tile looks at the whole block; both find the same, so that they meet below
+        // only where something has to be mended.
         uint32_t bad = 0;
-        for (int ch = c0; ch < c1; ++ch) {
-          uint4* p = reinterpret_cast<uint4*>(vrow + (ch >> 3) * C::PANEL + ((ch & 7) << 4));
+#pragma unroll
+        for (int ch = 0; ch < HD / 8; ++ch) {
+          uint4* p = reinterpret_cast<uint4*>(vrow + (ch >> 3) * C::PANEL + (((ch & 7) ^ (tr & 7)) << 4));
           if (in) {
             const uint4 q = *p;
             bad |= not_finite(q.x) | not_finite(q.y) | not_finite(q.z) | not_finite(q.w);
@@ -661,10 +666,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
         proxy_fence();
         wait_st();
         tc_before();
-        if (any_softmax(NSOFT * nt, bad != 0)) {
+        if (any_softmax(2 + tile, 128, bad != 0)) {
           tc_after();
 #pragma unroll 1
-          for (int d = d_begin; d < d_end; d += 32) {
+          for (int d = 0; d < HD; d += 32) {
             float o[32];
             ld32(to + d, o);
             wait_ld();
@@ -697,9 +702,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
             }
             st32(to + d, reinterpret_cast<uint32_t*>(o));
           }
-          any_softmax(NSOFT * nt, false);  // all rows have taken theirs
-          for (int ch = c0; ch < c1; ++ch) {
-            uint4* p = reinterpret_cast<uint4*>(vrow + (ch >> 3) * C::PANEL + ((ch & 7) << 4));
+          any_softmax(1, 128 * nt, false);  // all rows have taken theirs
+          for (int ch = tile * (HD / 8 / nt); ch < (tile + 1) * (HD / 8 / nt); ++ch) {
+            uint4* p = reinterpret_cast<uint4*>(vrow + (ch >> 3) * C::PANEL + (((ch & 7) ^ (tr & 7)) << 4));
             uint32_t* w = reinterpret_cast<uint32_t*>(p);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -708,8 +713,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
             }
           }
           proxy_fence();
-          any_softmax(NSOFT * nt, false);
-          if (tr == 0 && half == 0 && j == 0) *(volatile int*)&primed[tile] = 1;
+          any_softmax(1, 128 * nt, false);
+          if (tr == 0 && j == 0) *(volatile int*)&primed[tile] = 1;
         }
       }
       wait_st();
@@ -720,56 +725,72 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
       if (alive) alive = mbar_wait(&o_bar[tile], (uint32_t)((nb - 1) & 1), a.err, DEV_TIMEOUT_DRAIN);
       tc_after();
     }
-    if (kTpr == 2) {
-      xch[0][tile][half][tr] = l;  // all maxima are read: the last P V had both threads' p
-      asm volatile("bar.sync %0, 64;" ::"r"(2 + tile * 4 + (warp & 3)) : "memory");
-      l = xch[0][tile][0][tr] + xch[0][tile][kTpr - 1][tr];
-    }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int slot = u.slot + vec_id;
-    if (u.slot >= 0 && active && half == 0) a.part_ml[slot] = make_float2(m, l);
-    const size_t at = (size_t)row * a.ldo + (size_t)head * HD;
-    const bool vec = ((reinterpret_cast<uintptr_t>(a.out) | (size_t)a.ldo * (HL ? 4 : 2)) & 15) == 0;
+    const bool part = u.slot >= 0;
+    if (part && active) a.part_ml[u.slot + vec_id] = make_float2(m, l);
+    // O through the tile's place of q, which no product reads any more. Parts stay
+    // unnormalised in fp32; fp16 rows have room for half of such a row at a time.
+    const int out_esz = part || HL ? 4 : 2, passes = part && !HL ? 2 : 1, nd = HD / passes;
+    const unsigned long long mine =
+        !active ? 0ull
+        : part  ? (unsigned long long)(a.part_o + (size_t)(u.slot + vec_id) * HD)
+                : (unsigned long long)a.out + ((size_t)row * a.ldo + (size_t)head * HD) * ESZ;
+    const bool vec = part || ((reinterpret_cast<uintptr_t>(a.out) | (size_t)a.ldo * ESZ) & 15) == 0;
 #pragma unroll 1
-    for (int d = d_begin; d < d_end; d += 32) {
-      float o[32];
-      ld32(to + d, o);
-      wait_ld();
-      if (nb == 0 || l == 0.f)
+    for (int pass = 0; pass < passes; ++pass) {
+#pragma unroll 1
+      for (int d = 0; d < nd; d += 32) {
+        float o[32];
+        ld32(to + pass * nd + d, o);
+        wait_ld();
+        if (nb == 0 || l == 0.f)
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = 0.f;
-      if (!active) continue;
-      if (u.slot >= 0) {
-        float4* dst = reinterpret_cast<float4*>(a.part_o + (size_t)slot * HD + d);
+          for (int i = 0; i < 32; ++i) o[i] = 0.f;
+        if (!part)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-      } else if (HL) {
-        float* dst = reinterpret_cast<float*>(a.out) + at + d;
+          for (int i = 0; i < 32; ++i) o[i] *= inv;
+        if (out_esz == 4) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] *= inv;
-        if (vec) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            reinterpret_cast<float4*>(dst)[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          for (int i = 0; i < 8; ++i) {
+            const int c = d / 4 + i;
+            *chunk_at(tr, c / (HD / 8), c % (HD / 8)) =
+                make_uint4(__float_as_uint(o[4 * i]), __float_as_uint(o[4 * i + 1]), __float_as_uint(o[4 * i + 2]),
+                           __float_as_uint(o[4 * i + 3]));
+          }
         } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) dst[i] = o[i];
-        }
-      } else {
-        __half* dst = reinterpret_cast<__half*>(a.out) + at + d;
-        uint32_t h[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) h[i] = pack2(o[2 * i] * inv, o[2 * i + 1] * inv);
-        if (vec) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            reinterpret_cast<uint4*>(dst)[i] = make_uint4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            dst[i] = __ushort_as_half((unsigned short)((i & 1) ? h[i >> 1] >> 16 : h[i >> 1]));
+            *chunk_at(tr, 0, d / 8 + i) = make_uint4(pack2(o[8 * i], o[8 * i + 1]), pack2(o[8 * i + 2], o[8 * i + 3]),
+                                                     pack2(o[8 * i + 4], o[8 * i + 5]), pack2(o[8 * i + 6], o[8 * i + 7]));
         }
       }
+      __syncwarp();
+      const int nch = nd * out_esz / 16;  // chunks a row: 8, 16 or 32
+#pragma unroll 4
+      for (int i = 0; i < nch; ++i) {
+        const int at = i * 32 + lane, rr = at / nch, c = at % nch;
+        const unsigned long long p = __shfl_sync(0xffffffffu, mine, rr);
+        const uint4 v = *chunk_at(w0 + rr, c / (HD / 8), c % (HD / 8));
+        if (!p) continue;
+        if (vec) {
+          reinterpret_cast<uint4*>(p + (size_t)pass * nd * out_esz)[c] = v;
+        } else if (HL) {
+          uint32_t* dst = reinterpret_cast<uint32_t*>(p) + 4 * c;
+          dst[0] = v.x;
+          dst[1] = v.y;
+          dst[2] = v.z;
+          dst[3] = v.w;
+        } else {
+          uint16_t* dst = reinterpret_cast<uint16_t*>(p) + 8 * c;
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            dst[2 * e] = (uint16_t)w[e];
+            dst[2 * e + 1] = (uint16_t)(w[e] >> 16);
+          }
+        }
+      }
+      __syncwarp();
     }
   }
   tc_before();
