@@ -26,9 +26,57 @@ struct VecInfo {
   float slope;
 };
 
-// The last CTA that deposits a part of unit u's item joins all of them, in the order
-// of the keys whichever CTA that is, so the result depends on no order of arrival.
-// Every thread's parts are stored before. Ends with a barrier of the CTA.
+// Joins the parts of vector v of an item for the four elements at d, parts in the order
+// of the keys; their loads do not wait for one another.
+template <int HD, class TO>
+__device__ __forceinline__ void join_vec(const RowAttnArgs& a, const JoinItem& it, int v, int d) {
+  const float2* pml = a.part_ml + it.slot0 + v;
+  const float4* po = reinterpret_cast<const float4*>(a.part_o + (size_t)(it.slot0 + v) * HD + d);
+  float M = -INFINITY, L = 0.f;
+  float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p0 = 0; p0 < it.n_parts; p0 += 8) {
+    float2 ml[8];
+    float4 o[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const bool in = p0 + q < it.n_parts;
+      ml[q] = in ? __ldcg(pml + (size_t)(p0 + q) * it.nv) : make_float2(-INFINITY, 0.f);
+      o[q] = in ? __ldcg(po + (size_t)(p0 + q) * it.nv * (HD / 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float m8 = M;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) m8 = fmaxf(m8, ml[q].x);
+    const float f0 = m8 == -INFINITY ? 1.f : exp2f(M - m8);
+    L *= f0;
+    O.x *= f0;
+    O.y *= f0;
+    O.z *= f0;
+    O.w *= f0;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const float f = m8 == -INFINITY ? 1.f : exp2f(ml[q].x - m8);
+      L += ml[q].y * f;
+      O.x += o[q].x * f;
+      O.y += o[q].y * f;
+      O.z += o[q].z * f;
+      O.w += o[q].w * f;
+    }
+    M = m8;
+  }
+  const float r = L == 0.f ? 0.f : 1.f / L;
+  const float e[4] = {O.x * r, O.y * r, O.z * r, O.w * r};
+  const size_t at = (size_t)(it.row0 + (it.v0 + v) / a.n_rep) * a.ldo +
+                    (size_t)(it.kvh * a.n_rep + (it.v0 + v) % a.n_rep) * HD + d;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if constexpr (sizeof(TO) == 2) reinterpret_cast<__half*>(a.out)[at + q] = __float2half_rn(e[q]);
+    else reinterpret_cast<float*>(a.out)[at + q] = e[q];
+  }
+}
+
+// The last CTA that deposits a part of unit u's item joins all of them, whichever CTA
+// that is, so the result depends on no order of arrival. Every thread's parts are
+// stored before. Ends with a barrier of the CTA.
 template <int HD, class TO>
 __device__ void join_last(const RowAttnArgs& a, const AttnUnit& u) {
   __shared__ int last;
@@ -39,54 +87,9 @@ __device__ void join_last(const RowAttnArgs& a, const AttnUnit& u) {
     if (last) a.counters[u.join] = 0;
   }
   __syncthreads();
-  if (last) {
-    // a thread has four elements of one vector; the parts' loads do not wait for one another
-    for (int i = threadIdx.x; i < it.nv * (HD / 4); i += blockDim.x) {
-      const int v = i / (HD / 4), d = i % (HD / 4) * 4;
-      const float2* pml = a.part_ml + it.slot0 + v;
-      const float4* po = reinterpret_cast<const float4*>(a.part_o + (size_t)(it.slot0 + v) * HD + d);
-      float M = -INFINITY, L = 0.f;
-      float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int p0 = 0; p0 < it.n_parts; p0 += 8) {
-        float2 ml[8];
-        float4 o[8];
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const bool in = p0 + q < it.n_parts;
-          ml[q] = in ? __ldcg(pml + (size_t)(p0 + q) * it.nv) : make_float2(-INFINITY, 0.f);
-          o[q] = in ? __ldcg(po + (size_t)(p0 + q) * it.nv * (HD / 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-        float m8 = M;
-#pragma unroll
-        for (int q = 0; q < 8; ++q) m8 = fmaxf(m8, ml[q].x);
-        const float f0 = m8 == -INFINITY ? 1.f : exp2f(M - m8);
-        L *= f0;
-        O.x *= f0;
-        O.y *= f0;
-        O.z *= f0;
-        O.w *= f0;
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const float f = m8 == -INFINITY ? 1.f : exp2f(ml[q].x - m8);
-          L += ml[q].y * f;
-          O.x += o[q].x * f;
-          O.y += o[q].y * f;
-          O.z += o[q].z * f;
-          O.w += o[q].w * f;
-        }
-        M = m8;
-      }
-      const float r = L == 0.f ? 0.f : 1.f / L;
-      const float e[4] = {O.x * r, O.y * r, O.z * r, O.w * r};
-      const size_t at = (size_t)(it.row0 + (it.v0 + v) / a.n_rep) * a.ldo +
-                        (size_t)(it.kvh * a.n_rep + (it.v0 + v) % a.n_rep) * HD + d;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if constexpr (sizeof(TO) == 2) reinterpret_cast<__half*>(a.out)[at + q] = __float2half_rn(e[q]);
-        else reinterpret_cast<float*>(a.out)[at + q] = e[q];
-      }
-    }
-  }
+  if (last)
+    for (int i = threadIdx.x; i < it.nv * (HD / 4); i += blockDim.x)
+      join_vec<HD, TO>(a, it, i / (HD / 4), i % (HD / 4) * 4);
   __syncthreads();
 }
 
@@ -682,28 +685,12 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) rows_mma_kernel(const __gri
   }
 }
 
-// Joins the parts of a tile item: a CTA for every 32nd vector, parts in order.
-template <int HD>
-__global__ void __launch_bounds__(HD) rows_join_kernel(const __grid_constant__ RowAttnArgs a) {
+// Joins the parts of the tile items.
+template <int HD, class TO>
+__global__ void __launch_bounds__(256) rows_join_kernel(const __grid_constant__ RowAttnArgs a) {
   const JoinItem it = a.joins[a.n_small_joins + blockIdx.x];
-  const int d = threadIdx.x;
-  for (int v = blockIdx.y; v < it.nv; v += gridDim.y) {
-    float M = -INFINITY;
-    for (int p = 0; p < it.n_parts; ++p) M = fmaxf(M, a.part_ml[it.slot0 + p * it.nv + v].x);
-    float L = 0.f, O = 0.f;
-    for (int p = 0; p < it.n_parts; ++p) {
-      const int s = it.slot0 + p * it.nv + v;
-      const float2 ml = a.part_ml[s];
-      const float f = M == -INFINITY ? 1.f : exp2f(ml.x - M);
-      L += ml.y * f;
-      O += a.part_o[(size_t)s * HD + d] * f;
-    }
-    const float r = L == 0.f ? 0.f : M == -INFINITY ? L : O / L;
-    const int row = it.row0 + (it.v0 + v) / a.n_rep, head = it.kvh * a.n_rep + (it.v0 + v) % a.n_rep;
-    const size_t at = (size_t)row * a.ldo + (size_t)head * HD + d;
-    if (a.q16) reinterpret_cast<__half*>(a.out)[at] = __float2half_rn(r);
-    else reinterpret_cast<float*>(a.out)[at] = r;
-  }
+  const int v = blockIdx.y * (256 / (HD / 4)) + threadIdx.x / (HD / 4);
+  if (v < it.nv) join_vec<HD, TO>(a, it, v, threadIdx.x % (HD / 4) * 4);
 }
 
 }  // namespace
@@ -751,9 +738,14 @@ cudaError_t rows_small_launch(const RowAttnArgs& a, cudaStream_t s) {
 cudaError_t rows_join_launch(const RowAttnArgs& a, cudaStream_t s) {
   const int n = a.n_joins - a.n_small_joins;
   if (n < 1) return cudaSuccess;
-  const dim3 g(n, 32);
-  if (a.kv.hd == 128) rows_join_kernel<128><<<g, 128, 0, s>>>(a);
-  else rows_join_kernel<64><<<g, 64, 0, s>>>(a);
+  const dim3 g(n, kTileVecs * a.kv.hd / 4 / 256);
+  if (a.kv.hd == 128) {
+    if (a.q16) rows_join_kernel<128, __half><<<g, 256, 0, s>>>(a);
+    else rows_join_kernel<128, float><<<g, 256, 0, s>>>(a);
+  } else {
+    if (a.q16) rows_join_kernel<64, __half><<<g, 256, 0, s>>>(a);
+    else rows_join_kernel<64, float><<<g, 256, 0, s>>>(a);
+  }
   return cudaGetLastError();
 }
 

@@ -96,16 +96,18 @@ void rows_partition(const std::vector<RowInfo>& rows, int n_heads, int n_kv, int
   }
   out.n_small_joins = (int)out.joins.size();
 
-  // tile items: one CTA per unit, the longest first. Items of more blocks than half an
-  // SM's even share are cut, so that the last ones to run do not leave SMs idle, but
-  // not below four blocks: a unit's start and end cost about as much as those.
+  // tile items: one CTA per unit, the longest first. Their keys are cut only where
+  // the items are fewer than the SMs, and not below four blocks: a unit's start and
+  // end cost about as much as those. (Cutting the longest of 256 uneven items as well,
+  // for the balance at the end, took 257 us and 19 us of joining instead of 237 us.)
   if (!tile.empty()) {
     long long blocks = 0;
     for (const Item& it : tile) blocks += (long long)n_kv * std::max(1, blocks_of(it, kTileKeys));
-    const long long seg = std::max<long long>(4, (blocks + 2 * num_sms - 1) / (2 * num_sms));
+    const long long seg = std::max<long long>(4, (blocks + num_sms - 1) / num_sms);
+    const bool cut = (long long)tile.size() * n_kv < num_sms;
     for (const Item& it : tile) {
       const int nb = blocks_of(it, kTileKeys);
-      const int parts = nb > seg ? (int)((nb + seg - 1) / seg) : 1;
+      const int parts = cut && nb > seg ? (int)((nb + seg - 1) / seg) : 1;
       for (int h = 0; h < n_kv; ++h) {
         if (parts > 1) {
           out.joins.push_back({it.row0, it.v0, it.nv, h, out.n_slots, parts});
