@@ -282,7 +282,7 @@ typedef struct rb_attention_desc {
 int32_t rb_plan_attention(rb_ctx* ctx, int32_t plan, uint32_t layer, const rb_attention_desc* desc, uint32_t flags);
 /* Test hook, host only: the work lists for rows [n_rows][4] (position, first key,
  * one past the last, tenant) as rb_plan_create makes them. Writes at most cap units
- * of 10 values (kernel 0 small / 1 tile, CTA, row0, v0, nv, kv head, tenant, k0, k1,
+ * of 10 values (kernel 0 small / 1 tile, its warp / CTA, row0, v0, nv, kv head, tenant, k0, k1,
  * slot) and returns their number. */
 int32_t rb_plan_partition(uint32_t n_rows, const int32_t* rows, uint32_t n_heads, uint32_t n_kv, uint32_t num_sms,
                           int32_t f16_cache, int32_t* units, uint32_t cap);

@@ -282,8 +282,8 @@ struct RowPlanTenant {
 struct RowSet {
   int pool = -1, n_heads = 0, n_rows = 0, max_pos = 0;
   std::vector<RowPlanTenant> tenants;
-  int n_cta = 0, n_tile = 0, n_joins = 0, n_small_joins = 0, max_nv = 0;
-  DevBuf rows, small, cta, tile, spans, joins, counters, part_o, part_ml;
+  int n_warps = 0, n_tile = 0, n_joins = 0, join_nv = 0, max_nv = 0;
+  DevBuf rows, small, warps, tile, spans, joins, part_o, part_ml;
 };
 
 struct Ctx {
@@ -2249,8 +2249,8 @@ int32_t rb_plan_partition(uint32_t n_rows, const int32_t* rows, uint32_t n_heads
     }
     ++n;
   };
-  for (size_t b = 0; b + 1 < w.small_cta.size(); ++b)
-    for (int i = w.small_cta[b]; i < w.small_cta[b + 1]; ++i) put(0, (int)b, w.small[i]);
+  for (size_t b = 0; b + 1 < w.small_warp.size(); ++b)
+    for (int i = w.small_warp[b]; i < w.small_warp[b + 1]; ++i) put(0, (int)b, w.small[i]);
   for (size_t i = 0; i < w.tile.size(); ++i) put(1, (int)i, w.tile[i]);
   return (int32_t)n;
 }
@@ -2296,18 +2296,17 @@ int32_t rb_plan_create(rb_ctx* c, int32_t pool, const rb_plan_desc* d, int32_t* 
     want.push_back({r.tenant, std::max(r.hi, S->tenants[of[r.tenant]].ascending ? r.pos + 1 : 0)});
   RowWork w;
   rows_partition(rows, S->n_heads, P->n_kv, c->num_sms, P->f16 != 0, w);
-  S->n_cta = (int)w.small_cta.size() ? (int)w.small_cta.size() - 1 : 0;
+  S->n_warps = w.small_warp.empty() ? 0 : (int)w.small_warp.size() - 1;
   S->n_tile = (int)w.tile.size();
   S->n_joins = (int)w.joins.size();
-  S->n_small_joins = w.n_small_joins;
+  S->join_nv = w.join_nv;
   S->max_nv = w.max_nv;
   if (int rc = upload_vec(c, S->rows, rows)) return rc;
   if (int rc = upload_vec(c, S->small, w.small)) return rc;
-  if (int rc = upload_vec(c, S->cta, w.small_cta)) return rc;
+  if (int rc = upload_vec(c, S->warps, w.small_warp)) return rc;
   if (int rc = upload_vec(c, S->tile, w.tile)) return rc;
   if (int rc = upload_vec(c, S->spans, w.spans)) return rc;
   if (int rc = upload_vec(c, S->joins, w.joins)) return rc;
-  if (int rc = upload_vec(c, S->counters, std::vector<int32_t>(w.n_small_joins, 0))) return rc;
   if (w.n_slots) {
     if (S->part_o.alloc((size_t)w.n_slots * P->hd * 4) != cudaSuccess ||
         S->part_ml.alloc((size_t)w.n_slots * 8) != cudaSuccess)
@@ -2445,13 +2444,12 @@ int32_t rb_plan_attention(rb_ctx* c, int32_t plan, uint32_t layer, const rb_atte
   a.part_ml = S->part_ml.as<float2>();
   a.err = c->err.as<uint32_t>();
   a.units = S->small.as<AttnUnit>();
-  a.cta = S->cta.as<int32_t>();
-  a.n_cta = S->n_cta;
+  a.warps = S->warps.as<int32_t>();
+  a.n_warps = S->n_warps;
   a.max_nv = S->max_nv;
   a.joins = S->joins.as<JoinItem>();
   a.n_joins = S->n_joins;
-  a.n_small_joins = S->n_small_joins;
-  a.counters = S->counters.as<int32_t>();
+  a.join_nv = S->join_nv;
   RB_CUDA(rows_small_launch(a, c->stream));
   a.units = S->tile.as<AttnUnit>();
   a.n_units = S->n_tile;

@@ -13,6 +13,7 @@ constexpr int kSmallVecs = 8;     // query vectors per item of the small kernels
 constexpr int kTileVecs = 256;    // query vectors per item of the tile kernel (two tiles of 128)
 constexpr int kTileKeys = 128;    // keys per block of the tile kernel
 constexpr int kMaxRep = 64;       // query heads per kv head
+constexpr int kRowWarps = 4;      // warps a CTA of the small kernels, two CTAs an SM
 
 // One row as the kernels see it: the keys [lo, hi) of its tenant (hi <= lo: none).
 struct RowInfo {
@@ -26,7 +27,9 @@ struct RowInfo {
 // whole item and writes the output; else its vectors' partial results go to
 // slot .. slot + nv.
 struct AttnUnit {
-  int32_t row0, v0, nv, kvh, tenant, k0, k1, slot, join;  // join: its entry of the item list, or -1
+  int32_t row0, v0, nv, kvh, tenant, k0, k1, slot;
+  int32_t all0, all1;        // keys that every row of the item sees [all0, all1)
+  int32_t in0, in1;          // and that some row sees [in0, in1)
 };
 
 // An item cut into n_parts units: part p of vector i lies at slot0 + p * nv + i.
@@ -40,14 +43,14 @@ struct TileSpan {
   int32_t all0[2], all1[2], in0, in1;
 };
 
-// Work lists of one plan. CTA b of the small (tile) kernel runs the units
-// [cta[b], cta[b + 1]) of its list.
+// Work lists of one plan. Warp w of the small kernels runs the units
+// [small_warp[w], small_warp[w + 1]), CTA b of the tile kernel unit b.
 struct RowWork {
   std::vector<AttnUnit> small, tile;
   std::vector<TileSpan> spans;       // of the tile units
-  std::vector<int32_t> small_cta;
-  std::vector<JoinItem> joins;       // the small kernels' items first: their last CTA joins them
-  int32_t n_small_joins = 0;
+  std::vector<int32_t> small_warp;
+  std::vector<JoinItem> joins;       // items that were cut
+  int32_t join_nv = 0;               // vectors of the largest of them
   int32_t n_slots = 0;      // partial result vectors
   int32_t max_nv = 0;       // vectors of the largest small item
 };
@@ -75,12 +78,11 @@ struct RowAttnArgs {
   KvView kv;
   const RowInfo* rows = nullptr;
   const AttnUnit* units = nullptr;
-  const int32_t* cta = nullptr;  // small kernels
-  int32_t n_cta = 0, n_units = 0, max_nv = 0;  // max_nv: vectors of the largest small item
+  const int32_t* warps = nullptr;  // small kernels: [n_warps + 1]
+  int32_t n_warps = 0, n_units = 0, max_nv = 0;  // max_nv: vectors of the largest small item
   const TileSpan* spans = nullptr;  // tile kernel
   const JoinItem* joins = nullptr;
-  int32_t n_small_joins = 0, n_joins = 0;
-  int32_t* counters = nullptr;  // [n_small_joins], zero between launches
+  int32_t n_joins = 0, join_nv = 0;  // join_nv: vectors of the largest cut item
   float* part_o = nullptr;   // [n_slots][hd]
   float2* part_ml = nullptr; // [n_slots] (maximum in base-2 units, sum)
   uint32_t* err = nullptr;
@@ -101,11 +103,11 @@ struct RowAppendArgs {
 };
 
 cudaError_t rows_append_launch(const RowAppendArgs& a, int num_sms, cudaStream_t s);
-// the small kernel over a.units / a.cta
+// the small kernel over a.units / a.warps
 cudaError_t rows_small_launch(const RowAttnArgs& a, cudaStream_t s);
 // the tile kernel over a.units (one CTA each)
 cudaError_t rows_tile_launch(const RowAttnArgs& a, cudaStream_t s);
-// joins the tile kernel's items
+// joins the items that were cut, after both
 cudaError_t rows_join_launch(const RowAttnArgs& a, cudaStream_t s);
 
 }  // namespace rb

@@ -5,6 +5,8 @@
 //   s_k = cap tanh(x_k / cap)  (cap 0: s_k = x_k),  s_k -= slope |t - k|,
 //   out = sum_k exp(s_k - m) v_k / sum_k exp(s_k - m),  m = max_k s_k,
 // and 0 for a row that sees no key.
+#include <type_traits>
+
 #include "common.cuh"
 #include "rows.cuh"
 
@@ -12,7 +14,6 @@ namespace rb {
 
 namespace {
 
-constexpr int kRowWarps = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <class T>
@@ -22,170 +23,151 @@ __device__ __forceinline__ float ld_f32(const void* p, size_t i) {
 }
 
 struct VecInfo {
-  int lo, hi, pos, head;
+  int lo, hi, pos;
   float slope;
 };
 
-// Joins the parts of vector v of an item for the four elements at d, parts in the order
-// of the keys; their loads do not wait for one another.
-template <int HD, class TO>
-__device__ __forceinline__ void join_vec(const RowAttnArgs& a, const JoinItem& it, int v, int d) {
-  const float2* pml = a.part_ml + it.slot0 + v;
-  const float4* po = reinterpret_cast<const float4*>(a.part_o + (size_t)(it.slot0 + v) * HD + d);
-  float M = -INFINITY, L = 0.f;
-  float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int p0 = 0; p0 < it.n_parts; p0 += 8) {
-    float2 ml[8];
-    float4 o[8];
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const bool in = p0 + q < it.n_parts;
-      ml[q] = in ? __ldcg(pml + (size_t)(p0 + q) * it.nv) : make_float2(-INFINITY, 0.f);
-      o[q] = in ? __ldcg(po + (size_t)(p0 + q) * it.nv * (HD / 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    float m8 = M;
-#pragma unroll
-    for (int q = 0; q < 8; ++q) m8 = fmaxf(m8, ml[q].x);
-    const float f0 = m8 == -INFINITY ? 1.f : exp2f(M - m8);
-    L *= f0;
-    O.x *= f0;
-    O.y *= f0;
-    O.z *= f0;
-    O.w *= f0;
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const float f = m8 == -INFINITY ? 1.f : exp2f(ml[q].x - m8);
-      L += ml[q].y * f;
-      O.x += o[q].x * f;
-      O.y += o[q].y * f;
-      O.z += o[q].z * f;
-      O.w += o[q].w * f;
-    }
-    M = m8;
+// Vector v of a unit: the row of the call and the query head.
+__device__ __forceinline__ int vec_row(const RowAttnArgs& a, int row0, int v0, int v) { return row0 + (v0 + v) / a.n_rep; }
+__device__ __forceinline__ int vec_head(const RowAttnArgs& a, int kvh, int v0, int v) {
+  return kvh * a.n_rep + (v0 + v) % a.n_rep;
+}
+__device__ __forceinline__ VecInfo vec_info(const RowAttnArgs& a, const AttnUnit& u, int v) {
+  VecInfo w{0, 0, 0, 0.f};
+  if (v < u.nv) {
+    const RowInfo r = a.rows[vec_row(a, u.row0, u.v0, v)];
+    w.lo = r.lo;
+    w.hi = r.hi;
+    w.pos = r.pos;
+    if (a.slopes) w.slope = a.slopes[vec_head(a, u.kvh, u.v0, v)] * kLog2e;
   }
-  const float r = L == 0.f ? 0.f : 1.f / L;
-  const float e[4] = {O.x * r, O.y * r, O.z * r, O.w * r};
-  const size_t at = (size_t)(it.row0 + (it.v0 + v) / a.n_rep) * a.ldo +
-                    (size_t)(it.kvh * a.n_rep + (it.v0 + v) % a.n_rep) * HD + d;
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    if constexpr (sizeof(TO) == 2) reinterpret_cast<__half*>(a.out)[at + q] = __float2half_rn(e[q]);
-    else reinterpret_cast<float*>(a.out)[at + q] = e[q];
-  }
+  return w;
+}
+template <class TO>
+__device__ __forceinline__ void store_out(const RowAttnArgs& a, size_t at, float x) {
+  if constexpr (sizeof(TO) == 2) reinterpret_cast<__half*>(a.out)[at] = __float2half_rn(x);
+  else reinterpret_cast<float*>(a.out)[at] = x;
 }
 
-// The last CTA that deposits a part of unit u's item joins all of them, whichever CTA
-// that is, so the result depends on no order of arrival. Every thread's parts are
-// stored before. Ends with a barrier of the CTA.
-template <int HD, class TO>
-__device__ void join_last(const RowAttnArgs& a, const AttnUnit& u) {
-  __shared__ int last;
-  const JoinItem it = a.joins[u.join];
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    last = atom_add_acq_rel(&a.counters[u.join], 1) == it.n_parts - 1;
-    if (last) a.counters[u.join] = 0;
+// This warp's loads run ahead of its math, over the ends of units: unit pu, key pk.
+struct Ahead {
+  int pu, end, pk, pk1, tenant, kvh;
+  __device__ __forceinline__ void open(const RowAttnArgs& a) {  // the first unit from pu on that has keys
+    for (; pu < end; ++pu) {
+      const AttnUnit& u = a.units[pu];
+      pk = u.k0;
+      pk1 = u.k1;
+      tenant = u.tenant;
+      kvh = u.kvh;
+      if (pk < pk1) return;
+    }
   }
-  __syncthreads();
-  if (last)
-    for (int i = threadIdx.x; i < it.nv * (HD / 4); i += blockDim.x)
-      join_vec<HD, TO>(a, it, i / (HD / 4), i % (HD / 4) * 4);
-  __syncthreads();
-}
+  __device__ __forceinline__ void next(const RowAttnArgs& a) {
+    pk += kRowPage;
+    if (pk >= pk1) {
+      ++pu;
+      open(a);
+    }
+  }
+};
+// The page of a tenant's token k; a warp keeps 32 entries of the table, one a lane.
+struct PageCache {
+  int tenant = -1, first = 0, val = 0;
+  __device__ __forceinline__ int page(const RowAttnArgs& a, int t, int k) {
+    const int p = k >> 4;
+    if (t != tenant || p < first || p >= first + 32) {
+      tenant = t;
+      first = p;
+      const int at = p + (threadIdx.x & 31);
+      val = at < a.kv.ptab_stride ? a.kv.ptab[(size_t)t * a.kv.ptab_stride + at] : 0;
+    }
+    return __shfl_sync(0xffffffffu, val, p - first);
+  }
+};
 
-// fp32 caches: K and V in fp32 on the CUDA cores. Each warp streams every fourth page
-// of its CTA's share through a ring of its own (bulk copies). Scores: lane (j, hh)
-// has key j and half of its elements, starting at chunk j, so that eight lanes meet
-// all banks; P V: a lane owns HD / 32 elements. NVT: the vectors an item of this
+// fp32 caches: K and V in fp32 on the CUDA cores. Each warp streams its share of the
+// pages through a ring of its own (bulk copies, K and V blocks in turn). Scores: lane
+// (j, hh) has key j and half of its elements, starting at chunk j, so that eight lanes
+// meet all banks; P V: a lane owns HD / 32 elements. NV: the vectors an item of this
 // launch may have, so that a query head without others on its kv head (1) does not
 // pay for eight.
 template <int HD>
 struct F32Cfg {
   static constexpr int BLK = 16 * HD * 4;
-  static constexpr int STAGE = 2 * BLK;
-  static constexpr int NST = HD == 128 ? 1 : 3;   // 64 / 96 KB a CTA
-  static constexpr int SMEM = 128 + kRowWarps * NST * STAGE + kRowWarps * NST * 8;
+  static constexpr int NST = HD == 128 ? 3 : 6;   // blocks a warp: 96 KB a CTA
+  static constexpr int SMEM = 128 + kRowWarps * NST * (BLK + 8);
 };
 
 template <int HD, int NV, class TQ>
-__global__ void __launch_bounds__(kRowWarps * 32) rows_f32_kernel(const __grid_constant__ RowAttnArgs a) {
+__global__ void __launch_bounds__(kRowWarps * 32, 2) rows_f32_kernel(const __grid_constant__ RowAttnArgs a) {
   using C = F32Cfg<HD>;
   constexpr int DPL = HD / 32, NST = C::NST, NCH = HD / 8;  // 16-byte chunks in half a key
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 127) & ~uintptr_t(127));
-  __shared__ __align__(16) float qs[NV][HD];
-  __shared__ VecInfo vi[NV];
-  __shared__ float pb[kRowWarps][NV][16];
-  __shared__ float mo[kRowWarps][NV][HD];
-  __shared__ float mm[kRowWarps][NV], ml[kRowWarps][NV];
+  __shared__ __align__(16) float q_all[kRowWarps][NV][HD];
+  __shared__ VecInfo vi_all[kRowWarps][NV];
+  __shared__ float pb_all[kRowWarps][NV][16];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, j = lane & 15, hh = lane >> 4;
+  const int me = blockIdx.x * kRowWarps + warp;
+  pdl_launch_dependents();
+  if (me >= a.n_warps) return;
+  auto qs = q_all[warp];
+  VecInfo* vi = vi_all[warp];
+  auto pb = pb_all[warp];
   const float* pool = reinterpret_cast<const float*>(a.kv.pool);
-  uint8_t* ring = smem + warp * NST * C::STAGE;
-  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + kRowWarps * NST * C::STAGE) + warp * NST;
+  uint8_t* ring = smem + warp * NST * C::BLK;
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + kRowWarps * NST * C::BLK) + warp * NST;
   if (lane == 0) {
     for (int i = 0; i < NST; ++i) mbar_init(&bar[i], 1);
     fence_barrier_init();
   }
   __syncwarp();
-  const int u_begin = a.cta[blockIdx.x], u_end = a.cta[blockIdx.x + 1];
-  int pu = u_begin, pk = 0, pk1 = 0, pten = 0, pkvh = 0;
-  auto open = [&]() {
-    for (; pu < u_end; ++pu) {
-      const AttnUnit u = a.units[pu];
-      pk = u.k0 + 16 * warp;
-      pk1 = u.k1;
-      pten = u.tenant;
-      pkvh = u.kvh;
-      if (pk < pk1) return;
-    }
-  };
-  open();
-  int issued = 0, used = 0;
+  const int u_begin = a.warps[me], u_end = a.warps[me + 1];
+  Ahead ah{u_begin, u_end, 0, 0, 0, 0};
+  PageCache pages;
+  ah.open(a);
+  int issued = 0, used = 0, which = 0;
+  const float* block = nullptr;
   auto issue = [&](int limit) {
-    while (issued < limit && pu < u_end) {
+    while (issued < limit && ah.pu < u_end) {
+      if (which == 0) {
+        const int page = pages.page(a, ah.tenant, ah.pk);
+        block = pool + ((((size_t)page * a.kv.n_layers + a.layer) * 2) * a.kv.n_kv + ah.kvh) * 16 * HD;
+      }
       if (lane == 0) {
-        const int page = a.kv.ptab[(size_t)pten * a.kv.ptab_stride + (pk >> 4)], s = issued % NST;
-        const float* kb = pool + ((((size_t)page * a.kv.n_layers + a.layer) * 2) * a.kv.n_kv + pkvh) * 16 * HD;
-        mbar_arrive_expect_tx(&bar[s], C::STAGE);
-        bulk_g2s(ring + s * C::STAGE, kb, C::BLK, &bar[s]);
-        bulk_g2s(ring + s * C::STAGE + C::BLK, kb + (size_t)a.kv.n_kv * 16 * HD, C::BLK, &bar[s]);
+        const int s = issued % NST;
+        mbar_arrive_expect_tx(&bar[s], C::BLK);
+        bulk_g2s(ring + s * C::BLK, block + (which ? (size_t)a.kv.n_kv * 16 * HD : 0), C::BLK, &bar[s]);
       }
       ++issued;
-      pk += 16 * kRowWarps;
-      if (pk >= pk1) {
-        ++pu;
-        open();
-      }
+      which ^= 1;
+      if (which == 0) ah.next(a);
     }
   };
   issue(NST);
   bool alive = true;
+  // the next block of the ring; done with it: release()
+  auto take = [&]() {
+    const int s = used % NST;
+    if (alive) alive = mbar_wait(&bar[s], (used / NST) & 1, a.err, DEV_TIMEOUT_FULL);
+    return reinterpret_cast<const float*>(ring + s * C::BLK);
+  };
+  auto release = [&]() {
+    __syncwarp();
+    ++used;
+    issue(used + NST);
+  };
   for (int ui = u_begin; ui < u_end; ++ui) {
     const AttnUnit u = a.units[ui];
-    __syncthreads();
-    for (int i = threadIdx.x; i < NV * HD; i += blockDim.x) {
-      const int v = i / HD, d = i % HD;
-      float x = 0.f;
-      if (v < u.nv) {
-        const int row = u.row0 + (u.v0 + v) / a.n_rep, head = u.kvh * a.n_rep + (u.v0 + v) % a.n_rep;
-        x = ld_f32<TQ>(a.q, (size_t)row * a.ldq + (size_t)head * HD + d);
-      }
-      qs[v][d] = x;
+    __syncwarp();
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const size_t at = (size_t)vec_row(a, u.row0, u.v0, v) * a.ldq + (size_t)vec_head(a, u.kvh, u.v0, v) * HD + lane;
+#pragma unroll
+      for (int i = 0; i < DPL; ++i) qs[v][lane + 32 * i] = v < u.nv ? ld_f32<TQ>(a.q, at + 32 * i) : 0.f;
     }
-    if (threadIdx.x < NV) {
-      VecInfo w{0, 0, 0, 0, 0.f};
-      if ((int)threadIdx.x < u.nv) {
-        const int v = u.v0 + threadIdx.x;
-        const RowInfo r = a.rows[u.row0 + v / a.n_rep];
-        w.lo = r.lo;
-        w.hi = r.hi;
-        w.pos = r.pos;
-        w.head = u.kvh * a.n_rep + v % a.n_rep;
-        w.slope = a.slopes ? a.slopes[w.head] : 0.f;
-      }
-      vi[threadIdx.x] = w;
-    }
-    __syncthreads();
+    if (lane < NV) vi[lane] = vec_info(a, u, lane);
+    __syncwarp();
     float m[NV], l[NV], o[NV][DPL];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
@@ -194,12 +176,8 @@ __global__ void __launch_bounds__(kRowWarps * 32) rows_f32_kernel(const __grid_c
 #pragma unroll
       for (int d = 0; d < DPL; ++d) o[v][d] = 0.f;
     }
-    for (int k = u.k0 + 16 * warp; k < u.k1; k += 16 * kRowWarps) {
-      issue(used + NST);
-      const int s = used % NST;
-      if (alive) alive = mbar_wait(&bar[s], (used / NST) & 1, a.err, DEV_TIMEOUT_FULL);
-      const float* kb = reinterpret_cast<const float*>(ring + s * C::STAGE);
-      const float* vb = kb + 16 * HD;
+    for (int k = u.k0; k < u.k1; k += kRowPage) {
+      const float* kb = take();
       float dot[NV];
 #pragma unroll
       for (int v = 0; v < NV; ++v) dot[v] = 0.f;
@@ -213,12 +191,13 @@ __global__ void __launch_bounds__(kRowWarps * 32) rows_f32_kernel(const __grid_c
           dot[v] = fmaf(q.x, kf.x, fmaf(q.y, kf.y, fmaf(q.z, kf.z, fmaf(q.w, kf.w, dot[v]))));
         }
       }
+      release();
       const int key = k + j;
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         float x = (dot[v] + __shfl_xor_sync(0xffffffffu, dot[v], 16)) * a.scale;
         if (a.cap > 0.f) x = a.cap * tanhf(x / a.cap);
-        x = (x - vi[v].slope * fabsf((float)(vi[v].pos - key))) * kLog2e;
+        x = fmaf(x, kLog2e, -vi[v].slope * fabsf((float)(vi[v].pos - key)));
         const bool in = key >= vi[v].lo && key < vi[v].hi;
         // the maximum is raised only when some score passes it; the sums stay per lane
         if (__any_sync(0xffffffffu, in && x > m[v])) {
@@ -235,9 +214,10 @@ __global__ void __launch_bounds__(kRowWarps * 32) rows_f32_kernel(const __grid_c
         const float p = in ? exp2f(x - (m[v] == -INFINITY ? 0.f : m[v])) : 0.f;
         if (hh == 0) {
           l[v] += p;
-          pb[warp][v][j] = p;
+          pb[v][j] = p;
         }
       }
+      const float* vb = take();
       __syncwarp();
       const int nk = min(16, u.k1 - k);
 #pragma unroll 4
@@ -247,49 +227,30 @@ __global__ void __launch_bounds__(kRowWarps * 32) rows_f32_kernel(const __grid_c
         else *reinterpret_cast<float2*>(vf) = *reinterpret_cast<const float2*>(vb + t * HD + lane * DPL);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-          const float p = pb[warp][v][t];
+          const float p = pb[v][t];
           // a masked key adds nothing, whatever its value holds
 #pragma unroll
           for (int d = 0; d < DPL; ++d) o[v][d] = p == 0.f ? o[v][d] : fmaf(p, vf[d], o[v][d]);
         }
       }
-      __syncwarp();
-      ++used;
+      release();
     }
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
 #pragma unroll
-      for (int w = 8; w > 0; w >>= 1) l[v] += __shfl_xor_sync(0xffffffffu, l[v], w);
-#pragma unroll
-      for (int d = 0; d < DPL; ++d) mo[warp][v][lane * DPL + d] = o[v][d];
-      if (lane == 0) {
-        mm[warp][v] = m[v];
-        ml[warp][v] = l[v];
-      }
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < u.nv * HD; i += blockDim.x) {
-      const int v = i / HD, d = i % HD;
-      float M = -INFINITY, L = 0.f, O = 0.f;
-#pragma unroll
-      for (int w = 0; w < kRowWarps; ++w) M = fmaxf(M, mm[w][v]);
-#pragma unroll
-      for (int w = 0; w < kRowWarps; ++w) {
-        const float f = M == -INFINITY ? 1.f : exp2f(mm[w][v] - M);
-        L += ml[w][v] * f;
-        O += mo[w][v][d] * f;
-      }
+      for (int w = 16; w > 0; w >>= 1) l[v] += __shfl_xor_sync(0xffffffffu, l[v], w);
+      if (v >= u.nv) continue;
       if (u.slot >= 0) {
-        a.part_o[(size_t)(u.slot + v) * HD + d] = O;
-        if (d == 0) a.part_ml[u.slot + v] = make_float2(M, L);
+#pragma unroll
+        for (int d = 0; d < DPL; ++d) a.part_o[(size_t)(u.slot + v) * HD + lane * DPL + d] = o[v][d];
+        if (lane == 0) a.part_ml[u.slot + v] = make_float2(m[v], l[v]);
       } else {
-        const float r = L == 0.f ? 0.f : O / L;
-        const size_t at = (size_t)(u.row0 + (u.v0 + v) / a.n_rep) * a.ldo + (size_t)vi[v].head * HD + d;
-        if constexpr (sizeof(TQ) == 2) reinterpret_cast<__half*>(a.out)[at] = __float2half_rn(r);
-        else reinterpret_cast<float*>(a.out)[at] = r;
+        const float r = l[v] == 0.f ? 0.f : 1.f / l[v];
+        const size_t at = (size_t)vec_row(a, u.row0, u.v0, v) * a.ldo + (size_t)vec_head(a, u.kvh, u.v0, v) * HD;
+#pragma unroll
+        for (int d = 0; d < DPL; ++d) store_out<TQ>(a, at + lane * DPL + d, o[v][d] * r);
       }
     }
-    if (u.slot >= 0) join_last<HD, TQ>(a, u);
   }
 }
 
@@ -303,9 +264,11 @@ __global__ void __launch_bounds__(kRowWarps * 32) rows_f32_kernel(const __grid_c
 // and round p. q is brought to a power of two near 2^8 first and p counts from
 // 2^12 down, so that neither part meets fp16's subnormals where it matters.
 //
-// Bound by memory: each warp streams every fourth page of its CTA's share through
-// a ring of its own (TMA boxes of 16 rows x 128 bytes with 128-byte swizzle);
-// the loads run ahead over the ends of units.
+// Bound by memory: each warp streams its share of the pages through a ring of its own
+// (TMA boxes of 16 rows x 128 bytes with 128-byte swizzle); the loads run ahead over
+// the ends of units. Warps share nothing: with the four warps of a CTA on one unit,
+// its start and end (barriers, merges) took 6 us a unit, 72 us for 16 tenants of
+// 512-8192 tokens.
 // ---------------------------------------------------------------------------
 template <int HD>
 struct MmaCfg {
@@ -313,7 +276,7 @@ struct MmaCfg {
   static constexpr int STAGE = 2 * BLK;
   static constexpr int NST = HD == 128 ? 3 : 6;           // 96 KB a CTA, two CTAs an SM
   static constexpr int RING = kRowWarps * NST * STAGE;
-  static constexpr int SMEM = 1024 + RING + 2 * kSmallVecs * (HD + 2) * 4 + kRowWarps * NST * 8;
+  static constexpr int SMEM = 1024 + RING + kRowWarps * NST * 8;
 };
 constexpr float kPBias = 12.f;  // p = 2^(s - m + 12)
 
@@ -353,57 +316,49 @@ __device__ __forceinline__ uint32_t pack2_lo(float a, float b, uint32_t hi) {
   return pack2(a - f.x, b - f.y);
 }
 
+// Two consecutive elements of a query vector as the B operand wants them
+template <int HL>
+__device__ __forceinline__ float2 load_q2(const RowAttnArgs& a, size_t at, bool whole) {
+  if (HL) {
+    const float* p = reinterpret_cast<const float*>(a.q) + at;
+    return whole ? *reinterpret_cast<const float2*>(p) : make_float2(p[0], p[1]);
+  }
+  const __half* p = reinterpret_cast<const __half*>(a.q) + at;
+  return __half22float2(whole ? *reinterpret_cast<const __half2*>(p) : __halves2half2(p[0], p[1]));
+}
+
 template <int HD, int HL>
 __global__ void __launch_bounds__(kRowWarps * 32, 2) rows_mma_kernel(const __grid_constant__ RowAttnArgs a) {
   using C = MmaCfg<HD>;
+  using TO = typename std::conditional<HL != 0, float, __half>::type;
   constexpr int NV = kSmallVecs, KS = HD / 16, NST = C::NST;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  float* qs = reinterpret_cast<float*>(smem + C::RING);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(qs + 2 * NV * (HD + 2));
-  auto mrg = reinterpret_cast<float(*)[NV][HD + 2]>(qs);  // [2], over the queries
-  __shared__ float pt[kRowWarps][16][NV];
-  __shared__ VecInfo vi[NV];
-  __shared__ float qmul[NV];
+  __shared__ float pt_all[kRowWarps][16][NV];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const int u_begin = a.cta[blockIdx.x], u_end = a.cta[blockIdx.x + 1];
+  const int me = blockIdx.x * kRowWarps + warp;
+  pdl_launch_dependents();
+  if (me >= a.n_warps) return;
+  auto pt = pt_all[warp];
   uint8_t* ring = smem + warp * NST * C::STAGE;
-  uint64_t* bar = bars + warp * NST;
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + C::RING) + warp * NST;
   if (lane == 0) {
     for (int i = 0; i < NST; ++i) mbar_init(&bar[i], 1);
     fence_barrier_init();
   }
   __syncwarp();
-
-  // this warp's loads: unit pu, key pk (its page), running ahead of the math
-  int pu = u_begin, pk = 0, pk1 = 0, pten = 0, pkvh = 0;
-  auto open = [&]() {  // the first unit at or after pu with a page for this warp
-    for (; pu < u_end; ++pu) {
-      const AttnUnit u = a.units[pu];
-      pk = u.k0 + 16 * warp;
-      pk1 = u.k1;
-      pten = u.tenant;
-      pkvh = u.kvh;
-      if (pk < pk1) return;
-    }
-  };
-  open();
-  int cached_t = -1, cached_p = 0, cached = 0;  // lane i: the page of page index cached_p + 4 i
+  const int u_begin = a.warps[me], u_end = a.warps[me + 1];
+  Ahead ah{u_begin, u_end, 0, 0, 0, 0};
+  PageCache pages;
+  ah.open(a);
   int issued = 0, used = 0;
   auto issue = [&](int limit) {
-    while (issued < limit && pu < u_end) {
-      const int p = pk >> 4, off = p - cached_p;
-      if (pten != cached_t || off < 0 || (off & 3) || off >= 128) {
-        cached_t = pten;
-        cached_p = p;
-        const int at = p + 4 * lane;
-        cached = at < a.kv.ptab_stride ? a.kv.ptab[(size_t)pten * a.kv.ptab_stride + at] : 0;
-      }
-      const int page = __shfl_sync(0xffffffffu, cached, (p - cached_p) >> 2);
+    while (issued < limit && ah.pu < u_end) {
+      const int page = pages.page(a, ah.tenant, ah.pk);
       if (lane == 0) {
         const int s = issued % NST;
         mbar_arrive_expect_tx(&bar[s], C::STAGE);
-        const int y = (((page * a.kv.n_layers + a.layer) * 2) * a.kv.n_kv + pkvh) * 16;
+        const int y = (((page * a.kv.n_layers + a.layer) * 2) * a.kv.n_kv + ah.kvh) * 16;
 #pragma unroll
         for (int w = 0; w < 2; ++w)
 #pragma unroll
@@ -411,11 +366,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) rows_mma_kernel(const __gri
             tma_2d(ring + s * C::STAGE + w * C::BLK + b * 2048, &a.tmap, b * 64, y + w * a.kv.n_kv * 16, &bar[s]);
       }
       ++issued;
-      pk += 16 * kRowWarps;
-      if (pk >= pk1) {
-        ++pu;
-        open();
-      }
+      ah.next(a);
     }
   };
   issue(NST);
@@ -429,87 +380,54 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) rows_mma_kernel(const __gri
       voff[ks] = swz16(rr + (mi >> 1) * 8, ks * 2 + (mi & 1));
     }
   }
+  const bool whole = ((reinterpret_cast<uintptr_t>(a.q) | (size_t)a.ldq * (HL ? 4 : 2)) & (HL ? 7 : 3)) == 0;
   for (int ui = u_begin; ui < u_end; ++ui) {
     const AttnUnit u = a.units[ui];
-    __syncthreads();  // the last unit's queries and partial results are read
-    for (int v = warp; v < NV; v += kRowWarps) {  // a warp per vector: load, largest magnitude
-      float top = 0.f;
-      const int at_v = u.v0 + v;
-      const size_t at = (size_t)(u.row0 + at_v / a.n_rep) * a.ldq + (size_t)(u.kvh * a.n_rep + at_v % a.n_rep) * HD;
+    uint32_t qb[KS][1 + HL][2];
+    float mul = 1.f;
+    {  // lane (g, c) holds elements 2c, 2c + 1 and 2c + 8, 2c + 9 of every 16 of vector g
+      const size_t at = (size_t)vec_row(a, u.row0, u.v0, g) * a.ldq + (size_t)vec_head(a, u.kvh, u.v0, g) * HD + 2 * c;
+      float2 x[KS][2];
 #pragma unroll
-      for (int i = 0; i < HD / 32; ++i) {
-        float x = 0.f;
-        if (v < u.nv) x = HL ? ld_f32<float>(a.q, at + lane + 32 * i) : ld_f32<__half>(a.q, at + lane + 32 * i);
-        qs[v * HD + lane + 32 * i] = x;
-        top = fmaxf(top, fabsf(x));
-      }
-      float mul = 1.f;
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+          x[ks][b] = g < u.nv ? load_q2<HL>(a, at + ks * 16 + 8 * b, whole) : make_float2(0.f, 0.f);
       if (HL) {
+        float top = 0.f;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) top = fmaxf(top, fmaxf(fabsf(x[ks][b].x), fabsf(x[ks][b].y)));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         // 2^(8 - exponent of top), for normal finite tops
         const int e = (int)(__float_as_uint(top) >> 23);
         if (e > 8 && e < 255) mul = __uint_as_float((uint32_t)min(254, 127 + 8 + 127 - e) << 23);
       }
-      if (lane == 0) qmul[v] = mul;
-      if (lane == 1) {
-        VecInfo w{0, 0, 0, 0, 0.f};
-        if (v < u.nv) {
-          const RowInfo r = a.rows[u.row0 + at_v / a.n_rep];
-          w.lo = r.lo;
-          w.hi = r.hi;
-          w.pos = r.pos;
-          w.head = u.kvh * a.n_rep + at_v % a.n_rep;
-          w.slope = a.slopes ? a.slopes[w.head] : 0.f;
-        }
-        vi[v] = w;
-      }
-    }
-    __syncthreads();
-    uint32_t qb[KS][1 + HL][2];
-    {
-      const float mul = HL ? qmul[g] : 1.f;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          const float x0 = qs[g * HD + ks * 16 + 2 * c + 8 * b] * mul, x1 = qs[g * HD + ks * 16 + 2 * c + 8 * b + 1] * mul;
-          qb[ks][0][b] = pack2(x0, x1);
-          if (HL) qb[ks][HL][b] = pack2_lo(x0, x1, qb[ks][0][b]);
+          qb[ks][0][b] = pack2(x[ks][b].x * mul, x[ks][b].y * mul);
+          if (HL) qb[ks][HL][b] = pack2_lo(x[ks][b].x * mul, x[ks][b].y * mul, qb[ks][0][b]);
         }
     }
-    __syncthreads();  // the queries' place takes the warps' results
-    // this lane's two vectors (columns 2c, 2c + 1)
+    // this lane's two vectors in the scores (columns 2c, 2c + 1)
     VecInfo w[2];
     float sv[2];
-    int in0 = 0x7fffffff, in1 = 0;      // keys that some vector sees
-    int all0 = 0, all1 = 0x7fffffff;    // keys that every vector sees
-    bool one_row = true;
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
-      if (v < u.nv) {
-        const int lo = vi[v].lo, hi = vi[v].hi;
-        if (hi > lo) {
-          in0 = min(in0, lo);
-          in1 = max(in1, hi);
-        }
-        all0 = max(all0, lo);
-        all1 = min(all1, hi);
-      }
-    one_row = u.v0 + u.nv <= a.n_rep;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      w[h] = vi[2 * c + h];
-      sv[h] = a.scale / (HL ? qmul[2 * c + h] : 1.f);
+      w[h] = vec_info(a, u, 2 * c + h);
+      sv[h] = a.scale / __shfl_sync(0xffffffffu, mul, (2 * c + h) * 4);
       if (!(a.cap > 0.f)) sv[h] *= kLog2e;
-      w[h].slope *= kLog2e;
     }
+    const bool one_row = u.v0 + u.nv <= a.n_rep;
     const float icap = a.cap > 0.f ? 1.f / a.cap : 0.f, cap2 = a.cap * kLog2e;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, ot[KS][4];
 #pragma unroll
     for (int i = 0; i < KS; ++i) ot[i][0] = ot[i][1] = ot[i][2] = ot[i][3] = 0.f;
-    for (int k = u.k0 + 16 * warp; k < u.k1; k += 16 * kRowWarps) {
-      issue(used + NST);
+    for (int k = u.k0; k < u.k1; k += kRowPage) {
       const int s = used % NST;
       if (alive) alive = mbar_wait(&bar[s], (used / NST) & 1, a.err, DEV_TIMEOUT_FULL);
       const uint8_t* kb = ring + s * C::STAGE;
@@ -528,7 +446,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) rows_mma_kernel(const __gri
           mma_16816(sa[ks & 3], af, qb[ks][0][0], qb[ks][0][1]);
         }
       }
-      const bool full = k >= all0 && k + 16 <= all1;  // the same in every lane
+      const bool full = k >= u.all0 && k + 16 <= u.all1;  // the same in every lane
       float x[4];  // (key g, vector 2c), (g, 2c + 1), (g + 8, 2c), (g + 8, 2c + 1)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -579,7 +497,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) rows_mma_kernel(const __gri
         // values of keys that no vector sees do not enter the product
         uint32_t z0 = 0xffffffffu, z1 = 0xffffffffu;
         if (!full) {
-          auto half_mask = [&](int key) { return key >= in0 && key < in1 ? 0xffffu : 0u; };
+          auto half_mask = [&](int key) { return key >= u.in0 && key < u.in1 ? 0xffffu : 0u; };
           z0 = half_mask(k + 2 * c) | half_mask(k + 2 * c + 1) << 16;
           z1 = half_mask(k + 2 * c + 8) | half_mask(k + 2 * c + 9) << 16;
         }
@@ -598,13 +516,13 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) rows_mma_kernel(const __gri
         }
       } else {
         // rows that see different keys of this page: in fp32, each vector over its own keys
-        pt[warp][g][2 * c] = p[0];
-        pt[warp][g][2 * c + 1] = p[1];
-        pt[warp][g + 8][2 * c] = p[2];
-        pt[warp][g + 8][2 * c + 1] = p[3];
+        pt[g][2 * c] = p[0];
+        pt[g][2 * c + 1] = p[1];
+        pt[g + 8][2 * c] = p[2];
+        pt[g + 8][2 * c + 1] = p[3];
         __syncwarp();
         for (int t = 0; t < 16; ++t) {
-          const float p0 = pt[warp][t][2 * c], p1 = pt[warp][t][2 * c + 1];
+          const float p0 = pt[t][2 * c], p1 = pt[t][2 * c + 1];
 #pragma unroll
           for (int i = 0; i < KS; ++i)
 #pragma unroll
@@ -618,79 +536,87 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) rows_mma_kernel(const __gri
       }
       __syncwarp();  // the stage is read before it is loaded again
       ++used;
+      issue(used + NST);
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], o);
-    // the warps' results in pairs (2 and 3 into 0 and 1), then those two
-    auto deposit = [&](float (*b)[HD + 2]) {
+    // 32-byte runs of a vector in eight lanes
 #pragma unroll
-      for (int i = 0; i < KS; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) b[2 * c + (e & 1)][i * 16 + g + (e >> 1) * 8] = ot[i][e];
-      if (g == 0)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          b[2 * c + h][HD] = m[h];
-          b[2 * c + h][HD + 1] = l[h];
-        }
-    };
-    if (warp >= 2) deposit(mrg[warp - 2]);
-    __syncthreads();
-    if (warp < 2) {
-      const float(*b)[HD + 2] = mrg[warp];
-      float f1[2], f2[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float m2 = b[2 * c + h][HD], M = fmaxf(m[h], m2);
-        f1[h] = M == -INFINITY ? 1.f : ex2(m[h] - M);
-        f2[h] = M == -INFINITY ? 1.f : ex2(m2 - M);
-        l[h] = l[h] * f1[h] + b[2 * c + h][HD + 1] * f2[h];
-        m[h] = M;
-      }
-#pragma unroll
-      for (int i = 0; i < KS; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          ot[i][e] = ot[i][e] * f1[e & 1] + b[2 * c + (e & 1)][i * 16 + g + (e >> 1) * 8] * f2[e & 1];
-      __syncwarp();
-      deposit(mrg[warp]);
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < u.nv * HD; i += kRowWarps * 32) {
-      const int v = i / HD, d = i % HD;
-      const float M = fmaxf(mrg[0][v][HD], mrg[1][v][HD]);
-      float L = 0.f, O = 0.f;
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const float f = M == -INFINITY ? 1.f : ex2(mrg[q][v][HD] - M);
-        L += mrg[q][v][HD + 1] * f;
-        O += mrg[q][v][d] * f;
-      }
+    for (int h = 0; h < 2; ++h) {
+      const int v = 2 * c + h;
+      if (v >= u.nv) continue;
       if (u.slot >= 0) {
-        a.part_o[(size_t)(u.slot + v) * HD + d] = O;
-        if (d == 0) a.part_ml[u.slot + v] = make_float2(M, L);
+        float* dst = a.part_o + (size_t)(u.slot + v) * HD + g;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          dst[i * 16] = ot[i][h];
+          dst[i * 16 + 8] = ot[i][2 + h];
+        }
+        if (g == 0) a.part_ml[u.slot + v] = make_float2(m[h], l[h]);
       } else {
-        const float r = L == 0.f ? 0.f : O / L;
-        const size_t at = (size_t)(u.row0 + (u.v0 + v) / a.n_rep) * a.ldo + (size_t)vi[v].head * HD + d;
-        if (HL) reinterpret_cast<float*>(a.out)[at] = r;
-        else reinterpret_cast<__half*>(a.out)[at] = __float2half_rn(r);
+        const float r = l[h] == 0.f ? 0.f : 1.f / l[h];
+        const size_t at = (size_t)vec_row(a, u.row0, u.v0, v) * a.ldo + (size_t)vec_head(a, u.kvh, u.v0, v) * HD + g;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          store_out<TO>(a, at + i * 16, ot[i][h] * r);
+          store_out<TO>(a, at + i * 16 + 8, ot[i][2 + h] * r);
+        }
       }
-    }
-    if (u.slot >= 0) {
-      if (HL) join_last<HD, float>(a, u);
-      else join_last<HD, __half>(a, u);
     }
   }
 }
 
-// Joins the parts of the tile items.
+// Joins the parts of the items that were cut, parts in the order of the keys: a thread
+// has four elements of one vector, and sixteen parts' loads do not wait for one another.
+// A kernel of its own, launched ahead of its start (its launch costs nothing then): the
+// last warp of an item joining its parts took 40 us for 37 parts of 8 vectors.
 template <int HD, class TO>
-__global__ void __launch_bounds__(256) rows_join_kernel(const __grid_constant__ RowAttnArgs a) {
-  const JoinItem it = a.joins[a.n_small_joins + blockIdx.x];
-  const int v = blockIdx.y * (256 / (HD / 4)) + threadIdx.x / (HD / 4);
-  if (v < it.nv) join_vec<HD, TO>(a, it, v, threadIdx.x % (HD / 4) * 4);
+__global__ void __launch_bounds__(128) rows_join_kernel(const __grid_constant__ RowAttnArgs a) {
+  constexpr int LPV = HD / 4, NP = 16;
+  const JoinItem it = a.joins[blockIdx.x];
+  const int v = blockIdx.y * (128 / LPV) + threadIdx.x / LPV, d = threadIdx.x % LPV * 4;
+  if (v >= it.nv) return;
+  pdl_wait();
+  float M = -INFINITY, L = 0.f;
+  float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p0 = 0; p0 < it.n_parts; p0 += NP) {
+    float2 ml[NP];
+    float4 o[NP];
+#pragma unroll
+    for (int q = 0; q < NP; ++q) {
+      const bool in = p0 + q < it.n_parts;
+      const size_t s = (size_t)it.slot0 + (size_t)(p0 + q) * it.nv + v;
+      ml[q] = in ? __ldcg(a.part_ml + s) : make_float2(-INFINITY, 0.f);
+      o[q] = in ? __ldcg(reinterpret_cast<const float4*>(a.part_o + s * HD + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float mn = M;
+#pragma unroll
+    for (int q = 0; q < NP; ++q) mn = fmaxf(mn, ml[q].x);
+    const float f0 = mn == -INFINITY ? 1.f : exp2f(M - mn);
+    L *= f0;
+    O.x *= f0;
+    O.y *= f0;
+    O.z *= f0;
+    O.w *= f0;
+#pragma unroll
+    for (int q = 0; q < NP; ++q) {
+      const float f = mn == -INFINITY ? 1.f : exp2f(ml[q].x - mn);
+      L += ml[q].y * f;
+      O.x += o[q].x * f;
+      O.y += o[q].y * f;
+      O.z += o[q].z * f;
+      O.w += o[q].w * f;
+    }
+    M = mn;
+  }
+  const float r = L == 0.f ? 0.f : 1.f / L;
+  const size_t at = (size_t)vec_row(a, it.row0, it.v0, v) * a.ldo + (size_t)vec_head(a, it.kvh, it.v0, v) * HD + d;
+  store_out<TO>(a, at, O.x * r);
+  store_out<TO>(a, at + 1, O.y * r);
+  store_out<TO>(a, at + 2, O.z * r);
+  store_out<TO>(a, at + 3, O.w * r);
 }
 
 }  // namespace
@@ -700,7 +626,7 @@ static cudaError_t launch_mma(const RowAttnArgs& a, cudaStream_t s) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (cudaError_t e = ensure_smem_attr(rows_mma_kernel<HD, HL>, MmaCfg<HD>::SMEM, dev)) return e;
-  rows_mma_kernel<HD, HL><<<a.n_cta, kRowWarps * 32, MmaCfg<HD>::SMEM, s>>>(a);
+  rows_mma_kernel<HD, HL><<<(a.n_warps + kRowWarps - 1) / kRowWarps, kRowWarps * 32, MmaCfg<HD>::SMEM, s>>>(a);
   return cudaGetLastError();
 }
 
@@ -711,10 +637,10 @@ static cudaError_t launch_f32(const RowAttnArgs& a, cudaStream_t s) {
   constexpr int smem = F32Cfg<HD>::SMEM;
   if (a.q16) {
     if (cudaError_t e = ensure_smem_attr(rows_f32_kernel<HD, NV, __half>, smem, dev)) return e;
-    rows_f32_kernel<HD, NV, __half><<<a.n_cta, kRowWarps * 32, smem, s>>>(a);
+    rows_f32_kernel<HD, NV, __half><<<(a.n_warps + kRowWarps - 1) / kRowWarps, kRowWarps * 32, smem, s>>>(a);
   } else {
     if (cudaError_t e = ensure_smem_attr(rows_f32_kernel<HD, NV, float>, smem, dev)) return e;
-    rows_f32_kernel<HD, NV, float><<<a.n_cta, kRowWarps * 32, smem, s>>>(a);
+    rows_f32_kernel<HD, NV, float><<<(a.n_warps + kRowWarps - 1) / kRowWarps, kRowWarps * 32, smem, s>>>(a);
   }
   return cudaGetLastError();
 }
@@ -727,7 +653,7 @@ static cudaError_t launch_f32_vecs(const RowAttnArgs& a, cudaStream_t s) {
 }
 
 cudaError_t rows_small_launch(const RowAttnArgs& a, cudaStream_t s) {
-  if (a.n_cta < 1) return cudaSuccess;
+  if (a.n_warps < 1) return cudaSuccess;
   if (a.kv.f16) {
     if (a.kv.hd == 128) return a.q16 ? launch_mma<128, 0>(a, s) : launch_mma<128, 1>(a, s);
     return a.q16 ? launch_mma<64, 0>(a, s) : launch_mma<64, 1>(a, s);
@@ -735,18 +661,24 @@ cudaError_t rows_small_launch(const RowAttnArgs& a, cudaStream_t s) {
   return a.kv.hd == 128 ? launch_f32_vecs<128>(a, s) : launch_f32_vecs<64>(a, s);
 }
 
+template <int HD, class TO>
+static cudaError_t launch_join(const RowAttnArgs& a, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)a.n_joins, (unsigned)((a.join_nv * (HD / 4) + 127) / 128));
+  cfg.blockDim = dim3(128);
+  cfg.stream = s;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, rows_join_kernel<HD, TO>, a);
+}
+
 cudaError_t rows_join_launch(const RowAttnArgs& a, cudaStream_t s) {
-  const int n = a.n_joins - a.n_small_joins;
-  if (n < 1) return cudaSuccess;
-  const dim3 g(n, kTileVecs * a.kv.hd / 4 / 256);
-  if (a.kv.hd == 128) {
-    if (a.q16) rows_join_kernel<128, __half><<<g, 256, 0, s>>>(a);
-    else rows_join_kernel<128, float><<<g, 256, 0, s>>>(a);
-  } else {
-    if (a.q16) rows_join_kernel<64, __half><<<g, 256, 0, s>>>(a);
-    else rows_join_kernel<64, float><<<g, 256, 0, s>>>(a);
-  }
-  return cudaGetLastError();
+  if (a.n_joins < 1) return cudaSuccess;
+  if (a.kv.hd == 128) return a.q16 ? launch_join<128, __half>(a, s) : launch_join<128, float>(a, s);
+  return a.q16 ? launch_join<64, __half>(a, s) : launch_join<64, float>(a, s);
 }
 
 }  // namespace rb

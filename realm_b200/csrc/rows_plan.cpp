@@ -9,7 +9,7 @@ namespace rb {
 namespace {
 
 struct Item {
-  int row0, v0, nv, tenant, k0, k1;
+  int row0, v0, nv, tenant, k0, k1, all0, all1, in0, in1;
 };
 
 // Cuts the rows [r0, r1) (one tenant) into items of at most `vecs` query vectors
@@ -18,24 +18,31 @@ void cut_run(const std::vector<RowInfo>& rows, int r0, int r1, int n_rep, int ve
   const long long total = (long long)(r1 - r0) * n_rep;
   for (long long v = 0; v < total; v += vecs) {
     const int nv = (int)std::min<long long>(vecs, total - v);
-    Item it{r0 + (int)(v / n_rep), (int)(v % n_rep), nv, rows[r0].tenant, 0, 0};
-    int lo = 0, hi = 0;
+    Item it{r0 + (int)(v / n_rep), (int)(v % n_rep), nv, rows[r0].tenant, 0, 0, 0, 0x7fffffff, 0, 0};
     bool any = false;
-    for (int r = it.row0; r <= r0 + (int)((v + nv - 1) / n_rep); ++r)
-      if (rows[r].hi > rows[r].lo) {
-        lo = any ? std::min(lo, rows[r].lo) : rows[r].lo;
-        hi = any ? std::max(hi, rows[r].hi) : rows[r].hi;
-        any = true;
-      }
+    for (int r = it.row0; r <= r0 + (int)((v + nv - 1) / n_rep); ++r) {
+      it.all0 = std::max(it.all0, rows[r].lo);
+      it.all1 = std::min(it.all1, rows[r].hi);
+      if (rows[r].hi <= rows[r].lo) continue;
+      it.in0 = any ? std::min(it.in0, rows[r].lo) : rows[r].lo;
+      it.in1 = std::max(it.in1, rows[r].hi);
+      any = true;
+    }
     if (any) {
-      it.k0 = lo / align * align;
-      it.k1 = hi;
+      it.k0 = it.in0 / align * align;
+      it.k1 = it.in1;
     }
     out.push_back(it);
   }
 }
 
 int blocks_of(const Item& it, int width) { return (it.k1 - it.k0 + width - 1) / width; }
+
+// The unit of blocks [b0, b1) of an item, of `width` keys each.
+AttnUnit unit_of(const Item& it, int kvh, int b0, int b1, int width) {
+  return {it.row0, it.v0, it.nv, kvh, it.tenant, it.k0 + b0 * width, std::min(it.k1, it.k0 + b1 * width), -1,
+          it.all0, it.all1, it.in0, it.in1};
+}
 
 }  // namespace
 
@@ -53,49 +60,67 @@ void rows_partition(const std::vector<RowInfo>& rows, int n_heads, int n_kv, int
     r = e;
   }
 
-  // small items: the pages of all (item, kv head) pairs form one sequence; every
-  // CTA takes an equal contiguous share of it, at least four pages (one a warp)
-  long long pages = 0;
-  for (const Item& it : small) pages += (long long)n_kv * blocks_of(it, kRowPage);
-  const long long most = 2ll * num_sms;
-  const long long G = std::max<long long>(1, std::min(most, (pages + 3) / 4));
+  // Small items: every warp works for itself. The warps go in groups of n_kv, one for
+  // each kv head, and every group takes an equal contiguous share of all items' pages:
+  // the heads of a page lie next to one another in memory and are read at the same
+  // time. With few pages a group (at least four), a share does not cross into another
+  // item, since starting on a second one takes a warp as long as several pages.
   if (!small.empty()) {
-    out.small_cta.assign(1, 0);
-    long long at = 0, cta = 0;  // pages handed out so far, CTA being filled
-    auto cta_end = [&](long long c) { return pages * (c + 1) / G; };
+    long long pages = 0;
     for (const Item& it : small) {
+      pages += blocks_of(it, kRowPage);
       out.max_nv = std::max(out.max_nv, it.nv);
-      for (int h = 0; h < n_kv; ++h) {
-        const int np = blocks_of(it, kRowPage);
-        const size_t first = out.small.size();
+    }
+    const long long most = std::max(1ll, 2ll * kRowWarps * num_sms / n_kv);  // groups
+    const long long share = std::max<long long>(4, (pages + most - 1) / most);
+    const bool apart = share <= 8;
+    struct Piece {
+      int item, p0, p1, slot, parts;
+    };
+    std::vector<std::vector<Piece>> groups;
+    long long at = 0, g = 0;  // pages handed out so far, group whose share they are in
+    for (int i = 0; i < (int)small.size(); ++i) {
+      const Item& it = small[i];
+      const int np = blocks_of(it, kRowPage);
+      std::vector<std::pair<long long, int>> cuts;  // group and end of each piece
+      if (apart) {
+        const int n = std::max(1, (int)((np + share - 1) / share));
+        for (int q = 1; q <= n; ++q) cuts.push_back({(long long)groups.size() + q - 1, (int)((long long)np * q / n)});
+      } else {
         int p = 0;
         do {
-          while (cta + 1 < G && at >= cta_end(cta)) {
-            out.small_cta.push_back((int)out.small.size());
-            ++cta;
-          }
-          const int take = (int)std::min<long long>(np - p, cta + 1 < G ? cta_end(cta) - at : np - p);
-          AttnUnit u{it.row0, it.v0, it.nv, h, it.tenant, it.k0 + p * kRowPage,
-                     std::min(it.k1, it.k0 + (p + take) * kRowPage), -1, -1};
-          out.small.push_back(u);
-          p += take;
-          at += take;
+          while (g + 1 < most && pages * (g + 1) / most <= at + p) ++g;
+          p = g + 1 < most ? (int)std::min<long long>(np, pages * (g + 1) / most - at) : np;
+          cuts.push_back({g, p});
         } while (p < np);
-        const int parts = (int)(out.small.size() - first);
-        if (parts > 1) {
+      }
+      const int parts = (int)cuts.size();
+      const int slot = out.n_slots;
+      if (parts > 1)
+        for (int h = 0; h < n_kv; ++h) {
           out.joins.push_back({it.row0, it.v0, it.nv, h, out.n_slots, parts});
-          for (size_t i = first; i < out.small.size(); ++i) {
-            out.small[i].join = (int)out.joins.size() - 1;
-            out.small[i].slot = out.n_slots;
-            out.n_slots += it.nv;
-          }
+          out.n_slots += parts * it.nv;
         }
+      for (int q = 0; q < parts; ++q) {
+        if ((long long)groups.size() <= cuts[q].first) groups.resize(cuts[q].first + 1);
+        groups[cuts[q].first].push_back({i, q ? cuts[q - 1].second : 0, cuts[q].second, parts > 1 ? slot + q * it.nv : -1, parts});
+      }
+      at += np;
+    }
+    out.small_warp.push_back(0);
+    for (const auto& group : groups) {
+      if (group.empty()) continue;
+      for (int h = 0; h < n_kv; ++h) {
+        for (const Piece& pc : group) {
+          const Item& it = small[pc.item];
+          AttnUnit u = unit_of(it, h, pc.p0, pc.p1, kRowPage);
+          if (pc.slot >= 0) u.slot = pc.slot + h * pc.parts * it.nv;
+          out.small.push_back(u);
+        }
+        out.small_warp.push_back((int)out.small.size());
       }
     }
-    while ((long long)out.small_cta.size() <= G) out.small_cta.push_back((int)out.small.size());
   }
-  out.n_small_joins = (int)out.joins.size();
-
   // tile items: one CTA per unit, the longest first. Their keys are cut only where
   // the items are fewer than the SMs, and not below four blocks: a unit's start and
   // end cost about as much as those. (Cutting the longest of 256 uneven items as well,
@@ -114,8 +139,7 @@ void rows_partition(const std::vector<RowInfo>& rows, int n_heads, int n_kv, int
         }
         for (int p = 0; p < parts; ++p) {
           const int b0 = (int)((long long)nb * p / parts), b1 = (int)((long long)nb * (p + 1) / parts);
-          AttnUnit u{it.row0, it.v0, it.nv, h, it.tenant, it.k0 + b0 * kTileKeys,
-                     std::min(it.k1, it.k0 + b1 * kTileKeys), -1, -1};
+          AttnUnit u = unit_of(it, h, b0, b1, kTileKeys);
           if (parts > 1) {
             u.slot = out.n_slots;
             out.n_slots += it.nv;
@@ -145,6 +169,7 @@ void rows_partition(const std::vector<RowInfo>& rows, int n_heads, int n_kv, int
       out.spans.push_back(s);
     }
   }
+  for (const JoinItem& j : out.joins) out.join_nv = std::max(out.join_nv, j.nv);
 }
 
 }  // namespace rb

@@ -232,6 +232,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
   __shared__ uint32_t tmem_slot;
   __shared__ int primed[2];    // O holds something before the first product
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_launch_dependents();
   const AttnUnit u = a.units[blockIdx.x];
   const TileSpan sp = a.spans[blockIdx.x];
   const int nt = u.nv > 128 ? 2 : 1, nb = (u.k1 - u.k0 + B - 1) / B;

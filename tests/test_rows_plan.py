@@ -67,13 +67,15 @@ def test_units_cover_every_key_once(name, heads, kv, f16, sms):
     assert slots == set(range(len(slots)))
 
 
-def test_ctas_share_pages_evenly():
+def test_warps_share_pages_evenly():
     from realm_b200 import rows as R
     rows = _rows(sum([_causal(t, 511 + 480 * t, 1) for t in range(16)], []))
     units = R.partition(rows, 32, 8, 148, True)
     load = np.zeros(units[:, 1].max() + 1, np.int64)
     np.add.at(load, units[:, 1], (units[:, 8] - units[:, 7] + 15) // 16)
-    assert len(load) == 296 and load.max() - load.min() <= 1
+    # warps in groups of eight, one a kv head, on the same keys
+    assert (units[:, 5] == units[:, 1] % 8).all()
+    assert len(load) == 2 * 4 * 148 and load.max() - load.min() <= 1
 
 
 def test_refusals():
