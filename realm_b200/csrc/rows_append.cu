@@ -7,6 +7,8 @@
 //
 // in fp32, rounded once into q_out and the cache. Bound by memory: every element
 // is read once and written once.
+#include <type_traits>
+
 #include "common.cuh"
 #include "rows.cuh"
 
@@ -30,31 +32,6 @@ __device__ __forceinline__ void store_vec(T* p, const float* x) {
   for (int i = 0; i < E; ++i) {
     if constexpr (sizeof(T) == 2) p[i] = __float2half_rn(x[i]);
     else p[i] = x[i];
-  }
-}
-
-// N floats at a place aligned to them (8 or 16 bytes)
-template <int N>
-__device__ __forceinline__ void load_f32(const float* p, float* x) {
-  if constexpr (N == 2) {
-    *reinterpret_cast<float2*>(x) = __ldg(reinterpret_cast<const float2*>(p));
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(x + i) = __ldg(reinterpret_cast<const float4*>(p + i));
-  }
-}
-// E elements at a place aligned to them
-template <class T, int E>
-__device__ __forceinline__ void store_vec16(T* p, const float* x) {
-  if constexpr (sizeof(T) == 2) {
-    uint32_t h[E / 2];
-#pragma unroll
-    for (int i = 0; i < E / 2; ++i) h[i] = h2_as_u32(__floats2half2_rn(x[2 * i], x[2 * i + 1]));
-    if constexpr (E == 8) *reinterpret_cast<uint4*>(p) = make_uint4(h[0], h[1], h[2], h[3]);
-    else *reinterpret_cast<uint2*>(p) = make_uint2(h[0], h[1]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < E; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
   }
 }
 
@@ -128,125 +105,159 @@ __global__ void __launch_bounds__(256) rows_append_kernel(const __grid_constant_
   }
 }
 
-// The same with 16-byte accesses: a head vector takes LPH lanes of E elements, a
-// warp HPW of them at a time and U such groups in flight. Needs the tables and every
-// row of q, k, v and q_out on 16 bytes, and rotation pairs that lie E-aligned in one lane each (or
-// adjacent ones).
+// The same with wide accesses. A lane has two chunks of four elements, the two that the
+// rotation pairs with one another where it does (so nothing is exchanged for it), and a
+// head takes HD / 8 lanes; a warp takes 32 / (HD / 8) heads at a time and U such groups
+// in flight. Needs chunks and tables aligned to their size.
+// 8188 rows of 32 + 8 + 8 heads of 128 (fp16, 205 MB): APPEND_US us; with 8 elements in a row
+// a lane and the partners' fetched by shuffles 56 us, with 2-byte accesses 97 us.
+template <class T>
+__device__ __forceinline__ void load4(const T* p, float* x) {
+  if constexpr (sizeof(T) == 2) {
+    const uint2 r = *reinterpret_cast<const uint2*>(p);
+    const float2 a = __half22float2(u32_as_h2(r.x)), b = __half22float2(u32_as_h2(r.y));
+    x[0] = a.x;
+    x[1] = a.y;
+    x[2] = b.x;
+    x[3] = b.y;
+  } else {
+    *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(p);
+  }
+}
+template <class T>
+__device__ __forceinline__ void store4(T* p, const float* x) {
+  if constexpr (sizeof(T) == 2)
+    *reinterpret_cast<uint2*>(p) =
+        make_uint2(h2_as_u32(__floats2half2_rn(x[0], x[1])), h2_as_u32(__floats2half2_rn(x[2], x[3])));
+  else
+    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+}
+
+template <class TD, int U, int HPW>
+__device__ __forceinline__ void store_heads(TD* dst, int stride, int h0, int n, int d0, int d1, float (&x)[U][8]) {
+#pragma unroll
+  for (int i = 0; i < U; ++i)
+    if (h0 + i * HPW < n) {
+      store4(dst + i * HPW * stride + d0, x[i]);
+      store4(dst + i * HPW * stride + d1, x[i] + 4);
+    }
+}
+
+// A warp's heads are all of q, of k or of v (gq, gk groups, and then v's).
 template <int HD, class TI, class TC, int U>
-__global__ void __launch_bounds__(256) rows_append_vec_kernel(const __grid_constant__ RowAppendArgs a, int groups) {
-  constexpr int E = 16 / sizeof(TI), LPH = HD / E, HPW = 32 / LPH;
-  const int lane = threadIdx.x & 31, sub = lane / LPH, d = (lane % LPH) * E;
-  const int n_q = a.q ? a.n_heads : 0, n_kv = a.kv.n_kv, per = n_q + 2 * n_kv;
-  const long long w = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-  const int row = (int)(w / groups), h0 = (int)(w % groups) * (HPW * U) + sub;
+__global__ void __launch_bounds__(256) rows_append_vec_kernel(const __grid_constant__ RowAppendArgs a, int groups, int gq,
+                                                              int gk) {
+  constexpr int LPH = HD / 8, HPW = 32 / LPH;
+  const int lane = threadIdx.x & 31, l = lane % LPH;
+  const unsigned w = (blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const int row = (int)(w / (unsigned)groups), g = (int)(w % (unsigned)groups);
   if (row >= a.n_rows) return;
+  const int kind = g < gq ? 0 : g < gq + gk ? 1 : 2;
+  const int n = kind == 0 ? a.n_heads : a.kv.n_kv;
+  const int h0 = (kind == 0 ? g : kind == 1 ? g - gq : g - gq - gk) * (HPW * U) + lane / LPH;
+  // the first `pairs` lanes have the rotated chunks l and l + pairs, the others what follows
+  const int pairs = a.rotary / 8;
+  const bool turned = l < pairs;
+  const int d0 = turned ? 4 * l : 8 * l, d1 = turned ? 4 * (l + pairs) : 8 * l + 4;
   const RowInfo r = a.rows[row];
-  uint4 raw[U];
+  float x[U][8];
+  {
+    const TI* src = reinterpret_cast<const TI*>(kind == 0 ? a.q : kind == 1 ? a.k : a.v) +
+                    (size_t)row * (kind == 0 ? a.ldq : kind == 1 ? a.ldk : a.ldv) + h0 * HD;
 #pragma unroll
-  for (int i = 0; i < U; ++i) {
-    const int h = h0 + i * HPW;
-    const TI* p = nullptr;
-    if (h < n_q) p = reinterpret_cast<const TI*>(a.q) + (size_t)row * a.ldq + (size_t)h * HD;
-    else if (h < n_q + n_kv) p = reinterpret_cast<const TI*>(a.k) + (size_t)row * a.ldk + (size_t)(h - n_q) * HD;
-    else if (h < per) p = reinterpret_cast<const TI*>(a.v) + (size_t)row * a.ldv + (size_t)(h - n_q - n_kv) * HD;
-    raw[i] = p ? *reinterpret_cast<const uint4*>(p + d) : make_uint4(0, 0, 0, 0);
-  }
-  const int page = a.kv.ptab[(size_t)r.tenant * a.kv.ptab_stride + (r.pos >> 4)];
-  // the lane's cosines and sines: E of each (half split) or E / 2 (adjacent pairs)
-  const bool turned = d < a.rotary;
-  const int half = a.rotary / 2;
-  const bool low = d < half;
-  float cs[E], sn[E];
-  if (turned) {
-    const float* t = a.rope + (size_t)r.pos * a.rotary;
-    if (a.adjacent) {
-      float c2[E / 2], s2[E / 2];
-      load_f32<E / 2>(t + d / 2, c2);
-      load_f32<E / 2>(t + half + d / 2, s2);
+    for (int i = 0; i < U; ++i)
+      if (h0 + i * HPW < n) {
+        load4(src + i * HPW * HD + d0, x[i]);
+        load4(src + i * HPW * HD + d1, x[i] + 4);
+      } else {
 #pragma unroll
-      for (int i = 0; i < E; ++i) {
-        cs[i] = c2[i / 2];
-        sn[i] = s2[i / 2];
+        for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
       }
-    } else {
-      const int at = low ? d : d - half;
-      load_f32<E>(t + at, cs);
-      load_f32<E>(t + half + at, sn);
-    }
   }
-  // the lane with the other halves of this lane's pairs, in the same head
-  const int partner = low ? lane + half / E : lane - half / E;
+  const float* norm = kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr;
+  const int page = kind ? a.kv.ptab[(size_t)r.tenant * a.kv.ptab_stride + (r.pos >> 4)] : 0;
+  if (kind < 2) {
+    float cs[4], sn[4];
+    if (turned) {
+      const float* t = a.rope + (size_t)r.pos * a.rotary;
+      if (a.adjacent) {  // chunk c has pairs 2 c and 2 c + 1: those of chunk l, then of chunk l + pairs
+        *reinterpret_cast<float2*>(cs) = *reinterpret_cast<const float2*>(t + d0 / 2);
+        *reinterpret_cast<float2*>(cs + 2) = *reinterpret_cast<const float2*>(t + d1 / 2);
+        *reinterpret_cast<float2*>(sn) = *reinterpret_cast<const float2*>(t + a.rotary / 2 + d0 / 2);
+        *reinterpret_cast<float2*>(sn + 2) = *reinterpret_cast<const float2*>(t + a.rotary / 2 + d1 / 2);
+      } else {
+        *reinterpret_cast<float4*>(cs) = *reinterpret_cast<const float4*>(t + d0);
+        *reinterpret_cast<float4*>(sn) = *reinterpret_cast<const float4*>(t + a.rotary / 2 + d0);
+      }
+    }
+    if (norm) {
+      const float4 w0 = *reinterpret_cast<const float4*>(norm + d0), w1 = *reinterpret_cast<const float4*>(norm + d1);
+      const float wn[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-  for (int i = 0; i < U; ++i) {
-    const int h = h0 + i * HPW;
-    float x[E];
-    load_vec<TI, E>(reinterpret_cast<const TI*>(&raw[i]), x);
-    const float* norm = h < n_q ? a.q_norm : h < n_q + n_kv ? a.k_norm : nullptr;
-    if (a.q_norm || a.k_norm) {
-      float ss = 0.f;
+      for (int i = 0; i < U; ++i) {
+        float ss = 0.f;
 #pragma unroll
-      for (int e = 0; e < E; ++e) ss = fmaf(x[e], x[e], ss);
+        for (int e = 0; e < 8; ++e) ss = fmaf(x[i][e], x[i][e], ss);
 #pragma unroll
-      for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      if (norm) {
+        for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         const float inv = rsqrtf(ss * (1.f / HD) + a.eps);
-        float wn[E];
-        load_f32<E>(norm + d, wn);
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] *= inv * wn[e];
+        for (int e = 0; e < 8; ++e) x[i][e] *= inv * wn[e];
       }
     }
-    if (a.rotary) {
-      const bool turn = turned && h < n_q + n_kv;
+    if (turned) {
       if (a.adjacent) {
-        if (turn)
 #pragma unroll
-          for (int e = 0; e < E; e += 2) {
-            const float y0 = x[e] * cs[e] - x[e + 1] * sn[e], y1 = x[e + 1] * cs[e] + x[e] * sn[e];
-            x[e] = y0;
-            x[e + 1] = y1;
+        for (int i = 0; i < U; ++i)
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            const float u = x[i][e] * cs[e / 2] - x[i][e + 1] * sn[e / 2], v = x[i][e + 1] * cs[e / 2] + x[i][e] * sn[e / 2];
+            x[i][e] = u;
+            x[i][e + 1] = v;
           }
       } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float y = __shfl_sync(0xffffffffu, x[e], partner & 31);
-          if (turn) x[e] = low ? x[e] * cs[e] - y * sn[e] : x[e] * cs[e] + y * sn[e];
-        }
+        for (int i = 0; i < U; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float u = x[i][e] * cs[e] - x[i][e + 4] * sn[e], v = x[i][e + 4] * cs[e] + x[i][e] * sn[e];
+            x[i][e] = u;
+            x[i][e + 4] = v;
+          }
       }
     }
-    if (h >= per) continue;
-    if (h < n_q) {
-      store_vec16<TI, E>(reinterpret_cast<TI*>(a.q_out) + (size_t)row * a.ldo + (size_t)h * HD + d, x);
-    } else {
-      const int which = h >= n_q + n_kv, kvh = h - n_q - which * n_kv;
-      const size_t at = ((((size_t)page * a.kv.n_layers + a.layer) * 2 + which) * n_kv + kvh) * 16 + (r.pos & 15);
-      store_vec16<TC, E>(reinterpret_cast<TC*>(a.kv.pool) + at * HD + d, x);
-    }
+  }
+  if (kind == 0) {
+    store_heads<TI, U, HPW>(reinterpret_cast<TI*>(a.q_out) + (size_t)row * a.ldo + h0 * HD, HD, h0, n, d0, d1, x);
+  } else {
+    const size_t at = ((((size_t)page * a.kv.n_layers + a.layer) * 2 + (kind - 1)) * n + h0) * 16 + (r.pos & 15);
+    store_heads<TC, U, HPW>(reinterpret_cast<TC*>(a.kv.pool) + at * HD, 16 * HD, h0, n, d0, d1, x);
   }
 }
 
 template <int HD, class TI, class TC>
 cudaError_t launch_types(const RowAppendArgs& a, int num_sms, cudaStream_t s) {
-  constexpr int E = 16 / sizeof(TI), HPW = 32 / (HD / E);
+  constexpr int HPW = 32 / (HD / 8), CHUNK = 4 * sizeof(TI);
   const long long per = (a.q ? a.n_heads : 0) + 2 * a.kv.n_kv;
-  auto bad = [&](const void* p, int64_t ld) { return p && ((reinterpret_cast<uintptr_t>(p) | (size_t)ld * sizeof(TI)) & 15); };
+  auto bad = [&](const void* p, int64_t ld) {
+    return p && ((reinterpret_cast<uintptr_t>(p) | (size_t)ld * sizeof(TI)) & (CHUNK - 1));
+  };
   const uintptr_t tables = reinterpret_cast<uintptr_t>(a.rope) | reinterpret_cast<uintptr_t>(a.q_norm) |
                            reinterpret_cast<uintptr_t>(a.k_norm);
-  const bool vec = !(tables & 15) && !bad(a.q, a.ldq) && !bad(a.k, a.ldk) && !bad(a.v, a.ldv) && !bad(a.q_out, a.ldo) &&
-                   (a.adjacent || a.rotary / 2 % E == 0);
-  if (!vec) {
+  if ((tables & 15) || bad(a.q, a.ldq) || bad(a.k, a.ldk) || bad(a.v, a.ldv) || bad(a.q_out, a.ldo)) {
     const long long warps = a.n_rows * per;
     rows_append_kernel<HD, TI, TC><<<(unsigned)((warps + 7) / 8), 256, 0, s>>>(a);
     return cudaGetLastError();
   }
-  // one group a warp while that leaves no SM with more than a few warps, else four
-  const long long one = (per + HPW - 1) / HPW;
-  if (a.n_rows * one <= 32ll * num_sms) {
-    rows_append_vec_kernel<HD, TI, TC, 1><<<(unsigned)((a.n_rows * one + 7) / 8), 256, 0, s>>>(a, (int)one);
-  } else {
-    const long long four = (per + 4 * HPW - 1) / (4 * HPW);
-    rows_append_vec_kernel<HD, TI, TC, 4><<<(unsigned)((a.n_rows * four + 7) / 8), 256, 0, s>>>(a, (int)four);
-  }
+  auto run = [&](auto u) {
+    constexpr int U = decltype(u)::value, S = HPW * U;
+    const int gq = a.q ? (a.n_heads + S - 1) / S : 0, gk = (a.kv.n_kv + S - 1) / S, groups = gq + 2 * gk;
+    rows_append_vec_kernel<HD, TI, TC, U>
+        <<<(unsigned)(((long long)a.n_rows * groups + 7) / 8), 256, 0, s>>>(a, groups, gq, gk);
+  };
+  // one group of heads a warp while that leaves no SM with more than 32 warps, else four
+  if (a.n_rows * ((per + HPW - 1) / HPW) <= 32ll * num_sms) run(std::integral_constant<int, 1>());
+  else run(std::integral_constant<int, 4>());
   return cudaGetLastError();
 }
 
