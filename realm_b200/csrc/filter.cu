@@ -11,7 +11,7 @@
 // and the draw takes the first index whose running sum of kept W exceeds
 // floor(u sum W). t < 1e-7 takes the first rank.
 //
-// A cluster of CTAs holds one row in registers: each CTA a contiguous share of its
+// A cluster of CTAs holds one row in shared memory: each CTA a contiguous share of its
 // 16-byte vectors, thread t the vectors t, t + 1024, ... of the share. Thresholds come
 // from a radix walk over the bits of w: first its binade (W has 40 bits, so 41 of
 // them), then the 23 bits of its mantissa in digits of 8, 8 and 7, until a bin is kept
@@ -22,9 +22,10 @@
 // two lanes of a warp meet); mantissas are spread, and there only the elements of the
 // chosen binade count.
 //
-// Bound by instructions (about 50 an element) and, for few rows, by the chain of
-// barriers: 96 rows of 151937 took 315 us with the rows in shared memory and 64-bit
-// atomics, 208 us with the 32-bit histograms.
+// Bound by the chain of barriers (about ten) and by instructions: 96 rows of 151937 take
+// 101 us with the elements in shared memory and two CTAs an SM, took 129 us with them in
+// registers (one CTA an SM), 208 us with chunks of consecutive elements a thread, 315 us
+// with 64-bit atomics. One row of 32000: 12 us.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -137,6 +138,31 @@ struct Cluster {
   }
 };
 
+// A thread's elements: NQ quads, kFT apart in shared memory, which no other thread touches.
+template <int NQ, class F>
+__device__ __forceinline__ void each(const float4* mine, F f) {
+#pragma unroll 2
+  for (int q = 0; q < NQ; ++q) {
+    const float4 v = mine[q * kFT];
+    f(v.x);
+    f(v.y);
+    f(v.z);
+    f(v.w);
+  }
+}
+template <int NQ, class F>
+__device__ __forceinline__ void change(float4* mine, F f) {
+#pragma unroll 2
+  for (int q = 0; q < NQ; ++q) {
+    float4 v = mine[q * kFT];
+    v.x = f(v.x);
+    v.y = f(v.y);
+    v.z = f(v.z);
+    v.w = f(v.w);
+    mine[q * kFT] = v;
+  }
+}
+
 // What is kept: weights with more than `bits`, and the first `ties` of those with
 // just these bits, of which there are `equal`.
 struct Cut {
@@ -190,8 +216,8 @@ __device__ void choose(uint32_t c, u64 w, int n, u64 want, u64& acc_c, u64& acc_
 
 // The cut of one rule. bc, bw: this thread's binade (thread t < kBinades holds binade
 // t). total: the sum of what it keeps.
-template <bool COUNT, int NEL, int N>
-__device__ Cut radix_cut(const float (&x)[NEL], uint32_t bc, u64 bw, u64 want, Cluster<N>& cl, u64& total) {
+template <bool COUNT, int NQ, int N>
+__device__ Cut radix_cut(const float4* mine, uint32_t bc, u64 bw, u64 want, Cluster<N>& cl, u64& total) {
   FilterShared& s = cl.s;
   const int tid = threadIdx.x;
   u64 acc_c = 0, acc_s = 0;
@@ -209,17 +235,16 @@ __device__ Cut radix_cut(const float (&x)[NEL], uint32_t bc, u64 bw, u64 want, C
     uint32_t *cnt = s.cnt[turn], *lo = s.lo[turn], *hi = s.hi[turn];
     if (tid < kBins) cnt[tid] = lo[tid] = hi[tid] = 0;
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < NEL; ++i) {
-      const uint32_t b = __float_as_uint(x[i]);
+    each<NQ>(mine, [&](float x) {
+      const uint32_t b = __float_as_uint(x);
       if ((b & hmask) == pre) {
         int e;
-        const uint32_t v = part_of(x[i], e), bin = (b >> sh) & ((1u << width) - 1);
+        const uint32_t v = part_of(x, e), bin = (b >> sh) & ((1u << width) - 1);
         atomicAdd(&cnt[bin], 1u);
         atomicAdd(&lo[bin], v & 1023u);
         atomicAdd(&hi[bin], v >> 10);
       }
-    }
+    });
     cl.sync();
     // thread t owns bin 2^width - 1 - t
     uint32_t c = 0;
@@ -244,9 +269,17 @@ __device__ Cut radix_cut(const float (&x)[NEL], uint32_t bc, u64 bw, u64 want, C
   return r;
 }
 
+// Two CTAs an SM (32 registers a thread) where their elements fit and keep a CTA busy
+// for long enough: one works while the other waits at a barrier.
+template <class T, int NV>
+constexpr int two_ctas() {
+  return NV >= 3 && NV * (16 / (int)sizeof(T)) <= 24 ? 2 : 1;
+}
+
 template <class T, int NV, int N>
-__global__ void __launch_bounds__(kFT) filter_kernel(const __grid_constant__ FilterArgs a) {
-  constexpr int E = 16 / sizeof(T), NEL = NV * E;
+__global__ void __launch_bounds__(kFT, two_ctas<T, NV>()) filter_kernel(const __grid_constant__ FilterArgs a) {
+  constexpr int E = 16 / sizeof(T), Q = E / 4, NQ = NV * Q;  // quads of a vector, of a thread
+  extern __shared__ float4 quads[];
   __shared__ FilterShared s;
   Cluster<N> cl(s);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -261,28 +294,31 @@ __global__ void __launch_bounds__(kFT) filter_kernel(const __grid_constant__ Fil
   const int vecs = (V + mis + E - 1) / E, share = (vecs + N - 1) / N;
   const int v0 = cl.rank * share, v1 = min(vecs, v0 + share);
   auto index = [&](int r) { return (v0 + r * kFT + tid) * E - mis; };  // of vector round r's first element
-  float x[NEL];
+  float4* mine = quads + tid;
 #pragma unroll
   for (int r = 0; r < NV; ++r) {
     const int i = index(r);
     const bool in = v0 + r * kFT + tid < v1;
+    float x[E];
     if (in && i >= 0 && i + E <= V) {
       const uint4 q = __ldcs(reinterpret_cast<const uint4*>(lg + i));
       const T* y = reinterpret_cast<const T*>(&q);
 #pragma unroll
-      for (int e = 0; e < E; ++e) x[r * E + e] = (float)y[e];
+      for (int e = 0; e < E; ++e) x[e] = (float)y[e];
     } else {
 #pragma unroll
-      for (int e = 0; e < E; ++e) x[r * E + e] = in && i + e >= 0 && i + e < V ? (float)lg[i + e] : -INFINITY;
+      for (int e = 0; e < E; ++e) x[e] = in && i + e >= 0 && i + e < V ? (float)lg[i + e] : -INFINITY;
     }
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (x[e] != x[e]) x[e] = -INFINITY;
+#pragma unroll
+    for (int h = 0; h < Q; ++h) mine[(r * Q + h) * kFT] = make_float4(x[4 * h], x[4 * h + 1], x[4 * h + 2], x[4 * h + 3]);
   }
   for (int i = tid; i < kBinades * 32; i += kFT) s.ba[i] = s.bb[i] = 0;
   const float t = p.temperature;
   const bool greedy = !(t >= 1e-7f);
   float top = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < NEL; ++i)
-    if (x[i] != x[i]) x[i] = -INFINITY;
   if (a.prev_off && p.repetition_penalty != 1.0f) {
     // one thread applies all occurrences of a token, in order
     const uint32_t j1 = a.prev_off[row + 1];
@@ -290,24 +326,20 @@ __global__ void __launch_bounds__(kFT) filter_kernel(const __grid_constant__ Fil
       const uint32_t tok = a.prev[j];
       const int at = tok < (uint32_t)V ? (int)tok + mis : -1, local = at / E - v0;
       if (at >= 0 && local >= 0 && at / E < v1 && local % kFT == tid) {
-        const int k = local / kFT * E + at % E;
-#pragma unroll
-        for (int i = 0; i < NEL; ++i)
-          if (i == k) x[i] = x[i] > 0.f ? __fdiv_rn(x[i], p.repetition_penalty) : __fmul_rn(x[i], p.repetition_penalty);
+        float& x = reinterpret_cast<float*>(mine + (local / kFT * Q + at % E / 4) * kFT)[at % 4];
+        x = x > 0.f ? __fdiv_rn(x, p.repetition_penalty) : __fmul_rn(x, p.repetition_penalty);
       }
     }
   }
-  if (!greedy && t != 1.f)
-#pragma unroll
-    for (int i = 0; i < NEL; ++i) x[i] = __fdiv_rn(x[i], t);
-#pragma unroll
-  for (int i = 0; i < NEL; ++i) top = fmaxf(top, x[i]);
+  if (!greedy && t != 1.f) change<NQ>(mine, [&](float x) { return __fdiv_rn(x, t); });
+  each<NQ>(mine, [&](float x) { top = fmaxf(top, x); });
   u64 best = (u64)float_order_key(top) << 32;
   if (greedy) {  // and the lowest index that has it
     uint32_t at = 0xffffffffu;
-#pragma unroll
-    for (int i = NEL - 1; i >= 0; --i)
-      if (x[i] == top && top != -INFINITY) at = (uint32_t)(index(i / E) + i % E);
+    for (int q = NQ - 1; q >= 0; --q)
+      for (int e = 3; e >= 0; --e)
+        if (reinterpret_cast<float*>(mine + q * kFT)[e] == top && top != -INFINITY)
+          at = (uint32_t)(index(q / Q) + q % Q * 4 + e);
     best |= 0xffffffffu - at;
   }
   best = warp_max(best);
@@ -332,18 +364,17 @@ __global__ void __launch_bounds__(kFT) filter_kernel(const __grid_constant__ Fil
   }
   const bool use_k = p.top_k > 0 && p.top_k < (uint32_t)V, use_p = p.top_p > 0.f && p.top_p < 1.f;
   const bool hist = use_k || use_p;
-#pragma unroll
-  for (int i = 0; i < NEL; ++i) {
-    float w = x[i] == m ? 1.f : expf(x[i] - m);
+  change<NQ>(mine, [&](float x) {
+    const float w = x == m ? 1.f : expf(x - m);
     int b;
     const uint32_t v = part_of(w, b);
     const bool in = w >= p.min_p && v != 0;  // v 0: below the fixed point, never drawn
-    x[i] = in ? w : 0.f;
     if (hist && in) {
       atomicAdd(&s.ba[b * 32 + lane], 1u << 21 | (v & 1023u));
       atomicAdd(&s.bb[b * 32 + lane], v >> 10);
     }
-  }
+    return in ? w : 0.f;
+  });
   if (hist) {
     Cut cut{0u, 0xffffffffu, 0xffffffffu};
     // the row's binades: sums over the lanes' copies, then over the cluster
@@ -368,7 +399,7 @@ __global__ void __launch_bounds__(kFT) filter_kernel(const __grid_constant__ Fil
     }
     u64 total = 0;
     if (use_k) {
-      cut = radix_cut<true, NEL, N>(x, bc, bw, p.top_k, cl, total);
+      cut = radix_cut<true, NQ, N>(mine, bc, bw, p.top_k, cl, total);
     } else {
       if (tid < 64) {  // two warps hold the binades
         const u64 y = warp_scan(bw);
@@ -381,45 +412,37 @@ __global__ void __launch_bounds__(kFT) filter_kernel(const __grid_constant__ Fil
     if (use_p) {
       u64 want = (u64)((double)total * (double)p.top_p);
       if (want < 1) want = 1;
-      const Cut c = radix_cut<false, NEL, N>(x, bc, bw, want, cl, total);
+      const Cut c = radix_cut<false, NQ, N>(mine, bc, bw, want, cl, total);
       // never below the first cut; at the same weight, the fewer ties
       if (c.bits > cut.bits || (c.bits == cut.bits && c.ties < cut.ties)) cut = c;
     }
     // kept: bits above the cut, and its ties with the lowest indices
-#pragma unroll
-    for (int i = 0; i < NEL; ++i)
-      if (__float_as_uint(x[i]) < cut.bits) x[i] = 0.f;
+    change<NQ>(mine, [&](float x) { return __float_as_uint(x) < cut.bits ? 0.f : x; });
     if (cut.ties < cut.equal) {  // the same in every thread of the cluster
-      u64 mine = 0, cta;
-#pragma unroll
-      for (int i = 0; i < NEL; ++i) mine += __float_as_uint(x[i]) == cut.bits;
-      block_scan(mine, s.red, cta);
+      u64 count = 0, cta;
+      each<NQ>(mine, [&](float x) { count += __float_as_uint(x) == cut.bits; });
+      block_scan(count, s.red, cta);
       u64 before = 0;
       if (N > 1) {
         const u64* all = cl.share(cta);
         for (int r = 0; r < cl.rank; ++r) before += all[r];
       }
-#pragma unroll
       for (int r = 0; r < NV; ++r) {
         u64 eq = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) eq += __float_as_uint(x[r * E + e]) == cut.bits;
+        each<Q>(mine + r * Q * kFT, [&](float x) { eq += __float_as_uint(x) == cut.bits; });
         u64 round;
         u64 rank = before + block_scan(eq, s.red, round);
         before += round;
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (__float_as_uint(x[r * E + e]) == cut.bits && rank++ >= cut.ties) x[r * E + e] = 0.f;
+        change<Q>(mine + r * Q * kFT, [&](float x) { return __float_as_uint(x) == cut.bits && rank++ >= cut.ties ? 0.f : x; });
       }
     }
   }
   // the draw: rounds of vectors, then warps, then lanes are in the order of the indices
-#pragma unroll
   for (int r = 0; r < NV; ++r) {
     u64 w = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (x[r * E + e] != 0.f) w += fix(x[r * E + e]);
+    each<Q>(mine + r * Q * kFT, [&](float x) {
+      if (x != 0.f) w += fix(x);
+    });
     w = warp_sum43(w);
     if (lane == 0) s.part[r][warp] = w;
   }
@@ -458,31 +481,34 @@ __global__ void __launch_bounds__(kFT) filter_kernel(const __grid_constant__ Fil
   if (warp != (int)s.warp) return;
   const int round = (int)s.round;
   u64 w = 0;
-#pragma unroll
-  for (int i = 0; i < NEL; ++i)
-    if (i / E == round) w += fix(x[i]);
+  each<Q>(mine + round * Q * kFT, [&](float x) { w += fix(x); });
   u64 at = s.base + warp_scan(w) - w;
   if (at <= target && target < at + w) {
+    int i = index(round);
     bool found = false;
-#pragma unroll
-    for (int i = 0; i < NEL; ++i)
-      if (i / E == round && !found) {
-        const u64 f = fix(x[i]);
-        if (at + f > target) {
-          a.tokens[row] = (uint32_t)(index(i / E) + i % E);
-          if (a.probs) a.probs[row] = (float)((double)f / (double)total);
-          found = true;
-        }
-        at += f;
+    each<Q>(mine + round * Q * kFT, [&](float x) {
+      const u64 f = fix(x);
+      if (!found && at + f > target) {
+        a.tokens[row] = (uint32_t)i;
+        if (a.probs) a.probs[row] = (float)((double)f / (double)total);
+        found = true;
       }
+      at += f;
+      ++i;
+    });
   }
 }
 
 template <class T, int NV, int N>
 cudaError_t launch(const FilterArgs& a, cudaStream_t s) {
+  constexpr int smem = NV * kFT * (16 / (int)sizeof(T)) * 4;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (cudaError_t e = ensure_smem_attr(filter_kernel<T, NV, N>, smem, dev)) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.n_rows * N));
   cfg.blockDim = dim3(kFT);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute at;
   at.id = cudaLaunchAttributeClusterDimension;
@@ -499,6 +525,10 @@ cudaError_t launch_type(const FilterArgs& a, cudaStream_t s) {
   // vectors of a row, wherever it starts, and of a thread in a cluster of n
   const int vecs = (a.vocab + E - 1 + E - 1) / E;
   auto rounds = [&](int n) { return ((vecs + n - 1) / n + kFT - 1) / kFT; };
+  // as few CTAs as give every thread one vector, up to eight
+  if (rounds(1) <= 1) return launch<T, 1, 1>(a, s);
+  if (rounds(2) <= 1) return launch<T, 1, 2>(a, s);
+  if (rounds(4) <= 1) return launch<T, 1, 4>(a, s);
   const int r8 = rounds(8);
   if (r8 <= 1) return launch<T, 1, 8>(a, s);
   if (r8 <= 2) return launch<T, 2, 8>(a, s);
