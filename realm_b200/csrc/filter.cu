@@ -519,33 +519,44 @@ cudaError_t launch(const FilterArgs& a, cudaStream_t s) {
   return cudaLaunchKernelEx(&cfg, filter_kernel<T, NV, N>, a);
 }
 
-template <class T>
-cudaError_t launch_type(const FilterArgs& a, cudaStream_t s) {
+template <class T, int N>
+cudaError_t launch_rounds(const FilterArgs& a, int rounds, cudaStream_t s) {
   constexpr int E = 16 / sizeof(T);
-  // vectors of a row, wherever it starts, and of a thread in a cluster of n
-  const int vecs = (a.vocab + E - 1 + E - 1) / E;
-  auto rounds = [&](int n) { return ((vecs + n - 1) / n + kFT - 1) / kFT; };
-  // as few CTAs as give every thread one vector, up to eight
-  if (rounds(1) <= 1) return launch<T, 1, 1>(a, s);
-  if (rounds(2) <= 1) return launch<T, 1, 2>(a, s);
-  if (rounds(4) <= 1) return launch<T, 1, 4>(a, s);
-  const int r8 = rounds(8);
-  if (r8 <= 1) return launch<T, 1, 8>(a, s);
-  if (r8 <= 2) return launch<T, 2, 8>(a, s);
-  if (r8 <= 3) return launch<T, 3, 8>(a, s);
+  if (rounds <= 1) return launch<T, 1, N>(a, s);
+  if (rounds <= 2) return launch<T, 2, N>(a, s);
+  if (rounds <= 3) return launch<T, 3, N>(a, s);
   if constexpr (E == 4) {
-    if (r8 <= 5) return launch<T, 5, 8>(a, s);
-    return launch<T, 9, 8>(a, s);
+    if (rounds <= 5) return launch<T, 5, N>(a, s);
+    if constexpr (N == 8) return launch<T, 9, N>(a, s);
   } else {
-    return r8 <= 4 ? launch<T, 4, 8>(a, s) : launch<T, 5, 8>(a, s);
+    if constexpr (N == 8) return launch<T, 5, N>(a, s);
+  }
+  return cudaErrorInvalidValue;
+}
+
+// CTAs a row: as few as hold it with two CTAs an SM, and then more while all rows'
+// CTAs stay resident at once and a thread has more than one vector. 96 rows of 32000
+// (2 CTAs a row, one wave): 36 us; with 8 CTAs a row 79 us; one row of 32000 wants 8.
+template <class T>
+cudaError_t launch_type(const FilterArgs& a, int num_sms, cudaStream_t s) {
+  constexpr int E = 16 / sizeof(T);
+  const int vecs = (a.vocab + E - 1 + E - 1) / E;  // of a row, wherever it starts
+  auto rounds = [&](int n) { return ((vecs + n - 1) / n + kFT - 1) / kFT; };
+  int n = 1;
+  while (n < kMaxCluster && rounds(n) > (E == 4 ? 5 : 3)) n *= 2;
+  while (n < kMaxCluster && rounds(n) > 1 && (long long)a.n_rows * n * 2 <= 2ll * num_sms) n *= 2;
+  switch (n) {
+    case 1: return launch_rounds<T, 1>(a, rounds(1), s);
+    case 2: return launch_rounds<T, 2>(a, rounds(2), s);
+    case 4: return launch_rounds<T, 4>(a, rounds(4), s);
+    default: return launch_rounds<T, 8>(a, rounds(8), s);
   }
 }
 
 }  // namespace
 
 cudaError_t filter_launch(const FilterArgs& a, int num_sms, cudaStream_t s) {
-  (void)num_sms;
-  return a.x16 ? launch_type<__half>(a, s) : launch_type<float>(a, s);
+  return a.x16 ? launch_type<__half>(a, num_sms, s) : launch_type<float>(a, num_sms, s);
 }
 
 }  // namespace rb

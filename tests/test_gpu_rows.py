@@ -512,7 +512,7 @@ FILTERS = [(0.0, 0, 1.0, 0.0), (1.0, 0, 1.0, 0.0), (0.7, 40, 1.0, 0.0), (1.0, 0,
            (1.0, 0, 1.0, 0.1), (1.0, 1, 1.0, 0.0), (0.9, 10 ** 6, 0.5, 0.0), (2.0, 7, 1e-9, 0.0), (1.0, 0, 0.8, 5.0)]
 
 
-@pytest.mark.parametrize("V", [1, 2, 7, 1000, 8193, 32000, 151937])
+@pytest.mark.parametrize("V", [1, 2, 7, 1000, 8193, 21000, 32000, 100000, 151937, 262144])
 @pytest.mark.parametrize("typ", ["float32", "float16"])
 def test_sample_filtered(ctx, V, typ):
     import torch
@@ -583,3 +583,23 @@ def test_sample_frequencies(ctx):
     got = rb.sample_filtered(ctx, x, [f] * n, ((np.arange(n) + 0.5) / n).astype(np.float32))
     p = np.array([_sample_ref(x[0], f, (i + 0.5) / n)[0] for i in range(n)])
     assert (np.bincount(got, minlength=V) == np.bincount(p, minlength=V)).all()
+
+
+@pytest.mark.parametrize("typ", ["float32", "float16"])
+@pytest.mark.parametrize("V", [3000, 9001, 23001, 40003, 90001])
+def test_sample_many_rows(ctx, V, typ):
+    """Many rows take fewer CTAs each: the same tokens as one row at a time, for every vocabulary range."""
+    import torch
+    import realm_b200 as rb
+    n = 300
+    g = torch.Generator("cuda").manual_seed(V)
+    x = (torch.randn(n, V, device="cuda", generator=g) * 3).to(getattr(torch, typ))
+    u = torch.rand(n, device="cuda", generator=g)
+    fs = [rb.SamplingFilter(0.9, 60 if i % 2 else 0, 0.9 if i % 3 else 1.0, 0.001) for i in range(n)]
+    probs = torch.empty(n, device="cuda")
+    got = rb.sample_filtered(ctx, x, rb.pack_filters(fs, "cuda"), u, probs=probs)
+    for i in range(0, n, 23):
+        tok, p = _sample_ref(x[i].cpu().numpy(), fs[i], float(u[i]))
+        assert got[i].item() == tok and abs(probs[i].item() - p) <= 2.0 ** -22 * p
+        one = rb.sample_filtered(ctx, x[i:i + 1], rb.pack_filters(fs[i:i + 1], "cuda"), u[i:i + 1])
+        assert one.item() == tok
