@@ -63,17 +63,29 @@ void rows_partition(const std::vector<RowInfo>& rows, int n_heads, int n_kv, int
   // Small items: every warp works for itself. The warps go in groups of n_kv, one for
   // each kv head, and every group takes an equal contiguous share of all items' pages:
   // the heads of a page lie next to one another in memory and are read at the same
-  // time. With few pages a group (at least four), a share does not cross into another
-  // item, since starting on a second one takes a warp as long as several pages.
+  // time. With few pages a group, a share does not cross into another item, since
+  // starting on a second one takes a warp as long as several pages.
   if (!small.empty()) {
-    long long pages = 0;
+    long long pages = 0, longest = 0;
     for (const Item& it : small) {
       pages += blocks_of(it, kRowPage);
+      longest = std::max<long long>(longest, blocks_of(it, kRowPage));
       out.max_nv = std::max(out.max_nv, it.nv);
     }
     const long long most = std::max(1ll, 2ll * kRowWarps * num_sms / n_kv);  // groups
-    const long long share = std::max<long long>(4, (pages + most - 1) / most);
+    long long share = (pages + most - 1) / most;
     const bool apart = share <= 8;
+    if (apart) {
+      // A page takes a warp about 0.8 us, sixteen parts their join about 1 us: for one
+      // tenant of 513 tokens 3 pages a warp and one round of joining (10.3 us in all)
+      // against 4 pages (12.3 us); of 4096 tokens 4 and four (16.4) against 2 and eight (20.5).
+      long long best = 0, at = share;
+      for (long long s = std::max(2ll, share); s <= 8; ++s) {
+        const long long parts = (longest + s - 1) / s, cost = 8 * s + (parts > 1 ? 10 * ((parts + 15) / 16) : 0);
+        if (!best || cost < best) best = cost, at = s;
+      }
+      share = at;
+    }
     struct Piece {
       int item, p0, p1, slot, parts;
     };
