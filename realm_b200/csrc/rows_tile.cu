@@ -14,6 +14,8 @@
 //
 // Warps: 0-3 softmax of tile 0, 4-7 of tile 1, 8 issues the products, 9 the loads (10
 // and 11 fill the last warpgroup, which gives registers to the others).
+#include <type_traits>
+
 #include "common.cuh"
 #include "rows.cuh"
 
@@ -169,13 +171,17 @@ struct Fused {
     return HL ? k[i] : k3[i < 3 ? i : 0];
   }
 };
-// The wider form, 4e-09.
+// For larger scores: 3e-07 and 5e-09.
+template <int HL>
 struct Wide {
-  static constexpr int N = 6;
-  static constexpr float limit = 0.625f;
+  static constexpr int N = HL ? 9 : 7;
+  static constexpr float limit = 1.2f;
   static __device__ __forceinline__ float c(int i) {
-    constexpr float k[6] = {0.999999996f, -0.333332605f, 0.133311275f, -0.053721068f, 0.0205909884f, -0.00565998907f};
-    return k[i];
+    constexpr float k[9] = {1.f,           -0.333332747f,  0.133322015f,   -0.0538841411f, 0.0215497930f,
+                            -0.00815800484f, 0.00262519997f, -0.000594539568f, 6.65760599e-05f},
+                    k7[7] = {0.999999583f,    -0.333305687f,  0.133013666f,  -0.0525437407f,
+                             0.0187073722f, -0.00493616611f, 0.000659012294f};
+    return HL ? k[i] : k7[i < 7 ? i : 0];
   }
 };
 // named barrier `id` of n threads, with the "or" of their values
@@ -191,11 +197,6 @@ __device__ __forceinline__ bool any_softmax(int id, int n, bool v) {
 }
 // the sign bits of the two halves of w that are infinite or not a number
 __device__ __forceinline__ uint32_t not_finite(uint32_t w) { return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u; }
-
-template <bool V>
-struct Flag {
-  static constexpr bool value = V;
-};
 
 template <int HD, int HL>
 struct TileCfg {
@@ -470,6 +471,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
       if (!HL) kp *= kcap * kcap;
     }
     const bool fuse_ok = HL || (kcap > 1e-6f && kcap < 1e4f && cap2 < 1e6f);
+    // How the warp applies the cap: 1 Fused and 2 Wide, together with the exponential; 3 on its
+    // own, with no bound on the scores. One prompt of 8192, 32 heads of 128: fp16 rows 575,
+    // 713 and 1000 us, fp32 rows 1027, about 1200 and 1290. A larger score raises the form for
+    // good: with one chosen for each block, warps that went back and forth between two of
+    // them took longer than with either (fp16 rows, 1 and 2: 993 us).
+    int form = !__all_sync(0xffffffffu, kcap > 1e-30f) ? 3 : BIAS || !__all_sync(0xffffffffu, fuse_ok) ? 2 : 1;
     float m = -INFINITY, l = 0.f;
     for (int j = 0; j < nb; ++j) {
       const int kb = u.k0 + j * B;
@@ -484,9 +491,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
         mbar_arrive(&s_free);
       }
       const bool partial = kb < all0 || kb + B > all1;  // the same for the whole tile
-      bool fused = false;  // the cap is applied together with the exponential
-      if (CAP) {
-        // the largest magnitude of the warp's scores, unseen keys' included
+      if (CAP && kb + B > u.k1) {  // keys past the end may be anything and do not choose the form
+        const int n = u.k1 - kb;
+#pragma unroll
+        for (int i = 0; i < B; ++i) x[i] = i < n ? x[i] : 0.f;
+      }
+      if (CAP && form < 3) {  // the largest magnitude of the warp's scores, unseen keys' included
         float lo4[4] = {0.f, 0.f, 0.f, 0.f}, hi4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < B; i += 8)
@@ -498,24 +508,28 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
           for (int q = 0; q < 4; ++q) hi4[q] = max3(hi4[q], x[i + 2 * q], x[i + 2 * q + 1]);
         const float top = fmaxf(max3(fmaxf(hi4[0], hi4[1]), hi4[2], hi4[3]),
                                 -min3(fminf(lo4[0], lo4[1]), lo4[2], lo4[3]));
-        fused = !BIAS && fuse_ok && __all_sync(0xffffffffu, top * kcap <= Fused<HL>::limit);
-        if (!fused) {
-          if (__all_sync(0xffffffffu, top * kcap <= Wide::limit)) {
-            const f2 k2 = pair(kcap, kcap);
+        const float far = top * kcap;
+        if (!__all_sync(0xffffffffu, far <= Wide<HL>::limit)) form = 3;
+        else if (!__all_sync(0xffffffffu, far <= Fused<HL>::limit)) form = 2;
+      }
+      const bool fused = CAP && !BIAS && form < 3;
+      if (CAP && !fused) {
+        if (form == 2) {
+          using P = Wide<HL>;
+          const f2 k2 = pair(kcap, kcap);
 #pragma unroll
-            for (int i = 0; i < B; i += 2) {
-              const f2 y = mul2(pair(x[i], x[i + 1]), k2), z = mul2(y, y);
-              f2 t = pair(cap2 * Wide::c(Wide::N - 1), cap2 * Wide::c(Wide::N - 1));
+          for (int i = 0; i < B; i += 2) {
+            const f2 y = mul2(pair(x[i], x[i + 1]), k2), z = mul2(y, y);
+            f2 t = pair(cap2 * P::c(P::N - 1), cap2 * P::c(P::N - 1));
 #pragma unroll
-              for (int q = Wide::N - 2; q >= 0; --q) t = fma2(t, z, pair(cap2 * Wide::c(q), cap2 * Wide::c(q)));
-              unpair(mul2(t, y), x[i], x[i + 1]);
-            }
-          } else {
-            // cap tanh(y) = cap - 2 cap / (1 + e^(2 y))
-            const float k = 2.f * kLog2e * kcap;
-#pragma unroll
-            for (int i = 0; i < B; ++i) x[i] = fmaf(-2.f * cap2, rcp(1.f + ex2(x[i] * k)), cap2);
+            for (int q = P::N - 2; q >= 0; --q) t = fma2(t, z, pair(cap2 * P::c(q), cap2 * P::c(q)));
+            unpair(mul2(t, y), x[i], x[i + 1]);
           }
+        } else {
+          // cap tanh(y) = cap - 2 cap / (1 + e^(2 y))
+          const float k = 2.f * kLog2e * kcap;
+#pragma unroll
+          for (int i = 0; i < B; ++i) x[i] = fmaf(-2.f * cap2, rcp(1.f + ex2(x[i] * k)), cap2);
         }
       }
       if (BIAS) {
@@ -580,11 +594,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
       // Groups of 16 keys, every step for the whole group before the next one: the
       // steps of a key wait for one another, the keys do not.
       auto exps = [&](auto capped) {
-        constexpr bool FUSED = decltype(capped)::value;
-        using P = Fused<HL>;
+        constexpr int FUSED = decltype(capped)::value;
+        using P = std::conditional_t<FUSED == 2, Wide<HL>, Fused<HL>>;
         f2 pc[P::N];
 #pragma unroll
-        for (int q = 0; q < P::N; ++q) pc[q] = pair(coef[q], coef[q]);
+        for (int q = 0; q < P::N; ++q) {
+          const float c = FUSED == 2 ? cap2 * P::c(q) : coef[q < Fused<HL>::N ? q : 0];
+          pc[q] = pair(c, c);
+        }
         constexpr int G = 8;  // pairs
 #pragma unroll
         for (int i = 0; i < B / 32; ++i) {
@@ -597,7 +614,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
             for (int g = 0; g < G; ++g) y[g] = pair(x[32 * i + 2 * G * h + 2 * g], x[32 * i + 2 * G * h + 2 * g + 1]);
             if (FUSED) {
               f2 z[G], t[G];
-              if (HL) {  // rows have scales of their own, too far apart for powers of them
+              if (HL || FUSED == 2) {  // fp32 rows have scales of their own, too far apart for powers of them
                 const f2 k2 = pair(kcap, kcap);
 #pragma unroll
                 for (int g = 0; g < G; ++g) y[g] = mul2(y[g], k2);
@@ -635,8 +652,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
           if (HL) st16(tp + C::pcol(2 * i, 1), lo);
         }
       };
-      if (CAP && fused) exps(Flag<true>());
-      else exps(Flag<false>());
+      if (fused && form == 1) exps(std::integral_constant<int, 1>());
+      else if (fused) exps(std::integral_constant<int, 2>());
+      else exps(std::integral_constant<int, 0>());
       {
         float p0, p1;
         unpair(add2(s2[0], s2[1]), p0, p1);

@@ -126,7 +126,7 @@ def _attn_ref(q, k, v, pos, lo, hi, scale, cap, slopes):
         for h in range(H):
             kk, vv = k[lo[r]:hi[r], h // rep], v[lo[r]:hi[r], h // rep]
             x = kk @ q[r, h] * scale
-            amp = max(amp, (np.abs(kk) @ np.abs(q[r, h])).max() * scale)
+            amp = max(amp, (np.abs(kk) @ np.abs(q[r, h])).max() * abs(scale))
             if cap:
                 x = cap * np.tanh(x / cap)
             if slopes is not None:
@@ -137,7 +137,7 @@ def _attn_ref(q, k, v, pos, lo, hi, scale, cap, slopes):
 
 
 def _check_attention(ctx, hd, H, kv, typ, cache, tenants, cap=0.0, bias=False, window=0, q_scale=1.0, strided=False,
-                     dirty=None, seed=0):
+                     dirty=None, seed=0, scale=None):
     """tenants: (cached length, rows' positions, begin, end) each; begin/end None: the defaults."""
     import torch
     import realm_b200 as rb
@@ -163,7 +163,7 @@ def _check_attention(ctx, hd, H, kv, typ, cache, tenants, cap=0.0, bias=False, w
         n = len(ten)
         q = (rng.normal(0, q_scale, (n, H, hd))).astype(typ)
         slopes = (2.0 ** -np.arange(1, H + 1)).astype(np.float32) if bias else None
-        scale = 1 / np.sqrt(hd)
+        scale = 1 / np.sqrt(hd) if scale is None else scale
         dq = torch.from_numpy(q).cuda()
         out = None
         if strided:
@@ -248,6 +248,23 @@ def test_masks(ctx, typ, cache, hd, H, kv, kind):
         beg, end = np.array([2, 200, 17, 0, 0]), np.array([3, 290, 18, 290, 1])
     _check_attention(ctx, hd, H, kv, typ, cache, [(n, pos, beg, end), (40, [39], [40], [40]), (40, [39], [0], [0])],
                      cap=10.0 if kind == "prefix" else 0.0, bias=kind == "prefix", window=window)
+
+
+@pytest.mark.parametrize("typ,cache", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("cap", [3.0, 10.0, 22.0, 60.0])
+def test_caps(ctx, typ, cache, hd, cap):
+    """Scores from far below the cap to far above it, in rows that see different keys, over several blocks."""
+    _check_attention(ctx, hd, 4, 1, typ, cache, [(700, np.arange(600, 700), None, None), (300, [299], None, None)], cap=cap,
+                     q_scale=3.0)
+
+
+@pytest.mark.parametrize("typ,cache", TYPES)
+@pytest.mark.parametrize("scale", [-0.125, 0.0, 1e-25])
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+def test_scales(ctx, typ, cache, scale, cap):
+    _check_attention(ctx, 128, 8, 2, typ, cache, [(300, np.arange(230, 300), None, None), (40, [39], None, None)], cap=cap,
+                     scale=scale)
 
 
 @pytest.mark.parametrize("typ,cache", TYPES)
