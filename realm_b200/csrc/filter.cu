@@ -11,22 +11,27 @@
 // and the draw takes the first index whose running sum of kept W exceeds
 // floor(u sum W). t < 1e-7 takes the first rank.
 //
-// A cluster of CTAs holds one row in shared memory: each CTA a contiguous share of its
-// 16-byte vectors, thread t the vectors t, t + 1024, ... of the share. Thresholds come
-// from a radix walk over the bits of w: first its binade (W has 40 bits, so 41 of
-// them), then the 23 bits of its mantissa in digits of 8, 8 and 7, until a bin is kept
-// whole; each step is a histogram of counts and sums that the cluster adds up through
-// distributed shared memory. Within a binade W is v << s with a v of 24 bits, so a sum
-// is that of v's low 10 and high 14 bits, in 32-bit words: 64-bit shared-memory atomics
-// are loops. The binades of a row are few, so their histogram has a copy per lane (no
-// two lanes of a warp meet); mantissas are spread, and there only the elements of the
-// chosen binade count.
+// Two kernels. The one for short lists (below) settles the rows that keep few tokens; the
+// other takes every row: a cluster of CTAs holds the row in shared memory, each CTA a
+// contiguous share of its 16-byte vectors, thread t the vectors t, t + 1024, ... of the
+// share. Thresholds come from a radix walk over the bits of w: first its binade (W has 40
+// bits, so 41 of them), then the 23 bits of its mantissa in digits of 8, 8 and 7, until a
+// bin is kept whole; each step is a histogram of counts and sums that the cluster adds up
+// through distributed shared memory. Within a binade W is v << s with a v of 24 bits, so a
+// sum is that of v's low 10 and high 14 bits, in 32-bit words: 64-bit shared-memory atomics
+// are loops. The binades of a row are few, so their histogram has a copy per lane (no two
+// lanes of a warp meet); mantissas are spread, and there only the elements of the chosen
+// binade count.
 //
 // Bound by the chain of barriers (about ten) and by instructions: 96 rows of 151937 take
 // 101 us with the elements in shared memory and two CTAs an SM, took 129 us with them in
 // registers (one CTA an SM), 208 us with chunks of consecutive elements a thread, 315 us
-// with 64-bit atomics. One row of 32000: 12 us.
+// with 64-bit atomics. With short lists 57 us (58 MB, 1.0 TB/s: about 15 us for the
+// maximum, 6 for the list, 7 for thresholds and draw, on two thirds of the SMs). One row of
+// 32000: 11 us.
 #include <cooperative_groups.h>
+
+#include <algorithm>
 
 #include "common.cuh"
 #include "filter.cuh"
@@ -41,11 +46,19 @@ constexpr int kFT = 1024, kFW = kFT / 32;
 constexpr int kBinades = 48;      // 41 in use: binade b holds exponents 127 - b
 constexpr int kBins = 256;
 constexpr int kMaxCluster = 8;
+constexpr uint32_t kLeft = 0xfffffffeu;  // in place of a token: a row left to the second kernel
+constexpr int kShortWarp = 384;   // candidates a warp may find
+constexpr int kShortBins = 512;
+constexpr int kShortMax = 8192;   // candidates of a row
+constexpr int kShortSums = 4095;  // of a bin: 4095 (2^20 + 2^20) fits the 32-bit sums of W's halves
+constexpr float kShortFloor = 0x1p-13f, kShortFloor2 = 0x1p-8f;
 constexpr int kMaxElems = 40;     // of a thread: one vector more than 262144 / 8 / 1024, for rows off 16 bytes
 using u64 = unsigned long long;
 
 struct FilterShared {
-  uint32_t ba[kBinades * 32], bb[kBinades * 32];  // per lane: count << 21 | sum of low parts; sum of high parts
+  // per lane: count << 21 | sum of low parts; sum of high parts. In short lists: two histograms.
+  uint32_t ba[2 * kBinades * 32];
+  __device__ uint32_t* bb() { return ba + kBinades * 32; }
   uint32_t cnt[2][kBins], lo[2][kBins], hi[2][kBins];
   u64 xch[2][kMaxCluster];  // one value of every CTA of the cluster
   u64 red[kFW], red2[kFW];
@@ -53,6 +66,7 @@ struct FilterShared {
   u64 above_c, above_s, in_s, base;
   uint32_t bin, in_bin, round, warp;
 };
+static_assert(2 * 3 * kShortBins <= 2 * kBinades * 32 && kFilterMaxVocab / kFW + 2 * 8 * 32 < 65536, "");
 // one lane's copy takes at most kMaxElems elements of each warp: 11 bits of count, 21 of low parts
 static_assert(kFW * kMaxElems < 2048 && kFilterMaxVocab + 8 <= kMaxCluster * kFT * kMaxElems, "");
 
@@ -269,6 +283,323 @@ __device__ Cut radix_cut(const float4* mine, uint32_t bc, u64 bw, u64 want, Clus
   return r;
 }
 
+// Rows with a short list. Most rows keep only tokens within a few binades of the first rank: a
+// min-p of at least kShortFloor keeps no others, nor does a top-k for which there are k above
+// that weight. They are some thousandth of the vocabulary, so a first kernel reads the row
+// twice (once for the maximum, once, from L2, for the list), and the first CTA of its
+// cluster does the rest by itself on the list, which is in the order of the indices. The
+// rows whose list does not fit, that need the whole vocabulary or have repetitions to
+// penalise are left to the other kernel, which holds all their elements.
+
+// A thread's candidates of the short list: K consecutive ones.
+struct ShortList {
+  uint2* mine;  // weight's bits, index
+  int K;
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {
+    for (int e = 0; e < K; ++e) f(mine[e]);
+  }
+};
+__device__ __forceinline__ uint32_t short_key(uint32_t bits) { return 0x3f800000u - bits; }  // below 2^27
+
+// Histogram of the digit at `sh` of the candidates whose key continues `pre`; thread t < kShortBins
+// gets bin t's count and sum. `turn` alternates; the other buffer is cleared for the next one.
+__device__ void short_hist(const ShortList& l, uint32_t pre, int sh, int& turn, uint32_t& c, u64& w, FilterShared& s) {
+  const int tid = threadIdx.x;
+  uint32_t* h = s.ba + (turn & 1) * 3 * kShortBins;
+  uint32_t* other = s.ba + (~turn & 1) * 3 * kShortBins;
+  ++turn;
+  l.each([&](uint2 v) {
+    const uint32_t key = short_key(v.x);
+    if (v.x && key >> (sh + 9) == pre) {
+      const uint32_t b = (key >> sh) & (kShortBins - 1);
+      const u64 f = fix(__uint_as_float(v.x));
+      atomicAdd(&h[b], 1u);
+      atomicAdd(&h[kShortBins + b], (uint32_t)f & 0xfffffu);
+      atomicAdd(&h[2 * kShortBins + b], (uint32_t)(f >> 20));
+    }
+  });
+  for (int i = tid; i < 3 * kShortBins; i += kFT) other[i] = 0;
+  __syncthreads();
+  c = 0;
+  w = 0;
+  if (tid < kShortBins) {
+    c = h[tid];
+    w = h[kShortBins + tid] + ((u64)h[2 * kShortBins + tid] << 20);
+  }
+}
+
+// The cut of one rule over the short list; (c, w): the first digit's bin of this thread.
+template <bool COUNT>
+__device__ Cut short_cut(const ShortList& l, uint32_t c, u64 w, u64 want, int& turn, u64& total, FilterShared& s) {
+  u64 acc_c = 0, acc_s = 0;
+  uint32_t pre = 0;
+  int sh = 27;
+  auto whole = [&]() { return s.in_bin == 1 || (COUNT && acc_c + s.in_bin <= want); };
+  do {
+    sh -= 9;
+    if (sh < 18) short_hist(l, pre, sh, turn, c, w, s);
+    choose<COUNT>(c, w, kShortBins, want, acc_c, acc_s, s);
+    pre = pre << 9 | s.bin;
+  } while (sh > 0 && !whole());
+  const uint32_t bits = 0x3f800000u - (((pre + 1) << sh) - 1);  // the least of the bin
+  if (whole()) {
+    total = acc_s + s.in_s;
+    return Cut{bits, 0xffffffffu, 0xffffffffu};
+  }
+  const u64 tq = fix(__uint_as_float(bits));
+  const u64 ties = COUNT ? want - acc_c : (want - acc_s + tq - 1) / tq;
+  Cut r{bits, ties < s.in_bin ? (uint32_t)ties : s.in_bin, s.in_bin};
+  total = acc_s + r.ties * tq;
+  return r;
+}
+
+// Thresholds and draw over the n candidates of `list`, by one CTA. False: more of one bin than its sums hold.
+__device__ bool short_finish(uint2* list, int n, const rb_sampling_filter& p, bool use_k, bool use_p, const FilterArgs& a,
+                             int row, FilterShared& s) {
+  const int tid = threadIdx.x;
+  const int K = (n + kFT - 1) / kFT;
+  for (int i = tid; i < 6 * kShortBins; i += kFT) s.ba[i] = 0;
+  for (int i = n + tid; i < K * kFT; i += kFT) list[i] = make_uint2(0, 0);
+  __syncthreads();
+  const ShortList l{list + tid * K, K};
+  int turn = 0;
+  Cut cut{0u, 0xffffffffu, 0xffffffffu};
+  u64 total = 0;
+  if (use_k || use_p) {
+    uint32_t c;
+    u64 w;
+    short_hist(l, 0, 18, turn, c, w, s);
+    if (n > kShortSums && __syncthreads_or(c > kShortSums)) return false;
+    if (use_k) {
+      cut = short_cut<true>(l, c, w, p.top_k, turn, total, s);
+    } else {
+      block_scan(w, s.red, total);
+    }
+    if (use_p) {
+      u64 want = (u64)((double)total * (double)p.top_p);
+      if (want < 1) want = 1;
+      __syncthreads();  // s.in_bin and the like have been read
+      const Cut q = short_cut<false>(l, c, w, want, turn, total, s);
+      if (q.bits > cut.bits || (q.bits == cut.bits && q.ties < cut.ties)) cut = q;
+    }
+    if (cut.ties < cut.equal) {  // the same in every thread
+      u64 eq = 0, all;
+      l.each([&](uint2 v) { eq += v.x == cut.bits; });
+      u64 rank = block_scan(eq, s.red, all);
+      for (int e = 0; e < K; ++e)
+        if (l.mine[e].x == cut.bits && rank++ >= cut.ties) l.mine[e].x = 0;
+    }
+  }
+  u64 sum = 0;
+  l.each([&](uint2 v) {
+    if (v.x >= cut.bits) sum += fix(__uint_as_float(v.x));
+  });
+  u64 at = block_scan(sum, s.red, total);
+  const u64 target = (u64)((double)a.uniforms[row] * (double)total);
+  if (target < at || target >= at + sum) return true;
+  for (int e = 0; e < K; ++e) {
+    const uint2 v = l.mine[e];
+    const u64 f = v.x >= cut.bits ? fix(__uint_as_float(v.x)) : 0;
+    if (at + f > target) {
+      a.tokens[row] = v.y;
+      if (a.probs) a.probs[row] = (float)((double)f / (double)total);
+      return true;
+    }
+    at += f;
+  }
+  return true;
+}
+
+template <class T, int N>
+__global__ void __launch_bounds__(kFT, 2) filter_short_kernel(const __grid_constant__ FilterArgs a) {
+  constexpr int E = 16 / sizeof(T), U = 2;
+  extern __shared__ uint2 list[];            // of the first CTA: all candidates
+  __shared__ uint16_t own[kFW][kShortWarp];  // each warp's, as places in its part of the row
+  __shared__ FilterShared s;
+  __shared__ uint32_t kept;  // of the first CTA
+  Cluster<N> cl(s);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_launch_dependents();
+  const int row = blockIdx.x / N;
+  rb_sampling_filter p = a.params[row];
+  p.min_p = fminf(p.min_p, 1.f);  // the first rank always stays
+  const int V = a.vocab;
+  const float t = p.temperature;
+  const bool greedy = !(t >= 1e-7f);
+  const bool use_k = p.top_k > 0 && p.top_k < (uint32_t)V, use_p = p.top_p > 0.f && p.top_p < 1.f;
+  bool all_of = p.min_p >= kShortFloor;  // the list has all that is kept
+  if (!(greedy || use_k || all_of) ||
+      (a.prev_off && p.repetition_penalty != 1.0f && a.prev_off[row + 1] > a.prev_off[row])) {
+    if (cl.rank == 0 && tid == 0) a.tokens[row] = kLeft;
+    return;  // the whole cluster
+  }
+  if (tid == 0) kept = 0;
+  if (N > 1) cg::this_cluster().barrier_arrive();
+  const T* lg = reinterpret_cast<const T*>(a.logits) + (size_t)row * a.ld;
+  // the row's 16-byte vectors, the first one up to E - 1 elements before the row; each CTA has a
+  // contiguous share of them, and each of its warps of those
+  const int mis = (int)((reinterpret_cast<uintptr_t>(lg) & 15) / sizeof(T));
+  const int vecs = (V + mis + E - 1) / E, share = (vecs + N - 1) / N, ours = (share + kFW - 1) / kFW;
+  const int v0 = cl.rank * share + warp * ours, v1 = min(min(vecs, (cl.rank + 1) * share), v0 + ours);
+  // f(elements, vector) for U vectors a lane; -inf where there is none
+  auto scan = [&](auto f) {
+#pragma unroll 1
+    for (int b = v0; b < v1; b += 32 * U) {
+      constexpr uint32_t none = sizeof(T) == 2 ? 0xfc00fc00u : 0xff800000u;
+      uint4 q[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int v = b + 32 * j + lane, i = v * E - mis;
+        q[j] = make_uint4(none, none, none, none);
+        if (v < v1 && i >= 0 && i + E <= V) q[j] = __ldg(reinterpret_cast<const uint4*>(lg + i));
+      }
+      if (b == 0 || b + 32 * U >= vecs) {  // the row's ends may be within a vector
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+          const int v = b + 32 * j + lane, i = v * E - mis;
+          if (v < v1 && (i < 0 || i + E > V)) {
+            T y[E];
+            *reinterpret_cast<uint4*>(y) = q[j];
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+              if (i + e >= 0 && i + e < V) y[e] = lg[i + e];
+            q[j] = *reinterpret_cast<uint4*>(y);
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const T* y = reinterpret_cast<const T*>(&q[j]);
+        float x[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = (float)y[e];
+        f(x, b + 32 * j + lane);
+      }
+    }
+  };
+  float top = -INFINITY;
+  scan([&](const float (&x)[E], int) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) top = fmaxf(top, x[e]);  // not of what is not a number
+  });
+  uint32_t key = __reduce_max_sync(0xffffffffu, float_order_key(top));
+  if (lane == 0) s.red[warp] = key;
+  __syncthreads();
+  key = __reduce_max_sync(0xffffffffu, (uint32_t)s.red[lane]);
+  if (N > 1) {
+    cg::this_cluster().barrier_wait();  // every CTA of the cluster runs before its shared memory is written
+    const u64* all = cl.share(key);
+#pragma unroll
+    for (int r = 0; r < N; ++r) key = max(key, (uint32_t)all[r]);
+  }
+  top = __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
+  if (top == -INFINITY) {
+    if (cl.rank == 0 && tid == 0) {
+      a.tokens[row] = 0xffffffffu;
+      if (a.probs) a.probs[row] = 0.f;
+    }
+    return;
+  }
+  if (greedy) {  // the lowest index that has it
+    uint32_t at = 0xffffffffu;
+    scan([&](const float (&x)[E], int v) {
+#pragma unroll
+      for (int e = E - 1; e >= 0; --e)
+        if (x[e] == top) at = min(at, (uint32_t)(v * E + e - mis));
+    });
+    at = __reduce_min_sync(0xffffffffu, at);
+    if (lane == 0) s.red2[warp] = at;
+    __syncthreads();
+    at = __reduce_min_sync(0xffffffffu, (uint32_t)s.red2[lane]);
+    if (N > 1) {
+      const u64* all = cl.share(at);
+#pragma unroll
+      for (int r = 0; r < N; ++r) at = min(at, (uint32_t)all[r]);
+    }
+    if (cl.rank == 0 && tid == 0) {
+      a.tokens[row] = at;
+      if (a.probs) a.probs[row] = 1.f;
+    }
+    return;
+  }
+  const float m = t == 1.f ? top : __fdiv_rn(top, t);  // the largest quotient: division keeps the order
+  float least = all_of ? p.min_p : kShortFloor;
+  uint32_t count, before;
+  int n;
+#pragma unroll 1
+  while (true) {
+    // below `far` no quotient's weight reaches `least` (where this overflows or is not a number, all are listed)
+    const float ln = logf(least) - 1e-3f, far = (m + ln) * t - (fabsf(m) - ln) * t * 1e-6f;
+    n = 0;
+    scan([&](const float (&x)[E], int v) {
+      bool some = false;
+#pragma unroll
+      for (int e = 0; e < E; ++e) some |= !(x[e] < far);
+      if (!__any_sync(0xffffffffu, some)) return;
+      int at = n;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const unsigned b = __ballot_sync(0xffffffffu, !(x[e] < far));
+        at += __popc(b & ((1u << lane) - 1));
+        n += __popc(b);
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (!(x[e] < far)) {
+          if (at < kShortWarp) own[warp][at] = (uint16_t)((v - v0) * E + e);
+          ++at;
+        }
+    });
+    if (lane == 0) s.red2[warp] = (u64)n;
+    __syncthreads();
+    const uint32_t warps_n = (uint32_t)s.red2[lane], scanned = (uint32_t)warp_scan(warps_n);
+    before = __shfl_sync(0xffffffffu, scanned - warps_n, warp);
+    count = __shfl_sync(0xffffffffu, scanned, 31);
+    if (__any_sync(0xffffffffu, warps_n > kShortWarp)) count = 1u << 24;
+    if (N > 1) {
+      const u64* all = cl.share(count);
+      count = 0;
+#pragma unroll
+      for (int r = 0; r < N; ++r) {
+        if (r < cl.rank) before += (uint32_t)all[r];
+        count += (uint32_t)all[r];
+      }
+    }
+    // too many: fewer do for a top-k
+    if (count <= kShortMax || !use_k || least >= kShortFloor2) break;
+    least = kShortFloor2;
+    all_of = false;
+    __syncthreads();  // s.red2 has been read
+  }
+  if (count > kShortMax) {  // the same in every thread of the cluster
+    if (cl.rank == 0 && tid == 0) a.tokens[row] = kLeft;
+    return;
+  }
+  {
+    uint2* first = N > 1 ? cl.g.map_shared_rank(list, 0) : list;
+    uint32_t found = 0;
+    for (int b = 0; b < n; b += 32) {
+      bool in = false;
+      if (b + lane < n) {
+        const int place = own[warp][b + lane], i = v0 * E + place - mis;
+        float x = -INFINITY;  // where all are listed, places past the warp's part are too
+        if (v0 + place / E < v1 && i >= 0 && i < V) x = (float)lg[i];
+        if (t != 1.f) x = __fdiv_rn(x, t);
+        const float w = x == m ? 1.f : expf(x - m);
+        in = w >= least;
+        first[before + b + lane] = make_uint2(in ? __float_as_uint(w) : 0u, (uint32_t)i);
+      }
+      found += __popc(__ballot_sync(0xffffffffu, in));
+    }
+    if (lane == 0 && found) atomicAdd(N > 1 ? cl.g.map_shared_rank(&kept, 0) : &kept, found);
+  }
+  cl.sync();
+  if (cl.rank) return;
+  if ((!all_of && kept < p.top_k) || !short_finish(list, (int)count, p, use_k, use_p, a, row, s))
+    if (tid == 0) a.tokens[row] = kLeft;
+}
+
 // Two CTAs an SM (32 registers a thread) where their elements fit and keep a CTA busy
 // for long enough: one works while the other waits at a barrier (96 rows of 151937: 101 us
 // against 129 with one).
@@ -284,8 +615,10 @@ __global__ void __launch_bounds__(kFT, two_ctas<T, NV>()) filter_kernel(const __
   __shared__ FilterShared s;
   Cluster<N> cl(s);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (N > 1) cg::this_cluster().barrier_arrive();
   const int row = blockIdx.x / N;
+  pdl_wait();
+  if (!a.all && a.tokens[row] != kLeft) return;  // the whole cluster
+  if (N > 1) cg::this_cluster().barrier_arrive();
   rb_sampling_filter p = a.params[row];
   p.min_p = fminf(p.min_p, 1.f);  // the first rank always stays
   const int V = a.vocab;
@@ -316,7 +649,7 @@ __global__ void __launch_bounds__(kFT, two_ctas<T, NV>()) filter_kernel(const __
 #pragma unroll
     for (int h = 0; h < Q; ++h) mine[(r * Q + h) * kFT] = make_float4(x[4 * h], x[4 * h + 1], x[4 * h + 2], x[4 * h + 3]);
   }
-  for (int i = tid; i < kBinades * 32; i += kFT) s.ba[i] = s.bb[i] = 0;
+  for (int i = tid; i < 2 * kBinades * 32; i += kFT) s.ba[i] = 0;
   const float t = p.temperature;
   const bool greedy = !(t >= 1e-7f);
   float top = -INFINITY;
@@ -372,7 +705,7 @@ __global__ void __launch_bounds__(kFT, two_ctas<T, NV>()) filter_kernel(const __
     const bool in = w >= p.min_p && v != 0;  // v 0: below the fixed point, never drawn
     if (hist && in) {
       atomicAdd(&s.ba[b * 32 + lane], 1u << 21 | (v & 1023u));
-      atomicAdd(&s.bb[b * 32 + lane], v >> 10);
+      atomicAdd(&s.bb()[b * 32 + lane], v >> 10);
     }
     return in ? w : 0.f;
   });
@@ -382,7 +715,7 @@ __global__ void __launch_bounds__(kFT, two_ctas<T, NV>()) filter_kernel(const __
     const int turn = cl.turn & 1;
     __syncthreads();
     for (int b = warp; b < kBinades; b += kFW) {
-      const uint32_t y = s.ba[b * 32 + lane], z = s.bb[b * 32 + lane];
+      const uint32_t y = s.ba[b * 32 + lane], z = s.bb()[b * 32 + lane];
       const uint32_t c = __reduce_add_sync(0xffffffffu, y >> 21), l = __reduce_add_sync(0xffffffffu, y & 0x1fffffu),
                      h = __reduce_add_sync(0xffffffffu, z);
       if (lane == 0) {
@@ -511,13 +844,48 @@ cudaError_t launch(const FilterArgs& a, cudaStream_t s) {
   cfg.blockDim = dim3(kFT);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = N;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, filter_kernel<T, NV, N>, a);
+}
+
+template <class T, int N>
+cudaError_t launch_short(const FilterArgs& a, cudaStream_t s) {
+  constexpr int smem = kShortMax * 8;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (cudaError_t e = ensure_smem_attr(filter_short_kernel<T, N>, smem, dev)) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.n_rows * N));
+  cfg.blockDim = dim3(kFT);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
   cudaLaunchAttribute at;
   at.id = cudaLaunchAttributeClusterDimension;
   at.val.clusterDim.x = N;
   at.val.clusterDim.y = at.val.clusterDim.z = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, filter_kernel<T, NV, N>, a);
+  return cudaLaunchKernelEx(&cfg, filter_short_kernel<T, N>, a);
+}
+
+// CTAs a row: one for each SM, with a vector a thread at least. 1, 2, 4 and 8 CTAs a row, us:
+// 96 rows of 151937 65, 69, 67, 75; 16 rows 56, 42, 32, 32; 96 rows of 32000 24, 30, 34, 46.
+template <class T>
+cudaError_t launch_shorts(const FilterArgs& a, int num_sms, cudaStream_t s) {
+  const int vecs = a.vocab / (16 / (int)sizeof(T)), n = std::min(num_sms / a.n_rows, vecs / kFT);
+  if (n >= 8) return launch_short<T, 8>(a, s);
+  if (n >= 6) return launch_short<T, 6>(a, s);
+  if (n >= 4) return launch_short<T, 4>(a, s);
+  if (n >= 3) return launch_short<T, 3>(a, s);
+  if (n >= 2) return launch_short<T, 2>(a, s);
+  return launch_short<T, 1>(a, s);
 }
 
 template <class T, int N>
@@ -546,11 +914,18 @@ cudaError_t launch_type(const FilterArgs& a, int num_sms, cudaStream_t s) {
   int n = 1;
   while (n < kMaxCluster && rounds(n) > (E == 4 ? 5 : 3)) n *= 2;
   while (n < kMaxCluster && rounds(n) > 1 && (long long)a.n_rows * n * 2 <= 2ll * num_sms) n *= 2;
+  // Short lists first, unless a thread would have one vector and a CTA an SM of its own: one and
+  // eight rows of 32000 took 14 and 18 us without them, 17 and 22 with; 32 rows 37 and 24, one
+  // row of 151937 25 and 22, 96 rows 105 and 65.
+  FilterArgs b = a;
+  b.all = rounds(n) <= 1 && (long long)a.n_rows * n <= num_sms;
+  if (!b.all)
+    if (cudaError_t e = launch_shorts<T>(a, num_sms, s)) return e;
   switch (n) {
-    case 1: return launch_rounds<T, 1>(a, rounds(1), s);
-    case 2: return launch_rounds<T, 2>(a, rounds(2), s);
-    case 4: return launch_rounds<T, 4>(a, rounds(4), s);
-    default: return launch_rounds<T, 8>(a, rounds(8), s);
+    case 1: return launch_rounds<T, 1>(b, rounds(1), s);
+    case 2: return launch_rounds<T, 2>(b, rounds(2), s);
+    case 4: return launch_rounds<T, 4>(b, rounds(4), s);
+    default: return launch_rounds<T, 8>(b, rounds(8), s);
   }
 }
 

@@ -13,6 +13,7 @@ struct FilterArgs {
   const void* logits = nullptr;
   int64_t ld = 0;
   int32_t x16 = 0;  // 1: fp16 logits, 0: fp32
+  int32_t all = 0;  // 1: the kernel that holds whole rows takes every row, 0: those left to it
   int32_t n_rows = 0, vocab = 0;
   const rb_sampling_filter* params = nullptr;
   const uint32_t* prev = nullptr;

@@ -620,3 +620,37 @@ def test_sample_many_rows(ctx, V, typ):
         assert got[i].item() == tok and abs(probs[i].item() - p) <= 2.0 ** -22 * p
         one = rb.sample_filtered(ctx, x[i:i + 1], rb.pack_filters(fs[i:i + 1], "cuda"), u[i:i + 1])
         assert one.item() == tok
+
+
+@pytest.mark.parametrize("typ", ["float32", "float16"])
+@pytest.mark.parametrize("V", [6007, 50000, 140001])
+def test_sample_few_and_many_candidates(ctx, V, typ):
+    """Rows of which few or most tokens weigh enough, together, at one end, equal or all over the vocabulary."""
+    import torch
+    import realm_b200 as rb
+    rng = np.random.default_rng(V)
+    i = np.arange(V)
+    kinds = [np.zeros(V),                                   # all equal
+             np.where(i < 5000, 1.0, -30.0),                # 5000 equal ones at the front
+             np.where(i >= V - 300, 2.0 + i % 7, -40.0),    # all at the end
+             np.where(i % 97 == 5, 3.0, -50.0 + i % 3),     # spread, with ties
+             np.where(i == V // 2, 40.0, -5.0 * (i % 11)),  # one token
+             -np.sqrt(i) / 4.0,                             # sorted
+             rng.normal(0, 4, V), rng.normal(0, 0.5, V), rng.normal(0, 12, V),
+             np.where(i % 1999 == 7, np.inf, 1.0)]          # infinities
+    filters = [(1.0, 0, 0.9, 0.01), (0.7, 40, 0.95, 0.0), (1.0, 3000, 1.0, 0.0), (1.3, 7000, 0.5, 1e-3), (0.0, 0, 1.0, 0.0),
+               (2.0, 1, 1.0, 0.5), (1.0, 0, 1.0, 0.2), (1e4, 50, 0.3, 0.0), (3e38, 0, 0.4, 0.5)]
+    fs, x = [], []
+    for k in kinds:
+        for f in filters:
+            fs.append(rb.SamplingFilter(*f))
+            x.append(k)
+    x = np.stack(x).astype(typ)
+    n = len(fs) * 3
+    u = (rng.integers(0, 2 ** 23, n) / 2 ** 23).astype(np.float32)
+    dx = torch.from_numpy(x).cuda().repeat(3, 1)
+    probs = torch.empty(n, device="cuda")
+    got = rb.sample_filtered(ctx, dx, rb.pack_filters(fs * 3, "cuda"), torch.from_numpy(u).cuda(), probs=probs)
+    for r in range(n):
+        tok, p = _sample_ref(x[r % len(fs)], fs[r % len(fs)], float(u[r]))
+        assert got[r].item() == tok and abs(probs[r].item() - p) <= 2.0 ** -22 * p, (r, got[r].item(), tok)
