@@ -26,9 +26,9 @@
 // Bound by the chain of barriers (about ten) and by instructions: 96 rows of 151937 take
 // 101 us with the elements in shared memory and two CTAs an SM, took 129 us with them in
 // registers (one CTA an SM), 208 us with chunks of consecutive elements a thread, 315 us
-// with 64-bit atomics. With short lists 57 us (58 MB, 1.0 TB/s: about 15 us for the
-// maximum, 6 for the list, 7 for thresholds and draw, on two thirds of the SMs). One row of
-// 32000: 11 us.
+// with 64-bit atomics. With short lists 44 us (58 MB, 1.3 TB/s, on two thirds of the
+// SMs: reading for the maximum, from L2 for the list, 7 us for thresholds and draw, 3 for
+// the second kernel, which finds nothing left). One row of 32000: 11 us.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -411,9 +411,11 @@ __device__ bool short_finish(uint2* list, int n, const rb_sampling_filter& p, bo
   return true;
 }
 
+// One CTA an SM, for the registers of four vectors in flight a thread: 96 rows of 151937
+// 50 us, with two vectors and two CTAs 65 us; 200 rows 93 and 114.
 template <class T, int N>
-__global__ void __launch_bounds__(kFT, 2) filter_short_kernel(const __grid_constant__ FilterArgs a) {
-  constexpr int E = 16 / sizeof(T), U = 2;
+__global__ void __launch_bounds__(kFT, 1) filter_short_kernel(const __grid_constant__ FilterArgs a) {
+  constexpr int E = 16 / sizeof(T), U = 4;
   extern __shared__ uint2 list[];            // of the first CTA: all candidates
   __shared__ uint16_t own[kFW][kShortWarp];  // each warp's, as places in its part of the row
   __shared__ FilterShared s;
@@ -875,8 +877,9 @@ cudaError_t launch_short(const FilterArgs& a, cudaStream_t s) {
   return cudaLaunchKernelEx(&cfg, filter_short_kernel<T, N>, a);
 }
 
-// CTAs a row: one for each SM, with a vector a thread at least. 1, 2, 4 and 8 CTAs a row, us:
-// 96 rows of 151937 65, 69, 67, 75; 16 rows 56, 42, 32, 32; 96 rows of 32000 24, 30, 34, 46.
+// CTAs a row: one for each SM, with a vector a thread at least. 1, 2, 4 and 8 CTAs a row, us
+// (with two vectors in flight a thread): 96 rows of 151937 65, 69, 67, 75; 16 rows 56, 42,
+// 32, 32; 96 rows of 32000 24, 30, 34, 46.
 template <class T>
 cudaError_t launch_shorts(const FilterArgs& a, int num_sms, cudaStream_t s) {
   const int vecs = a.vocab / (16 / (int)sizeof(T)), n = std::min(num_sms / a.n_rows, vecs / kFT);
