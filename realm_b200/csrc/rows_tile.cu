@@ -402,61 +402,76 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
       const unsigned long long mine =
           active ? (unsigned long long)a.q + ((size_t)row * a.ldq + (size_t)head * HD) * ESZ : 0ull;
       const bool vec = ((reinterpret_cast<uintptr_t>(a.q) | (size_t)a.ldq * ESZ) & 15) == 0;
-      const float sign = a.scale < 0.f ? -1.f : 1.f;
-      const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
-      float my_mul = 1.f;
-#pragma unroll 1
-      for (int i0 = 0; i0 < 32; i0 += 8 * RPI) {
-        uint4 raw[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const unsigned long long p = __shfl_sync(0xffffffffu, mine, i0 + i * RPI + sub);
-          raw[i] = make_uint4(0, 0, 0, 0);
-          if (p) {
-            if (vec) {
-              raw[i] = reinterpret_cast<const uint4*>(p)[ch];
-            } else if (HL) {
-              const uint32_t* q = reinterpret_cast<const uint32_t*>(p) + 4 * ch;
-              raw[i] = make_uint4(q[0], q[1], q[2], q[3]);
-            } else {
-              const uint16_t* q = reinterpret_cast<const uint16_t*>(p) + 8 * ch;
-              raw[i] = make_uint4(q[0] | (uint32_t)q[1] << 16, q[2] | (uint32_t)q[3] << 16,
-                                  q[4] | (uint32_t)q[5] << 16, q[6] | (uint32_t)q[7] << 16);
-            }
-          }
+      // All of the warp's rows at once, asynchronously: fp16 to their place, an fp32 row to those of
+      // its two parts, which then replace it. (Loops stay rolled: this code runs once a unit, and
+      // fetching it unrolled took 16 K clocks of the 51 K of a short unit.)
+      if (vec) {
+#pragma unroll 4
+        for (int i = 0; i < 32; i += RPI) {
+          const unsigned long long p = __shfl_sync(0xffffffffu, mine, i + sub);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                           smem_u32(chunk_at(w0 + i + sub, ch / (HD / 8), ch % (HD / 8)))),
+                       "l"(p ? p + 16 * ch : (unsigned long long)a.q), "r"(p ? 16 : 0)
+                       : "memory");
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int rr = i0 + i * RPI + sub;  // of the warp's rows
-          if (HL) {
-            float x[4] = {__uint_as_float(raw[i].x), __uint_as_float(raw[i].y), __uint_as_float(raw[i].z),
-                          __uint_as_float(raw[i].w)};
-            float top = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-#pragma unroll
-            for (int o = LPR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            float mul = 1.f;  // 2^(8 - exponent of top), for normal finite tops
-            const int e = (int)(__float_as_uint(top) >> 23);
-            if (e > 8 && e < 255) mul = __uint_as_float((uint32_t)min(254, 127 + 8 + 127 - e) << 23);
-#pragma unroll
-            for (int q = 0; q < RPI; ++q) {
-              const float m = __shfl_sync(0xffffffffu, mul, q * LPR);
-              if (lane == i0 + i * RPI + q) my_mul = m;
-            }
-            mul *= sign;
-            uint2 hi, lo;
-            hi.x = pack2(x[0] * mul, x[1] * mul);
-            hi.y = pack2(x[2] * mul, x[3] * mul);
-            lo.x = pack2_lo(x[0] * mul, x[1] * mul, hi.x);
-            lo.y = pack2_lo(x[2] * mul, x[3] * mul, hi.y);
-            reinterpret_cast<uint2*>(chunk_at(w0 + rr, 0, ch >> 1))[ch & 1] = hi;
-            reinterpret_cast<uint2*>(chunk_at(w0 + rr, HL, ch >> 1))[ch & 1] = lo;
-          } else {
-            raw[i].x ^= flip;
-            raw[i].y ^= flip;
-            raw[i].z ^= flip;
-            raw[i].w ^= flip;
-            *chunk_at(w0 + rr, 0, ch) = raw[i];
+        asm volatile("cp.async.wait_all;" ::: "memory");
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < 32; i += RPI) {
+          const unsigned long long p = __shfl_sync(0xffffffffu, mine, i + sub);
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (p && HL) {
+            const uint32_t* q = reinterpret_cast<const uint32_t*>(p) + 4 * ch;
+            v = make_uint4(q[0], q[1], q[2], q[3]);
+          } else if (p) {
+            const uint16_t* q = reinterpret_cast<const uint16_t*>(p) + 8 * ch;
+            v = make_uint4(q[0] | (uint32_t)q[1] << 16, q[2] | (uint32_t)q[3] << 16, q[4] | (uint32_t)q[5] << 16,
+                           q[6] | (uint32_t)q[7] << 16);
           }
+          *chunk_at(w0 + i + sub, ch / (HD / 8), ch % (HD / 8)) = v;
+        }
+      }
+      __syncwarp();
+      float my_mul = 1.f;
+      if (HL) {
+        const float sign = a.scale < 0.f ? -1.f : 1.f;
+#pragma unroll 4
+        for (int i = 0; i < 32; i += RPI) {
+          const int rr = w0 + i + sub;
+          const uint4 raw = *chunk_at(rr, ch / (HD / 8), ch % (HD / 8));
+          const float x[4] = {__uint_as_float(raw.x), __uint_as_float(raw.y), __uint_as_float(raw.z),
+                              __uint_as_float(raw.w)};
+          const float big = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+          uint32_t top = __float_as_uint(big);  // magnitudes in the order of their bits
+          if (LPR == 32) {
+            top = __reduce_max_sync(0xffffffffu, top);
+          } else {
+#pragma unroll
+            for (int o = LPR / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+          }
+          float mul = 1.f;  // 2^(8 - exponent of top), for normal finite tops
+          const int e = (int)(top >> 23);
+          if (e > 8 && e < 255) mul = __uint_as_float((uint32_t)min(254, 127 + 8 + 127 - e) << 23);
+#pragma unroll
+          for (int q = 0; q < RPI; ++q) {
+            const float m = __shfl_sync(0xffffffffu, mul, q * LPR);
+            if (lane == i + q) my_mul = m;
+          }
+          mul *= sign;
+          uint2 hi, lo;
+          hi.x = pack2(x[0] * mul, x[1] * mul);
+          hi.y = pack2(x[2] * mul, x[3] * mul);
+          lo.x = pack2_lo(x[0] * mul, x[1] * mul, hi.x);
+          lo.y = pack2_lo(x[2] * mul, x[3] * mul, hi.y);
+          __syncwarp();  // the whole row has been read
+          reinterpret_cast<uint2*>(chunk_at(rr, 0, ch >> 1))[ch & 1] = hi;
+          reinterpret_cast<uint2*>(chunk_at(rr, HL, ch >> 1))[ch & 1] = lo;
+        }
+      } else if (a.scale < 0.f) {
+#pragma unroll 1
+        for (int i = 0; i < 32; i += RPI) {
+          uint4* v = chunk_at(w0 + i + sub, 0, ch);
+          *v = make_uint4(v->x ^ 0x80008000u, v->y ^ 0x80008000u, v->z ^ 0x80008000u, v->w ^ 0x80008000u);
         }
       }
       if (HL) sv /= my_mul;
@@ -791,28 +806,29 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
         }
       }
       __syncwarp();
-      const int nch = nd * out_esz / 16;  // chunks a row: 8, 16 or 32
+      const int nch = nd * out_esz / 16, lg = 31 - __clz(nch);  // chunks a row: 8, 16 or 32
+      if (vec) {
 #pragma unroll 4
-      for (int i = 0; i < nch; ++i) {
-        const int at = i * 32 + lane, rr = at / nch, c = at % nch;
-        const unsigned long long p = __shfl_sync(0xffffffffu, mine, rr);
-        const uint4 v = *chunk_at(w0 + rr, c / (HD / 8), c % (HD / 8));
-        if (!p) continue;
-        if (vec) {
-          reinterpret_cast<uint4*>(p + (size_t)pass * nd * out_esz)[c] = v;
-        } else if (HL) {
-          uint32_t* dst = reinterpret_cast<uint32_t*>(p) + 4 * c;
-          dst[0] = v.x;
-          dst[1] = v.y;
-          dst[2] = v.z;
-          dst[3] = v.w;
-        } else {
-          uint16_t* dst = reinterpret_cast<uint16_t*>(p) + 8 * c;
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        for (int i = 0; i < nch; ++i) {
+          const int at = i * 32 + lane, rr = at >> lg, c = at & (nch - 1);
+          const unsigned long long p = __shfl_sync(0xffffffffu, mine, rr);
+          const uint4 v = *chunk_at(w0 + rr, c / (HD / 8), c % (HD / 8));
+          if (p) reinterpret_cast<uint4*>(p + (size_t)pass * nd * out_esz)[c] = v;
+        }
+      } else {  // rows off 16 bytes (never parts)
+        constexpr int EO = HL ? 4 : 2;
+#pragma unroll 1
+        for (int i = 0; i < nch; ++i) {
+          const int at = i * 32 + lane, rr = at >> lg, c = at & (nch - 1);
+          const unsigned long long p = __shfl_sync(0xffffffffu, mine, rr);
+          const uint4* v = chunk_at(w0 + rr, c / (HD / 8), c % (HD / 8));
+          if (!p) continue;
+          if (HL) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            dst[2 * e] = (uint16_t)w[e];
-            dst[2 * e + 1] = (uint16_t)(w[e] >> 16);
+            for (int e = 0; e < 4; ++e) reinterpret_cast<uint32_t*>(p)[4 * c + e] = (&v->x)[e];
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16 / EO; ++e) reinterpret_cast<uint16_t*>(p)[8 * c + e] = reinterpret_cast<const uint16_t*>(v)[e];
           }
         }
       }
