@@ -50,14 +50,15 @@ void rows_partition(const std::vector<RowInfo>& rows, int n_heads, int n_kv, int
   out = RowWork();
   const int n_rep = n_heads / n_kv, n = (int)rows.size();
   std::vector<Item> small, tile;
-  // Runs of at least 32 query vectors a kv head take the tile kernel. Tiles against small
-  // items, us, for runs of 16, 32 and 64 vectors, 64 tenants x 1024 tokens, 8 kv heads:
-  // fp16 rows at head size 128 100/99, 105/200, 106/341; at 64 83/69, 84/120, 85/214;
-  // fp32 rows at 128 146/99, 158/200, 161/342; at 64 111/71, 117/124, 119/222.
+  // Runs of at least 24 query vectors a kv head take the tile kernel. Tiles against small
+  // items, us, for runs of 16, 24, 32 and 64 vectors, 64 tenants x 1024 tokens, 8 kv heads:
+  // fp16 rows at head size 128 92/99, 93/159, 94/198, 94/337; at 64 73/69, 73/97, 74/120,
+  // 74/214; fp32 rows at 128 137/99, 138/173, 139/202, 141/341; at 64 96/71, 96/99, 98/124,
+  // 98/222. (16 tenants x 2048, fp32 rows at 128: 77/67, 79/69, 81/93, 87/155.)
   for (int r = 0; r < n;) {
     int e = r + 1;
     while (e < n && rows[e].tenant == rows[r].tenant) ++e;
-    if (use_tile && (long long)(e - r) * n_rep >= 32)
+    if (use_tile && (long long)(e - r) * n_rep >= 24)
       cut_run(rows, r, e, n_rep, kTileVecs, kRowPage, tile);
     else
       cut_run(rows, r, e, n_rep, kSmallVecs, kRowPage, small);
