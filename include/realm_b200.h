@@ -499,8 +499,10 @@ int32_t rb_sample_logits(rb_ctx* ctx, const float* logits, uint32_t ld, uint32_t
  * order. Tokens rank by weight, ties by the lowest index. Kept are the first top_k
  * ranks with w >= min_p, and of these the ranks with less than top_p of their
  * weight before them; the draw takes the first kept index whose running sum
- * exceeds uniform * total. A temperature below 1e-7 takes the first rank. A logit
- * that is not a number counts as -infinity. */
+ * exceeds uniform * total. Uniforms lie in [0, 1); one that rounding brought to 1, or
+ * past it, draws the last kept index, one below 0 or not a number the first. A
+ * temperature below 1e-7 takes the first rank. A logit that is not a number counts
+ * as -infinity. */
 typedef struct rb_sampling_filter {
   float temperature;
   uint32_t top_k;           /* used when 0 < top_k < vocab */

@@ -9,7 +9,7 @@
 //   min-p   those with w >= min_p (the first rank's w is 1),
 //   top-p   of these, the ranks with less than floor(p sum W) before them,
 // and the draw takes the first index whose running sum of kept W exceeds
-// floor(u sum W). t < 1e-7 takes the first rank.
+// floor(u sum W) (draw_target). t < 1e-7 takes the first rank.
 //
 // Two kernels. The one for short lists (below) settles the rows that keep few tokens; the
 // other takes every row: a cluster of CTAs holds the row in shared memory, each CTA a
@@ -175,6 +175,14 @@ __device__ __forceinline__ void change(float4* mine, F f) {
     v.w = f(v.w);
     mine[q * kFT] = v;
   }
+}
+
+// The running sum that the draw has to pass, below `total` (at least 1) for every u, so that each
+// row gets a token: u >= 1 draws the last kept one, u <= 0 or not a number the first.
+__device__ __forceinline__ u64 draw_target(float u, u64 total) {
+  const double x = (double)u * (double)total;
+  if (!(x > 0.0)) return 0;
+  return x < (double)total ? min((u64)x, total - 1) : total - 1;
 }
 
 // What is kept: weights with more than `bits`, and the first `ties` of those with
@@ -396,7 +404,7 @@ __device__ bool short_finish(uint2* list, int n, const rb_sampling_filter& p, bo
     if (v.x >= cut.bits) sum += fix(__uint_as_float(v.x));
   });
   u64 at = block_scan(sum, s.red, total);
-  const u64 target = (u64)((double)a.uniforms[row] * (double)total);
+  const u64 target = draw_target(a.uniforms[row], total);
   if (target < at || target >= at + sum) return true;
   for (int e = 0; e < K; ++e) {
     const uint2 v = l.mine[e];
@@ -797,7 +805,7 @@ __global__ void __launch_bounds__(kFT, two_ctas<T, NV>()) filter_kernel(const __
       total += all[r];
     }
   }
-  const u64 target = (u64)((double)a.uniforms[row] * (double)total);
+  const u64 target = draw_target(a.uniforms[row], total);
   if (target < run || target >= run + mass) return;  // the whole CTA
   // exactly one CTA's, warp's and lane's kept weights reach past the target (target < total)
   if (warp == 0) {

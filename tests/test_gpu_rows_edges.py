@@ -1,0 +1,73 @@
+"""Edges of the row plans' operators: what calls refuse, lifetimes, streams, and inputs
+on which a kernel's rounding shows. References are plain forms in 64 bits; each
+tolerance is derived where it stands, with U = 2^-24 (fp32) and HALF = 2^-11 (fp16)."""
+import os
+import subprocess
+import sys
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+U, HALF = 2.0 ** -24, 2.0 ** -11
+
+
+def _np(x):
+    return x.detach().cpu().double().numpy()
+
+
+def _cuda(a):
+    import torch
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def _code(f):
+    import realm_b200 as rb
+    with pytest.raises(rb.RealmError) as e:
+        f()
+    return e.value.code
+
+
+# ---------------------------------------------------------------------------
+# sampling
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("typ", ["float32", "float16"])
+@pytest.mark.parametrize("rows,V", [(1, 9), (3, 5000), (200, 33000), (40, 151937)])
+@pytest.mark.parametrize("top_k,min_p", [(0, 0.0), (5, 0.0), (0, 0.3), (2000, 0.0)])
+def test_a_uniform_of_one_draws_the_last_kept_token(ctx, typ, rows, V, top_k, min_p):
+    """Float64 draws just below 1 round to 1.0f: every row still writes a token, the last of those kept."""
+    import torch
+    import realm_b200 as rb
+    rng = np.random.default_rng(V + top_k)
+    x = np.round(rng.normal(0, 1.5, (rows, V)) * 4).astype(typ) / 4  # exact in both types: ties by the index
+    want = []
+    for r in range(rows):
+        order = np.lexsort((np.arange(V), -x[r].astype(np.float64)))
+        kept = order[:top_k] if 0 < top_k < V else order
+        if min_p:  # exp(-1.25) = 0.2865 < 0.3 < exp(-1) = 0.3679
+            kept = kept[x[r][kept].astype(np.float64) >= float(x[r].max()) - 1.0]
+        want.append(kept.max())
+    f = rb.SamplingFilter(1.0, top_k=top_k, min_p=min_p)
+    one = np.full(rows, np.nextafter(1.0, 0.0))
+    probs = np.full(rows, -7, np.float32)
+    assert (rb.sample_filtered(ctx, x, [f] * rows, one, probs=probs) == want).all()
+    assert (probs > 0).all()
+    for u in (1.0, 1.5, float("inf")):
+        out = torch.full((rows,), -7, dtype=torch.int32, device="cuda")
+        probs = torch.full((rows,), -7.0, device="cuda")
+        rb.sample_filtered(ctx, _cuda(x), rb.pack_filters([f] * rows, "cuda"), torch.full((rows,), u, device="cuda"),
+                           out=out, probs=probs)
+        assert (out.cpu().numpy() == want).all() and (probs > 0).all()
+    # below 0 and not a number: the first kept token
+    for u in (-1.0, float("nan")):
+        out = torch.full((rows,), -7, dtype=torch.int32, device="cuda")
+        rb.sample_filtered(ctx, _cuda(x), rb.pack_filters([f] * rows, "cuda"), torch.full((rows,), u, device="cuda"), out=out)
+        got = out.cpu().numpy()
+        for r in range(rows):
+            order = np.lexsort((np.arange(V), -x[r].astype(np.float64)))
+            kept = order[:top_k] if 0 < top_k < V else order
+            if min_p:
+                kept = kept[x[r][kept].astype(np.float64) >= float(x[r].max()) - 1.0]
+            assert got[r] == kept.min()
