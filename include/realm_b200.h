@@ -184,6 +184,11 @@ int32_t rb_kv_pool_free_pages(rb_ctx* ctx, int32_t pool);
 /* The pool's device memory, [page][layer][k | v][kv head][16 tokens][head_dim] in its
  * dtype, and its size in bytes. */
 int32_t rb_kv_pool_data(rb_ctx* ctx, int32_t pool, void** data, uint64_t* bytes);
+/* Keeps that memory when the pool, its model or the context is destroyed, until
+ * rb_kv_hold_release, which needs none of them. The last of those that had it frees
+ * it (cudaFree, which waits for the device). */
+int32_t rb_kv_pool_hold(rb_ctx* ctx, int32_t pool, void** hold);
+int32_t rb_kv_hold_release(void* hold);
 /* KVCache::new (kv_cache.rs:24-34) for one tenant. */
 int32_t rb_kv_create(rb_ctx* ctx, int32_t pool, uint32_t tenant);
 int32_t rb_kv_destroy(rb_ctx* ctx, int32_t pool, uint32_t tenant);

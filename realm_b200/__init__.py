@@ -97,6 +97,8 @@ _sig("rb_kv_pool_destroy", [_vp, _i32])
 _sig("rb_kv_pool_shuffle", [_vp, _i32, _u64])
 _sig("rb_kv_pool_free_pages", [_vp, _i32])
 _sig("rb_kv_pool_data", [_vp, _i32, C.POINTER(_vp), C.POINTER(_u64)])
+_sig("rb_kv_pool_hold", [_vp, _i32, C.POINTER(_vp)])
+_sig("rb_kv_hold_release", [_vp])
 _sig("rb_kv_create", [_vp, _i32, _u32])
 _sig("rb_kv_destroy", [_vp, _i32, _u32])
 _sig("rb_kv_clear", [_vp, _i32, _u32])
@@ -351,23 +353,22 @@ class Weight:
             self.handle = -1
 
 
-class _PoolMemory:
-    """Frees a closed pool once no KVPool and no tensor uses it."""
+class _PoolView:
+    """A pool's memory for torch, which keeps this object, and so the memory (rb_kv_pool_hold)."""
 
-    def __init__(self, ctx: Context, handle: int):
-        self.ctx, self.handle, self.closed = ctx, handle, False
+    def __init__(self, pool: "KVPool"):
+        self._hold = _vp()
+        _check(_lib.rb_kv_pool_hold(pool.ctx.handle, pool.handle, C.byref(self._hold)))
+        p, n = _vp(), _u64()
+        _check(_lib.rb_kv_pool_data(pool.ctx.handle, pool.handle, C.byref(p), C.byref(n)))
+        esz = 2 if pool.kv_dtype == F16 else 4
+        shape = (n.value // (esz * pool.n_layers * 2 * pool.n_kv * 16 * pool.hd), pool.n_layers, 2, pool.n_kv, 16,
+                 pool.hd)
+        self.__cuda_array_interface__ = {"shape": shape, "typestr": f"<f{esz}", "data": (p.value, False), "version": 3}
 
     def __del__(self):
-        if self.closed and self.ctx._h and _lib is not None:
-            _lib.rb_kv_pool_destroy(self.ctx.handle, self.handle)
-
-
-class _PoolView:
-    """A pool's memory for torch, which keeps this object, and so the memory."""
-
-    def __init__(self, memory, shape, typestr, ptr):
-        self._memory = memory
-        self.__cuda_array_interface__ = {"shape": shape, "typestr": typestr, "data": (ptr, False), "version": 3}
+        if self._hold and _lib is not None:
+            _lib.rb_kv_hold_release(self._hold)
 
 
 class KVPool:
@@ -385,26 +386,20 @@ class KVPool:
                                           max_tenants, max_seq, C.byref(h)))
             handle = h.value
         self.handle = handle
-        self._memory = _PoolMemory(ctx, handle) if self._owned else None
 
     def close(self):
         """Ends the use of the pool and its plans; its memory is freed once no tensor of pages() is left."""
         if not self._owned:
             raise ValueError("the pool belongs to a model")
-        if self._memory is not None:
-            self._memory.closed = True
-        self.handle, self._memory = -1, None
+        if self.handle >= 0 and self.ctx.handle:
+            _check(_lib.rb_kv_pool_destroy(self.ctx.handle, self.handle))
+        self.handle = -1
 
     def pages(self):
-        """The pool's memory as a CUDA tensor [page][layer][k | v][kv head][16][head_dim] (a view)."""
+        """The pool's memory as a CUDA tensor [page][layer][k | v][kv head][16][head_dim] (a view). The memory stays
+        while the tensor does, whatever becomes of the pool, its model and the context."""
         import torch
-        p, n = _vp(), _u64()
-        _check(_lib.rb_kv_pool_data(self.ctx.handle, self.handle, C.byref(p), C.byref(n)))
-        esz = 2 if self.kv_dtype == F16 else 4
-        shape = (n.value // (esz * self.n_layers * 2 * self.n_kv * 16 * self.hd), self.n_layers, 2, self.n_kv, 16,
-                 self.hd)
-        return torch.as_tensor(_PoolView(self._memory, shape, "<f2" if esz == 2 else "<f4", p.value),
-                               device=torch.device("cuda", self.ctx.device))
+        return torch.as_tensor(_PoolView(self), device=torch.device("cuda", self.ctx.device))
 
     def plan(self, tenants, n_heads: int, positions=None, begin=None, end=None, window: int = 0) -> "RowPlan":
         """The rows of one step: row r is tenants[r] at positions[r] (None: the tenants' next

@@ -228,14 +228,15 @@ struct KvTenant {
 struct KvPool {
   int n_layers = 0, n_kv = 0, hd = 0, f16 = 1, max_tenants = 0, max_seq = 0, max_pages_per_tenant = 0;
   int n_pages = 0;
-  DevBuf pool, ptab;
+  std::shared_ptr<DevBuf> pool = std::make_shared<DevBuf>();  // outlives this while someone holds it (rb_kv_pool_hold)
+  DevBuf ptab;
   CUtensorMap tmap;  // fp16 pools: the pool as a TMA tensor (kv_tensor_map)
   std::vector<int32_t> h_ptab;
   std::vector<int> free_list;  // stack; back() is handed out next
   std::vector<KvTenant> tenants;
   KvView view() const {
     KvView v;
-    v.pool = pool.p;
+    v.pool = pool->p;
     v.f16 = f16;
     v.n_layers = n_layers;
     v.n_kv = n_kv;
@@ -914,8 +915,8 @@ int pool_create(rb_ctx* c, int n_layers, int n_kv, int hd, int kv_dtype, int n_p
   P->max_seq = max_seq;
   P->max_pages_per_tenant = (max_seq + 15) / 16;
   const size_t page_bytes = (size_t)n_layers * 2 * n_kv * 16 * hd * (P->f16 ? 2 : 4);
-  if (P->pool.alloc(page_bytes * n_pages) != cudaSuccess) return fail(RB_ERR_OOM, "kv pool of %zu bytes", page_bytes * n_pages);
-  RB_CUDA(cudaMemsetAsync(P->pool.p, 0, page_bytes * n_pages, c->stream));
+  if (P->pool->alloc(page_bytes * n_pages) != cudaSuccess) return fail(RB_ERR_OOM, "kv pool of %zu bytes", page_bytes * n_pages);
+  RB_CUDA(cudaMemsetAsync(P->pool->p, 0, page_bytes * n_pages, c->stream));
   if (P->f16) RB_CUDA(kv_tensor_map(P->view(), (size_t)n_pages, &P->tmap));
   P->h_ptab.assign((size_t)max_tenants * P->max_pages_per_tenant, 0);
   RB_CUDA(P->ptab.alloc(P->h_ptab.size() * 4));
@@ -1396,8 +1397,22 @@ int32_t rb_kv_pool_data(rb_ctx* c, int32_t pool, void** data, uint64_t* bytes) {
   KvPool* P = get_pool(c, pool);
   if (!P) return fail(RB_ERR_BAD_HANDLE, "pool %d", pool);
   if (!data || !bytes) return fail(RB_ERR_INVALID, "null output");
-  *data = P->pool.p;
-  *bytes = P->pool.n;
+  *data = P->pool->p;
+  *bytes = P->pool->n;
+  return RB_OK;
+}
+
+int32_t rb_kv_pool_hold(rb_ctx* c, int32_t pool, void** hold) {
+  KvPool* P = get_pool(c, pool);
+  if (!P) return fail(RB_ERR_BAD_HANDLE, "pool %d", pool);
+  if (!hold) return fail(RB_ERR_INVALID, "null output");
+  *hold = new std::shared_ptr<DevBuf>(P->pool);
+  return RB_OK;
+}
+
+int32_t rb_kv_hold_release(void* hold) {
+  if (!hold) return fail(RB_ERR_BAD_HANDLE, "null hold");
+  delete (std::shared_ptr<DevBuf>*)hold;
   return RB_OK;
 }
 

@@ -71,3 +71,51 @@ def test_a_uniform_of_one_draws_the_last_kept_token(ctx, typ, rows, V, top_k, mi
             if min_p:
                 kept = kept[x[r][kept].astype(np.float64) >= float(x[r].max()) - 1.0]
             assert got[r] == kept.min()
+
+
+# ---------------------------------------------------------------------------
+# lifetimes
+# ---------------------------------------------------------------------------
+def _small_model(ctx, rb):
+    return rb.Model(ctx, dict(n_layers=2, hidden=256, n_heads=4, n_kv_heads=2, head_dim=64, ffn=256, vocab=256, max_seq=64,
+                              rms_eps=1e-5, layer_eps=1e-5, rope_theta=1e4, kv_dtype=rb.F32, max_tenants=2, kv_pages=8192))
+
+
+@pytest.mark.parametrize("owner", ["pool", "model"])
+def test_a_tensor_of_pages_outlives_the_context(owner):
+    import torch
+    import realm_b200 as rb
+    free = torch.cuda.mem_get_info()[0]
+    k = torch.randn(20, 2, 64, device="cuda")
+    with rb.Context(0) as c:
+        if owner == "pool":
+            pool = c.kv_pool(2, 2, 64, rb.F32, n_pages=8192, max_tenants=1, max_seq=64)  # 256 MB
+            pool.create(0)
+        else:
+            model = _small_model(c, rb)
+            model.tenant_create(0)
+            pool = model.kv
+        with pool.plan([0] * 20, 2) as p:
+            p.append(1, k, k)
+        view = pool.pages()[:, 1]
+    assert torch.equal(view[0, 1].permute(1, 0, 2), k[:16])
+    view.fill_(3.0)  # the whole of it
+    assert (view == 3.0).all()
+    assert free - torch.cuda.mem_get_info()[0] >= 256 << 20
+    del view
+    assert free - torch.cuda.mem_get_info()[0] < 256 << 20
+
+
+def test_a_tensor_of_pages_outlives_its_model(ctx):
+    import torch
+    import realm_b200 as rb
+    model = _small_model(ctx, rb)
+    model.tenant_create(0)
+    k = torch.randn(20, 2, 64, device="cuda")
+    with model.kv.plan([0] * 20, 2) as p:
+        p.append(0, k, k)
+    view = model.kv.pages()
+    kv = model.kv
+    model.close()
+    assert torch.equal(view[0, 0, 0].permute(1, 0, 2), k[:16])
+    assert _code(kv.pages) == -20 and _code(lambda: kv.create(1)) == -20
