@@ -239,7 +239,8 @@ typedef struct rb_plan_desc {
  * RB_ERR_NOT_FOUND (tenant), RB_ERR_KV_OVERFLOW (position or end past max_seq),
  * RB_ERR_UNSUPPORTED (heads). Returns RB_OK. */
 int32_t rb_plan_create(rb_ctx* ctx, int32_t pool, const rb_plan_desc* desc, int32_t* plan);
-/* Waits for the context's stream, then frees the plan. Cached tokens stay. */
+/* Waits for the context's stream, then frees the plan. Cached tokens stay. The plans
+ * of a pool go with it. A plan's handle is not given out again. */
 int32_t rb_plan_destroy(rb_ctx* ctx, int32_t plan);
 
 /* Layouts of the rows that go in: element (row, head, i) of q lies at

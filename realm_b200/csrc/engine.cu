@@ -303,7 +303,8 @@ struct Ctx {
   std::vector<std::unique_ptr<Weight>> weights;
   std::vector<std::unique_ptr<KvPool>> pools;
   std::vector<std::unique_ptr<Model>> models;
-  std::vector<std::unique_ptr<RowSet>> plans;
+  std::map<int, std::unique_ptr<RowSet>> plans;  // by handle; no handle is given out twice
+  int next_plan = 0;
   bool own_stream = true;
   float last_ms = 0.f;
   int last_launches = 0;
@@ -929,6 +930,13 @@ int pool_create(rb_ctx* c, int n_layers, int n_kv, int hd, int kv_dtype, int n_p
   return (int)c->pools.size() - 1;
 }
 
+// Ends a pool and the plans of its rows (the stream is idle).
+void drop_pool(rb_ctx* c, int pool) {
+  for (auto it = c->plans.begin(); it != c->plans.end();)
+    it = it->second->pool == pool ? c->plans.erase(it) : std::next(it);
+  c->pools[pool].reset();
+}
+
 void tenant_release(KvPool& P, int t) {
   KvTenant& T = P.tenants[t];
   for (auto it = T.pages.rbegin(); it != T.pages.rend(); ++it) P.free_list.push_back(*it);
@@ -1373,9 +1381,7 @@ int32_t rb_kv_pool_create(rb_ctx* c, uint32_t n_layers, uint32_t n_kv, uint32_t 
 int32_t rb_kv_pool_destroy(rb_ctx* c, int32_t pool) {
   if (!get_pool(c, pool)) return fail(RB_ERR_BAD_HANDLE, "pool %d", pool);
   cudaStreamSynchronize(c->stream);
-  for (auto& p : c->plans)
-    if (p && p->pool == pool) p.reset();
-  c->pools[pool].reset();
+  drop_pool(c, pool);
   return RB_OK;
 }
 
@@ -1628,7 +1634,7 @@ int32_t rb_model_destroy(rb_ctx* c, int32_t model) {
   for (auto& g : M->graphs) cudaGraphExecDestroy(g.second);
   const int p = M->pool;
   c->models[model].reset();
-  if (p >= 0 && p < (int)c->pools.size()) c->pools[p].reset();
+  if (p >= 0 && p < (int)c->pools.size()) drop_pool(c, p);
   return RB_OK;
 }
 
@@ -2186,8 +2192,9 @@ extern "C" int32_t rb_weight_matmul_noalloc(rb_ctx* c, int32_t h, const float* i
 namespace {
 
 RowSet* get_plan(rb_ctx* c, int32_t plan) {
-  if (!c || plan < 0 || plan >= (int)c->plans.size() || !c->plans[plan]) return nullptr;
-  return c->plans[plan].get();
+  if (!c) return nullptr;
+  auto it = c->plans.find(plan);
+  return it == c->plans.end() ? nullptr : it->second.get();
 }
 
 template <class T>
@@ -2277,6 +2284,7 @@ int32_t rb_plan_create(rb_ctx* c, int32_t pool, const rb_plan_desc* d, int32_t* 
   if (d->n_rows == 0 || d->n_rows > (1u << 24)) return fail(RB_ERR_INVALID, "n_rows %u not in [1, 2^24]", d->n_rows);
   if (d->n_heads == 0 || d->n_heads % P->n_kv || d->n_heads / P->n_kv > (uint32_t)kMaxRep)
     return fail(RB_ERR_UNSUPPORTED, "n_heads %u for %d kv heads", d->n_heads, P->n_kv);
+  if (c->next_plan == INT32_MAX) return fail(RB_ERR_UNSUPPORTED, "no plan handle left");
   RB_CUDA(cudaSetDevice(c->device));
   auto S = std::make_unique<RowSet>();
   S->pool = pool;
@@ -2330,18 +2338,15 @@ int32_t rb_plan_create(rb_ctx* c, int32_t pool, const rb_plan_desc* d, int32_t* 
   if (int rc = reserve_pages(c, *P, want)) return rc;
   // the lists are copied from this call's own memory
   RB_CUDA(cudaStreamSynchronize(c->stream));
-  size_t h = 0;
-  while (h < c->plans.size() && c->plans[h]) ++h;
-  if (h == c->plans.size()) c->plans.emplace_back();
-  c->plans[h] = std::move(S);
-  *plan = (int32_t)h;
+  *plan = c->next_plan++;
+  c->plans[*plan] = std::move(S);
   return RB_OK;
 }
 
 int32_t rb_plan_destroy(rb_ctx* c, int32_t plan) {
   if (!get_plan(c, plan)) return fail(RB_ERR_BAD_HANDLE, "plan %d", plan);
   cudaStreamSynchronize(c->stream);
-  c->plans[plan].reset();
+  c->plans.erase(plan);
   return RB_OK;
 }
 

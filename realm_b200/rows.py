@@ -25,6 +25,7 @@ from .sampling import _prev_arrays
 
 _vp, _u32, _u64, _i32, _f = C.c_void_p, C.c_uint32, C.c_uint64, C.c_int32, C.c_float
 ASYNC = 2
+BAD_HANDLE = -20  # RB_ERR_BAD_HANDLE
 MAX_VOCAB = 262144
 
 
@@ -169,11 +170,13 @@ def _call(ctx, flags, fn, *args):
 
 
 class RowPlan:
-    """The rows of one step over a KV pool (rb_plan_create); see KVPool.plan."""
+    """The rows of one step over a KV pool (rb_plan_create); see KVPool.plan. Ends with close(), with its pool, or
+    when nothing refers to it."""
+
+    handle = -1
 
     def __init__(self, pool, tenants, n_heads: int, positions=None, begin=None, end=None, window: int = 0):
         self.pool, self.ctx, self.n_heads = pool, pool.ctx, int(n_heads)
-        self.handle = -1
         arr = [None if a is None else np.ascontiguousarray(a, np.uint32) for a in (tenants, positions, begin, end)]
         self.n_rows = len(arr[0])
         for a in arr[1:]:
@@ -237,9 +240,15 @@ class RowPlan:
 
     def close(self):
         """Frees the plan; its pool's tokens stay."""
-        if self.handle >= 0 and self.ctx.handle and self.pool.handle >= 0:
-            _check(_lib.rb_plan_destroy(self.ctx.handle, self.handle))
-        self.handle = -1
+        h, self.handle = self.handle, -1
+        if h >= 0 and self.ctx.handle:
+            rc = _lib.rb_plan_destroy(self.ctx.handle, h)
+            if rc != BAD_HANDLE:  # gone with its pool
+                _check(rc)
+
+    def __del__(self):
+        if self.handle >= 0 and _lib is not None:
+            self.close()
 
     def __enter__(self):
         return self

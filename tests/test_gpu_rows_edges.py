@@ -119,3 +119,60 @@ def test_a_tensor_of_pages_outlives_its_model(ctx):
     model.close()
     assert torch.equal(view[0, 0, 0].permute(1, 0, 2), k[:16])
     assert _code(kv.pages) == -20 and _code(lambda: kv.create(1)) == -20
+
+
+def test_a_plan_ends_with_its_pool(ctx):
+    """A plan of a closed pool stays refused when other pools and plans have come, and leaves them alone."""
+    import torch
+    import realm_b200 as rb
+    a = ctx.kv_pool(1, 4, 128, rb.F32, n_pages=8, max_tenants=1, max_seq=64)
+    a.create(0)
+    old = a.plan([0] * 2, 8)
+    x, y = torch.zeros(2, 4, 128, device="cuda"), torch.zeros(2, 8, 128, device="cuda")
+    a.close()
+    b = ctx.kv_pool(1, 4, 128, rb.F32, n_pages=8, max_tenants=1, max_seq=64)
+    try:
+        b.create(0)
+        for plan in (b.plan([0] * 60, 8), b.plan([0] * 60, 8)):
+            assert _code(lambda: old.append(0, x, x)) == -20
+            assert _code(lambda: old.attention(0, y, 1.0)) == -20
+            assert b.len(0) == 0
+            plan.close()
+            plan.close()
+        old.close()
+        assert b.plan([0], 8).handle > old.handle
+    finally:
+        b.close()
+
+
+def test_a_plan_ends_with_its_model(ctx):
+    import torch
+    import realm_b200 as rb
+    model = _small_model(ctx, rb)
+    model.tenant_create(0)
+    k = torch.randn(20, 2, 64, device="cuda")
+    plan = model.kv.plan([0] * 20, 4)
+    plan.append(0, k, k)
+    model.close()
+    other = ctx.kv_pool(1, 2, 64, rb.F16, n_pages=8, max_tenants=1, max_seq=64)
+    try:
+        assert _code(lambda: plan.append(0, k, k)) == -20
+        assert _code(lambda: plan.attention(0, torch.zeros(20, 4, 64, device="cuda"), 1.0)) == -20
+        plan.close()
+    finally:
+        other.close()
+
+
+def test_a_plan_that_nothing_refers_to_is_freed(ctx):
+    import torch
+    import realm_b200 as rb
+    pool = ctx.kv_pool(1, 1, 128, rb.F16, n_pages=16, max_tenants=16, max_seq=64)
+    try:
+        pool.create(0)
+        rows = np.zeros(1 << 20, np.uint32)
+        free = torch.cuda.mem_get_info()[0]
+        for _ in range(4):  # 2^20 rows of 64 heads are 16 MB and more of lists
+            pool.plan(rows, 64, positions=rows)
+        assert free - torch.cuda.mem_get_info()[0] < 16 << 20
+    finally:
+        pool.close()
