@@ -177,7 +177,9 @@ def _flags(*arrays) -> int:
         ctx = _ORDER_CTX[0]
         dev = next(a for a in arrays if a is not None).device
         if ctx is not None and ctx._h:
-            torch.cuda.ExternalStream(ctx.stream, device=dev).wait_stream(torch.cuda.current_stream(dev))
+            cur = torch.cuda.current_stream(dev)
+            if cur.cuda_stream != ctx.stream:
+                ctx.torch_stream().wait_stream(cur)
         return PTR_DEVICE
     return PTR_HOST
 
@@ -208,7 +210,7 @@ class Context:
             _check(_lib.rb_ctx_create_on_stream(C.byref(cfg), stream, C.byref(h)))
         self._h = h
         self.device = device
-        self._stream_id = self.stream or 0
+        self._stream_id = self.stream
         _ORDER_CTX[0] = self
 
     def close(self):
@@ -235,7 +237,15 @@ class Context:
 
     @property
     def stream(self) -> int:
-        return _lib.rb_stream(self._h)
+        """The cudaStream_t; 0: the legacy default stream."""
+        return _lib.rb_stream(self._h) or 0
+
+    def torch_stream(self):
+        """The stream as torch's."""
+        import torch
+        dev = torch.device("cuda", self.device)
+        # ExternalStream does not stand for the default stream: it takes 0 as no stream given
+        return torch.cuda.ExternalStream(self.stream, device=dev) if self.stream else torch.cuda.default_stream(dev)
 
     def sync(self):
         _check(_lib.rb_sync(self._h))

@@ -151,7 +151,7 @@ class _Order:
     def __init__(self, ctx):
         import torch
         self.cur = torch.cuda.current_stream(ctx.device)
-        self.ext = torch.cuda.ExternalStream(ctx.stream, device=self.cur.device)
+        self.ext = ctx.torch_stream()
         self.ext.wait_stream(self.cur)
 
     def done(self):

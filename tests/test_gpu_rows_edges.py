@@ -176,3 +176,50 @@ def test_a_plan_that_nothing_refers_to_is_freed(ctx):
         assert free - torch.cuda.mem_get_info()[0] < 16 << 20
     finally:
         pool.close()
+
+
+# ---------------------------------------------------------------------------
+# streams
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("which", ["default", "side"])
+@pytest.mark.parametrize("current", ["default", "side"])
+def test_every_call_takes_cuda_tensors_on_a_context_of_the_callers_stream(which, current):
+    """The calls that were there before row plans, and row plans, whatever torch's current stream is."""
+    import torch
+    import realm_b200 as rb
+    side = torch.cuda.Stream()
+    own = torch.cuda.default_stream() if which == "default" else side
+    rng = np.random.default_rng(0)
+    with rb.Context(0, stream=own.cuda_stream) as c:
+        assert c.stream == own.cuda_stream
+        blocks = c.quantize(rb.Q4_K, rng.normal(0, 0.1, (256, 256)).astype(np.float32))
+        w = c.upload_weight(rb.Q4_K, 256, 256, blocks)
+        pool = c.kv_pool(1, 2, 64, rb.F16, n_pages=8, max_tenants=2, max_seq=64)
+        pool.create(0)
+        pool.create(1)
+        with torch.cuda.stream(torch.cuda.default_stream() if current == "default" else torch.cuda.Stream()):
+            x = _cuda(rng.normal(0, 1, (3, 256)).astype(np.float32))
+            got = w.matmul(x, 3, out=torch.empty(3, 256, device="cuda"))
+            host = w.matmul(x.cpu().numpy(), 3)
+            assert np.array_equal(got.cpu().numpy(), host)
+            k = torch.ones(5, 2, 64, device="cuda")
+            pool.append(0, 0, k, k * 3)
+            o = pool.attention_forward(0, [0], k[:1], 2, 0.1, positions=[4], out=torch.empty(1, 2, 64, device="cuda"))
+            # five equal keys: 3 within the rounding of five weights and their sum
+            assert (o - 3).abs().max() <= 3 * 16 * U
+            with pool.plan([1] * 5, 2) as p:
+                p.append(0, k, k * 3)
+                o = p.attention(0, k, 0.1)
+            assert (o - 3).abs().max() <= 3 * 2.0 ** -20  # probabilities in two fp16 parts: 22 bits
+            t = rb.sample_filtered(c, torch.zeros(2, 4, device="cuda"), rb.pack_filters([rb.SamplingFilter()] * 2, "cuda"),
+                                   torch.tensor([0.1, 0.9], device="cuda"))
+            assert t.tolist() == [0, 3]
+        pool.close()
+        w.free()
+
+
+def test_the_example_runs():
+    r = subprocess.run([sys.executable, os.path.join(ROOT, "examples", "local_global_decode.py")], capture_output=True,
+                       text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+    assert r.stdout.count("prompt of") == 3
