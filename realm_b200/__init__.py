@@ -163,20 +163,16 @@ def _ptr(a):
     return a.ctypes.data_as(C.c_void_p)
 
 
-_ORDER_CTX = [None]  # the context whose stream device-tensor calls are ordered on
-
-
-def _flags(*arrays) -> int:
+def _flags(ctx: "Context", *arrays) -> int:
     devs = [_is_dev(a) for a in arrays if a is not None]
     if any(devs) and not all(devs):
         raise ValueError("mix of host and device buffers in one call")
     if devs and devs[0]:
-        # torch produced these tensors on its current stream; make the library's
+        # torch produced these tensors on its current stream; make the context's
         # stream wait for that work (stream-ordered, no host synchronisation)
         import torch
-        ctx = _ORDER_CTX[0]
         dev = next(a for a in arrays if a is not None).device
-        if ctx is not None and ctx._h:
+        if ctx._h:
             cur = torch.cuda.current_stream(dev)
             if cur.cuda_stream != ctx.stream:
                 ctx.torch_stream().wait_stream(cur)
@@ -211,7 +207,6 @@ class Context:
         self._h = h
         self.device = device
         self._stream_id = self.stream
-        _ORDER_CTX[0] = self
 
     def close(self):
         if getattr(self, "_h", None) and _lib is not None:
@@ -262,7 +257,7 @@ class Context:
         nb = (blocks.numel() if _is_dev(blocks) else blocks.nbytes) // BLOCK_BYTES[dtype]
         if out is None:
             out = np.empty(nb * BLOCK_ELEMS[dtype], np.float32)
-        _check(_lib.rb_dequantize(self._h, dtype, _ptr(blocks), nb, _ptr(out), _flags(blocks, out)))
+        _check(_lib.rb_dequantize(self._h, dtype, _ptr(blocks), nb, _ptr(out), _flags(self, blocks, out)))
         return out
 
     def quantize(self, dtype: int, x, out=None):
@@ -270,7 +265,7 @@ class Context:
         n = x.numel() if _is_dev(x) else x.size
         if out is None:
             out = np.empty(n // BLOCK_ELEMS[dtype] * BLOCK_BYTES[dtype], np.uint8)
-        _check(_lib.rb_quantize(self._h, dtype, _ptr(x), n, _ptr(out), _flags(x, out)))
+        _check(_lib.rb_quantize(self._h, dtype, _ptr(x), n, _ptr(out), _flags(self, x, out)))
         return out
 
     # ---- GpuBackendTrait::fused_dequant_matmul_* ----
@@ -283,7 +278,7 @@ class Context:
         if out is None:
             out = np.empty((batch_size, n), np.float32)
         _check(_lib.rb_fused_dequant_matmul(self._h, dtype, _ptr(blocks), nblocks, _ptr(input), _ptr(out),
-                                            batch_size, n, k, _flags(blocks, input, out)))
+                                            batch_size, n, k, _flags(self, blocks, input, out)))
         return out
 
     def fused_dequant_matmul_q4k(self, blocks, input, batch_size, n, k):
@@ -316,7 +311,7 @@ class Context:
         if out is None:
             out = np.empty((m, n), np.float32)
         fn = _lib.rb_candle_matmul_transposed if transposed else _lib.rb_candle_matmul
-        _check(fn(self._h, _ptr(a), _ptr(b), _ptr(out), m, k, n, _flags(a, b, out)))
+        _check(fn(self._h, _ptr(a), _ptr(b), _ptr(out), m, k, n, _flags(self, a, b, out)))
         return out
 
     def kv_pool(self, n_layers, n_kv_heads, head_dim, kv_dtype=F16, n_pages=1024, max_tenants=64,
@@ -332,14 +327,15 @@ class Weight:
         blocks = _u8(blocks)
         nbytes = blocks.numel() if _is_dev(blocks) else blocks.nbytes
         h = C.c_int32()
-        _check(_lib.rb_weight_upload(ctx.handle, dtype, n, k, _ptr(blocks), nbytes, _flags(blocks), C.byref(h)))
+        _check(_lib.rb_weight_upload(ctx.handle, dtype, n, k, _ptr(blocks), nbytes, _flags(ctx, blocks), C.byref(h)))
         self.handle = h.value
 
     def matmul(self, x, batch_size: int, out=None):
         x = _f32(x)
         if out is None:
             out = np.empty((batch_size, self.n), np.float32)
-        _check(_lib.rb_weight_matmul(self.ctx.handle, self.handle, _ptr(x), _ptr(out), batch_size, _flags(x, out)))
+        _check(_lib.rb_weight_matmul(self.ctx.handle, self.handle, _ptr(x), _ptr(out), batch_size,
+                                     _flags(self.ctx, x, out)))
         return out
 
     def matmul_noalloc(self, x, out, batch_size: int):
@@ -349,7 +345,7 @@ class Weight:
         if not (_is_dev(x) and _is_dev(out)):
             raise ValueError("matmul_noalloc takes CUDA tensors only")
         _check(_lib.rb_weight_matmul_noalloc(self.ctx.handle, self.handle, _ptr(x), _ptr(out), batch_size,
-                                             _flags(x, out)))
+                                             _flags(self.ctx, x, out)))
         return out
 
     def export(self) -> np.ndarray:
@@ -440,7 +436,7 @@ class KVPool:
         n = k.numel() if _is_dev(k) else k.size
         seq = n // (self.n_kv * self.hd)
         return _check(_lib.rb_kv_append(self.ctx.handle, self.handle, tenant, layer, _ptr(k), _ptr(v), seq,
-                                         _flags(k, v)))
+                                         _flags(self.ctx, k, v)))
 
     def gather(self, tenant: int, layer: int):
         n = self.len(tenant, layer) * self.n_kv * self.hd
@@ -462,7 +458,7 @@ class KVPool:
             out = np.empty((len(t), n_heads * self.hd), np.float32)
         _check(_lib.rb_attention_forward(self.ctx.handle, self.handle, layer, len(t), _ptr(t), _ptr(p), _ptr(q),
                                          _ptr(k_new), _ptr(v_new), _ptr(out), n_heads, scale,
-                                         _flags(q, k_new, v_new, out)))
+                                         _flags(self.ctx, q, k_new, v_new, out)))
         return out
 
 
@@ -530,7 +526,7 @@ class Model:
             data = np.ascontiguousarray(data).view(np.uint8).ravel()
         nbytes = (data.numel() * data.element_size()) if _is_dev(data) else data.nbytes
         _check(_lib.rb_model_set_weight(self.ctx.handle, self.handle, which, layer, dtype, _ptr(data), nbytes,
-                                        _flags(data)))
+                                        _flags(self.ctx, data)))
 
     def set_weights(self, weights: dict):
         for (which, layer), (dtype, data) in weights.items():
@@ -625,7 +621,7 @@ class Model:
         caller's linear memory `mem` (a uint8 array or CUDA tensor) at mem_offset."""
         nbytes = (mem.numel() * mem.element_size()) if _is_dev(mem) else mem.nbytes
         return _check(_lib.rb_memory64_read(self.ctx.handle, self.handle, offset, _ptr(mem), nbytes, mem_offset,
-                                            size, _flags(mem)))
+                                            size, _flags(self.ctx, mem)))
 
     def close(self):
         if self.handle >= 0:

@@ -223,3 +223,24 @@ def test_the_example_runs():
                        text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
     assert r.stdout.count("prompt of") == 3
+
+
+def test_calls_wait_on_their_own_contexts_stream(ctx):
+    """Another context that came and went changes nothing."""
+    import torch
+    import realm_b200 as rb
+    rng = np.random.default_rng(1)
+    w = ctx.upload_weight(rb.Q4_K, 256, 256, ctx.quantize(rb.Q4_K, rng.normal(0, 0.1, (256, 256)).astype(np.float32)))
+    value = rng.normal(0, 1, (3, 256)).astype(np.float32)
+    want = w.matmul(value, 3)
+    value, x, out = _cuda(value), torch.zeros(3, 256, device="cuda"), torch.empty(3, 256, device="cuda")
+    big = torch.randn(4096, 4096, device="cuda")
+    with rb.Context(0), rb.Context(0):
+        pass
+    torch.cuda.synchronize()
+    for _ in range(20):
+        big = (big @ big).clamp(-1, 1)  # keeps torch's stream busy, so that a missing wait shows
+    x.copy_(value + big[:3, :256] * 0)
+    w.matmul(x, 3, out=out)
+    assert np.array_equal(out.cpu().numpy(), want)
+    w.free()
