@@ -2490,6 +2490,8 @@ int32_t rb_sample_filtered(rb_ctx* c, int32_t dtype, const void* logits, uint64_
   if (!c) return fail(RB_ERR_BAD_HANDLE, "null context");
   if (int rc = row_dtype(dtype)) return rc;
   if (!logits || !params || !uniforms || !out) return fail(RB_ERR_INVALID, "logits/params/uniforms/out NULL");
+  const bool dev = flags & RB_PTR_DEVICE;
+  if (!dev && !prev && prev_off && n_rows && prev_off[n_rows] == 0) prev_off = nullptr;  // no row has a history
   if ((prev == nullptr) != (prev_off == nullptr)) return fail(RB_ERR_INVALID, "prev_tokens and prev_offsets go together");
   if (vocab == 0 || vocab > (uint32_t)kFilterMaxVocab || ld < vocab)
     return fail(RB_ERR_UNSUPPORTED, "vocab %u not in [1, %d] or ld %llu < vocab", vocab, kFilterMaxVocab,
@@ -2497,7 +2499,6 @@ int32_t rb_sample_filtered(rb_ctx* c, int32_t dtype, const void* logits, uint64_
   if (n_rows == 0) return 0;
   if (n_rows > (1u << 24)) return fail(RB_ERR_INVALID, "n_rows %u > 2^24", n_rows);
   RB_CUDA(cudaSetDevice(c->device));
-  const bool dev = flags & RB_PTR_DEVICE;
   const size_t esz = dtype == RB_F16 ? 2 : 4;
   Staged sl, sp, sprev, soff, su;
   if (int rc = stage_rows(c, "logits", logits, ld, n_rows, vocab, esz, flags, sl)) return rc;

@@ -322,6 +322,9 @@ def sample_filtered(ctx, logits, filters, uniforms, prev=None, out=None, probs=N
         out = torch.empty(n, dtype=torch.int32, device=logits.device)
     prev = prev or (None, None)
     _space([logits, filters, uniforms, out, probs, *prev], ctx)
+    if prev[0] is not None and prev[0].numel() == 0 and prev[1] is not None:  # no row has a history; no memory either
+        _vec(prev[1], "int32", n + 1, "prev offsets")
+        prev = (None, None)
     _call(
         ctx, flags, _lib.rb_sample_filtered, ctx._h, dt, logits.data_ptr(), logits.stride(0) if n > 1 else v, n, v,
         _vec(filters, "uint8", n * C.sizeof(_Filter), "filters"),

@@ -244,3 +244,14 @@ def test_calls_wait_on_their_own_contexts_stream(ctx):
     w.matmul(x, 3, out=out)
     assert np.array_equal(out.cpu().numpy(), want)
     w.free()
+
+
+def test_empty_histories_on_cuda_tensors(ctx):
+    """The first token of a batch: no row has a history, and the tensor of all of them is empty."""
+    import torch
+    import realm_b200 as rb
+    x = torch.randn(3, 1000, device="cuda", generator=torch.Generator("cuda").manual_seed(0))
+    u = torch.tensor([0.2, 0.5, 0.8], device="cuda")
+    f = rb.pack_filters([rb.SamplingFilter(0.7, top_k=20, repetition_penalty=1.3)] * 3, "cuda")
+    none = (torch.empty(0, dtype=torch.int32, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda"))
+    assert torch.equal(rb.sample_filtered(ctx, x, f, u, prev=none), rb.sample_filtered(ctx, x, f, u))
