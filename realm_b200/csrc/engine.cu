@@ -2489,6 +2489,7 @@ int32_t rb_sample_filtered(rb_ctx* c, int32_t dtype, const void* logits, uint64_
                            uint32_t flags) {
   if (!c) return fail(RB_ERR_BAD_HANDLE, "null context");
   if (int rc = row_dtype(dtype)) return rc;
+  if (n_rows == 0) return 0;  // an empty batch has no memory
   if (!logits || !params || !uniforms || !out) return fail(RB_ERR_INVALID, "logits/params/uniforms/out NULL");
   const bool dev = flags & RB_PTR_DEVICE;
   if (!dev && !prev && prev_off && n_rows && prev_off[n_rows] == 0) prev_off = nullptr;  // no row has a history
@@ -2496,7 +2497,6 @@ int32_t rb_sample_filtered(rb_ctx* c, int32_t dtype, const void* logits, uint64_
   if (vocab == 0 || vocab > (uint32_t)kFilterMaxVocab || ld < vocab)
     return fail(RB_ERR_UNSUPPORTED, "vocab %u not in [1, %d] or ld %llu < vocab", vocab, kFilterMaxVocab,
                 (unsigned long long)ld);
-  if (n_rows == 0) return 0;
   if (n_rows > (1u << 24)) return fail(RB_ERR_INVALID, "n_rows %u > 2^24", n_rows);
   RB_CUDA(cudaSetDevice(c->device));
   const size_t esz = dtype == RB_F16 ? 2 : 4;

@@ -286,6 +286,8 @@ class SamplingFilter:
 def pack_filters(filters: Sequence[SamplingFilter], device):
     """The filters as a tensor on `device` ([n][20] bytes), for sample_filtered on CUDA tensors."""
     import torch
+    if not filters:
+        return torch.empty((0, C.sizeof(_Filter)), dtype=torch.uint8, device=device)
     arr = (_Filter * len(filters))(*[f.c() for f in filters])
     return torch.frombuffer(bytearray(arr), dtype=torch.uint8).view(len(filters), C.sizeof(_Filter)).to(device)
 

@@ -255,3 +255,12 @@ def test_empty_histories_on_cuda_tensors(ctx):
     f = rb.pack_filters([rb.SamplingFilter(0.7, top_k=20, repetition_penalty=1.3)] * 3, "cuda")
     none = (torch.empty(0, dtype=torch.int32, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda"))
     assert torch.equal(rb.sample_filtered(ctx, x, f, u, prev=none), rb.sample_filtered(ctx, x, f, u))
+
+
+def test_empty_batches_on_cuda_tensors(ctx):
+    import torch
+    import realm_b200 as rb
+    for typ in (torch.float32, torch.float16):
+        t = rb.sample_filtered(ctx, torch.empty(0, 1000, dtype=typ, device="cuda"), rb.pack_filters([], "cuda"),
+                               torch.empty(0, device="cuda"), probs=torch.empty(0, device="cuda"))
+        assert t.shape == (0,) and t.dtype == torch.int32
