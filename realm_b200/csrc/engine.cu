@@ -2220,6 +2220,12 @@ int stage_rows(Ctx* c, const char* name, const void* p, uint64_t ld, size_t rows
   return stage(c, p, ((rows - 1) * ld + width) * esz, flags, out);
 }
 
+// The same for `count` values of 4 bytes (floats, or structures of such).
+int stage_words(Ctx* c, const char* name, const void* p, size_t count, uint32_t flags, Staged& out) {
+  if ((flags & RB_PTR_DEVICE) && (uintptr_t)p % 4) return fail(RB_ERR_INVALID, "%s is not aligned to 4 bytes", name);
+  return stage(c, p, count * 4, flags, out);
+}
+
 // Takes pages so that want[i].second tokens of tenant want[i].first fit, in the
 // order of `want`, all or none, and copies the new page-table entries to the device.
 int reserve_pages(Ctx* c, KvPool& P, const std::vector<std::pair<int, int>>& want) {
@@ -2384,11 +2390,11 @@ int32_t rb_plan_append(rb_ctx* c, int32_t plan, uint32_t layer, const rb_append_
   if (int rc = stage_rows(c, "k", d->k, d->ldk, n, wk, esz, flags, sk)) return rc;
   if (int rc = stage_rows(c, "v", d->v, d->ldv, n, wk, esz, flags, sv)) return rc;
   if (d->q_norm)
-    if (int rc = stage(c, d->q_norm, (size_t)P.hd * 4, flags, nq)) return rc;
+    if (int rc = stage_words(c, "q_norm", d->q_norm, P.hd, flags, nq)) return rc;
   if (d->k_norm)
-    if (int rc = stage(c, d->k_norm, (size_t)P.hd * 4, flags, nk)) return rc;
+    if (int rc = stage_words(c, "k_norm", d->k_norm, P.hd, flags, nk)) return rc;
   if (d->rotary)
-    if (int rc = stage(c, d->rope, (size_t)(S->max_pos + 1) * d->rotary * 4, flags, sr)) return rc;
+    if (int rc = stage_words(c, "rope", d->rope, (size_t)(S->max_pos + 1) * d->rotary, flags, sr)) return rc;
   RowAppendArgs a;
   a.q = sq.dptr;
   a.k = sk.dptr;
@@ -2444,7 +2450,7 @@ int32_t rb_plan_attention(rb_ctx* c, int32_t plan, uint32_t layer, const rb_atte
   if (int rc = stage_rows(c, "q", d->q, d->ldq, n, w, esz, flags, sq)) return rc;
   if (int rc = stage_rows(c, "out", d->out, d->ldo, n, w, esz, flags, so)) return rc;
   if (d->slopes)
-    if (int rc = stage(c, d->slopes, (size_t)S->n_heads * 4, flags, ss)) return rc;
+    if (int rc = stage_words(c, "slopes", d->slopes, S->n_heads, flags, ss)) return rc;
   RowAttnArgs a;
   if (P.f16) a.tmap = P.tmap;
   a.q = sq.dptr;
@@ -2502,12 +2508,14 @@ int32_t rb_sample_filtered(rb_ctx* c, int32_t dtype, const void* logits, uint64_
   const size_t esz = dtype == RB_F16 ? 2 : 4;
   Staged sl, sp, sprev, soff, su;
   if (int rc = stage_rows(c, "logits", logits, ld, n_rows, vocab, esz, flags, sl)) return rc;
-  if (int rc = stage(c, params, (size_t)n_rows * sizeof(rb_sampling_filter), flags, sp)) return rc;
+  if (int rc = stage_words(c, "params", params, (size_t)n_rows * (sizeof(rb_sampling_filter) / 4), flags, sp)) return rc;
   if (prev_off) {
-    if (int rc = stage(c, prev_off, (size_t)(n_rows + 1) * 4, flags, soff)) return rc;
-    if (int rc = stage(c, prev, dev ? 0 : (size_t)prev_off[n_rows] * 4, flags, sprev)) return rc;
+    if (int rc = stage_words(c, "prev_offsets", prev_off, (size_t)n_rows + 1, flags, soff)) return rc;
+    if (int rc = stage_words(c, "prev_tokens", prev, dev ? 0 : prev_off[n_rows], flags, sprev)) return rc;
   }
-  if (int rc = stage(c, uniforms, (size_t)n_rows * 4, flags, su)) return rc;
+  if (int rc = stage_words(c, "uniforms", uniforms, n_rows, flags, su)) return rc;
+  if (dev && ((uintptr_t)out % 4 || (uintptr_t)probs % 4))
+    return fail(RB_ERR_INVALID, "out_tokens or probs is not aligned to 4 bytes");
   DevBuf dout;
   FilterArgs a;
   a.logits = sl.dptr;

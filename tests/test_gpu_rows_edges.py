@@ -264,3 +264,46 @@ def test_empty_batches_on_cuda_tensors(ctx):
         t = rb.sample_filtered(ctx, torch.empty(0, 1000, dtype=typ, device="cuda"), rb.pack_filters([], "cuda"),
                                torch.empty(0, device="cuda"), probs=torch.empty(0, device="cuda"))
         assert t.shape == (0,) and t.dtype == torch.int32
+
+
+# ---------------------------------------------------------------------------
+# refusals
+# ---------------------------------------------------------------------------
+def test_memory_off_its_alignment_is_refused(ctx):
+    """Device memory that a kernel could not read by words: an error from the call, nothing launched."""
+    import ctypes as C
+    import torch
+    import realm_b200 as rb
+    from realm_b200 import rows as R
+    x = torch.zeros(2, 8, device="cuda")
+    u = torch.zeros(2, device="cuda")
+    packed = rb.pack_filters([rb.SamplingFilter()] * 2, "cuda")
+    odd = torch.zeros(41, dtype=torch.uint8, device="cuda")[1:]
+    odd.copy_(packed.reshape(-1))
+    assert _code(lambda: rb.sample_filtered(ctx, x, odd, u)) == -3
+    ok = dict(params=packed.data_ptr(), prev=u.data_ptr(), prev_off=u.data_ptr(), uniforms=u.data_ptr(),
+              out=torch.zeros(2, device="cuda").data_ptr(), probs=u.data_ptr())
+    for name in ok:
+        a = dict(ok, **{name: ok[name] + 2})
+        rc = rb.lib().rb_sample_filtered(ctx.handle, rb.F32, x.data_ptr(), 8, 2, 8, a["params"], a["prev"], a["prev_off"],
+                                         a["uniforms"], a["out"], a["probs"], rb.PTR_DEVICE)
+        assert rc == -3, name
+    pool = ctx.kv_pool(1, 2, 64, rb.F16, n_pages=2, max_tenants=1, max_seq=32)
+    try:
+        pool.create(0)
+        with pool.plan([0], 4) as p:
+            k = torch.zeros(1, 4, 64, device="cuda")
+            at = k.data_ptr()
+            good = dict(q=at, k=at, v=at, q_out=at, q_norm=at, k_norm=at, rope=at)
+            for name in good:
+                d = R._AppendDesc(dtype=rb.F32, ldq=256, ldk=128, ldv=128, ldo=256, eps=1e-6, rotary=64, rope_len=1,
+                                  **dict(good, **{name: at + 2}))
+                assert rb.lib().rb_plan_append(ctx.handle, p.handle, 0, C.byref(d), rb.PTR_DEVICE) == -3, name
+            assert pool.len(0) == 0
+            p.append(0, k[:, :2], k[:, :2])
+            good = dict(q=at, out=at, slopes=at)
+            for name in good:
+                d = R._AttentionDesc(dtype=rb.F32, scale=1.0, ldq=256, ldo=256, **dict(good, **{name: at + 2}))
+                assert rb.lib().rb_plan_attention(ctx.handle, p.handle, 0, C.byref(d), rb.PTR_DEVICE) == -3, name
+    finally:
+        pool.close()
