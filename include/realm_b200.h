@@ -244,8 +244,8 @@ int32_t rb_plan_create(rb_ctx* ctx, int32_t pool, const rb_plan_desc* desc, int3
 int32_t rb_plan_destroy(rb_ctx* ctx, int32_t plan);
 
 /* Layouts of the rows that go in: element (row, head, i) of q lies at
- * q[row * ldq + head * head_dim + i], and so on; ld* count elements, and at least
- * heads * head_dim of them, so q, k and v may be slices of one projection's output. */
+ * q[row * ldq + head * head_dim + i], and so on; ld* count elements, at least
+ * heads * head_dim of them and at most 2^36, so q, k and v may be slices of one projection's output. */
 #define RB_ROPE_HALF 0     /* pairs (i, i + rotary / 2) */
 #define RB_ROPE_ADJACENT 1 /* pairs (2i, 2i + 1), crates/realm-models/src/attention.rs:171-240 */
 typedef struct rb_append_desc {

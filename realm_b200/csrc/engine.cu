@@ -2216,6 +2216,8 @@ int stage_rows(Ctx* c, const char* name, const void* p, uint64_t ld, size_t rows
                uint32_t flags, Staged& out) {
   if (!p) return fail(RB_ERR_INVALID, "%s NULL", name);
   if (ld < width) return fail(RB_ERR_INVALID, "ld %llu of %s below its row of %zu", (unsigned long long)ld, name, width);
+  if (rows > 1 && ld > (1ull << 36))  // of 2^24 rows at most: the bytes fit 64 bits
+    return fail(RB_ERR_INVALID, "ld %llu of %s above 2^36", (unsigned long long)ld, name);
   if ((uintptr_t)p % esz) return fail(RB_ERR_INVALID, "%s is not aligned to its elements", name);
   return stage(c, p, ((rows - 1) * ld + width) * esz, flags, out);
 }

@@ -307,3 +307,33 @@ def test_memory_off_its_alignment_is_refused(ctx):
                 assert rb.lib().rb_plan_attention(ctx.handle, p.handle, 0, C.byref(d), rb.PTR_DEVICE) == -3, name
     finally:
         pool.close()
+
+
+def test_rows_too_far_apart_are_refused(ctx):
+    """Distances whose bytes would not fit 64 bits."""
+    import ctypes as C
+    import realm_b200 as rb
+    from realm_b200 import rows as R
+    x = np.zeros(1024, np.float32)
+    at = x.ctypes.data
+    pool = ctx.kv_pool(1, 1, 64, rb.F16, n_pages=2, max_tenants=1, max_seq=32)
+    try:
+        pool.create(0)
+        with pool.plan([0, 0], 1) as p:
+            for ld in ((1 << 62) + 64, 1 << 61, (1 << 36) + 1):
+                d = R._AppendDesc(dtype=rb.F32, k=at, v=at, ldk=64, ldv=ld)
+                assert rb.lib().rb_plan_append(ctx.handle, p.handle, 0, C.byref(d), rb.PTR_HOST) == -3
+                d = R._AppendDesc(dtype=rb.F32, k=at, v=at, ldk=ld, ldv=64)
+                assert rb.lib().rb_plan_append(ctx.handle, p.handle, 0, C.byref(d), rb.PTR_HOST) == -3
+                assert pool.len(0) == 0
+                f = rb.SamplingFilter().c()
+                rc = rb.lib().rb_sample_filtered(ctx.handle, rb.F32, at, ld, 2, 8, (R._Filter * 2)(f, f), None, None, at, at,
+                                                 None, rb.PTR_HOST)
+                assert rc == -3
+            p.append(0, x[:128].reshape(2, 1, 64), x[:128].reshape(2, 1, 64))
+            for ld in ((1 << 62) + 64, 1 << 61, (1 << 36) + 1):
+                for ldq, ldo in ((ld, 64), (64, ld)):
+                    d = R._AttentionDesc(dtype=rb.F32, scale=1.0, q=at, out=at, ldq=ldq, ldo=ldo)
+                    assert rb.lib().rb_plan_attention(ctx.handle, p.handle, 0, C.byref(d), rb.PTR_HOST) == -3
+    finally:
+        pool.close()
