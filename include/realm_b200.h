@@ -517,7 +517,8 @@ typedef struct rb_sampling_filter {
   float repetition_penalty; /* 1: off */
 } rb_sampling_filter;
 /* One token per row of logits [n_rows][ld] (dtype RB_F32 or RB_F16). params, prev_*,
- * uniforms and pointer spaces as rb_sample_logits; probs: NULL, or [n_rows] the
+ * uniforms and pointer spaces as rb_sample_logits; prev_offsets never fall (checked
+ * where they are host memory) and end within prev_tokens; probs: NULL, or [n_rows] the
  * tokens' probabilities among those kept. A row without a finite or +infinite
  * logit gets token 0xffffffff; unless RB_ASYNC, the call then returns
  * RB_ERR_INVALID ("Failed to create weighted index"). Returns n_rows. */

@@ -2506,6 +2506,9 @@ int32_t rb_sample_filtered(rb_ctx* c, int32_t dtype, const void* logits, uint64_
     return fail(RB_ERR_UNSUPPORTED, "vocab %u not in [1, %d] or ld %llu < vocab", vocab, kFilterMaxVocab,
                 (unsigned long long)ld);
   if (n_rows > (1u << 24)) return fail(RB_ERR_INVALID, "n_rows %u > 2^24", n_rows);
+  if (prev_off && !dev)
+    for (uint32_t r = 0; r < n_rows; ++r)
+      if (prev_off[r] > prev_off[r + 1]) return fail(RB_ERR_INVALID, "row %u: prev_offsets fall", r);
   RB_CUDA(cudaSetDevice(c->device));
   const size_t esz = dtype == RB_F16 ? 2 : 4;
   Staged sl, sp, sprev, soff, su;

@@ -337,3 +337,17 @@ def test_rows_too_far_apart_are_refused(ctx):
                     assert rb.lib().rb_plan_attention(ctx.handle, p.handle, 0, C.byref(d), rb.PTR_HOST) == -3
     finally:
         pool.close()
+
+
+def test_histories_out_of_order_are_refused(ctx):
+    """Host offsets that fall, or pass the last one: the kernel would read past the tokens."""
+    import realm_b200 as rb
+    from realm_b200 import rows as R
+    x, u = np.zeros((2, 8), np.float32), np.zeros(2, np.float32)
+    f = rb.SamplingFilter(repetition_penalty=1.2).c()
+    tokens, out = np.zeros(4, np.uint32), np.zeros(2, np.uint32)
+    for off, rc in (([0, 9, 4], -3), ([5, 2, 4], -3), ([0, 3, 2], -3), ([0, 1, 4], 2), ([2, 2, 4], 2)):
+        off = np.array(off, np.uint32)
+        assert rb.lib().rb_sample_filtered(ctx.handle, rb.F32, x.ctypes.data, 8, 2, 8, (R._Filter * 2)(f, f),
+                                           tokens.ctypes.data, off.ctypes.data, u.ctypes.data, out.ctypes.data, None,
+                                           rb.PTR_HOST) == rc, off
