@@ -128,10 +128,11 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) rows_f32_kernel(const __gri
   Ahead ah{u_begin, u_end, 0, 0, 0, 0};
   PageCache pages;
   ah.open(a);
-  int issued = 0, used = 0, which = 0;
+  int issued = 0, landed = 0, used = 0, which = 0;
+  bool alive = true;  // the same in every lane; a wait that ran out ends the warp's work
   const float* block = nullptr;
   auto issue = [&](int limit) {
-    while (issued < limit && ah.pu < u_end) {
+    while (alive && issued < limit && ah.pu < u_end) {
       if (which == 0) {
         const int page = pages.page(a, ah.tenant, ah.pk);
         block = pool + ((((size_t)page * a.kv.n_layers + a.layer) * 2) * a.kv.n_kv + ah.kvh) * 16 * HD;
@@ -147,11 +148,11 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) rows_f32_kernel(const __gri
     }
   };
   issue(NST);
-  bool alive = true;
   // the next block of the ring; done with it: release()
   auto take = [&]() {
     const int s = used % NST;
-    if (alive) alive = mbar_wait(&bar[s], (used / NST) & 1, a.err, DEV_TIMEOUT_FULL);
+    if (alive) alive = __all_sync(0xffffffffu, mbar_wait(&bar[s], (used / NST) & 1, a.err, DEV_TIMEOUT_FULL));
+    landed += alive;
     return reinterpret_cast<const float*>(ring + s * C::BLK);
   };
   auto release = [&]() {
@@ -159,7 +160,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) rows_f32_kernel(const __gri
     ++used;
     issue(used + NST);
   };
-  for (int ui = u_begin; ui < u_end; ++ui) {
+  for (int ui = u_begin; ui < u_end && alive; ++ui) {
     const AttnUnit u = a.units[ui];
     __syncwarp();
 #pragma unroll
@@ -178,7 +179,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) rows_f32_kernel(const __gri
 #pragma unroll
       for (int d = 0; d < DPL; ++d) o[v][d] = 0.f;
     }
-    for (int k = u.k0; k < u.k1; k += kRowPage) {
+    for (int k = u.k0; k < u.k1 && alive; k += kRowPage) {
       const float* kb = take();
       float dot[NV];
 #pragma unroll
@@ -237,6 +238,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) rows_f32_kernel(const __gri
       }
       release();
     }
+    if (!alive) break;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
 #pragma unroll
@@ -254,6 +256,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) rows_f32_kernel(const __gri
       }
     }
   }
+  // after a wait that ran out: what is in flight lands before the shared memory goes away
+  for (; landed < issued; ++landed) mbar_wait(&bar[landed % NST], (landed / NST) & 1, a.err, DEV_TIMEOUT_FULL);
 }
 
 // ---------------------------------------------------------------------------
@@ -354,9 +358,10 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) rows_mma_kernel(const __gri
   Ahead ah{u_begin, u_end, 0, 0, 0, 0};
   PageCache pages;
   ah.open(a);
-  int issued = 0, used = 0;
+  int issued = 0, landed = 0, used = 0;
+  bool alive = true;  // the same in every lane; a wait that ran out ends the warp's work
   auto issue = [&](int limit) {
-    while (issued < limit && ah.pu < u_end) {
+    while (alive && issued < limit && ah.pu < u_end) {
       const int page = pages.page(a, ah.tenant, ah.pk);
       if (lane == 0) {
         const int s = issued % NST;
@@ -373,7 +378,6 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) rows_mma_kernel(const __gri
     }
   };
   issue(NST);
-  bool alive = true;
   int koff[KS], voff[KS];
   {
     const int mi = lane >> 3, rr = lane & 7;
@@ -384,7 +388,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) rows_mma_kernel(const __gri
     }
   }
   const bool whole = ((reinterpret_cast<uintptr_t>(a.q) | (size_t)a.ldq * (HL ? 4 : 2)) & (HL ? 7 : 3)) == 0;
-  for (int ui = u_begin; ui < u_end; ++ui) {
+  for (int ui = u_begin; ui < u_end && alive; ++ui) {
     const AttnUnit u = a.units[ui];
     uint32_t qb[KS][1 + HL][2];
     float mul = 1.f;
@@ -432,7 +436,9 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) rows_mma_kernel(const __gri
     for (int i = 0; i < KS; ++i) ot[i][0] = ot[i][1] = ot[i][2] = ot[i][3] = 0.f;
     for (int k = u.k0; k < u.k1; k += kRowPage) {
       const int s = used % NST;
-      if (alive) alive = mbar_wait(&bar[s], (used / NST) & 1, a.err, DEV_TIMEOUT_FULL);
+      alive = __all_sync(0xffffffffu, mbar_wait(&bar[s], (used / NST) & 1, a.err, DEV_TIMEOUT_FULL));
+      if (!alive) break;
+      ++landed;
       const uint8_t* kb = ring + s * C::STAGE;
       const uint8_t* vb = kb + C::BLK;
       float sa[4][4];
@@ -541,6 +547,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) rows_mma_kernel(const __gri
       ++used;
       issue(used + NST);
     }
+    if (!alive) break;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -569,6 +576,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) rows_mma_kernel(const __gri
       }
     }
   }
+  // after a wait that ran out: what is in flight lands before the shared memory goes away
+  for (; landed < issued; ++landed) mbar_wait(&bar[landed % NST], (landed / NST) & 1, a.err, DEV_TIMEOUT_FULL);
 }
 
 // Joins the parts of the items that were cut, parts in the order of the keys: a thread
