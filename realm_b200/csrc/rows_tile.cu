@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
     return;
   }
   uint8_t* ring = smem + 2 * (1 + HL) * C::QT;
-  __shared__ uint64_t q_bar[2], s_bar[2], p_bar[2], o_bar[2], s_free, full[NS], freeb[NS], drain;
+  __shared__ uint64_t q_bar[2], s_bar[2], p_bar[2], o_bar[2], s_free, full[NS], freeb[NS], drain, mend_bar;
   __shared__ uint32_t tmem_slot;
   __shared__ int primed[2];    // O holds something before the first product
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -265,6 +265,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
     }
     mbar_init(&drain, 1);
     mbar_init(&s_free, 128);
+    mbar_init(&mend_bar, 128 * nt);
     fence_barrier_init();
   }
   tc_before();
@@ -501,6 +502,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
     // them took longer than with either (fp16 rows, 1 and 2: 993 us).
     int form = !__all_sync(0xffffffffu, kcap > 1e-30f) ? 3 : BIAS || !__all_sync(0xffffffffu, fuse_ok) ? 2 : 1;
     float m = -INFINITY, l = 0.f;
+    // Both tiles meet. Not a named barrier, which has no limit: after a wait that ran out
+    // one of them may have read other values and not come.
+    int met = 0;
+    auto meet = [&]() {
+      mbar_arrive(&mend_bar);
+      if (alive) alive = mbar_wait(&mend_bar, (uint32_t)(met & 1), a.err, DEV_TIMEOUT_DRAIN);
+      ++met;
+    };
     for (int j = 0; j < nb; ++j) {
       const int kb = u.k0 + j * B;
       if (alive) alive = mbar_wait(&s_bar[tile], (uint32_t)(j & 1), a.err, DEV_TIMEOUT_FULL);
@@ -744,7 +753,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
             }
             st32(to + d, reinterpret_cast<uint32_t*>(o));
           }
-          any_softmax(1, 128 * nt, false);  // all rows have taken theirs
+          meet();  // all rows have taken theirs
           for (int ch = tile * (HD / 8 / nt); ch < (tile + 1) * (HD / 8 / nt); ++ch) {
             uint4* p = reinterpret_cast<uint4*>(vrow + (ch >> 3) * C::PANEL + (((ch & 7) ^ (tr & 7)) << 4));
             uint32_t* w = reinterpret_cast<uint32_t*>(p);
@@ -755,7 +764,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
             }
           }
           proxy_fence();
-          any_softmax(1, 128 * nt, false);
+          meet();
           if (tr == 0 && j == 0) *(volatile int*)&primed[tile] = 1;
         }
       }
