@@ -282,9 +282,11 @@ typedef struct rb_attention_desc {
 /* Attention of the plan's rows over `layer` of the cache: out = softmax(s) . v over
  * the keys that a row sees, s = cap(scale * q . k) - slope * distance; 0 for a row
  * that sees none. What lies in keys that a row does not see never reaches it.
- * Every key of the plan has to be cached (RB_ERR_OUT_OF_BOUNDS). fp32 rows are
- * computed to fp32 accuracy on either cache type, fp16 rows with probabilities
- * rounded to fp16 on fp16 caches. Returns n_rows. */
+ * Every key of the plan has to be cached (RB_ERR_OUT_OF_BOUNDS). Sums are fp32. On
+ * fp32 caches so is all else. On fp16 caches fp32 rows have q and the probabilities
+ * in 22 bits (each probability to 2^-22 of itself and 2^-37 of the row's largest),
+ * fp16 rows probabilities rounded to fp16 (2^-12 and 2^-34): a caller who wants fp16
+ * rows without that passes them as fp32. Returns n_rows. */
 int32_t rb_plan_attention(rb_ctx* ctx, int32_t plan, uint32_t layer, const rb_attention_desc* desc, uint32_t flags);
 /* Test hook, host only: the work lists for rows [n_rows][4] (position, first key,
  * one past the last, tenant) as rb_plan_create makes them. Writes at most cap units

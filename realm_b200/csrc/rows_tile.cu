@@ -15,9 +15,14 @@
 // documents are bound by those (6 prompts of 200-1500 in documents of 300: 123 us).
 //
 // fp32 rows: q and p as fp16 hi + lo parts, two products each (22 bits); q is
-// brought to a power of two near 2^8 first. p counts from 2^kBias and the running
-// maximum is raised only when a score passes it by 2^kSlack, so p stays below
-// 2^15, fp16's range, and O is rarely rescaled.
+// brought to a power of two near 2^8 first. p counts from 2^bias and the running
+// maximum is raised only when a score passes it by 2^slack, so p stays below 2^16,
+// fp16's range, and O is rarely rescaled. What the bias leaves is the steps of light
+// keys, 2^-24 of p: 2^-37 of the heaviest weight for fp32 rows, 2^-34 for fp16 ones
+// (Scale). More slack saves rescaling: a prompt of 8192, cap 50, fp16 rows with bias and
+// slack 6 and 8 653 us, 10 and 5.9 664, 11 and 4.9 676, 13 and 2.9 688; but with 6 and 8
+// weights from 2^-20 of the heaviest on lost bits and were 0 below 2^-31, which shows in
+// the output of thousands of such keys beside a heavy one whose value is small.
 //
 // Warps: 0-3 softmax of tile 0, 4-7 of tile 1, 8 issues the products, 9 the loads (10
 // and 11 fill the last warpgroup, which gives registers to the others).
@@ -31,7 +36,10 @@ namespace rb {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kBias = 6.f, kSlack = 8.f;
+template <int HL>
+struct Scale {
+  static constexpr float bias = HL ? 13.f : 10.f, slack = HL ? 2.9f : 5.9f;
+};
 constexpr int kSoftWarps = 8;
 constexpr int kTileThreads = (kSoftWarps + 4) * 32;
 // registers a thread at launch, of a softmax warp and of the others: the split uses what the launch gave
@@ -598,7 +606,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
       // the cap keeps the order: where it is fused, it is applied to the maximum alone
       if (CAP && fused && mx != -INFINITY) mx = fmaf(-2.f * cap2, rcp(1.f + ex2(mx * (2.f * kLog2e * kcap))), cap2);
       // each row raises its maximum by its own scores alone
-      const bool up = mx > (m == -INFINITY ? m : m + kSlack);
+      const bool up = mx > (m == -INFINITY ? m : m + Scale<HL>::slack);
       float alpha = 1.f;
       if (up) {
         alpha = ex2(m - mx);
@@ -620,7 +628,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
           st32(to + d, reinterpret_cast<uint32_t*>(o));
         }
       }
-      const float off = kBias - (m == -INFINITY ? 0.f : m);
+      const float off = Scale<HL>::bias - (m == -INFINITY ? 0.f : m);
       const f2 mult2 = pair(mult, mult), off2 = pair(off, off);
       f2 s2[2] = {0ull, 0ull};
       // Groups of 16 keys, every step for the whole group before the next one: the

@@ -351,3 +351,42 @@ def test_histories_out_of_order_are_refused(ctx):
         assert rb.lib().rb_sample_filtered(ctx.handle, rb.F32, x.ctypes.data, 8, 2, 8, (R._Filter * 2)(f, f),
                                            tokens.ctypes.data, off.ctypes.data, u.ctypes.data, out.ctypes.data, None,
                                            rb.PTR_HOST) == rc, off
+
+
+# ---------------------------------------------------------------------------
+# rounding
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("typ", ["float32", "float16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("shape", ["row of 32 heads", "run of 40 rows"])
+def test_light_keys_beside_a_heavy_one_whose_value_is_zero(ctx, typ, hd, shape):
+    """One key has nearly all the weight and a value of 0, and thousands of equal ones 2^-u of it each: the
+    output is theirs alone, and shows what their weights are rounded to. Another u for every query vector.
+
+    A weight of fp32 rows is off by 2^-22 of itself (two fp16 parts) and by what its score is off, and by
+    2^-37 of the heaviest one (p counts from 2^12 and more, in steps of 2^-24). The score has a magnitude
+    of u ln 2, made of q in 22 bits and a few fp32 roundings: 2^-22 (u + 4) with some room. fp16 rows: q is
+    an exact input; probabilities and output are rounded to fp16, h / 2 each, with room 2 h together."""
+    import realm_b200 as rb
+    n, H, L = (1, 32, 5000) if shape[0:3] == "row" else (40, 1, 5000)
+    u = np.linspace(9.3, 30.7, n * H).reshape(n, H)
+    q = np.zeros((n, H, hd), typ)
+    k = np.zeros((L, 1, hd), np.float16)
+    k[0, 0, 5], k[1:, 0, 5] = 8.0, -8.0
+    q[:, :, 5] = u * np.log(2) / 16  # scale 1: the scores differ by u ln 2
+    v = np.ones((L, 1, hd), np.float16)
+    v[0] = 0
+    pool = ctx.kv_pool(1, 1, hd, rb.F16, n_pages=L // 16 + 1, max_tenants=1, max_seq=L)
+    try:
+        pool.create(0)
+        with pool.plan([0] * L, H) as p:
+            p.append(0, _cuda(k), _cuda(v))
+        with pool.plan([0] * n, H, positions=[L - 1] * n) as p:
+            got = _np(p.attention(0, _cuda(q), 1.0))
+    finally:
+        pool.close()
+    w = (L - 1) * np.exp(-16.0 * q[:, :, 5].astype(np.float64))
+    ref = (w / (1 + w))[:, :, None]
+    rel = 2.0 ** -21 * (u + 4) if typ == "float32" else 2 * HALF + 2.0 ** -21 * (u + 4)
+    tol = rel[:, :, None] * ref + (L - 1) * 2.0 ** -37 + (2.0 ** -25 if typ == "float16" else 0)
+    assert (np.abs(got - ref) <= tol).all(), (np.abs(got - ref) / tol).max()
