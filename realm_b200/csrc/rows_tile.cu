@@ -504,8 +504,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
     }
     const bool fuse_ok = HL || (kcap > 1e-6f && kcap < 1e4f && cap2 < 1e6f);
     // How the warp applies the cap: 1 Fused and 2 Wide, together with the exponential; 3 on its
-    // own, with no bound on the scores. One prompt of 8192, 32 heads of 128: fp16 rows 575,
-    // 713 and 1000 us, fp32 rows 1027, about 1200 and 1290. A larger score raises the form for
+    // own, with no bound on the scores. One prompt of 8192, 32 heads of 128: fp16 rows 583,
+    // 713 and 990 us, fp32 rows 1040, 1235 and 1555. A larger score raises the form for
     // good: with one chosen for each block, warps that went back and forth between two of
     // them took longer than with either (fp16 rows, 1 and 2: 993 us).
     int form = !__all_sync(0xffffffffu, kcap > 1e-30f) ? 3 : BIAS || !__all_sync(0xffffffffu, fuse_ok) ? 2 : 1;
@@ -554,8 +554,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
       }
       const bool fused = CAP && !BIAS && form < 3;
       if (CAP && !fused) {
+        using P = Wide<HL>;
         if (form == 2) {
-          using P = Wide<HL>;
           const f2 k2 = pair(kcap, kcap);
 #pragma unroll
           for (int i = 0; i < B; i += 2) {
@@ -565,11 +565,30 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
             for (int q = P::N - 2; q >= 0; --q) t = fma2(t, z, pair(cap2 * P::c(q), cap2 * P::c(q)));
             unpair(mul2(t, y), x[i], x[i + 1]);
           }
-        } else {
-          // cap tanh(y) = cap - 2 cap / (1 + e^(2 y))
+        } else if constexpr (!HL) {
+          // cap tanh(y) = cap - 2 cap / (1 + e^(2 y)), off by 2^-22 of the cap: for caps up to 128
+          // a weight by 2^-15 of itself, an eighth of what fp16 rows round it by
           const float k = 2.f * kLog2e * kcap;
 #pragma unroll
           for (int i = 0; i < B; ++i) x[i] = fmaf(-2.f * cap2, rcp(1.f + ex2(x[i] * k)), cap2);
+        } else {
+          // the same, but small scores, which other rows' large ones brought here, take the
+          // polynomial (prompt of 8192, cap 4, head size 128: 1555 us, without it 1290)
+          const f2 k2 = pair(kcap, kcap);
+#pragma unroll
+          for (int i = 0; i < B; i += 2) {
+            const f2 y = mul2(pair(x[i], x[i + 1]), k2), z = mul2(y, y);
+            f2 t = pair(cap2 * P::c(P::N - 1), cap2 * P::c(P::N - 1));
+#pragma unroll
+            for (int q = P::N - 2; q >= 0; --q) t = fma2(t, z, pair(cap2 * P::c(q), cap2 * P::c(q)));
+            float s0, s1, y0, y1;
+            unpair(mul2(t, y), s0, s1);
+            unpair(y, y0, y1);
+            const float b0 = fmaf(-2.f * cap2, rcp(1.f + ex2(y0 * (2.f * kLog2e))), cap2);
+            const float b1 = fmaf(-2.f * cap2, rcp(1.f + ex2(y1 * (2.f * kLog2e))), cap2);
+            x[i] = fabsf(y0) <= P::limit ? s0 : b0;
+            x[i + 1] = fabsf(y1) <= P::limit ? s1 : b1;
+          }
         }
       }
       if (BIAS) {

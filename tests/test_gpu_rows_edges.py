@@ -390,3 +390,38 @@ def test_light_keys_beside_a_heavy_one_whose_value_is_zero(ctx, typ, hd, shape):
     rel = 2.0 ** -21 * (u + 4) if typ == "float32" else 2 * HALF + 2.0 ** -21 * (u + 4)
     tol = rel[:, :, None] * ref + (L - 1) * 2.0 ** -37 + (2.0 ** -25 if typ == "float16" else 0)
     assert (np.abs(got - ref) <= tol).all(), (np.abs(got - ref) / tol).max()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("bias", [False, True])
+def test_small_capped_scores_beside_rows_with_large_ones(ctx, hd, bias):
+    """Rows of one warp: every other one has scores of several caps, the rest scores of up to 1.5, where two
+    kinds of keys with values 1 and -1 show the ratio of their weights. fp32 rows.
+
+    A small score x is off by 2^-22 |x| (q in 22 bits) and a few fp32 roundings of its size, so a weight by
+    2^-20 with |x| <= 1.5, and by 2^-22 for its own two parts; the output, a difference of two such shares,
+    by no more than 2^-19."""
+    import realm_b200 as rb
+    n, L, cap = 64, 256, 50.0
+    q = np.zeros((n, 1, hd), np.float32)
+    a = np.linspace(0.02, 1.5, n)
+    q[:, 0, 3] = np.where(np.arange(n) % 2, 100.0 * (1 + a), a)
+    k = np.zeros((L, 1, hd), np.float16)
+    k[0::2, 0, 3], k[1::2, 0, 3] = 1.0, -0.75
+    v = np.ones((L, 1, hd), np.float16)
+    v[1::2] = -1
+    slopes = np.zeros(1, np.float32) if bias else None
+    pool = ctx.kv_pool(1, 1, hd, rb.F16, n_pages=L // 16, max_tenants=1, max_seq=L)
+    try:
+        pool.create(0)
+        with pool.plan([0] * L, 1) as p:
+            p.append(0, _cuda(k), _cuda(v))
+        with pool.plan([0] * n, 1, positions=[L - 1] * n) as p:
+            got = _np(p.attention(0, _cuda(q), 1.0, softcap=cap, slopes=None if slopes is None else _cuda(slopes)))
+    finally:
+        pool.close()
+    x = cap * np.tanh(q[:, 0, 3].astype(np.float64)[:, None] * np.array([1.0, -0.75]) / cap)
+    ref = np.tanh((x[:, 0] - x[:, 1]) / 2)
+    err = np.abs(got[:, 0] - ref[:, None]).max(1)
+    assert (err[0::2] <= 2.0 ** -19).all(), err[0::2].max()
+    assert (err[1::2] <= 2.0 ** -18).all()  # one kind of key has the whole weight
