@@ -2464,7 +2464,8 @@ int32_t rb_plan_attention(rb_ctx* c, int32_t plan, uint32_t layer, const rb_atte
   a.n_heads = S->n_heads;
   a.n_rep = S->n_heads / P.n_kv;
   a.scale = d->scale;
-  a.cap = d->softcap;
+  // beyond these a cap is none, or leaves no difference between scores, to fp32; its inverse stays normal
+  a.cap = d->softcap > 0.f ? std::min(std::max(d->softcap, 1e-30f), 1e30f) : 0.f;
   a.slopes = (const float*)ss.dptr;
   a.kv = P.view();
   a.rows = S->rows.as<RowInfo>();

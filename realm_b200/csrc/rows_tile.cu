@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
     const int all0 = sp.all0[tile], all1 = sp.all1[tile], in0 = sp.in0, in1 = sp.in1;
     const int both0 = max(sp.all0[0], sp.all0[1]), both1 = min(sp.all1[0], sp.all1[1]);
     const float slope = BIAS && active ? a.slopes[head] * kLog2e : 0.f;
-    const float cap2 = a.cap * kLog2e, kcap = CAP ? sv / a.cap : 0.f;
+    const float cap2 = a.cap * kLog2e, kcap = CAP ? fmaxf(sv / a.cap, 1.2e-38f) : 0.f;  // above 0: -inf stays -inf
     const float mult = (CAP || BIAS) ? 1.f : fmaxf(sv * kLog2e, 1e-30f);  // scores to base-2 units (-inf stays)
     const float sv2 = sv * kLog2e;
     // coefficients of the fused form, for fp16 rows in powers of the raw score (kept normal)
@@ -508,7 +508,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
     // 713 and 990 us, fp32 rows 1040, 1235 and 1555. A larger score raises the form for
     // good: with one chosen for each block, warps that went back and forth between two of
     // them took longer than with either (fp16 rows, 1 and 2: 993 us).
-    int form = !__all_sync(0xffffffffu, kcap > 1e-30f) ? 3 : BIAS || !__all_sync(0xffffffffu, fuse_ok) ? 2 : 1;
+    int form = BIAS || !__all_sync(0xffffffffu, fuse_ok) ? 2 : 1;
     float m = -INFINITY, l = 0.f;
     // Both tiles meet. Not a named barrier, which has no limit: after a wait that ran out
     // one of them may have read other values and not come.
@@ -622,8 +622,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
 #pragma unroll
         for (int q = 0; q < 4; ++q) mx4[q] = max3(mx4[q], x[i + 2 * q], x[i + 2 * q + 1]);
       float mx = max3(fmaxf(mx4[0], mx4[1]), mx4[2], mx4[3]) * mult;
-      // the cap keeps the order: where it is fused, it is applied to the maximum alone
-      if (CAP && fused && mx != -INFINITY) mx = fmaf(-2.f * cap2, rcp(1.f + ex2(mx * (2.f * kLog2e * kcap))), cap2);
+      // the cap keeps the order: where it is fused, it is applied to the maximum alone (by the polynomial
+      // as well: an error in proportion to the cap would move all of p)
+      if (CAP && fused && mx != -INFINITY) {
+        using P = Wide<HL>;
+        const float y = mx * kcap, z = y * y;
+        float t = P::c(P::N - 1);
+#pragma unroll
+        for (int q = P::N - 2; q >= 0; --q) t = fmaf(t, z, P::c(q));
+        mx = t * y * cap2;
+      }
       // each row raises its maximum by its own scores alone
       const bool up = mx > (m == -INFINITY ? m : m + Scale<HL>::slack);
       float alpha = 1.f;

@@ -425,3 +425,40 @@ def test_small_capped_scores_beside_rows_with_large_ones(ctx, hd, bias):
     err = np.abs(got[:, 0] - ref[:, None]).max(1)
     assert (err[0::2] <= 2.0 ** -19).all(), err[0::2].max()
     assert (err[1::2] <= 2.0 ** -18).all()  # one kind of key has the whole weight
+
+
+@pytest.mark.parametrize("typ,cache", [("float16", "F16"), ("float32", "F16"), ("float32", "F32"), ("float16", "F32")])
+@pytest.mark.parametrize("shape", ["row", "run"])
+@pytest.mark.parametrize("bias", [False, True])
+def test_caps_far_from_the_scores(ctx, typ, cache, shape, bias):
+    """A cap so large that it changes nothing gives what no cap gives, and one so small that all scores are equal the mean
+    of the values; one score is exactly 0. Bounds: twice the error of one of them, scores of up to 8."""
+    import torch
+    import realm_b200 as rb
+    L, H, hd = 300, 4, 64
+    n = 1 if shape == "row" else 40
+    g = torch.Generator("cuda").manual_seed(5)
+    k = torch.randn(L, 1, hd, device="cuda", generator=g)
+    k[17] = 0
+    v = torch.randn(L, 1, hd, device="cuda", generator=g)
+    q = (torch.randn(n, H, hd, device="cuda", generator=g) * 2).to(getattr(torch, typ))
+    slopes = torch.full((H,), 2.0 ** -6, device="cuda") if bias else None
+    pool = ctx.kv_pool(1, 1, hd, rb.F16 if cache == "F16" else rb.F32, n_pages=L // 16 + 1, max_tenants=1, max_seq=L)
+    try:
+        pool.create(0)
+        with pool.plan([0] * L, H) as p:
+            p.append(0, k, v)
+        with pool.plan([0] * n, H, positions=[L - 1] * n) as p:
+            run = lambda cap: p.attention(0, q, 0.125, softcap=cap, slopes=slopes).double()  # noqa: E731
+            none = run(0.0)
+            top = v.abs().max().item()
+            tol = top * (4 * HALF if typ == "float16" else 2.0 ** -18)
+            for cap in (1e9, 1e20, 1e30, 3e38):
+                assert ((run(cap) - none).abs() <= tol).all(), cap
+            d = torch.arange(L - 1, -1, -1, device="cuda", dtype=torch.float64)
+            w = torch.softmax(-d * 2.0 ** -6 if bias else d * 0, 0)
+            c = v.to(torch.float16 if cache == "F16" else torch.float32).double()[:, 0]
+            for cap in (1e-9, 1e-30, 1e-38, 1e-40, 1e-45):
+                assert ((run(cap) - w @ c).abs() <= tol).all(), cap
+    finally:
+        pool.close()
