@@ -93,29 +93,36 @@ struct PageCache {
 // pay for eight: 8 tenants of 100-3001 tokens, 16 kv heads of 64, one, two and four
 // vectors 38, 40 and 44 us, with the form for eight 56, 56 and 58. Bound by memory:
 // with a window of 1024 16 us for 55 MB (3.4 TB/s; 12 pages a warp are little to stream).
-template <int HD>
+template <int HD, int NV>
 struct F32Cfg {
   static constexpr int BLK = 16 * HD * 4;
   static constexpr int NST = HD == 128 ? 3 : 6;   // blocks a warp: 96 KB a CTA
   static constexpr int SMEM = 128 + kRowWarps * NST * (BLK + 8);
+  // Two CTAs an SM, as the plan counts its warps: 228 KB, of which each takes 1 KB for the system.
+  // The probabilities go through shared memory where that leaves room (PB), else by shuffles: eight
+  // vectors at 128, 8 tenants x 64 rows after 2000 tokens, 32 heads on 8, 1115 us against 1510 with one
+  // CTA; eight at 64, where both fit, 790 us by shuffles, 730 through shared memory.
+  static constexpr int Q = kRowWarps * NV * (HD * 4 + (int)sizeof(VecInfo)), P = kRowWarps * NV * 16 * 4;
+  static constexpr bool PB = 2 * (SMEM + Q + P + 1024) <= 228 * 1024;
+  static_assert(2 * (SMEM + Q + 1024) <= 228 * 1024, "");
 };
 
 template <int HD, int NV, class TQ>
 __global__ void __launch_bounds__(kRowWarps * 32, 2) rows_f32_kernel(const __grid_constant__ RowAttnArgs a) {
-  using C = F32Cfg<HD>;
+  using C = F32Cfg<HD, NV>;
   constexpr int DPL = HD / 32, NST = C::NST, NCH = HD / 8;  // 16-byte chunks in half a key
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 127) & ~uintptr_t(127));
   __shared__ __align__(16) float q_all[kRowWarps][NV][HD];
   __shared__ VecInfo vi_all[kRowWarps][NV];
-  __shared__ float pb_all[kRowWarps][NV][16];
+  __shared__ float pb_all[C::PB ? kRowWarps : 1][C::PB ? NV : 1][16];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, j = lane & 15, hh = lane >> 4;
   const int me = blockIdx.x * kRowWarps + warp;
   pdl_launch_dependents();
   if (me >= a.n_warps) return;
   auto qs = q_all[warp];
   VecInfo* vi = vi_all[warp];
-  auto pb = pb_all[warp];
+  auto pb = pb_all[C::PB ? warp : 0];
   const float* pool = reinterpret_cast<const float*>(a.kv.pool);
   uint8_t* ring = smem + warp * NST * C::BLK;
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + kRowWarps * NST * C::BLK) + warp * NST;
@@ -196,6 +203,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) rows_f32_kernel(const __gri
       }
       release();
       const int key = k + j;
+      float pk[NV];  // of key j, in both lanes that have it
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         float x = (dot[v] + __shfl_xor_sync(0xffffffffu, dot[v], 16)) * a.scale;
@@ -215,13 +223,12 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) rows_f32_kernel(const __gri
           for (int d = 0; d < DPL; ++d) o[v][d] *= alpha;
         }
         const float p = in ? exp2f(x - (m[v] == -INFINITY ? 0.f : m[v])) : 0.f;
-        if (hh == 0) {
-          l[v] += p;
-          pb[v][j] = p;
-        }
+        if (hh == 0) l[v] += p;
+        pk[v] = p;
+        if (C::PB && hh == 0) pb[v][j] = p;
       }
       const float* vb = take();
-      __syncwarp();
+      if (C::PB) __syncwarp();
       const int nk = min(16, u.k1 - k);
 #pragma unroll 4
       for (int t = 0; t < nk; ++t) {
@@ -230,7 +237,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) rows_f32_kernel(const __gri
         else *reinterpret_cast<float2*>(vf) = *reinterpret_cast<const float2*>(vb + t * HD + lane * DPL);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-          const float p = pb[v][t];
+          const float p = C::PB ? pb[v][t] : __shfl_sync(0xffffffffu, pk[v], t);
           // a masked key adds nothing, whatever its value holds
 #pragma unroll
           for (int d = 0; d < DPL; ++d) o[v][d] = p == 0.f ? o[v][d] : fmaf(p, vf[d], o[v][d]);
@@ -646,7 +653,7 @@ template <int HD, int NV>
 static cudaError_t launch_f32(const RowAttnArgs& a, cudaStream_t s) {
   int dev = 0;
   cudaGetDevice(&dev);
-  constexpr int smem = F32Cfg<HD>::SMEM;
+  constexpr int smem = F32Cfg<HD, NV>::SMEM;
   if (a.q16) {
     if (cudaError_t e = ensure_smem_attr(rows_f32_kernel<HD, NV, __half>, smem, dev)) return e;
     rows_f32_kernel<HD, NV, __half><<<(a.n_warps + kRowWarps - 1) / kRowWarps, kRowWarps * 32, smem, s>>>(a);
