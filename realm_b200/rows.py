@@ -169,6 +169,18 @@ def _call(ctx, flags, fn, *args):
         _check(rc)
 
 
+def _indices(a, name):
+    """One 32-bit unsigned value per row, or None; anything that would not keep its value is refused."""
+    if a is None:
+        return None
+    a = np.asarray(a)
+    if a.size == 0:
+        return np.empty(0, np.uint32)
+    if a.ndim != 1 or a.dtype.kind not in "iu" or int(a.min()) < 0 or int(a.max()) > 0xffffffff:
+        raise ValueError(f"{name}: integers of at least 0, one per row, wanted")
+    return np.ascontiguousarray(a, np.uint32)
+
+
 class RowPlan:
     """The rows of one step over a KV pool (rb_plan_create); see KVPool.plan. Ends with close(), with its pool, or
     when nothing refers to it."""
@@ -177,7 +189,10 @@ class RowPlan:
 
     def __init__(self, pool, tenants, n_heads: int, positions=None, begin=None, end=None, window: int = 0):
         self.pool, self.ctx, self.n_heads = pool, pool.ctx, int(n_heads)
-        arr = [None if a is None else np.ascontiguousarray(a, np.uint32) for a in (tenants, positions, begin, end)]
+        arr = [_indices(tenants, "tenants"), _indices(positions, "positions"), _indices(begin, "begin"),
+               _indices(end, "end")]
+        if int(window) != window or not 0 <= window <= 0xffffffff:
+            raise ValueError("window: a length of at least 0, or 0 for none, wanted")
         self.n_rows = len(arr[0])
         for a in arr[1:]:
             if a is not None and len(a) != self.n_rows:

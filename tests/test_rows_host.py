@@ -1,0 +1,44 @@
+"""What row plans and the operators' bindings check on the host, without a GPU."""
+import os
+import subprocess
+import sys
+
+import numpy as np
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+class _Pool:
+    """Stands in for a pool where a call has to be refused before it reaches the library."""
+    n_kv, hd, handle = 2, 64, 0
+
+    class ctx:
+        handle, _h, device = None, None, 0
+
+
+@pytest.mark.parametrize("name", ["tenants", "positions", "begin", "end"])
+@pytest.mark.parametrize("bad", [np.array([3, -1]), np.array([0, 2 ** 32]), np.array([-5, 0], np.int8), [1, -2], [0.5, 1.0],
+                                 np.array([1.0, 2.0]), [[0, 1]], np.array([True, False])])
+def test_rows_that_are_not_indices_are_refused(name, bad):
+    """Before, a begin of -1 wrapped around to a key past all others, and the row saw none."""
+    from realm_b200 import RowPlan
+    rows = dict(tenants=[0, 1], positions=[4, 5], begin=[0, 0], end=[5, 6])
+    with pytest.raises(ValueError, match=name):
+        RowPlan(_Pool, n_heads=4, **dict(rows, **{name: bad}))
+
+
+@pytest.mark.parametrize("bad", [-1, 2 ** 32, 1.5])
+def test_windows_that_are_not_lengths_are_refused(bad):
+    from realm_b200 import RowPlan
+    with pytest.raises(ValueError, match="window"):
+        RowPlan(_Pool, [0, 1], 4, window=bad)
+
+
+def test_integer_rows_of_any_type_reach_the_library():
+    import realm_b200 as rb
+    for t in (np.int8, np.int64, np.uint64, np.uint32, list, tuple):
+        a = t([0, 1]) if t in (list, tuple) else np.array([0, 1], t)
+        with pytest.raises(rb.RealmError) as e:  # there is no context
+            rb.RowPlan(_Pool, a, 4, positions=a, end=a, window=np.int64(7))
+        assert e.value.code == -20
