@@ -10,6 +10,7 @@
 #include <cstring>
 #include <map>
 #include <memory>
+#include <new>
 #include <mutex>
 #include <random>
 #include <string>
@@ -1412,8 +1413,8 @@ int32_t rb_kv_pool_hold(rb_ctx* c, int32_t pool, void** hold) {
   KvPool* P = get_pool(c, pool);
   if (!P) return fail(RB_ERR_BAD_HANDLE, "pool %d", pool);
   if (!hold) return fail(RB_ERR_INVALID, "null output");
-  *hold = new std::shared_ptr<DevBuf>(P->pool);
-  return RB_OK;
+  *hold = new (std::nothrow) std::shared_ptr<DevBuf>(P->pool);
+  return *hold ? RB_OK : fail(RB_ERR_OOM, "host memory");
 }
 
 int32_t rb_kv_hold_release(void* hold) {
@@ -2230,23 +2231,27 @@ int stage_words(Ctx* c, const char* name, const void* p, size_t count, uint32_t 
 
 // Takes pages so that want[i].second tokens of tenant want[i].first fit, in the
 // order of `want`, all or none, and copies the new page-table entries to the device.
+// Nothing is allocated once the first page has been taken.
 int reserve_pages(Ctx* c, KvPool& P, const std::vector<std::pair<int, int>>& want) {
-  std::vector<int> taken;         // tenant of every page taken, in order
-  std::map<int, int> had;         // pages a tenant had before its first
+  std::map<int, int> pages, had;  // pages a tenant is to have; and had, of those that get some
   for (auto [t, upto] : want) {
-    KvTenant& T = P.tenants[t];
-    while ((int)T.pages.size() * kRowPage < upto) {
-      if (P.free_list.empty()) {
-        for (auto it = taken.rbegin(); it != taken.rend(); ++it) {
-          P.free_list.push_back(P.tenants[*it].pages.back());
-          P.tenants[*it].pages.pop_back();
-        }
-        return fail(RB_ERR_KV_POOL_EXHAUSTED, "KV page pool exhausted");
-      }
-      had.emplace(t, (int)T.pages.size());
-      T.pages.push_back(P.free_list.back());
+    int& n = pages[t];
+    n = std::max(n, (upto + kRowPage - 1) / kRowPage);
+  }
+  size_t missing = 0;
+  for (auto [t, n] : pages) {
+    std::vector<int>& pg = P.tenants[t].pages;
+    if (n <= (int)pg.size()) continue;
+    missing += n - pg.size();
+    had.emplace(t, (int)pg.size());
+    pg.reserve(n);
+  }
+  if (missing > P.free_list.size()) return fail(RB_ERR_KV_POOL_EXHAUSTED, "KV page pool exhausted");
+  for (auto [t, upto] : want) {
+    std::vector<int>& pg = P.tenants[t].pages;
+    while ((int)pg.size() * kRowPage < upto) {
+      pg.push_back(P.free_list.back());
       P.free_list.pop_back();
-      taken.push_back(t);
     }
   }
   for (auto [t, n0] : had) {
@@ -2259,12 +2264,18 @@ int reserve_pages(Ctx* c, KvPool& P, const std::vector<std::pair<int, int>>& wan
   return RB_OK;
 }
 
-}  // namespace
+// The work of a C entry that allocates on the host: no exception leaves it.
+template <class F>
+int32_t guarded(F f) {
+  try {
+    return f();
+  } catch (const std::exception& e) {
+    return fail(RB_ERR_OOM, "host memory: %s", e.what());
+  }
+}
 
-extern "C" {
-
-int32_t rb_plan_partition(uint32_t n_rows, const int32_t* rows, uint32_t n_heads, uint32_t n_kv, uint32_t num_sms,
-                          int32_t f16_cache, int32_t* units, uint32_t cap) {
+int32_t plan_partition(uint32_t n_rows, const int32_t* rows, uint32_t n_heads, uint32_t n_kv, uint32_t num_sms,
+                       int32_t f16_cache, int32_t* units, uint32_t cap) {
   if (!rows || !n_rows || !n_kv || !n_heads || n_heads % n_kv || !num_sms || (cap && !units))
     return fail(RB_ERR_INVALID, "bad partition arguments");
   std::vector<RowInfo> r(n_rows);
@@ -2285,7 +2296,7 @@ int32_t rb_plan_partition(uint32_t n_rows, const int32_t* rows, uint32_t n_heads
   return (int32_t)n;
 }
 
-int32_t rb_plan_create(rb_ctx* c, int32_t pool, const rb_plan_desc* d, int32_t* plan) {
+int32_t plan_create(rb_ctx* c, int32_t pool, const rb_plan_desc* d, int32_t* plan) {
   KvPool* P = get_pool(c, pool);
   if (!P) return fail(RB_ERR_BAD_HANDLE, "pool %d", pool);
   if (!d || !plan || !d->tenants) return fail(RB_ERR_INVALID, "null argument");
@@ -2346,9 +2357,80 @@ int32_t rb_plan_create(rb_ctx* c, int32_t pool, const rb_plan_desc* d, int32_t* 
   if (int rc = reserve_pages(c, *P, want)) return rc;
   // the lists are copied from this call's own memory
   RB_CUDA(cudaStreamSynchronize(c->stream));
+  c->plans[c->next_plan] = std::move(S);
   *plan = c->next_plan++;
-  c->plans[*plan] = std::move(S);
   return RB_OK;
+}
+
+int32_t sample_filtered(rb_ctx* c, int32_t dtype, const void* logits, uint64_t ld, uint32_t n_rows, uint32_t vocab,
+                        const rb_sampling_filter* params, const uint32_t* prev, const uint32_t* prev_off,
+                        const float* uniforms, uint32_t* out, float* probs, uint32_t flags) {
+  if (!c) return fail(RB_ERR_BAD_HANDLE, "null context");
+  if (int rc = row_dtype(dtype)) return rc;
+  if (n_rows == 0) return 0;  // an empty batch has no memory
+  if (!logits || !params || !uniforms || !out) return fail(RB_ERR_INVALID, "logits/params/uniforms/out NULL");
+  const bool dev = flags & RB_PTR_DEVICE;
+  if (!dev && !prev && prev_off && n_rows && prev_off[n_rows] == 0) prev_off = nullptr;  // no row has a history
+  if ((prev == nullptr) != (prev_off == nullptr)) return fail(RB_ERR_INVALID, "prev_tokens and prev_offsets go together");
+  if (vocab == 0 || vocab > (uint32_t)kFilterMaxVocab || ld < vocab)
+    return fail(RB_ERR_UNSUPPORTED, "vocab %u not in [1, %d] or ld %llu < vocab", vocab, kFilterMaxVocab,
+                (unsigned long long)ld);
+  if (n_rows > (1u << 24)) return fail(RB_ERR_INVALID, "n_rows %u > 2^24", n_rows);
+  if (prev_off && !dev)
+    for (uint32_t r = 0; r < n_rows; ++r)
+      if (prev_off[r] > prev_off[r + 1]) return fail(RB_ERR_INVALID, "row %u: prev_offsets fall", r);
+  RB_CUDA(cudaSetDevice(c->device));
+  const size_t esz = dtype == RB_F16 ? 2 : 4;
+  Staged sl, sp, sprev, soff, su;
+  if (int rc = stage_rows(c, "logits", logits, ld, n_rows, vocab, esz, flags, sl)) return rc;
+  if (int rc = stage_words(c, "params", params, (size_t)n_rows * (sizeof(rb_sampling_filter) / 4), flags, sp)) return rc;
+  if (prev_off) {
+    if (int rc = stage_words(c, "prev_offsets", prev_off, (size_t)n_rows + 1, flags, soff)) return rc;
+    if (int rc = stage_words(c, "prev_tokens", prev, dev ? 0 : prev_off[n_rows], flags, sprev)) return rc;
+  }
+  if (int rc = stage_words(c, "uniforms", uniforms, n_rows, flags, su)) return rc;
+  if (dev && ((uintptr_t)out % 4 || (uintptr_t)probs % 4))
+    return fail(RB_ERR_INVALID, "out_tokens or probs is not aligned to 4 bytes");
+  DevBuf dout;
+  FilterArgs a;
+  a.logits = sl.dptr;
+  a.ld = (int64_t)ld;
+  a.x16 = dtype == RB_F16;
+  a.n_rows = (int)n_rows;
+  a.vocab = (int)vocab;
+  a.params = (const rb_sampling_filter*)sp.dptr;
+  a.prev = (const uint32_t*)sprev.dptr;
+  a.prev_off = prev_off ? (const uint32_t*)soff.dptr : nullptr;
+  a.uniforms = (const float*)su.dptr;
+  a.tokens = out;
+  a.probs = probs;
+  if (!dev) {
+    RB_CUDA(dout.alloc((size_t)n_rows * 8));
+    a.tokens = dout.as<uint32_t>();
+    a.probs = probs ? dout.as<float>() + n_rows : nullptr;
+  }
+  RB_CUDA(filter_launch(a, c->num_sms, c->stream));
+  if (dev && (flags & RB_ASYNC)) return (int32_t)n_rows;
+  std::vector<uint32_t> h(n_rows);
+  RB_CUDA(cudaMemcpyAsync(h.data(), a.tokens, (size_t)n_rows * 4, cudaMemcpyDeviceToHost, c->stream));
+  if (!dev && probs) RB_CUDA(cudaMemcpyAsync(probs, a.probs, (size_t)n_rows * 4, cudaMemcpyDeviceToHost, c->stream));
+  if (int rc = sync_ctx(c)) return rc;
+  for (uint32_t r = 0; r < n_rows; ++r)
+    if (h[r] == 0xffffffffu) return fail(RB_ERR_INVALID, "row %u: Failed to create weighted index", r);
+  if (!dev) std::copy(h.begin(), h.end(), out);
+  return (int32_t)n_rows;
+}
+}  // namespace
+
+extern "C" {
+
+int32_t rb_plan_partition(uint32_t n_rows, const int32_t* rows, uint32_t n_heads, uint32_t n_kv, uint32_t num_sms,
+                          int32_t f16_cache, int32_t* units, uint32_t cap) {
+  return guarded([&] { return plan_partition(n_rows, rows, n_heads, n_kv, num_sms, f16_cache, units, cap); });
+}
+
+int32_t rb_plan_create(rb_ctx* c, int32_t pool, const rb_plan_desc* d, int32_t* plan) {
+  return guarded([&] { return plan_create(c, pool, d, plan); });
 }
 
 int32_t rb_plan_destroy(rb_ctx* c, int32_t plan) {
@@ -2496,60 +2578,9 @@ int32_t rb_sample_filtered(rb_ctx* c, int32_t dtype, const void* logits, uint64_
                            uint32_t vocab, const rb_sampling_filter* params, const uint32_t* prev,
                            const uint32_t* prev_off, const float* uniforms, uint32_t* out, float* probs,
                            uint32_t flags) {
-  if (!c) return fail(RB_ERR_BAD_HANDLE, "null context");
-  if (int rc = row_dtype(dtype)) return rc;
-  if (n_rows == 0) return 0;  // an empty batch has no memory
-  if (!logits || !params || !uniforms || !out) return fail(RB_ERR_INVALID, "logits/params/uniforms/out NULL");
-  const bool dev = flags & RB_PTR_DEVICE;
-  if (!dev && !prev && prev_off && n_rows && prev_off[n_rows] == 0) prev_off = nullptr;  // no row has a history
-  if ((prev == nullptr) != (prev_off == nullptr)) return fail(RB_ERR_INVALID, "prev_tokens and prev_offsets go together");
-  if (vocab == 0 || vocab > (uint32_t)kFilterMaxVocab || ld < vocab)
-    return fail(RB_ERR_UNSUPPORTED, "vocab %u not in [1, %d] or ld %llu < vocab", vocab, kFilterMaxVocab,
-                (unsigned long long)ld);
-  if (n_rows > (1u << 24)) return fail(RB_ERR_INVALID, "n_rows %u > 2^24", n_rows);
-  if (prev_off && !dev)
-    for (uint32_t r = 0; r < n_rows; ++r)
-      if (prev_off[r] > prev_off[r + 1]) return fail(RB_ERR_INVALID, "row %u: prev_offsets fall", r);
-  RB_CUDA(cudaSetDevice(c->device));
-  const size_t esz = dtype == RB_F16 ? 2 : 4;
-  Staged sl, sp, sprev, soff, su;
-  if (int rc = stage_rows(c, "logits", logits, ld, n_rows, vocab, esz, flags, sl)) return rc;
-  if (int rc = stage_words(c, "params", params, (size_t)n_rows * (sizeof(rb_sampling_filter) / 4), flags, sp)) return rc;
-  if (prev_off) {
-    if (int rc = stage_words(c, "prev_offsets", prev_off, (size_t)n_rows + 1, flags, soff)) return rc;
-    if (int rc = stage_words(c, "prev_tokens", prev, dev ? 0 : prev_off[n_rows], flags, sprev)) return rc;
-  }
-  if (int rc = stage_words(c, "uniforms", uniforms, n_rows, flags, su)) return rc;
-  if (dev && ((uintptr_t)out % 4 || (uintptr_t)probs % 4))
-    return fail(RB_ERR_INVALID, "out_tokens or probs is not aligned to 4 bytes");
-  DevBuf dout;
-  FilterArgs a;
-  a.logits = sl.dptr;
-  a.ld = (int64_t)ld;
-  a.x16 = dtype == RB_F16;
-  a.n_rows = (int)n_rows;
-  a.vocab = (int)vocab;
-  a.params = (const rb_sampling_filter*)sp.dptr;
-  a.prev = (const uint32_t*)sprev.dptr;
-  a.prev_off = prev_off ? (const uint32_t*)soff.dptr : nullptr;
-  a.uniforms = (const float*)su.dptr;
-  a.tokens = out;
-  a.probs = probs;
-  if (!dev) {
-    RB_CUDA(dout.alloc((size_t)n_rows * 8));
-    a.tokens = dout.as<uint32_t>();
-    a.probs = probs ? dout.as<float>() + n_rows : nullptr;
-  }
-  RB_CUDA(filter_launch(a, c->num_sms, c->stream));
-  if (dev && (flags & RB_ASYNC)) return (int32_t)n_rows;
-  std::vector<uint32_t> h(n_rows);
-  RB_CUDA(cudaMemcpyAsync(h.data(), a.tokens, (size_t)n_rows * 4, cudaMemcpyDeviceToHost, c->stream));
-  if (!dev && probs) RB_CUDA(cudaMemcpyAsync(probs, a.probs, (size_t)n_rows * 4, cudaMemcpyDeviceToHost, c->stream));
-  if (int rc = sync_ctx(c)) return rc;
-  for (uint32_t r = 0; r < n_rows; ++r)
-    if (h[r] == 0xffffffffu) return fail(RB_ERR_INVALID, "row %u: Failed to create weighted index", r);
-  if (!dev) std::copy(h.begin(), h.end(), out);
-  return (int32_t)n_rows;
+  return guarded([&] {
+    return sample_filtered(c, dtype, logits, ld, n_rows, vocab, params, prev, prev_off, uniforms, out, probs, flags);
+  });
 }
 
 }  // extern "C"

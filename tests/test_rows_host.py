@@ -42,3 +42,24 @@ def test_integer_rows_of_any_type_reach_the_library():
         with pytest.raises(rb.RealmError) as e:  # there is no context
             rb.RowPlan(_Pool, a, 4, positions=a, end=a, window=np.int64(7))
         assert e.value.code == -20
+
+
+def test_no_memory_is_an_error_not_an_abort():
+    """The work lists of many short runs do not fit the address space that the process may use."""
+    code = """
+import resource, sys
+sys.path.insert(0, %r)
+import numpy as np, realm_b200 as rb
+from realm_b200 import rows as R
+n = 1 << 19
+rows = np.zeros((n, 4), np.int32)
+rows[:, 2], rows[:, 3] = 1, np.arange(n) %% 2
+have = int(open("/proc/self/statm").read().split()[0]) * resource.getpagesize()
+resource.setrlimit(resource.RLIMIT_AS, (have + (64 << 20),) * 2)
+try:
+    R.partition(rows, 64, 8, 148, False)
+except rb.RealmError as e:
+    print("refused", e.code)
+""" % ROOT
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and r.stdout.strip() == "refused -26", (r.returncode, r.stdout, r.stderr[-500:])
