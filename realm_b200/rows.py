@@ -88,6 +88,8 @@ def _rows3(a, n, heads, hd, name):
         shape, stride, ptr = a.shape, a.stride(), a.data_ptr()
     else:
         shape, ptr = a.shape, a.ctypes.data
+        if any(s % a.itemsize for s in a.strides):
+            raise ValueError(f"{name}: rows lie whole elements apart, got strides of {a.strides} bytes")
         stride = [s // a.itemsize for s in a.strides]
     if len(shape) == 3:
         ok = shape[0] == n and shape[1] == heads and shape[2] == hd and stride[2] == 1 and \

@@ -63,3 +63,33 @@ except rb.RealmError as e:
 """ % ROOT
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0 and r.stdout.strip() == "refused -26", (r.returncode, r.stdout, r.stderr[-500:])
+
+
+def _plan(n_rows, n_heads=2):
+    """A plan without a library behind it: its calls get past the binding's checks and then fail (-20)."""
+    from realm_b200 import RowPlan, rows as R
+    p = RowPlan.__new__(RowPlan)
+    p.pool, p.ctx, p.n_heads, p.n_rows = _Pool, _Pool.ctx, n_heads, n_rows
+    p._append, p._attention = R._AppendDesc(), R._AttentionDesc()
+    p._append_ref, p._attention_ref = R.C.byref(p._append), R.C.byref(p._attention)
+    return p
+
+
+def _code(f):
+    import realm_b200 as rb
+    with pytest.raises(rb.RealmError) as e:
+        f()
+    return e.value.code
+
+
+def test_rows_that_lie_parts_of_an_element_apart_are_refused():
+    """A field of packed records: 515 bytes from row to row. Before, the 3 were dropped and other memory was read."""
+    x = np.zeros(3, [("q", "f4", (2, 64)), ("tail", "u1", 3)])["q"]
+    k = np.zeros((3, 2, 64), np.float32)
+    for f in (lambda p: p.append(0, x, k), lambda p: p.append(0, k, x), lambda p: p.append(0, k, k, q=x),
+              lambda p: p.attention(0, x, 1.0), lambda p: p.attention(0, k, 1.0, out=x)):
+        with pytest.raises(ValueError, match="515"):
+            f(_plan(3))
+    wide = np.zeros((3, 2, 64 + 64), np.float32)
+    assert _code(lambda: _plan(3).append(0, k, k, q=k)) == -20 and wide[:, 0, :64].strides == (1024, 4)
+    assert _code(lambda: _plan(3).append(0, wide.reshape(3, 256)[:, :128].reshape(3, 2, 64), k)) == -20
