@@ -82,6 +82,13 @@ def _vec(a, dtype, n, name):
     raise ValueError(f"{name}: {n} contiguous {dtype} values wanted")
 
 
+def _writable(a, name):
+    """a, an output: not a numpy array that is read-only."""
+    if a is not None and not _is_tensor(a) and not a.flags.writeable:
+        raise ValueError(f"{name}: read-only")
+    return a
+
+
 def _rows3(a, n, heads, hd, name):
     """(pointer, elements between rows) of a [n][heads][hd] (or [n][heads * hd]) array."""
     if _is_tensor(a):
@@ -225,7 +232,7 @@ class RowPlan:
         d.k, d.ldk = _rows3(k, n, kv, hd, "k")
         d.v, d.ldv = _rows3(v, n, kv, hd, "v")
         d.q, d.ldq = (None, 0) if q is None else _rows3(q, n, H, hd, "q")
-        d.q_out, d.ldo = (None, 0) if q is None else _rows3(q_out, n, H, hd, "q_out")
+        d.q_out, d.ldo = (None, 0) if q is None else _rows3(_writable(q_out, "q_out"), n, H, hd, "q_out")
         d.q_norm, d.k_norm = _vec(q_norm, "float32", hd, "q_norm"), _vec(k_norm, "float32", hd, "k_norm")
         if rope is None:
             d.rope, d.rope_len, d.rotary = None, 0, 0
@@ -250,7 +257,7 @@ class RowPlan:
         d = self._attention
         d.dtype, d.scale, d.softcap = dt, scale, softcap
         d.q, d.ldq = _rows3(q, n, H, hd, "q")
-        d.out, d.ldo = _rows3(out, n, H, hd, "out")
+        d.out, d.ldo = _rows3(_writable(out, "out"), n, H, hd, "out")
         d.slopes = _vec(slopes, "float32", H, "slopes")
         _call(self.ctx, flags, _lib.rb_plan_attention, self.ctx._h, self.handle, layer, self._attention_ref)
         return out
@@ -327,7 +334,7 @@ def sample_filtered(ctx, logits, filters, uniforms, prev=None, out=None, probs=N
         u = np.ascontiguousarray(uniforms, np.float32).reshape(n)
         pf, po = _prev_arrays(prev, n)
         tok = np.empty(n, np.uint32)
-        pp = None if probs is None else _vec(probs, "float32", n, "probs")
+        pp = _vec(_writable(probs, "probs"), "float32", n, "probs")
         _check(_lib.rb_sample_filtered(ctx.handle, dt, x.ctypes.data, v, n, v, arr,
                                        None if pf is None else pf.ctypes.data, None if po is None else po.ctypes.data,
                                        u.ctypes.data, tok.ctypes.data, pp, PTR_HOST))

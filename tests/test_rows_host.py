@@ -93,3 +93,17 @@ def test_rows_that_lie_parts_of_an_element_apart_are_refused():
     wide = np.zeros((3, 2, 64 + 64), np.float32)
     assert _code(lambda: _plan(3).append(0, k, k, q=k)) == -20 and wide[:, 0, :64].strides == (1024, 4)
     assert _code(lambda: _plan(3).append(0, wide.reshape(3, 256)[:, :128].reshape(3, 2, 64), k)) == -20
+
+
+def test_read_only_outputs_are_refused():
+    """Before, the library wrote into them (a mapped file's pages, or memory that others share)."""
+    import realm_b200 as rb
+    k = np.zeros((3, 2, 64), np.float32)
+    ro = np.frombuffer(bytes(k.nbytes), np.float32).reshape(k.shape)
+    assert not ro.flags.writeable
+    for f in (lambda: _plan(3).append(0, k, k, q=k, q_out=ro), lambda: _plan(3).attention(0, k, 1.0, out=ro),
+              lambda: rb.sample_filtered(_Pool.ctx, np.zeros((2, 5), np.float32), [rb.SamplingFilter()] * 2, [0.1, 0.2],
+                                         probs=np.frombuffer(bytes(8), np.float32))):
+        with pytest.raises(ValueError, match="read-only"):
+            f()
+    assert _code(lambda: _plan(3).append(0, ro, ro, q=ro, q_out=k.copy())) == -20  # inputs may be
