@@ -320,24 +320,26 @@ def sample_filtered(ctx, logits, filters, uniforms, prev=None, out=None, probs=N
     """One token per row of logits [n][vocab] (rb_sample_filtered); returns the tokens.
 
     Host: numpy logits (float32 or float16), a list of SamplingFilter, uniforms, prev as per-row token
-    lists; probs: a float32 array that receives the tokens' probabilities. CUDA: tensors; filters from
-    pack_filters, prev a pair (tokens, offsets) of int32 tensors; the call does not wait, and a row
-    without a token left holds -1."""
+    lists; out: a uint32 or int32 array; probs: a float32 array that receives the tokens' probabilities.
+    CUDA: tensors; filters from pack_filters, prev a pair (tokens, offsets) of int32 tensors; the call
+    does not wait, and a row without a token left holds -1."""
     if not _is_tensor(logits):
         x = np.ascontiguousarray(logits)
         x = x[None] if x.ndim == 1 else x
         n, v = x.shape
         dt, _ = _dtype([x], ctx)
+        _space([x, out, probs], ctx)
         if len(filters) != n:
             raise ValueError("one filter per row wanted")
         arr = (_Filter * n)(*[f.c() for f in filters])
         u = np.ascontiguousarray(uniforms, np.float32).reshape(n)
         pf, po = _prev_arrays(prev, n)
-        tok = np.empty(n, np.uint32)
+        tok = np.empty(n, np.uint32) if out is None else _writable(out, "out")
+        at = _vec(tok, "int32" if getattr(tok, "dtype", None) == np.int32 else "uint32", n, "out")
         pp = _vec(_writable(probs, "probs"), "float32", n, "probs")
         _check(_lib.rb_sample_filtered(ctx.handle, dt, x.ctypes.data, v, n, v, arr,
                                        None if pf is None else pf.ctypes.data, None if po is None else po.ctypes.data,
-                                       u.ctypes.data, tok.ctypes.data, pp, PTR_HOST))
+                                       u.ctypes.data, at, pp, PTR_HOST))
         return tok
     import torch
     n, v = logits.shape

@@ -353,6 +353,25 @@ def test_histories_out_of_order_are_refused(ctx):
                                            rb.PTR_HOST) == rc, off
 
 
+def test_sampled_tokens_go_to_the_callers_array(ctx):
+    """numpy: `out` as uint32 or int32, filled and returned, as on CUDA tensors."""
+    import torch
+    import realm_b200 as rb
+    x = np.random.default_rng(0).normal(0, 3, (6, 700)).astype(np.float32)
+    f, u = [rb.SamplingFilter(0.8, top_k=30)] * 6, np.linspace(0.05, 0.95, 6)
+    want = rb.sample_filtered(ctx, x, f, u)
+    for t in (np.uint32, np.int32):
+        out, probs = np.full(6, 12345, t), np.zeros(6, np.float32)
+        assert rb.sample_filtered(ctx, x, f, u, out=out, probs=probs) is out
+        assert (out == want).all() and (probs > 0).all()
+    for out in (np.zeros(5, np.uint32), np.zeros(6, np.int64), np.zeros(12, np.int32)[::2], torch.zeros(6, dtype=torch.int32),
+                torch.zeros(6, dtype=torch.int32, device="cuda")):
+        with pytest.raises(ValueError):
+            rb.sample_filtered(ctx, x, f, u, out=out)
+    with pytest.raises(ValueError):
+        rb.sample_filtered(ctx, x, f, u, probs=torch.zeros(6, device="cuda"))
+
+
 # ---------------------------------------------------------------------------
 # rounding
 # ---------------------------------------------------------------------------
