@@ -481,3 +481,106 @@ def test_caps_far_from_the_scores(ctx, typ, cache, shape, bias):
                 assert ((run(cap) - w @ c).abs() <= tol).all(), cap
     finally:
         pool.close()
+
+
+# ---------------------------------------------------------------------------
+# steps as a batcher makes them
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("typ,cache", [("float16", "F16"), ("float32", "F16"), ("float32", "F32"), ("float16", "F32")])
+@pytest.mark.parametrize("hd,H", [(64, 16), (128, 16), (128, 8), (64, 64)])
+@pytest.mark.parametrize("cap,bias,window", [(0.0, False, 0), (30.0, False, 0), (0.0, True, 0), (20.0, True, 3001)])
+def test_warps_with_several_units(ctx, typ, cache, hd, H, cap, bias, window):
+    """Twenty tenants of 500 to 8000 tokens on 8 kv heads: decode rows, runs of three rows, rows without keys between
+    them, and a chunk of 40 rows. Warps take shares of several items, so their loads run over the ends of units.
+
+    A score is known to 2^-22 of its parts (q in 22 bits, a few fp32 roundings) and a weight to twice that and the
+    2^-22 of its own two parts; the errors of different keys are independent, so the norm of the output's error is
+    at most 2^-21 (2 + S) of its norm, with S the largest weighted mean of |x| + |bias|. fp16 rows: probabilities
+    and outputs are rounded, each by 0.41 h in the mean square; 0.7 h together."""
+    import torch
+    import realm_b200 as rb
+    from realm_b200 import rows as R
+    kv = 8
+    rng = np.random.default_rng(hd + H)
+    g = torch.Generator("cuda").manual_seed(hd + H)
+    L = [int(n) for n in np.linspace(500, 8000, 20) + np.arange(20) % 16]
+    dt = torch.float16 if cache == "F16" else torch.float32
+    pool = ctx.kv_pool(1, kv, hd, rb.F16 if cache == "F16" else rb.F32, n_pages=sum((n + 15) // 16 for n in L),
+                       max_tenants=len(L), max_seq=max(L))
+    try:
+        pool.shuffle(3)
+        pool.pages().fill_(float("nan"))
+        K, V = [], []
+        for t, n in enumerate(L):
+            pool.create(t)
+            K.append(torch.randn(n, kv, hd, device="cuda", generator=g).to(dt))
+            V.append(torch.randn(n, kv, hd, device="cuda", generator=g).to(dt))
+            with pool.plan([t] * n, H) as p:
+                p.append(0, K[t], V[t])
+        ten, pos, beg, end = [], [], [], []
+        for t in rng.permutation(len(L)):
+            for i in range(40 if t == 11 else 3 if t % 4 == 2 else 1):
+                at = L[t] - 1 - 2 * i if t != 11 else L[t] - 40 + i
+                ten.append(t), pos.append(at), beg.append(0), end.append(at + 1)
+            if t % 5 == 3:
+                ten.append(t), pos.append(L[t] - 1), beg.append(7), end.append(7)
+        ten, pos, beg, end = (np.array(a) for a in (ten, pos, beg, end))
+        lo = np.maximum(beg, pos - window + 1) if window else beg
+        info = np.stack([pos, np.where(lo < end, lo, 0), np.where(lo < end, end, 0), ten], 1)
+        units = R.partition(info, H, kv, ctx.num_sms, cache == "F16")
+        small = units[units[:, 0] == 0]
+        assert np.bincount(small[:, 1]).max() >= 2 and (cache == "F32" or (units[:, 0] == 1).any())
+        n = len(ten)
+        q = (torch.randn(n, H, hd, device="cuda", generator=g) * 2).to(getattr(torch, typ))
+        slopes = torch.tensor(2.0 ** -np.linspace(1, 8, H), dtype=torch.float32, device="cuda") if bias else None
+        scale = 1 / np.sqrt(hd)
+        with pool.plan(ten, H, positions=pos, begin=beg, end=end, window=window) as p:
+            got = p.attention(0, q, scale, softcap=cap, slopes=slopes)
+            again = p.attention(0, q, scale, softcap=cap, slopes=slopes)
+        assert torch.equal(got, again)
+        ref, S = torch.zeros(n, H, hd, dtype=torch.float64, device="cuda"), 0.0
+        for r in range(n):
+            if lo[r] >= end[r]:
+                continue
+            k = K[ten[r]][lo[r]:end[r]].double().repeat_interleave(H // kv, 1)
+            v = V[ten[r]][lo[r]:end[r]].double().repeat_interleave(H // kv, 1)
+            x = torch.einsum("hd,khd->hk", q[r].double(), k) * scale
+            s = cap * torch.tanh(x / cap) if cap else x
+            if bias:
+                far = slopes.double()[:, None] * torch.arange(pos[r] - lo[r], pos[r] - end[r], -1, device="cuda").abs()
+                s, x = s - far, x.abs() + far
+            w = torch.softmax(s, -1)
+            S = max(S, (w * x.abs()).sum(-1).max().item())
+            ref[r] = torch.einsum("hk,khd->hd", w, v)
+        empty = torch.from_numpy(lo >= end).cuda()
+        assert empty.any() and (got[empty] == 0).all()
+        rel = ((got.double() - ref).norm() / ref.norm()).item()
+        assert rel <= 2.0 ** -21 * (2 + S) + (0.7 * HALF if typ == "float16" else 0), (rel, S)
+    finally:
+        pool.close()
+
+
+@pytest.mark.parametrize("typ", ["float32", "float16"])
+@pytest.mark.parametrize("rows,V", [(2, 3000), (5, 32000), (70, 40001), (3, 151937)])
+def test_long_histories(ctx, typ, rows, V):
+    """Histories of some thousand tokens, with repetitions and tokens past the vocabulary. The largest logit of a
+    row after its penalties is the greedy token; a token's penalty is applied once for each time that it is there."""
+    import torch
+    import realm_b200 as rb
+    rng = np.random.default_rng(V)
+    x = rng.normal(0, 3, (rows, V)).astype(typ)
+    prev = [rng.integers(0, V + 50, int(rng.integers(0, 4000))).tolist() + [int(np.argmax(x[r]))] * (r % 3) for r in range(rows)]
+    want = []
+    for r in range(rows):
+        y = x[r].astype(np.float32)
+        for t in prev[r]:
+            if t < V:
+                y[t] = y[t] / np.float32(1.3) if y[t] > 0 else y[t] * np.float32(1.3)
+        want.append(int(np.argmax(y)))
+    flat = torch.tensor([t for p in prev for t in p], dtype=torch.int32, device="cuda")
+    off = torch.tensor(np.concatenate([[0], np.cumsum([len(p) for p in prev])]), dtype=torch.int32, device="cuda")
+    u = np.full(rows, 0.5, np.float32)
+    for f in (rb.SamplingFilter(0.0, repetition_penalty=1.3), rb.SamplingFilter(0.7, top_k=1, repetition_penalty=1.3)):
+        assert rb.sample_filtered(ctx, x, [f] * rows, u, prev=prev).tolist() == want
+        dev = rb.sample_filtered(ctx, _cuda(x), rb.pack_filters([f] * rows, "cuda"), _cuda(u), prev=(flat, off))
+        assert dev.tolist() == want
