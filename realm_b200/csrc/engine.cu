@@ -2234,9 +2234,10 @@ int stage_words(Ctx* c, const char* name, const void* p, size_t count, uint32_t 
 // Nothing is allocated once the first page has been taken.
 int reserve_pages(Ctx* c, KvPool& P, const std::vector<std::pair<int, int>>& want) {
   std::map<int, int> pages, had;  // pages a tenant is to have; and had, of those that get some
+  auto at = pages.end();
   for (auto [t, upto] : want) {
-    int& n = pages[t];
-    n = std::max(n, (upto + kRowPage - 1) / kRowPage);
+    if (at == pages.end() || at->first != t) at = pages.emplace(t, 0).first;
+    at->second = std::max(at->second, (upto + kRowPage - 1) / kRowPage);
   }
   size_t missing = 0;
   for (auto [t, n] : pages) {

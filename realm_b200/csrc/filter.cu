@@ -26,9 +26,11 @@
 // Bound by the chain of barriers (about ten) and by instructions: 96 rows of 151937 take
 // 101 us with the elements in shared memory and two CTAs an SM, took 129 us with them in
 // registers (one CTA an SM), 208 us with chunks of consecutive elements a thread, 315 us
-// with 64-bit atomics. With short lists 44 us (58 MB, 1.3 TB/s, on two thirds of the
-// SMs: reading for the maximum, from L2 for the list, 7 us for thresholds and draw, 3 for
-// the second kernel, which finds nothing left). One row of 32000: 11-12 us.
+// with 64-bit atomics. With short lists 50 us with nothing of the row in L2, 42 us in a loop
+// over other inputs (58 MB, 1.2 to 1.4 TB/s, on two thirds of the SMs: reading for the
+// maximum, from L2 for the list, 7 us for thresholds and draw, 3 for the second kernel,
+// which finds nothing left). One row of 32000: 13-14 us. Without a min-p or top-k 128 us.
+// A history costs 0.6 us a token (96 rows with 500 each 425 us): every thread goes over it.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -420,7 +422,7 @@ __device__ bool short_finish(uint2* list, int n, const rb_sampling_filter& p, bo
 }
 
 // One CTA an SM, for the registers of four vectors in flight a thread: 96 rows of 151937
-// 50 us, with two vectors and two CTAs 65 us; 200 rows 93 and 114.
+// 50 us, with two vectors and two CTAs 65 us; 200 rows 93 and 114 (nothing in L2).
 template <class T, int N>
 __global__ void __launch_bounds__(kFT, 1) filter_short_kernel(const __grid_constant__ FilterArgs a) {
   constexpr int E = 16 / sizeof(T), U = 4;
@@ -885,9 +887,10 @@ cudaError_t launch_short(const FilterArgs& a, cudaStream_t s) {
   return cudaLaunchKernelEx(&cfg, filter_short_kernel<T, N>, a);
 }
 
-// CTAs a row: one for each SM, with a vector a thread at least. 1, 2, 4 and 8 CTAs a row, us
-// (with two vectors in flight a thread): 96 rows of 151937 65, 69, 67, 75; 16 rows 56, 42,
-// 32, 32; 96 rows of 32000 24, 30, 34, 46.
+// CTAs a row: one for each SM, with a vector a thread at least. 1, 2, 3, 4, 6 and 8 CTAs a row,
+// us: 200 rows of 151937 93, 93, 101, 109, 136, 154; 96 rows 50, 58, 60, 62, 73, 81; 48 rows 46,
+// 38, 43, 42, 44, 52; 16 rows 40, 32, 30, 28, 26, 30; one row 30, 26, 24, 21, 21, 19; 96 rows of
+// 32000 24, 36, 36, 41, 52, 60; 32 rows 24, 24, 22, 21, 28, 34.
 template <class T>
 cudaError_t launch_shorts(const FilterArgs& a, int num_sms, cudaStream_t s) {
   const int vecs = a.vocab / (16 / (int)sizeof(T)), n = std::min(num_sms / a.n_rows, vecs / kFT);
@@ -926,8 +929,8 @@ cudaError_t launch_type(const FilterArgs& a, int num_sms, cudaStream_t s) {
   while (n < kMaxCluster && rounds(n) > (E == 4 ? 5 : 3)) n *= 2;
   while (n < kMaxCluster && rounds(n) > 1 && (long long)a.n_rows * n * 2 <= 2ll * num_sms) n *= 2;
   // Short lists first, unless a thread would have one vector and a CTA an SM of its own: one and
-  // eight rows of 32000 took 14 and 18 us without them, 17 and 22 with; 32 rows 37 and 24, one
-  // row of 151937 25 and 22, 96 rows 105 and 65.
+  // eight rows of 32000 take 14 and 18.5 us without them, 17 and 21 with; 32 rows 39 and 21.5, one
+  // row of 151937 29 and 19.5, 96 rows 107 and 50.
   FilterArgs b = a;
   b.all = rounds(n) <= 1 && (long long)a.n_rows * n <= num_sms;
   if (!b.all)

@@ -185,7 +185,11 @@ def _indices(a, name):
     a = np.asarray(a)
     if a.size == 0:
         return np.empty(0, np.uint32)
-    if a.ndim != 1 or a.dtype.kind not in "iu" or int(a.min()) < 0 or int(a.max()) > 0xffffffff:
+    kind, size = a.dtype.kind, a.itemsize
+    # (a negative value of 8 bytes is a large one without its sign)
+    ok = kind == "u" and size <= 4 or \
+        (kind in "iu" and (a.view(np.uint64).max() <= 0xffffffff if size == 8 else a.min() >= 0))
+    if a.ndim != 1 or not ok:
         raise ValueError(f"{name}: integers of at least 0, one per row, wanted")
     return np.ascontiguousarray(a, np.uint32)
 
