@@ -15,14 +15,18 @@
 // documents are bound by those (6 prompts of 200-1500 in documents of 300: 123 us).
 //
 // fp32 rows: q and p as fp16 hi + lo parts, two products each (22 bits); q is
-// brought to a power of two near 2^8 first. p counts from 2^bias and the running
-// maximum is raised only when a score passes it by 2^slack, so p stays below 2^16,
-// fp16's range, and O is rarely rescaled. What the bias leaves is the steps of light
-// keys, 2^-24 of p: 2^-37 of the heaviest weight for fp32 rows, 2^-34 for fp16 ones
-// (Scale). More slack saves rescaling: a prompt of 8192, cap 50, fp16 rows with bias and
-// slack 6 and 8 653 us, 10 and 5.9 664, 11 and 4.9 676, 13 and 2.9 688; but with 6 and 8
-// weights from 2^-20 of the heaviest on lost bits and were 0 below 2^-31, which shows in
-// the output of thousands of such keys beside a heavy one whose value is small.
+// brought to a power of two near 2^8 first. The tensor core cuts a sum off (towards 0)
+// after every 16 products, so the low part comes first, while the sum is small: error
+// against 64 bits of the documents case 1.14e-6 with the high part first, 0.56e-6 so.
+//
+// p counts from 2^bias and the running maximum is raised only when a score passes it by
+// 2^slack, so p stays below 2^16, fp16's range, and O is rarely rescaled. What the bias
+// leaves is the steps of light keys, 2^-24 of p: 2^-37 of the heaviest weight for fp32
+// rows, 2^-34 for fp16 ones (Scale). More slack saves rescaling: a prompt of 8192, cap 50,
+// fp16 rows with bias and slack 6 and 8 653 us, 10 and 5.9 664, 11 and 4.9 676, 13 and 2.9
+// 688; but with 6 and 8 weights from 2^-20 of the heaviest on lost bits and were 0 below
+// 2^-31, which shows in the output of thousands of such keys beside a heavy one whose
+// value is small.
 //
 // Warps: 0-3 softmax of tile 0, 4-7 of tile 1, 8 issues the products, 9 the loads (10
 // and 11 fill the last warpgroup, which gives registers to the others).
@@ -336,12 +340,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
       auto scores = [&](int t, int slot) {
         const uint64_t kd = (desc128(ra + slot * C::SLOT, 16, 1024));
 #pragma unroll
-        for (int part = 0; part < 1 + HL; ++part) {
+        for (int part = HL; part >= 0; --part) {  // the low part first (below)
           const uint64_t qd = (desc128(qa + (t * (1 + HL) + part) * C::QT, 16, 1024));
 #pragma unroll
           for (int ks = 0; ks < HD / 16; ++ks) {
             const uint32_t off = ((ks >> 2) * C::PANEL + (ks & 3) * 32) >> 4;
-            mma_ss(on, tmem + C::S0 + t * C::SW, qd + off, kd + off, ids, part || ks);
+            mma_ss(on, tmem + C::S0 + t * C::SW, qd + off, kd + off, ids, part < HL || ks);
           }
         }
       };
@@ -370,11 +374,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
         const uint32_t more = j || *(volatile int*)&primed[t];
         const uint64_t vd = (desc128(ra + slot * C::SLOT, C::PANEL, 1024));
 #pragma unroll
-        for (int part = 0; part < 1 + HL; ++part)
+        for (int part = HL; part >= 0; --part)
 #pragma unroll
           for (int ks = 0; ks < B / 16; ++ks)
             mma_ts(on, tmem + t * HD, tmem + C::P0 + t * C::PW + C::pcol(ks, part), vd + ks * (2048 >> 4), ido,
-                   more || part || ks);
+                   more || part < HL || ks);
         tc_commit(on, &o_bar[t]);
         if (t == nt - 1) tc_commit(on, &freeb[slot]);
       };
