@@ -527,8 +527,11 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) rows_mma_kernel(const __gri
             af[2] &= z1;
             af[3] &= z1;
           }
-          mma_16816(ot[i], af, h0, h1);
-          if (HL) mma_16816(ot[i], af, l0, l1);
+          float t[4] = {0.f, 0.f, 0.f, 0.f};  // a page by itself: the tensor core cuts sums off, the adds below round
+          if (HL) mma_16816(t, af, l0, l1);
+          mma_16816(t, af, h0, h1);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ot[i][e] += t[e];
         }
       } else {
         // rows that see different keys of this page: in fp32, each vector over its own keys

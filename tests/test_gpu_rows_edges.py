@@ -527,6 +527,42 @@ def test_fp32_rows_lose_little_to_the_order_of_their_sums(ctx, hd, shape):
         torch.backends.cuda.matmul.allow_tf32 = before
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows", [1, 5])
+def test_long_sums_of_positive_values(ctx, hd, rows):
+    """fp32 rows over thousands of positive values: whatever is cut off a running sum adds up instead of cancelling.
+    The sums of a page cut off at most 2 x 2^-23 of themselves (two products of 16 keys each), the rest is rounded:
+    a page's share, some hundreds of shares and the parts' join 2^-24 each with any sign, and weights in 22 bits:
+    2^-21 in all, with room for the scores' 2^-22 S (S: the weighted mean of |x|, below 2 here)."""
+    import torch
+    import realm_b200 as rb
+    H, kv, T, L = 8, 2, 24, 8000
+    g = torch.Generator("cuda").manual_seed(hd)
+    pool = ctx.kv_pool(1, kv, hd, rb.F16, n_pages=T * L // 16, max_tenants=T, max_seq=L)
+    try:
+        K, V = [], []
+        for t in range(T):
+            pool.create(t)
+            K.append(torch.randn(L, kv, hd, device="cuda", generator=g).half())
+            V.append((torch.rand(L, kv, hd, device="cuda", generator=g) + 0.5).half())
+            with pool.plan([t] * L, H) as p:
+                p.append(0, K[t], V[t])
+        ten, pos = np.repeat(np.arange(T), rows), np.tile(np.arange(L - rows, L), T)
+        q = torch.randn(len(ten), H, hd, device="cuda", generator=g)
+        with pool.plan(ten, H, positions=pos) as p:
+            got = p.attention(0, q, hd ** -0.5)
+    finally:
+        pool.close()
+    num = den = 0.0
+    for r in range(len(ten)):
+        k = K[ten[r]][:pos[r] + 1].double().repeat_interleave(H // kv, 1)
+        v = V[ten[r]][:pos[r] + 1].double().repeat_interleave(H // kv, 1)
+        w = torch.softmax(torch.einsum("hd,khd->hk", q[r].double(), k) * hd ** -0.5, -1)
+        ref = torch.einsum("hk,khd->hd", w, v)
+        num, den = num + (got[r].double() - ref).square().sum().item(), den + ref.square().sum().item()
+    assert (num / den) ** 0.5 <= 2.0 ** -21 + 2.0 ** -21, (num / den) ** 0.5
+
+
 # ---------------------------------------------------------------------------
 # steps as a batcher makes them
 # ---------------------------------------------------------------------------
