@@ -306,6 +306,7 @@ struct Ctx {
   std::vector<std::unique_ptr<Model>> models;
   std::map<int, std::unique_ptr<RowSet>> plans;  // by handle; no handle is given out twice
   int next_plan = 0;
+  DevBuf tile_hold, tile_busy;  // RowAttnArgs::hold; made with the first fp16 pool
   bool own_stream = true;
   float last_ms = 0.f;
   int last_launches = 0;
@@ -903,6 +904,15 @@ int copy_out(rb_ctx* c, void* dst, const void* src, size_t bytes, uint32_t flags
   return RB_OK;
 }
 
+int ensure_tile_hold(Ctx* c) {
+  if (c->tile_busy.p) return RB_OK;
+  if (c->tile_hold.alloc((size_t)c->num_sms * kTileVecs * 128 * 4) != cudaSuccess)
+    return fail(RB_ERR_OOM, "sums of %d tiles", c->num_sms);
+  RB_CUDA(c->tile_busy.alloc((size_t)c->num_sms * 4));
+  RB_CUDA(cudaMemsetAsync(c->tile_busy.p, 0, (size_t)c->num_sms * 4, c->stream));
+  return RB_OK;
+}
+
 int pool_create(rb_ctx* c, int n_layers, int n_kv, int hd, int kv_dtype, int n_pages, int max_tenants, int max_seq) {
   if (n_layers < 1 || n_kv < 1 || (hd != 64 && hd != 128) || n_pages < 1 || max_tenants < 1 || max_seq < 1)
     return fail(RB_ERR_UNSUPPORTED, "kv pool geometry (layers %d, kv %d, hd %d) unsupported", n_layers, n_kv, hd);
@@ -927,6 +937,8 @@ int pool_create(rb_ctx* c, int n_layers, int n_kv, int hd, int kv_dtype, int n_p
   P->tenants.resize(max_tenants);
   const int n_rep_max = 8;
   if (int rc = ensure_attn_partials(c, attn_partials_floats(attn_grid(c->num_sms), n_rep_max, hd, n_kv))) return rc;
+  if (P->f16)
+    if (int rc = ensure_tile_hold(c)) return rc;
   c->pools.push_back(std::move(P));
   return (int)c->pools.size() - 1;
 }
@@ -2554,6 +2566,9 @@ int32_t rb_plan_attention(rb_ctx* c, int32_t plan, uint32_t layer, const rb_atte
   a.rows = S->rows.as<RowInfo>();
   a.part_o = S->part_o.as<float>();
   a.part_ml = S->part_ml.as<float2>();
+  a.hold = c->tile_hold.as<float>();
+  a.hold_busy = c->tile_busy.as<int32_t>();
+  a.n_hold = c->num_sms;
   a.err = c->err.as<uint32_t>();
   a.units = S->small.as<AttnUnit>();
   a.warps = S->warps.as<int32_t>();

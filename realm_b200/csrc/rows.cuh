@@ -85,6 +85,11 @@ struct RowAttnArgs {
   int32_t n_joins = 0, join_nv = 0;  // join_nv: vectors of the largest cut item
   float* part_o = nullptr;   // [n_slots][hd]
   float2* part_ml = nullptr; // [n_slots] (maximum in base-2 units, sum)
+  // tile kernel: places for kTileVecs vectors of up to 128 elements ([elements in fours][128 vectors] of
+  // each of their tiles), one for each CTA that runs at a time, and which are taken
+  float* hold = nullptr;
+  int32_t* hold_busy = nullptr;
+  int32_t n_hold = 0;
   uint32_t* err = nullptr;
 };
 

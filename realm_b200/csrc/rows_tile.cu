@@ -18,6 +18,12 @@
 // brought to a power of two near 2^8 first. The tensor core cuts a sum off (towards 0)
 // after every 16 products, so the low part comes first, while the sum is small: error
 // against 64 bits of the documents case 1.14e-6 with the high part first, 0.56e-6 so.
+// What is cut off a long sum still adds up, so O is taken out every CHAIN = 2 blocks and
+// added to what its row holds in memory (in L2: 128 KB an SM), with rounding, which takes
+// about the 2000 clocks that 128 KB take to L2. Rows over 4000 keys, random and positive
+// values: 0.8e-6 and 1.4e-6 (plain fp32 0.8e-6, 0.2e-6); in chains of 3 1.1e-6 and 2.2e-6,
+// of 4 1.4e-6 and 3.1e-6, without 9e-6 and 27e-6. One prompt of 8192, cap 50: 1203, 1178, 1133
+// and 1040 us. fp16 rows: 2e-5 at 8192 keys, a tenth of their own rounding.
 //
 // p counts from 2^bias and the running maximum is raised only when a score passes it by
 // 2^slack, so p stays below 2^16, fp16's range, and O is rarely rescaled. What the bias
@@ -122,6 +128,10 @@ __device__ __forceinline__ void st16(uint32_t ta, const uint32_t* r) {
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
+}
+// p[0..3] += v in memory, each sum rounded
+__device__ __forceinline__ void add4(float* p, float4 v) {
+  asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
 __device__ __forceinline__ float ld1(uint32_t ta) {
   float r;
@@ -232,6 +242,9 @@ struct TileCfg {
   static constexpr bool SEP = HD == 64 || !HL;
   static constexpr int PW = SEP ? 64 * (1 + HL) : kTileKeys;
   static constexpr int P0 = 2 * HD, S0 = SEP ? 512 - kTileKeys : P0, SW = SEP ? 0 : kTileKeys;
+  // fp32 rows: blocks that O sums up on the tensor core before it is added, with rounding, to
+  // what the row holds in memory.
+  static constexpr int CHAIN = 2;
   static_assert(P0 + 2 * PW + (SEP ? kTileKeys : 0) <= 512, "");
   // column, within a tile's P, of the 16 keys of k-step ks; lo: their low parts
   static constexpr __host__ __device__ int pcol(int ks, int lo) {
@@ -251,7 +264,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
   uint8_t* ring = smem + 2 * (1 + HL) * C::QT;
   __shared__ uint64_t q_bar[2], s_bar[2], p_bar[2], o_bar[2], s_free, full[NS], freeb[NS], drain, mend_bar;
   __shared__ uint32_t tmem_slot;
-  __shared__ int primed[2];    // O holds something before the first product
+  __shared__ int primed[2];    // 1 + the block before whose product O holds something already
+  __shared__ int hold_slot;    // this CTA's place in a.hold, or -1
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_launch_dependents();
   const AttnUnit u = a.units[blockIdx.x];
@@ -264,6 +278,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (tid == 0) {
+    int slot = -1;
+    if (HL && nb > C::CHAIN) {  // one of as many places as there are SMs, each of which runs one CTA
+      uint32_t at;
+      asm volatile("mov.u32 %0, %%smid;" : "=r"(at));
+      for (int i = 0; i < 4 * a.n_hold && slot < 0; ++i) {
+        const int p = (int)((at + i) % (uint32_t)a.n_hold);
+        if (atomicCAS(a.hold_busy + p, 0, 1) == 0) slot = p;
+      }
+      if (slot < 0) report_error(a.err, DEV_TIMEOUT_SMEM);
+    }
+    hold_slot = slot;
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_bar[t], 128);
       mbar_init(&s_bar[t], 1);
@@ -284,6 +309,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
   __syncthreads();
   tc_after();
   const uint32_t tmem = tmem_slot;
+  const bool hold = HL && hold_slot >= 0;
+  // whether O starts anew with block j
+  auto anew = [&](int j) { return j == 0 || (hold && j % C::CHAIN == 0); };
   // softmax warps: this thread has row tr of its tile
   const int tile = warp >> 2, tr = (warp & 3) * 32 + lane, vec_id = tile * 128 + tr;
   RowInfo r{0, 0, 0x7fffffff, 0};
@@ -371,7 +399,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
         if (t == 0) wait(&full[slot], (2 * j + 1) / NS, DEV_TIMEOUT_FULL);
         wait(&p_bar[t], j, DEV_TIMEOUT_DRAIN);
         if (!ok) return;
-        const uint32_t more = j || *(volatile int*)&primed[t];
+        const uint32_t more = !anew(j) || *(volatile int*)&primed[t] == j + 1;
         const uint64_t vd = (desc128(ra + slot * C::SLOT, C::PANEL, 1024));
 #pragma unroll
         for (int part = HL; part >= 0; --part)
@@ -514,6 +542,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
     // them took longer than with either (fp16 rows, 1 and 2: 993 us).
     int form = BIAS || !__all_sync(0xffffffffu, fuse_ok) ? 2 : 1;
     float m = -INFINITY, l = 0.f;
+    // elements d .. d + 3 of what this row holds, in units of 2^held: held_at[d * 128 .. + 3]
+    float* const held_at = a.hold + (size_t)((hold ? hold_slot : 0) * 2 + tile) * (HD * 128) + tr * 4;
+    float held = -INFINITY;
     // Both tiles meet. Not a named barrier, which has no limit: after a wait that ran out
     // one of them may have read other values and not come.
     int met = 0;
@@ -648,7 +679,33 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
         if (alive) alive = mbar_wait(&o_bar[tile], (uint32_t)((j - 1) & 1), a.err, DEV_TIMEOUT_DRAIN);
         tc_after();
       }
-      if (__any_sync(0xffffffffu, up) && j > 0) {
+      if (HL && j > 0 && anew(j)) {
+        if (held == -INFINITY) held = m;  // still so in a row that has seen no key: it holds zeros
+        const bool far = m - held > 60.f;
+        if (__any_sync(0xffffffffu, far)) {  // scores rose by much: other units
+          const float f = far ? ex2(held - m) : 1.f;
+#pragma unroll 1
+          for (int d = 0; d < HD; d += 4) {
+            float4 h = __ldcg(reinterpret_cast<const float4*>(held_at + d * 128));
+            h.x *= f, h.y *= f, h.z *= f, h.w *= f;
+            __stcg(reinterpret_cast<float4*>(held_at + d * 128), h);
+          }
+          if (far) held = m;
+        }
+        const float f = m == -INFINITY ? 1.f : alpha * ex2(m - held);
+#pragma unroll 1
+        for (int d = 0; d < HD; d += 32) {
+          float o[32];
+          ld32(to + d, o);
+          wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            const float4 v = make_float4(o[i] * f, o[i + 1] * f, o[i + 2] * f, o[i + 3] * f);
+            if (j > C::CHAIN) add4(held_at + (d + i) * 128, v);
+            else __stcg(reinterpret_cast<float4*>(held_at + (d + i) * 128), v);
+          }
+        }
+      } else if (__any_sync(0xffffffffu, up) && j > 0) {
 #pragma unroll 1
         for (int d = 0; d < HD; d += 32) {
           float o[32];
@@ -763,7 +820,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
             float o[32];
             ld32(to + d, o);
             wait_ld();
-            if (j == 0)
+            if (anew(j))
 #pragma unroll
               for (int i = 0; i < 32; ++i) o[i] = 0.f;
 #pragma unroll 1
@@ -804,7 +861,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
           }
           proxy_fence();
           meet();
-          if (tr == 0 && j == 0) *(volatile int*)&primed[tile] = 1;
+          if (tr == 0) *(volatile int*)&primed[tile] = j + 1;
         }
       }
       wait_st();
@@ -833,6 +890,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
         float o[32];
         ld32(to + pass * nd + d, o);
         wait_ld();
+        if (hold) {
+          const float f = ex2(held - m);
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            const float4 h = __ldcg(reinterpret_cast<const float4*>(held_at + (d + i) * 128));
+            o[i] = fmaf(h.x, f, o[i]);
+            o[i + 1] = fmaf(h.y, f, o[i + 1]);
+            o[i + 2] = fmaf(h.z, f, o[i + 2]);
+            o[i + 3] = fmaf(h.w, f, o[i + 3]);
+          }
+        }
         if (nb == 0 || l == 0.f)
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0.f;
@@ -887,6 +955,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
   tc_before();
   __syncthreads();
   tc_after();
+  if (tid == 0 && hold) {
+    __threadfence();
+    atomicExch(a.hold_busy + hold_slot, 0);
+  }
   if (warp == kSoftWarps)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }

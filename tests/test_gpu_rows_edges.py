@@ -563,6 +563,85 @@ def test_long_sums_of_positive_values(ctx, hd, rows):
     assert (num / den) ** 0.5 <= 2.0 ** -21 + 2.0 ** -21, (num / den) ** 0.5
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+@pytest.mark.parametrize("values", ["positive", "random"])
+def test_chunks_over_long_contexts(ctx, hd, cap, values):
+    """fp32 rows, chunks of 512 rows over 2500 tokens, more of them than SMs. Random values: the error against 64 bits stays
+    within 1.5 times that of plain fp32 products, or 1e-6. Positive values: what the tensor core cuts off has one sign;
+    at most 2^-23 of the running sum after each 16 keys of each part, 32 times before it is added to the rest: 2^-18."""
+    import torch
+    import realm_b200 as rb
+    H, kv, T, L, rows = 8, 2, 12, 2500, 512
+    g = torch.Generator("cuda").manual_seed(hd)
+    pool = ctx.kv_pool(1, kv, hd, rb.F16, n_pages=T * (L // 16 + 1), max_tenants=T, max_seq=L)
+    K, V = [], []
+    try:
+        for t in range(T):
+            pool.create(t)
+            K.append(torch.randn(L, kv, hd, device="cuda", generator=g).half())
+            v = torch.randn(L, kv, hd, device="cuda", generator=g)
+            V.append((v.abs() + 0.25 if values == "positive" else v).half())
+            with pool.plan([t] * L, H) as p:
+                p.append(0, K[t], V[t])
+        ten, pos = np.repeat(np.arange(T), rows), np.tile(np.arange(L - rows, L), T)
+        q = torch.randn(T, rows, H, hd, device="cuda", generator=g)
+        with pool.plan(ten, H, positions=pos) as p:
+            got = p.attention(0, q.view(-1, H, hd), hd ** -0.5, softcap=cap).view(q.shape)
+    finally:
+        pool.close()
+    seen = (torch.arange(L, device="cuda") <= torch.arange(L - rows, L, device="cuda")[:, None])[:, None]
+    before = torch.backends.cuda.matmul.allow_tf32
+    torch.backends.cuda.matmul.allow_tf32 = False
+    e = f = n = 0.0
+    try:
+        for t in range(T):
+            outs = []
+            for typ in (torch.float64, torch.float32):
+                k, v = (a[t].to(typ).repeat_interleave(H // kv, 1) for a in (K, V))
+                x = torch.einsum("nhd,lhd->nhl", q[t].to(typ), k) * hd ** -0.5
+                x = cap * torch.tanh(x / cap) if cap else x
+                outs.append(torch.einsum("nhl,lhd->nhd", torch.softmax(x.masked_fill(~seen, -torch.inf), -1), v).double())
+            e, f, n = (a + b.square().sum().item() for a, b in ((e, got[t].double() - outs[0]), (f, outs[1] - outs[0]),
+                                                                (n, outs[0])))
+    finally:
+        torch.backends.cuda.matmul.allow_tf32 = before
+    e, f = (e / n) ** 0.5, (f / n) ** 0.5
+    assert e <= (2.0 ** -18 if values == "positive" else max(1e-6, 1.5 * f)), (e, f)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_scores_that_rise_by_far(ctx, hd):
+    """fp32 rows whose scores climb block by block, by hundreds in all, so that what the earlier keys gave fades out,
+    and rows whose first keys come late. A weight is off by 2^-22 and by its score's rounding, 2^-23 of up to 400, twice:
+    2^-13 with room; values are up to 1."""
+    import torch
+    import realm_b200 as rb
+    H, L, n = 4, 2048, 300
+    g = torch.Generator("cuda").manual_seed(hd)
+    k = torch.zeros(L, 1, hd, dtype=torch.float16, device="cuda")
+    k[:, 0, 0] = torch.arange(L, device="cuda") / 64.0 + torch.rand(L, device="cuda", generator=g)
+    v = (torch.rand(L, 1, hd, device="cuda", generator=g) * 2 - 1).half()
+    q = torch.randn(n, H, hd, device="cuda", generator=g)
+    q[:, :, 0] = torch.linspace(-12, 12, n * H, device="cuda").view(n, H)
+    beg = np.where(np.arange(n) % 7 == 3, 1400, 0)
+    pool = ctx.kv_pool(1, 1, hd, rb.F16, n_pages=L // 16, max_tenants=1, max_seq=L)
+    try:
+        pool.create(0)
+        with pool.plan([0] * L, H) as p:
+            p.append(0, k, v)
+        rep = 40  # more items than SMs: none is cut
+        with pool.plan([0] * (n * rep), H, positions=[L - 1] * (n * rep), begin=np.tile(beg, rep)) as p:
+            got = p.attention(0, q.repeat(rep, 1, 1), 1.0).view(rep, n, H, hd)
+    finally:
+        pool.close()
+    assert (got - got[:1]).abs().max() <= 2.0 ** -13  # the same rows at other places of their tiles
+    seen = torch.arange(L, device="cuda") >= _cuda(beg)[:, None, None]
+    x = torch.einsum("nhd,ld->nhl", q.double(), k[:, 0].double()).masked_fill(~seen, -torch.inf)
+    ref = torch.einsum("nhl,ld->nhd", torch.softmax(x, -1), v[:, 0].double())
+    assert (got[0].double() - ref).abs().max() <= 2.0 ** -13
+
+
 # ---------------------------------------------------------------------------
 # steps as a batcher makes them
 # ---------------------------------------------------------------------------
