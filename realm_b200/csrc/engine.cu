@@ -2363,9 +2363,9 @@ int32_t plan_create(rb_ctx* c, int32_t pool, const rb_plan_desc* d, int32_t* pla
   if (int rc = upload_vec(c, S->spans, w.spans)) return rc;
   if (int rc = upload_vec(c, S->joins, w.joins)) return rc;
   if (w.n_slots) {
-    if (S->part_o.alloc((size_t)w.n_slots * P->hd * 4) != cudaSuccess ||
+    if (w.n_slots > INT32_MAX || S->part_o.alloc((size_t)w.n_slots * P->hd * 4) != cudaSuccess ||
         S->part_ml.alloc((size_t)w.n_slots * 8) != cudaSuccess)
-      return fail(RB_ERR_OOM, "partial results of %d vectors", w.n_slots);
+      return fail(RB_ERR_OOM, "partial results of %lld vectors", (long long)w.n_slots);
   }
   if (int rc = reserve_pages(c, *P, want)) return rc;
   // the lists are copied from this call's own memory

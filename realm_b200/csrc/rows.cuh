@@ -12,6 +12,7 @@ constexpr int kRowPage = 16;      // tokens per cache page
 constexpr int kSmallVecs = 8;     // query vectors per item of the small kernels
 constexpr int kTileVecs = 256;    // query vectors per item of the tile kernel (two tiles of 128)
 constexpr int kTileKeys = 128;    // keys per block of the tile kernel
+constexpr int kTileBlocks = 256;  // blocks of a unit of the tile kernel, at most
 constexpr int kMaxRep = 64;       // query heads per kv head
 constexpr int kRowWarps = 4;      // warps a CTA of the small kernels, two CTAs an SM
 
@@ -51,7 +52,7 @@ struct RowWork {
   std::vector<int32_t> small_warp;
   std::vector<JoinItem> joins;       // items that were cut
   int32_t join_nv = 0;               // vectors of the largest of them
-  int32_t n_slots = 0;      // partial result vectors
+  int64_t n_slots = 0;      // partial result vectors (a plan is refused where they pass 32 bits)
   int32_t max_nv = 0;       // vectors of the largest small item
 };
 

@@ -114,10 +114,10 @@ void rows_partition(const std::vector<RowInfo>& rows, int n_heads, int n_kv, int
         } while (p < np);
       }
       const int parts = (int)cuts.size();
-      const int slot = out.n_slots;
+      const int slot = (int)out.n_slots;
       if (parts > 1)
         for (int h = 0; h < n_kv; ++h) {
-          out.joins.push_back({it.row0, it.v0, it.nv, h, out.n_slots, parts});
+          out.joins.push_back({it.row0, it.v0, it.nv, h, (int)out.n_slots, parts});
           out.n_slots += parts * it.nv;
         }
       for (int q = 0; q < parts; ++q) {
@@ -144,6 +144,8 @@ void rows_partition(const std::vector<RowInfo>& rows, int n_heads, int n_kv, int
   // the items are fewer than the SMs, and not below four blocks: a unit's start and
   // end cost about as much as those. (Cutting the longest of 256 uneven items as well,
   // for the balance at the end, took 257 us and 19 us of joining instead of 237 us.)
+  // No unit has more than kTileBlocks: what the tensor core cuts off its running sums adds
+  // up, 5e-8 of the output a product of 16 keys, to 1e-4 there, which fp16 rows have room for.
   if (!tile.empty()) {
     long long blocks = 0;
     for (const Item& it : tile) blocks += (long long)n_kv * std::max(1, blocks_of(it, kTileKeys));
@@ -151,16 +153,17 @@ void rows_partition(const std::vector<RowInfo>& rows, int n_heads, int n_kv, int
     const bool cut = (long long)tile.size() * n_kv < num_sms;
     for (const Item& it : tile) {
       const int nb = blocks_of(it, kTileKeys);
-      const int parts = cut && nb > seg ? (int)((nb + seg - 1) / seg) : 1;
+      const int fit = (nb + kTileBlocks - 1) / kTileBlocks;
+      const int parts = std::max({1, fit, cut && nb > seg ? (int)((nb + seg - 1) / seg) : 1});
       for (int h = 0; h < n_kv; ++h) {
         if (parts > 1) {
-          out.joins.push_back({it.row0, it.v0, it.nv, h, out.n_slots, parts});
+          out.joins.push_back({it.row0, it.v0, it.nv, h, (int)out.n_slots, parts});
         }
         for (int p = 0; p < parts; ++p) {
           const int b0 = (int)((long long)nb * p / parts), b1 = (int)((long long)nb * (p + 1) / parts);
           AttnUnit u = unit_of(it, h, b0, b1, kTileKeys);
           if (parts > 1) {
-            u.slot = out.n_slots;
+            u.slot = (int)out.n_slots;
             out.n_slots += it.nv;
           }
           out.tile.push_back(u);

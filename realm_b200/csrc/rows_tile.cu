@@ -23,7 +23,8 @@
 // about the 2000 clocks that 128 KB take to L2. Rows over 4000 keys, random and positive
 // values: 0.8e-6 and 1.4e-6 (plain fp32 0.8e-6, 0.2e-6); in chains of 3 1.1e-6 and 2.2e-6,
 // of 4 1.4e-6 and 3.1e-6, without 9e-6 and 27e-6. One prompt of 8192, cap 50: 1203, 1178, 1133
-// and 1040 us. fp16 rows: 2e-5 at 8192 keys, a tenth of their own rounding.
+// and 1040 us. fp16 rows: 2e-5 at 8192 keys, a tenth of their own rounding; units end
+// after 32768.
 //
 // p counts from 2^bias and the running maximum is raised only when a score passes it by
 // 2^slack, so p stays below 2^16, fp16's range, and O is rarely rescaled. What the bias

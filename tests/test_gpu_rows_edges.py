@@ -642,6 +642,31 @@ def test_scores_that_rise_by_far(ctx, hd):
     assert (got[0].double() - ref).abs().max() <= 2.0 ** -13
 
 
+def test_fp16_chunks_over_very_long_contexts(ctx):
+    """fp16 rows over 200000 positive values, more items than SMs: the error stays that of the rows' own rounding, 2^-11
+    of the output in the mean square (probabilities' errors average out over the keys)."""
+    import torch
+    import realm_b200 as rb
+    H, hd, L, n = 1, 64, 200000, 64
+    g = torch.Generator("cuda").manual_seed(1)
+    k = torch.randn(L, 1, hd, device="cuda", generator=g).half()
+    v = (torch.rand(L, 1, hd, device="cuda", generator=g) + 0.5).half()
+    q = torch.randn(n, H, hd, device="cuda", generator=g).half()
+    pool = ctx.kv_pool(1, 1, hd, rb.F16, n_pages=L // 16, max_tenants=1, max_seq=L)
+    try:
+        pool.create(0)
+        with pool.plan([0] * L, H) as p:
+            p.append(0, k, v)
+        rep = 600
+        with pool.plan([0] * (n * rep), H, positions=[L - 1] * (n * rep)) as p:
+            got = p.attention(0, q.repeat(rep, 1, 1), hd ** -0.5)[:n].double()
+    finally:
+        pool.close()
+    w = torch.softmax(torch.einsum("nhd,ld->nhl", q.double(), k[:, 0].double()) * hd ** -0.5, -1)
+    ref = torch.einsum("nhl,ld->nhd", w, v[:, 0].double())
+    assert ((got - ref).norm() / ref.norm()).item() <= HALF
+
+
 # ---------------------------------------------------------------------------
 # steps as a batcher makes them
 # ---------------------------------------------------------------------------

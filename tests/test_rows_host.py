@@ -107,3 +107,23 @@ def test_read_only_outputs_are_refused():
         with pytest.raises(ValueError, match="read-only"):
             f()
     assert _code(lambda: _plan(3).append(0, ro, ro, q=ro, q_out=k.copy())) == -20  # inputs may be
+
+
+@pytest.mark.parametrize("heads,kv,rows", [(32, 8, 2000), (8, 1, 512), (4, 4, 3000)])
+def test_units_of_long_contexts_are_bounded(heads, kv, rows):
+    """Many rows over 131072 keys and more: no unit of the tile kernel takes more than 32768 keys, so that its sums on the
+    tensor core stay short; each key is in one unit."""
+    from realm_b200 import rows as R
+    end = 140001
+    pos = np.arange(end - rows, end)
+    r = np.stack([pos, np.zeros(rows, int), pos + 1, np.zeros(rows, int)], 1)
+    units = R.partition(r, heads, kv, 148, True)
+    assert (units[:, 0] == 1).all()
+    k0, k1 = units[:, 7], units[:, 8]
+    assert (k1 - k0).max() <= 256 * 128
+    items = {}
+    for u in units:
+        items.setdefault((u[2], u[3], u[5]), []).append((u[7], u[8]))
+    for spans in items.values():
+        spans.sort()
+        assert spans[0][0] == 0 and all(a[1] == b[0] for a, b in zip(spans, spans[1:])) and len(spans) >= 5
