@@ -26,7 +26,7 @@
 // Bound by the chain of barriers (about ten) and by instructions: 96 rows of 151937 take
 // 101 us with the elements in shared memory and two CTAs an SM, took 129 us with them in
 // registers (one CTA an SM), 208 us with chunks of consecutive elements a thread, 315 us
-// with 64-bit atomics. With short lists 50 us with nothing of the row in L2, 42 us in a loop
+// with 64-bit atomics. With short lists 50 us with nothing of the row in L2, 42 to 45 us in a loop
 // over other inputs (58 MB, 1.2 to 1.4 TB/s, on two thirds of the SMs: reading for the
 // maximum, from L2 for the list, 7 us for thresholds and draw, 3 for the second kernel,
 // which finds nothing left). One row of 32000: 13-14 us. Without a min-p or top-k 128 us.

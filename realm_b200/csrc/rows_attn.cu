@@ -281,8 +281,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) rows_f32_kernel(const __gri
 // (TMA boxes of 16 rows x 128 bytes with 128-byte swizzle); the loads run ahead over
 // the ends of units. Warps share nothing: with the four warps of a CTA on one unit,
 // its start and end (barriers, merges) took 6 us a unit, 72 us for 16 tenants of
-// 512-8192 tokens; so 61 us (285 MB, 4.7 TB/s). 4 tenants of 65537-131072 tokens with 64
-// heads: 269 us, 6.0 TB/s.
+// 512-8192 tokens; so 62 us (285 MB, 4.6 TB/s). 4 tenants of 65537-131072 tokens with 64
+// heads: 250 to 270 us, 6.0 to 6.4 TB/s.
 // ---------------------------------------------------------------------------
 template <int HD>
 struct MmaCfg {

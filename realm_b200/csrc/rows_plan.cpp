@@ -52,9 +52,9 @@ void rows_partition(const std::vector<RowInfo>& rows, int n_heads, int n_kv, int
   std::vector<Item> small, tile;
   // Runs of at least 24 query vectors a kv head take the tile kernel. Tiles against small
   // items, us, for runs of 16, 24, 32 and 64 vectors, 64 tenants x 1024 tokens, 8 kv heads:
-  // fp16 rows at head size 128 92/99, 93/159, 94/198, 94/337; at 64 73/69, 73/97, 74/120,
-  // 74/214; fp32 rows at 128 137/99, 138/173, 139/202, 141/341; at 64 96/71, 96/99, 98/124,
-  // 98/222. (16 tenants x 2048, fp32 rows at 128: 77/67, 79/69, 81/93, 87/155.)
+  // fp16 rows at head size 128 92/103, 92/161, 94/196, 94/335; at 64 72/71, 74/99, 74/122,
+  // 74/220; fp32 rows at 128 162/101, 164/167, 164/206, 166/339; at 64 106/73, 107/101,
+  // 109/126, 109/226. (16 tenants x 2048, fp32 rows at 128: 89/67, 91/71, 93/93, 97/159.)
   for (int r = 0; r < n;) {
     int e = r + 1;
     while (e < n && rows[e].tenant == rows[r].tenant) ++e;

@@ -9,10 +9,10 @@
 // the tensor core works on the other's.
 //
 // Bound by the softmax warps' instructions: one prompt of 8192, 32 heads of 128 on 8, cap
-// 50, fp16: 648 us, 849 TFLOP/s (issue slots 47 % used, tensor cores 44 %; without the cap
+// 50, fp16: 661 us, 832 TFLOP/s (issue slots 47 % used, tensor cores 44 %; without the cap
 // 0.91 of it). A unit's start and end (q, the first scores, O) cost 10 K clocks (fp16 rows,
 // head size 64) to 25 K (fp32 rows, 128), as much as two or three pairs of blocks: short
-// documents are bound by those (6 prompts of 200-1500 in documents of 300: 123 us).
+// documents are bound by those (6 prompts of 200-1500 in documents of 300: 129 us).
 //
 // fp32 rows: q and p as fp16 hi + lo parts, two products each (22 bits); q is
 // brought to a power of two near 2^8 first. The tensor core cuts a sum off (towards 0)
