@@ -667,6 +667,29 @@ def test_fp16_chunks_over_very_long_contexts(ctx):
     assert ((got - ref).norm() / ref.norm()).item() <= HALF
 
 
+def test_prompts_over_a_models_pool(ctx):
+    """Row plans on the pool of a model: a chunk of fp32 rows over several blocks of keys, as over a pool of the caller's."""
+    import torch
+    import realm_b200 as rb
+    cfg = dict(n_layers=1, hidden=256, n_heads=4, n_kv_heads=2, head_dim=64, ffn=256, vocab=256, max_seq=1024, rms_eps=1e-5,
+               layer_eps=1e-5, rope_theta=1e4, kv_dtype=rb.F16, max_tenants=1)
+    g = torch.Generator("cuda").manual_seed(0)
+    k, v = (torch.randn(1000, 2, 64, device="cuda", generator=g) for _ in range(2))
+    q = torch.randn(700, 8, 64, device="cuda", generator=g)
+    outs = []
+    with rb.Context(0) as c:
+        model = rb.Model(c, cfg)
+        model.tenant_create(0)
+        pool = c.kv_pool(1, 2, 64, rb.F16, n_pages=64, max_tenants=1, max_seq=1024)
+        pool.create(0)
+        for kv in (model.kv, pool):
+            with kv.plan([0] * 1000, 8) as p:
+                p.append(0, k, v)
+            with kv.plan([0] * 700, 8, positions=range(300, 1000)) as p:
+                outs.append(p.attention(0, q, 0.125))
+    assert torch.equal(*outs) and torch.isfinite(outs[0]).all()
+
+
 # ---------------------------------------------------------------------------
 # steps as a batcher makes them
 # ---------------------------------------------------------------------------
