@@ -17,7 +17,7 @@
 // fp32 rows: q and p as fp16 hi + lo parts, two products each (22 bits); q is
 // brought to a power of two near 2^8 first. The tensor core cuts a sum off (towards 0)
 // after every 16 products, so the low part comes first, while the sum is small: error
-// against 64 bits of the documents case 1.14e-6 with the high part first, 0.56e-6 so.
+// against 64 bits of 6 prompts in documents of 300 1.14e-6 with the high part first, 0.56e-6 so.
 // What is cut off a long sum still adds up, so O is taken out every CHAIN = 2 blocks and
 // added to what its row holds in memory (in L2: 128 KB an SM), with rounding, which takes
 // about the 2000 clocks that 128 KB take to L2. Rows over 4000 keys, random and positive
@@ -537,8 +537,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
     }
     const bool fuse_ok = HL || (kcap > 1e-6f && kcap < 1e4f && cap2 < 1e6f);
     // How the warp applies the cap: 1 Fused and 2 Wide, together with the exponential; 3 on its
-    // own, with no bound on the scores. One prompt of 8192, 32 heads of 128: fp16 rows 583,
-    // 713 and 990 us, fp32 rows 1040, 1235 and 1555. A larger score raises the form for
+    // own, with no bound on the scores. One prompt of 8192, 32 heads of 128: fp16 rows 575,
+    // 711 and 970 us, fp32 rows 1203, 1405 and 1708. A larger score raises the form for
     // good: with one chosen for each block, warps that went back and forth between two of
     // them took longer than with either (fp16 rows, 1 and 2: 993 us).
     int form = BIAS || !__all_sync(0xffffffffu, fuse_ok) ? 2 : 1;
@@ -609,7 +609,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) rows_tile_kernel(const __grid
           for (int i = 0; i < B; ++i) x[i] = fmaf(-2.f * cap2, rcp(1.f + ex2(x[i] * k)), cap2);
         } else {
           // the same, but small scores, which other rows' large ones brought here, take the
-          // polynomial (prompt of 8192, cap 4, head size 128: 1555 us, without it 1290)
+          // polynomial (a prompt of 8192 with cap 4 takes a fifth longer for it)
           const f2 k2 = pair(kcap, kcap);
 #pragma unroll
           for (int i = 0; i < B; i += 2) {
