@@ -80,12 +80,15 @@ def draw(rng):
         if rng.random() < 0.6:
             n = max(256, n // 64 * 64)
         typ = rng.choice(["f16", "f32"])
-        while rows * (k + 2 * n) > 4096 * (11008 + 2 * 4096):
-            rows = rows * 3 // 4
         lo = log(4, 128)
-        return dict(op=op, rows=rows, tenants=min(rows, log(1, 64)), k=k, n=n, rank_min=lo,
-                    rank_max=lo if rng.random() < 0.5 else log(lo, 128), type=typ, mixed=rng.random() < 0.5,
-                    bare=rng.choice([0.0, 0.0, 0.2]))
+        c = dict(op=op, rows=rows, tenants=log(1, 64), k=k, n=n, rank_min=lo,
+                 rank_max=lo if rng.random() < 0.5 else log(lo, 128), type=typ, mixed=rng.random() < 0.5,
+                 bare=rng.choice([0.0, 0.0, 0.2]))
+        while True:
+            c["tenants"] = min(c["tenants"], c["rows"])
+            if work(c)["bytes"] <= 3.3e8:
+                return c
+            c["rows"] = c["rows"] * 3 // 4
     if op == "norm":
         dim = log(64, 16384)
         if rng.random() < 0.6:
