@@ -54,7 +54,8 @@ extern "C" {
 #define RB_PTR_DEVICE 1u
 /* With RB_PTR_DEVICE: enqueue on the context stream and return without waiting
  * (rb_weight_matmul, rb_attention_forward, rb_plan_append, rb_plan_attention,
- * rb_sample_filtered); device-side failures surface at the
+ * rb_sample_filtered, rb_filter_probs, rb_verify_drafts, rb_residual_norm,
+ * rb_adapters_set, rb_adapters_add); device-side failures surface at the
  * next rb_sync. Without RB_PTR_DEVICE the flag is ignored. */
 #define RB_ASYNC 2u
 
@@ -528,6 +529,100 @@ int32_t rb_sample_filtered(rb_ctx* ctx, int32_t dtype, const void* logits, uint6
                            uint32_t vocab, const rb_sampling_filter* params, const uint32_t* prev_tokens,
                            const uint32_t* prev_offsets, const float* uniforms, uint32_t* out_tokens, float* probs,
                            uint32_t flags);
+/* The distribution that rb_sample_filtered draws from: probs [n_rows][ldp] (fp32), each
+ * kept token's share of the kept weight, rounded once, and 0 for the others. A row that
+ * has no finite or +infinite logit is 0 throughout. Arguments as rb_sample_filtered;
+ * probs must not overlap logits. Returns n_rows. */
+int32_t rb_filter_probs(rb_ctx* ctx, int32_t dtype, const void* logits, uint64_t ld, uint32_t n_rows, uint32_t vocab,
+                        const rb_sampling_filter* params, const uint32_t* prev_tokens, const uint32_t* prev_offsets,
+                        float* probs, uint64_t ldp, uint32_t flags);
+
+/* ---- verification of drafted tokens ----
+ * Draft/target decoding (crates/realm-runtime/src/speculative.rs) with random
+ * acceptance, which leaves the target's distribution as it is. Request r has the rows
+ * offsets[r] .. offsets[r + 1] of probs, one more than it has drafted tokens: row i is
+ * the target's distribution before drafts[i], the last one that after all of them. */
+typedef struct rb_verify_desc {
+  uint32_t n_requests, n_rows, vocab; /* vocab up to 262144 */
+  const uint32_t* offsets;   /* [n_requests + 1], never falling, up to n_rows; rows of no request are left as they are */
+  const float* probs;        /* [n_rows][ldp]; what lies outside [0, 1] counts as the nearer end, a NaN as 0 */
+  const float* draft_probs;  /* [n_rows][ldq] the distributions that the tokens were drawn from (a request's last row
+                              * is not read), or NULL: tokens that were not drawn, as by looking them up */
+  uint64_t ldp, ldq;
+  const uint32_t* drafts;    /* [n_rows]; a request's last entry is not read */
+  const float* uniforms;     /* [n_rows] in [0, 1): a request's last one draws its token, the others test its drafts */
+  uint32_t* tokens;          /* [n_rows] out; may be drafts itself */
+  int32_t* accepted;         /* [n_requests] out */
+} rb_verify_desc;
+/* Drafted token d of row i is accepted while uniforms[i] q(d) < p(d) (q(d) = 1 without
+ * draft_probs; p(d) = 0 for a d outside the vocabulary). At the first one that is not, a token is
+ * drawn from the positive part of p - q (without draft_probs from p without d), after the
+ * last from p. Weights of the draw are p - q in fixed point with 44 fractional bits, so it
+ * depends on no order: the first index whose running sum exceeds uniform * total
+ * (uniforms past either end draw the last and the first). Where p - q has no positive part
+ * the draw is from p. tokens gets the accepted tokens, then the drawn one, then 0xffffffff up
+ * to the request's last row; accepted the number of the accepted. A p without a positive
+ * value draws 0xffffffff; unless RB_ASYNC, the call then returns RB_ERR_INVALID ("Failed to create
+ * weighted index"). A request without rows gets accepted = 0, one whose offsets fall or pass
+ * n_rows -1 (device memory; on the host that is refused). Returns n_requests. */
+int32_t rb_verify_drafts(rb_ctx* ctx, const rb_verify_desc* desc, uint32_t flags);
+
+/* ---- norms around a block ----
+ *   z = y (y w1 / sqrt(mean y^2 + eps) with post_norm), h = x + scale * gate * z,
+ *   out = h w2 / sqrt(mean h^2 + eps)
+ * row by row in fp32: what lies between a block's last projection and the next block's
+ * first one. h goes to x_out, the norm of the unrounded h to out, each rounded once. */
+typedef struct rb_residual_desc {
+  int32_t dtype;          /* of y, gate and out: RB_F32 or RB_F16 */
+  int32_t x_dtype;        /* of x and x_out */
+  uint32_t n_rows, dim;   /* dim up to 32768 */
+  const void* y;          /* [n_rows][ldy] the block's output */
+  const void* x;          /* [n_rows][ldx] the residual stream */
+  const void* gate;       /* NULL: 1; else [n_rows][ldg], or with ldg 0 one row for all */
+  void* x_out;            /* [n_rows][ldxo]; may be x itself (ldxo == ldx) */
+  void* out;              /* [n_rows][ldo], or NULL: h alone; may be y itself (ldo == ldy) */
+  uint64_t ldy, ldx, ldg, ldxo, ldo;
+  const float* post_norm; /* [dim] w1, or NULL: no norm behind the block */
+  const float* pre_norm;  /* [dim] w2; with out, and only then */
+  float scale, eps;
+} rb_residual_desc;
+/* Apart from the two pairs named, outputs must not overlap inputs or one another
+ * (RB_ERR_INVALID). Returns n_rows. */
+int32_t rb_residual_norm(rb_ctx* ctx, const rb_residual_desc* desc, uint32_t flags);
+
+/* ---- low-rank adapters ----
+ * Adapters of many tenants beside one shared projection y = W x, W [n][k]
+ * (rb_weight_matmul): a row with adapter a gets scale_a * up_a (down_a x) added. The
+ * reference adds the product of the factors to dequantised weights, one model a tenant
+ * (crates/realm-runtime/src/lora.rs); here one call serves rows of any mix of adapters. A
+ * set holds n_slots adapters of one projection, each of up to max_rank, in fp16:
+ * n_slots * max_rank * (n + k) * 2 bytes, max_rank rounded up to a multiple of 8. */
+int32_t rb_adapters_create(rb_ctx* ctx, uint32_t n, uint32_t k, uint32_t n_slots, uint32_t max_rank, int32_t* set);
+/* Waits for the context's stream, then frees the set. Its handle is not given out again. */
+int32_t rb_adapters_destroy(rb_ctx* ctx, int32_t set);
+/* Puts an adapter in a slot, in place of what it held: down [rank][k], up [n][rank], both of
+ * dtype RB_F32 (rounded to fp16) or RB_F16. Ordered on the stream: rows of earlier calls
+ * have the slot's old adapter. Returns rank. */
+int32_t rb_adapters_set(rb_ctx* ctx, int32_t set, uint32_t slot, int32_t dtype, uint32_t rank, const void* down,
+                        const void* up, float scale, uint32_t flags);
+/* Empties a slot (RB_ERR_NOT_FOUND beyond n_slots). */
+int32_t rb_adapters_clear(rb_ctx* ctx, int32_t set, uint32_t slot);
+typedef struct rb_adapters_desc {
+  int32_t dtype;        /* of x, y and out: RB_F32 or RB_F16 */
+  uint32_t n_rows;
+  const int32_t* slots; /* [n_rows]; -1, or a slot that is empty or beyond n_slots: no adapter (host memory: the
+                         * last two are RB_ERR_NOT_FOUND) */
+  const void* x;        /* [n_rows][ldx] of k elements */
+  const void* y;        /* [n_rows][ldy] of n elements */
+  void* out;            /* [n_rows][ldo]: y with what the adapters add; may be y itself (ldo == ldy) */
+  uint64_t ldx, ldy, ldo;
+} rb_adapters_desc;
+/* Rows in any order; those without an adapter are copied as they are, whatever their x
+ * holds. All sums are fp32, x and down x in fp32 (x of RB_F32 in 22 bits where a call's
+ * rows are many), the result is rounded once. out must not overlap x, nor y unless it is y.
+ * Returns n_rows. */
+int32_t rb_adapters_add(rb_ctx* ctx, int32_t set, const rb_adapters_desc* desc, uint32_t flags);
+
 /* The counter-based uniform draw in [0, 1) (a multiple of 2^-23) of (seed, counter):
  * SplitMix64 of seed + counter * 0x9E3779B97F4A7C15, top 23 bits. */
 float rb_sampling_uniform(uint64_t seed, uint64_t counter);

@@ -318,6 +318,10 @@ class Context:
                 max_seq=8192) -> "KVPool":
         return KVPool(self, n_layers, n_kv_heads, head_dim, kv_dtype, n_pages, max_tenants, max_seq)
 
+    def adapters(self, n: int, k: int, n_slots: int, max_rank: int) -> "AdapterSet":
+        """Low-rank adapters of many tenants beside a projection [n][k]."""
+        return AdapterSet(self, n, k, n_slots, max_rank)
+
 
 class Weight:
     """A [n][k] GGUF weight resident on the device in the tiled GEMV layout."""
@@ -330,12 +334,19 @@ class Weight:
         _check(_lib.rb_weight_upload(ctx.handle, dtype, n, k, _ptr(blocks), nbytes, _flags(ctx, blocks), C.byref(h)))
         self.handle = h.value
 
-    def matmul(self, x, batch_size: int, out=None):
+    def matmul(self, x, batch_size: int, out=None, adapters: Optional["AdapterSet"] = None, slots=None):
+        """x W^T; with `adapters` and every row's slot, what its adapter adds is in it (AdapterSet.add)."""
         x = _f32(x)
+        if adapters is not None and (adapters.n, adapters.k, adapters.ctx) != (self.n, self.k, self.ctx):
+            raise ValueError(f"adapters of a [{adapters.n}][{adapters.k}] projection of their context, weight [{self.n}][{self.k}]")
+        if (adapters is None) != (slots is None):
+            raise ValueError("adapters and slots go together")
         if out is None:
             out = np.empty((batch_size, self.n), np.float32)
         _check(_lib.rb_weight_matmul(self.ctx.handle, self.handle, _ptr(x), _ptr(out), batch_size,
                                      _flags(self.ctx, x, out)))
+        if adapters is not None:
+            adapters.add(x.reshape(batch_size, self.k), slots, out.reshape(batch_size, self.n))
         return out
 
     def matmul_noalloc(self, x, out, batch_size: int):
@@ -634,3 +645,6 @@ from .batching import (BatchedRequest, BatchStats, ContinuousBatcher, Scheduler,
 from .gguf import GGUFFile, TensorDesc  # noqa: E402
 from .sampling import LogitsProcessor, SamplingParams, sample_logits, sampling_uniform  # noqa: E402
 from .rows import RowPlan, SamplingFilter, pack_filters, rope_table, sample_filtered  # noqa: E402
+from .adapters import AdapterSet  # noqa: E402
+from .drafts import filter_probs, verify_drafts  # noqa: E402
+from .norms import residual_norm  # noqa: E402

@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import concurrent.futures as cf
 import os
+import re
 import subprocess
 import sys
 
@@ -14,8 +15,7 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "librealm_b200.so")
 SOURCES = ["gemv.cu", "attention.cu", "engine.cu", "sample.cu", "scheduler.cpp", "gguf.cpp", "rows_plan.cpp",
-           "rows_append.cu", "rows_attn.cu", "rows_tile.cu", "filter.cu"]
-HEADERS = ["common.cuh", "quant.cuh", "gemv.cuh", "attention.cuh", "xfrag.cuh", "sample.cuh", "rows.cuh", "filter.cuh"]
+           "rows_append.cu", "rows_attn.cu", "rows_tile.cu", "filter.cu", "adapters.cu", "verify.cu", "residual.cu"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo",
          "-Xcompiler", "-fPIC"]
@@ -25,16 +25,21 @@ def _mtime(p: str) -> float:
     return os.path.getmtime(p) if os.path.exists(p) else 0.0
 
 
-def _deps_mtime() -> float:
-    files = [os.path.join(CSRC, h) for h in HEADERS]
-    files.append(os.path.join(HERE, "..", "include", "realm_b200.h"))
-    return max(_mtime(f) for f in files)
+def _newest(path: str, seen: set) -> float:
+    """The newest modification time of a source and of what it includes."""
+    path = os.path.normpath(path)
+    if path in seen:
+        return 0.0
+    seen.add(path)
+    with open(path) as f:
+        names = re.findall(r'^\s*#include "([^"]+)"', f.read(), re.M)
+    return max([_mtime(path)] + [_newest(os.path.join(os.path.dirname(path), n), seen) for n in names])
 
 
 def _compile(src: str, force: bool) -> str:
     obj = os.path.join(BUILD, os.path.splitext(src)[0] + ".o")
     path = os.path.join(CSRC, src)
-    if force or _mtime(obj) < max(_mtime(path), _deps_mtime()):
+    if force or _mtime(obj) < _newest(path, set()):
         cmd = [NVCC, *FLAGS, "-c", path, "-o", obj]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:

@@ -1,0 +1,289 @@
+// Low-rank adapters beside a shared projection: out_r = y_r + scale_a up_a (down_a x_r) for
+// the row's adapter a.
+//
+// A cluster of CTAs has up to R rows that share an adapter. Its CTAs split k for
+// v = down x and then n for up v; in between each sends its part of v to all of them
+// (distributed shared memory), which add the parts in CTA order. So there is one launch, nothing
+// is kept in memory between the two products, and no result depends on an order of atomics.
+// fp32 throughout, the weights' fp16 values are exact in it.
+//
+// The rows of an adapter find one another in the kernel: cluster i of a block of kBlock
+// rows takes the block's i-th item, an item being the next R rows of one slot, counted from the
+// block's first row; clusters past the last item have nothing to do.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+#include "adapters.cuh"
+#include "common.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace rb {
+
+namespace {
+
+constexpr int kT = 256, kWarps = kT / 32;
+constexpr int kBlock = 64;        // rows among which an item's rows are found
+constexpr int kGroup = 4;         // ranks a warp works on at a time
+constexpr int kTileK = 1536;      // elements of x in shared memory at a time
+constexpr int kMaxCluster = 8;
+static_assert(kWarps * kGroup <= kAdapterMaxRank && kTileK % 8 == 0, "");
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+template <class T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+
+__device__ __forceinline__ void unpack8(uint4 q, float (&f)[8]) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = __half22float2(u32_as_h2(w[i]));
+    f[2 * i] = v.x;
+    f[2 * i + 1] = v.y;
+  }
+}
+
+// Sums of V values (a power of two up to 32) over the warp: lane l gets that of value l / (32 / V).
+template <int V>
+__device__ __forceinline__ float fold(float (&v)[V]) {
+  const int lane = threadIdx.x & 31;
+  int o = 16;
+#pragma unroll
+  for (int h = V / 2; h > 0; h >>= 1, o >>= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int i = 0; i < h; ++i) {
+      const float give = up ? v[i] : v[i + h], keep = up ? v[i + h] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+    }
+  }
+  for (; o > 0; o >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+  return v[0];
+}
+
+// The slot of a row, or -1 where it has no adapter.
+__device__ __forceinline__ int slot_of(const AdapterArgs& a, int row) {
+  const int s = a.slots[row];
+  return s >= 0 && s < a.w.n_slots && a.w.meta[s].rank > 0 ? s : -1;
+}
+
+template <class T, int R>
+__global__ void __launch_bounds__(kT) adapters_kernel(const __grid_constant__ AdapterArgs a) {
+  __shared__ __align__(16) float xs[R][kTileK];
+  __shared__ float part[kAdapterMaxRank * R];                        // [k part][rank][row]
+  __shared__ float parts[kMaxCluster][kAdapterMaxRank * R];          // every CTA's v
+  __shared__ __align__(16) float v[kAdapterMaxRank * R];             // [rank][row]
+  __shared__ int s_slot[kBlock], s_rows[R], s_n, s_item;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = (int)cluster.num_blocks(), c = (int)cluster.block_rank();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int id = blockIdx.x / C;
+  int slot, rows[R], nr = 1;
+  if (R == 1) {
+    rows[0] = id;
+    slot = slot_of(a, id);
+  } else {
+    const int b0 = id / kBlock * kBlock, nb = min(kBlock, a.n_rows - b0);
+    if (tid < nb) s_slot[tid] = slot_of(a, b0 + tid);
+    if (tid == 0) s_n = s_item = 0;
+    __syncthreads();
+    if (warp == 0) {
+      // rows b0 + lane and b0 + 32 + lane: which of its slot's rows is it; a row without an adapter is one by itself
+      int lead[2], nth[2];
+      unsigned before = 0;
+      int first = -1;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = h * 32 + lane, s = r < nb ? s_slot[r] : -2;
+        const unsigned same = __match_any_sync(0xffffffffu, s);
+        int rank = __popc(same & ((1u << lane) - 1));
+        if (h == 1)
+          for (int j = 0; j < 32; ++j) rank += s_slot[j] == s;
+        nth[h] = rank;
+        lead[h] = r < nb && (s < 0 || rank % R == 0);
+        const unsigned leads = __ballot_sync(0xffffffffu, lead[h]);
+        const int item = (int)before + __popc(leads & ((1u << lane) - 1));
+        if (lead[h] && item == id - b0) first = r;
+        before += __popc(leads);
+      }
+      const unsigned who = __ballot_sync(0xffffffffu, first >= 0);
+      if (who) {
+        const int src = __ffs(who) - 1;
+        first = __shfl_sync(0xffffffffu, first, src);
+        const int s = s_slot[first], n0 = __shfl_sync(0xffffffffu, first < 32 ? nth[0] : nth[1], src);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = h * 32 + lane;
+          const bool in = r < nb && (s < 0 ? r == first : s_slot[r] == s && nth[h] >= n0 && nth[h] < n0 + R);
+          if (in) {
+            s_rows[s < 0 ? 0 : nth[h] - n0] = b0 + r;
+            atomicAdd(&s_n, 1);
+          }
+        }
+      }
+    }
+    __syncthreads();
+    nr = s_n;
+    if (nr == 0) return;  // the whole cluster: no item is left for it
+    slot = s_slot[s_rows[0] - b0];
+#pragma unroll
+    for (int r = 0; r < R; ++r) rows[r] = s_rows[min(r, nr - 1)];
+  }
+  const T* x = reinterpret_cast<const T*>(a.x);
+  const T* y = reinterpret_cast<const T*>(a.y);
+  T* out = reinterpret_cast<T*>(a.out);
+  // this CTA's columns of out
+  const int n0 = (int)((int64_t)a.w.n * c / C), n1 = (int)((int64_t)a.w.n * (c + 1) / C);
+  if (slot < 0) {
+    if (a.out != a.y)
+      for (int j = n0 + tid; j < n1; j += kT) out[rows[0] * a.ldo + j] = y[rows[0] * a.ldy + j];
+    return;  // the whole cluster
+  }
+  cluster.barrier_arrive();
+  const int rank = a.w.meta[slot].rank;
+  const float scale = a.w.meta[slot].scale;
+  const int groups = (rank + kGroup - 1) / kGroup;
+  // warps are split over groups of ranks, and with few of those over k
+  const int ks = groups >= kWarps ? 1 : kWarps / groups, kpart = ks == 1 ? 0 : warp / groups;
+  const int chunks = a.w.kp / 8, c0 = (int)((int64_t)chunks * c / C), c1 = (int)((int64_t)chunks * (c + 1) / C);
+  const uint16_t* down = a.w.down + (int64_t)slot * a.w.rp * a.w.kp;
+  const int nv = groups * kGroup * R;  // of a k part; ks > 1: at most kWarps groups in all
+  for (int i = tid; i < ks * nv; i += kT) part[i] = 0.f;
+  for (int t0 = c0; t0 < c1; t0 += kTileK / 8) {
+    const int t1 = min(c1, t0 + kTileK / 8), len = (t1 - t0) * 8, k0 = t0 * 8;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      for (int j = tid; j < len; j += kT) xs[r][j] = r < nr && k0 + j < a.w.k ? to_f(x[rows[r] * a.ldx + k0 + j]) : 0.f;
+    __syncthreads();
+    if (kpart < ks) {
+      const int b0 = (t1 - t0) * kpart / ks, b1 = (t1 - t0) * (kpart + 1) / ks;
+      for (int g = ks == 1 ? warp : warp % groups; g < groups; g += ks == 1 ? kWarps : groups) {
+        float acc[kGroup * R];
+#pragma unroll
+        for (int i = 0; i < kGroup * R; ++i) acc[i] = 0.f;
+        const uint16_t* w = down + (int64_t)(g * kGroup) * a.w.kp + k0;  // rows up to rp, a multiple of 8, exist
+        for (int b = b0 + lane; b < b1; b += 32) {
+          uint4 q[kGroup];
+#pragma unroll
+          for (int i = 0; i < kGroup; ++i) q[i] = __ldg(reinterpret_cast<const uint4*>(w + (int64_t)i * a.w.kp + b * 8));
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const float4 lo = *reinterpret_cast<const float4*>(&xs[r][b * 8]),
+                         hi = *reinterpret_cast<const float4*>(&xs[r][b * 8 + 4]);
+            const float xv[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+            for (int i = 0; i < kGroup; ++i) {
+              float f[8];
+              unpack8(q[i], f);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) acc[i * R + r] = fmaf(f[e], xv[e], acc[i * R + r]);
+            }
+          }
+        }
+        const float sum = fold<kGroup * R>(acc);
+        constexpr int per = 32 / (kGroup * R);
+        if (lane % per == 0) part[kpart * nv + g * kGroup * R + lane / per] += sum;
+      }
+    }
+  }
+  __syncthreads();
+  cluster.barrier_wait();  // every CTA of the cluster runs before its shared memory is written
+  for (int i = tid; i < nv; i += kT) {
+    float s = 0.f;
+    for (int p = 0; p < ks; ++p) s += part[p * nv + i];
+    for (int d = 0; d < C; ++d) *cluster.map_shared_rank(&parts[c][i], d) = s;
+  }
+  cluster.sync();
+  for (int i = tid; i < (rank + 7) / 8 * 8 * R; i += kT) {
+    float s = 0.f;
+    if (i < nv)
+      for (int d = 0; d < C; ++d) s += parts[d][i];
+    v[i] = s;
+  }
+  __syncthreads();
+  const uint16_t* up = a.w.up + (int64_t)slot * a.w.rp * a.w.n;
+  for (int j = n0 + tid; j < n1; j += kT) {
+    float acc[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) acc[r] = 0.f;
+    for (int h = 0; h < (rank + 7) / 8; ++h) {
+      float f[8];
+      unpack8(__ldg(reinterpret_cast<const uint4*>(up + ((int64_t)h * a.w.n + j) * 8)), f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int r = 0; r < R; ++r) acc[r] = fmaf(f[e], v[(h * 8 + e) * R + r], acc[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (r < nr) out[rows[r] * a.ldo + j] = from_f<T>(fmaf(scale, acc[r], to_f(y[rows[r] * a.ldy + j])));
+  }
+}
+
+template <class T, int R>
+cudaError_t launch(const AdapterArgs& a, int cluster, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)a.n_rows * cluster);
+  cfg.blockDim = dim3(kT);
+  cfg.stream = s;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)cluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, adapters_kernel<T, R>, a);
+}
+
+template <class S>
+__global__ void adapters_set_kernel(const __grid_constant__ AdapterSetArgs a) {
+  const S *sd = reinterpret_cast<const S*>(a.src_down), *su = reinterpret_cast<const S*>(a.src_up);
+  const int64_t nd = (int64_t)a.rp * a.kp, nu = (int64_t)a.rp * a.n;
+  const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, step = (int64_t)gridDim.x * blockDim.x;
+  for (int64_t i = at; i < nd; i += step) {
+    const int r = (int)(i / a.kp), j = (int)(i % a.kp);
+    a.down[i] = r < a.rank && j < a.k ? __half_as_ushort(from_f<__half>(to_f(sd[(int64_t)r * a.k + j]))) : 0;
+  }
+  for (int64_t i = at; i < nu; i += step) {  // [rank / 8][n][8]
+    const int64_t v = i / 8;
+    const int r = (int)(v / a.n) * 8 + (int)(i % 8), j = (int)(v % a.n);
+    a.up[i] = r < a.rank ? __half_as_ushort(from_f<__half>(to_f(su[(int64_t)j * a.rank + r]))) : 0;
+  }
+  if (at == 0) *a.meta = AdapterMeta{a.rank, a.scale};
+}
+
+__global__ void adapters_clear_kernel(AdapterMeta* meta) { *meta = AdapterMeta{0, 0.f}; }
+
+}  // namespace
+
+cudaError_t adapters_set_launch(const AdapterSetArgs& a, cudaStream_t s) {
+  const int64_t most = (int64_t)a.rp * std::max(a.kp, a.n);
+  const int blocks = (int)std::min<int64_t>(1184, (most + 255) / 256);
+  if (a.in16) adapters_set_kernel<__half><<<blocks, 256, 0, s>>>(a);
+  else adapters_set_kernel<float><<<blocks, 256, 0, s>>>(a);
+  return cudaGetLastError();
+}
+
+cudaError_t adapters_clear_launch(AdapterMeta* meta, cudaStream_t s) {
+  adapters_clear_kernel<<<1, 1, 0, s>>>(meta);
+  return cudaGetLastError();
+}
+
+cudaError_t adapters_launch(const AdapterArgs& a, int num_sms, cudaStream_t s) {
+  const int cluster = 8;
+  if (a.n_rows <= 16) return a.x16 ? launch<__half, 1>(a, cluster, s) : launch<float, 1>(a, cluster, s);
+  return a.x16 ? launch<__half, 4>(a, cluster, s) : launch<float, 4>(a, cluster, s);
+}
+
+}  // namespace rb

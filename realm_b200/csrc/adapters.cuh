@@ -1,0 +1,50 @@
+// Low-rank adapters of many tenants beside one projection (adapters.cu).
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace rb {
+
+constexpr int kAdapterMaxRank = 128;
+constexpr int kAdapterMaxSlots = 4096;
+constexpr int kAdapterMaxDim = 1 << 20;  // of k and n
+
+struct AdapterMeta {
+  int32_t rank;  // 0: the slot is empty
+  float scale;
+};
+
+// Adapters of one projection [n][k], in slots of equal size:
+//   down  [n_slots][rp][kp] fp16, zeros past the rank and past k
+//   up    [n_slots][rp / 8][n][8] fp16, zeros past the rank
+// rp, kp: max_rank and k rounded up to a multiple of 8.
+struct AdapterView {
+  const uint16_t *down = nullptr, *up = nullptr;
+  const AdapterMeta* meta = nullptr;
+  int32_t n = 0, k = 0, kp = 0, rp = 0, n_slots = 0;
+};
+
+struct AdapterArgs {
+  AdapterView w;
+  const void *x = nullptr, *y = nullptr;
+  void* out = nullptr;
+  int64_t ldx = 0, ldy = 0, ldo = 0;
+  int32_t x16 = 0;  // x, y and out are fp16, else fp32
+  int32_t n_rows = 0;
+  const int32_t* slots = nullptr;
+  uint32_t* err = nullptr;
+};
+
+struct AdapterSetArgs {
+  uint16_t *down = nullptr, *up = nullptr;  // of the slot
+  AdapterMeta* meta = nullptr;              // of the slot
+  int32_t n = 0, k = 0, kp = 0, rp = 0, rank = 0, in16 = 0;
+  float scale = 0.f;
+  const void *src_down = nullptr, *src_up = nullptr;  // [rank][k], [n][rank]
+};
+
+cudaError_t adapters_set_launch(const AdapterSetArgs& a, cudaStream_t s);
+cudaError_t adapters_clear_launch(AdapterMeta* meta, cudaStream_t s);
+cudaError_t adapters_launch(const AdapterArgs& a, int num_sms, cudaStream_t s);
+
+}  // namespace rb

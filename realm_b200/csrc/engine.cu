@@ -17,13 +17,16 @@
 #include <vector>
 
 #include "../../include/realm_b200.h"
+#include "adapters.cuh"
 #include "attention.cuh"
 #include "common.cuh"
 #include "filter.cuh"
 #include "gemv.cuh"
 #include "quant.cuh"
+#include "residual.cuh"
 #include "rows.cuh"
 #include "sample.cuh"
+#include "verify.cuh"
 #include "xfrag.cuh"
 
 namespace rb {
@@ -288,6 +291,13 @@ struct RowSet {
   DevBuf rows, small, warps, tile, spans, joins, part_o, part_ml;
 };
 
+// The adapters of one projection (rb_adapters_create).
+struct AdapterSet {
+  int n = 0, k = 0, kp = 0, max_rank = 0, rp = 0, n_slots = 0;
+  DevBuf down, up, meta;
+  std::vector<int> rank;  // by slot; 0: empty
+};
+
 struct Ctx {
   int device = 0, num_sms = 148, max_rows = 64;
   bool pdl = true, graphs = true;
@@ -306,6 +316,8 @@ struct Ctx {
   std::vector<std::unique_ptr<Model>> models;
   std::map<int, std::unique_ptr<RowSet>> plans;  // by handle; no handle is given out twice
   int next_plan = 0;
+  std::map<int, std::unique_ptr<AdapterSet>> adapters;  // the same
+  int next_adapters = 0;
   // RowAttnArgs::hold. Made with the first fp16 pool of a caller's, or the first plan with tile units over a
   // model's: a model's decode steps take 0.5 % longer when it lies between the memory of the model.
   DevBuf tile_hold, tile_busy;
@@ -2379,13 +2391,13 @@ int32_t plan_create(rb_ctx* c, int32_t pool, const rb_plan_desc* d, int32_t* pla
   return RB_OK;
 }
 
-int32_t sample_filtered(rb_ctx* c, int32_t dtype, const void* logits, uint64_t ld, uint32_t n_rows, uint32_t vocab,
-                        const rb_sampling_filter* params, const uint32_t* prev, const uint32_t* prev_off,
-                        const float* uniforms, uint32_t* out, float* probs, uint32_t flags) {
-  if (!c) return fail(RB_ERR_BAD_HANDLE, "null context");
-  if (int rc = row_dtype(dtype)) return rc;
-  if (n_rows == 0) return 0;  // an empty batch has no memory
-  if (!logits || !params || !uniforms || !out) return fail(RB_ERR_INVALID, "logits/params/uniforms/out NULL");
+// What filtered sampling and its distribution have in common: arguments checked and staged.
+struct FilterStaged {
+  Staged logits, params, prev, prev_off;
+};
+int stage_filter(Ctx* c, int32_t dtype, const void* logits, uint64_t ld, uint32_t n_rows, uint32_t vocab,
+                 const rb_sampling_filter* params, const uint32_t* prev, const uint32_t* prev_off, uint32_t flags,
+                 FilterStaged& st, FilterArgs& a) {
   const bool dev = flags & RB_PTR_DEVICE;
   if (!dev && !prev && prev_off && n_rows && prev_off[n_rows] == 0) prev_off = nullptr;  // no row has a history
   if ((prev == nullptr) != (prev_off == nullptr)) return fail(RB_ERR_INVALID, "prev_tokens and prev_offsets go together");
@@ -2398,26 +2410,39 @@ int32_t sample_filtered(rb_ctx* c, int32_t dtype, const void* logits, uint64_t l
       if (prev_off[r] > prev_off[r + 1]) return fail(RB_ERR_INVALID, "row %u: prev_offsets fall", r);
   RB_CUDA(cudaSetDevice(c->device));
   const size_t esz = dtype == RB_F16 ? 2 : 4;
-  Staged sl, sp, sprev, soff, su;
-  if (int rc = stage_rows(c, "logits", logits, ld, n_rows, vocab, esz, flags, sl)) return rc;
-  if (int rc = stage_words(c, "params", params, (size_t)n_rows * (sizeof(rb_sampling_filter) / 4), flags, sp)) return rc;
+  if (int rc = stage_rows(c, "logits", logits, ld, n_rows, vocab, esz, flags, st.logits)) return rc;
+  if (int rc = stage_words(c, "params", params, (size_t)n_rows * (sizeof(rb_sampling_filter) / 4), flags, st.params)) return rc;
   if (prev_off) {
-    if (int rc = stage_words(c, "prev_offsets", prev_off, (size_t)n_rows + 1, flags, soff)) return rc;
-    if (int rc = stage_words(c, "prev_tokens", prev, dev ? 0 : prev_off[n_rows], flags, sprev)) return rc;
+    if (int rc = stage_words(c, "prev_offsets", prev_off, (size_t)n_rows + 1, flags, st.prev_off)) return rc;
+    if (int rc = stage_words(c, "prev_tokens", prev, dev ? 0 : prev_off[n_rows], flags, st.prev)) return rc;
   }
-  if (int rc = stage_words(c, "uniforms", uniforms, n_rows, flags, su)) return rc;
-  if (dev && ((uintptr_t)out % 4 || (uintptr_t)probs % 4))
-    return fail(RB_ERR_INVALID, "out_tokens or probs is not aligned to 4 bytes");
-  DevBuf dout;
-  FilterArgs a;
-  a.logits = sl.dptr;
+  a.logits = st.logits.dptr;
   a.ld = (int64_t)ld;
   a.x16 = dtype == RB_F16;
   a.n_rows = (int)n_rows;
   a.vocab = (int)vocab;
-  a.params = (const rb_sampling_filter*)sp.dptr;
-  a.prev = (const uint32_t*)sprev.dptr;
-  a.prev_off = prev_off ? (const uint32_t*)soff.dptr : nullptr;
+  a.params = (const rb_sampling_filter*)st.params.dptr;
+  a.prev = (const uint32_t*)st.prev.dptr;
+  a.prev_off = prev_off ? (const uint32_t*)st.prev_off.dptr : nullptr;
+  return RB_OK;
+}
+
+int32_t sample_filtered(rb_ctx* c, int32_t dtype, const void* logits, uint64_t ld, uint32_t n_rows, uint32_t vocab,
+                        const rb_sampling_filter* params, const uint32_t* prev, const uint32_t* prev_off,
+                        const float* uniforms, uint32_t* out, float* probs, uint32_t flags) {
+  if (!c) return fail(RB_ERR_BAD_HANDLE, "null context");
+  if (int rc = row_dtype(dtype)) return rc;
+  if (n_rows == 0) return 0;  // an empty batch has no memory
+  if (!logits || !params || !uniforms || !out) return fail(RB_ERR_INVALID, "logits/params/uniforms/out NULL");
+  const bool dev = flags & RB_PTR_DEVICE;
+  FilterStaged st;
+  FilterArgs a;
+  if (int rc = stage_filter(c, dtype, logits, ld, n_rows, vocab, params, prev, prev_off, flags, st, a)) return rc;
+  Staged su;
+  if (int rc = stage_words(c, "uniforms", uniforms, n_rows, flags, su)) return rc;
+  if (dev && ((uintptr_t)out % 4 || (uintptr_t)probs % 4))
+    return fail(RB_ERR_INVALID, "out_tokens or probs is not aligned to 4 bytes");
+  DevBuf dout;
   a.uniforms = (const float*)su.dptr;
   a.tokens = out;
   a.probs = probs;
@@ -2437,6 +2462,320 @@ int32_t sample_filtered(rb_ctx* c, int32_t dtype, const void* logits, uint64_t l
   if (!dev) std::copy(h.begin(), h.end(), out);
   return (int32_t)n_rows;
 }
+// Whether two sets of n rows (`w` bytes wide, `ld` bytes apart) share a byte. Rows of one buffer that lie
+// side by side do not; those with unlike distances count as sharing where their ranges meet.
+bool rows_meet(const void* p, uint64_t ld, uint64_t w, const void* q, uint64_t ld2, uint64_t w2, uint64_t n) {
+  if (!p || !q || n == 0) return false;
+  const uint64_t a = (uint64_t)(uintptr_t)p, b = (uint64_t)(uintptr_t)q;
+  const uint64_t ea = a + (n - 1) * ld + w, eb = b + (n - 1) * ld2 + w2;
+  if (ea <= b || eb <= a) return false;
+  if (n == 1 || ld != ld2) return true;
+  const uint64_t off = a <= b ? (b - a) % ld : (ld - (a - b) % ld) % ld;  // of q's rows within p's
+  return off < w || ld - off < w2;
+}
+
+int32_t filter_probs(rb_ctx* c, int32_t dtype, const void* logits, uint64_t ld, uint32_t n_rows, uint32_t vocab,
+                     const rb_sampling_filter* params, const uint32_t* prev, const uint32_t* prev_off, float* probs,
+                     uint64_t ldp, uint32_t flags) {
+  if (!c) return fail(RB_ERR_BAD_HANDLE, "null context");
+  if (int rc = row_dtype(dtype)) return rc;
+  if (n_rows == 0) return 0;  // an empty batch has no memory
+  if (!logits || !params || !probs) return fail(RB_ERR_INVALID, "logits/params/probs NULL");
+  const bool dev = flags & RB_PTR_DEVICE;
+  FilterStaged st;
+  FilterArgs a;
+  if (int rc = stage_filter(c, dtype, logits, ld, n_rows, vocab, params, prev, prev_off, flags, st, a)) return rc;
+  const size_t esz = dtype == RB_F16 ? 2 : 4;
+  if (rows_meet(logits, ld * esz, vocab * esz, probs, ldp * 4, (uint64_t)vocab * 4, n_rows))
+    return fail(RB_ERR_INVALID, "probs overlaps logits");
+  Staged sp;  // host: a buffer of the same shape, whose gaps between rows go back as they came
+  if (int rc = stage_rows(c, "probs", probs, ldp, n_rows, vocab, 4, flags, sp)) return rc;
+  a.dist = (float*)const_cast<void*>(sp.dptr);
+  a.ldd = (int64_t)ldp;
+  RB_CUDA(filter_launch(a, c->num_sms, c->stream));
+  if (dev && (flags & RB_ASYNC)) return (int32_t)n_rows;
+  if (!dev)
+    RB_CUDA(cudaMemcpy2DAsync(probs, ldp * 4, a.dist, ldp * 4, (size_t)vocab * 4, n_rows, cudaMemcpyDeviceToHost, c->stream));
+  if (int rc = sync_ctx(c)) return rc;
+  return (int32_t)n_rows;
+}
+
+int32_t verify_drafts(rb_ctx* c, const rb_verify_desc* d, uint32_t flags) {
+  if (!c) return fail(RB_ERR_BAD_HANDLE, "null context");
+  if (!d) return fail(RB_ERR_INVALID, "null descriptor");
+  if (d->n_requests == 0) return 0;
+  if (d->n_requests > (1u << 24) || d->n_rows > (1u << 24))
+    return fail(RB_ERR_INVALID, "n_requests %u or n_rows %u > 2^24", d->n_requests, d->n_rows);
+  if (!d->offsets || !d->accepted) return fail(RB_ERR_INVALID, "offsets/accepted NULL");
+  if (d->n_rows && (!d->probs || !d->drafts || !d->uniforms || !d->tokens))
+    return fail(RB_ERR_INVALID, "probs/drafts/uniforms/tokens NULL");
+  if (d->vocab == 0 || d->vocab > (uint32_t)kFilterMaxVocab)
+    return fail(RB_ERR_UNSUPPORTED, "vocab %u not in [1, %d]", d->vocab, kFilterMaxVocab);
+  const bool dev = flags & RB_PTR_DEVICE;
+  const uint32_t n = d->n_rows, m = d->n_requests;
+  if (!dev)
+    for (uint32_t r = 0; r < m; ++r)
+      if (d->offsets[r] > d->offsets[r + 1] || d->offsets[r + 1] > n)
+        return fail(RB_ERR_INVALID, "request %u: rows [%u, %u) of %u", r, d->offsets[r], d->offsets[r + 1], n);
+  RB_CUDA(cudaSetDevice(c->device));
+  Staged so, sp, sq, sd, su, st;
+  VerifyArgs a;
+  if (int rc = stage_words(c, "offsets", d->offsets, (size_t)m + 1, flags, so)) return rc;
+  if (n) {
+    if (int rc = stage_rows(c, "probs", d->probs, d->ldp, n, d->vocab, 4, flags, sp)) return rc;
+    if (d->draft_probs)
+      if (int rc = stage_rows(c, "draft_probs", d->draft_probs, d->ldq, n, d->vocab, 4, flags, sq)) return rc;
+    if (int rc = stage_words(c, "drafts", d->drafts, n, flags, sd)) return rc;
+    if (int rc = stage_words(c, "uniforms", d->uniforms, n, flags, su)) return rc;
+    if (int rc = stage_words(c, "tokens", d->tokens, n, flags, st)) return rc;
+  }
+  if (dev && (uintptr_t)d->accepted % 4) return fail(RB_ERR_INVALID, "accepted is not aligned to 4 bytes");
+  auto meets = [&](const void* p, uint64_t w, const void* q, uint64_t w2) {
+    return rows_meet(p, w * 4, w * 4, q, w2 * 4, w2 * 4, 1);
+  };
+  const uint64_t np = n ? (n - 1) * d->ldp + d->vocab : 0, nq = n ? (n - 1) * d->ldq + d->vocab : 0;
+  if ((d->tokens != d->drafts && meets(d->tokens, n, d->drafts, n)) || meets(d->tokens, n, d->uniforms, n) ||
+      meets(d->tokens, n, d->offsets, (uint64_t)m + 1) || meets(d->tokens, n, d->probs, np) ||
+      meets(d->tokens, n, d->draft_probs, nq) || meets(d->tokens, n, d->accepted, m) || meets(d->accepted, m, d->drafts, n) ||
+      meets(d->accepted, m, d->uniforms, n) || meets(d->accepted, m, d->offsets, (uint64_t)m + 1) ||
+      meets(d->accepted, m, d->probs, np) || meets(d->accepted, m, d->draft_probs, nq))
+    return fail(RB_ERR_INVALID, "tokens or accepted overlaps an input, or one another");
+  DevBuf dacc;
+  a.n_requests = (int)m;
+  a.n_rows = (int)n;
+  a.vocab = (int)d->vocab;
+  a.offsets = (const uint32_t*)so.dptr;
+  a.probs = (const float*)sp.dptr;
+  a.draft_probs = (const float*)sq.dptr;
+  a.ldp = (int64_t)d->ldp;
+  a.ldq = (int64_t)d->ldq;
+  a.drafts = (const uint32_t*)sd.dptr;
+  a.uniforms = (const float*)su.dptr;
+  a.tokens = (uint32_t*)const_cast<void*>(st.dptr);
+  a.accepted = d->accepted;
+  if (!dev) {
+    RB_CUDA(dacc.alloc((size_t)m * 4));
+    a.accepted = dacc.as<int32_t>();
+  }
+  RB_CUDA(verify_launch(a, c->num_sms, c->stream));
+  if (dev && (flags & RB_ASYNC)) return (int32_t)m;
+  std::vector<uint32_t> tok(n), off(m + 1);
+  std::vector<int32_t> acc(m);
+  if (n) RB_CUDA(cudaMemcpyAsync(tok.data(), a.tokens, (size_t)n * 4, cudaMemcpyDeviceToHost, c->stream));
+  RB_CUDA(cudaMemcpyAsync(acc.data(), a.accepted, (size_t)m * 4, cudaMemcpyDeviceToHost, c->stream));
+  RB_CUDA(cudaMemcpyAsync(off.data(), a.offsets, ((size_t)m + 1) * 4, cudaMemcpyDeviceToHost, c->stream));
+  if (int rc = sync_ctx(c)) return rc;
+  for (uint32_t r = 0; r < m; ++r) {
+    if (acc[r] < 0) return fail(RB_ERR_INVALID, "request %u: rows [%u, %u) of %u", r, off[r], off[r + 1], n);
+    if (off[r] < off[r + 1] && tok[off[r] + acc[r]] == 0xffffffffu)
+      return fail(RB_ERR_INVALID, "request %u: Failed to create weighted index", r);
+  }
+  if (!dev) {
+    std::copy(tok.begin(), tok.end(), d->tokens);
+    std::copy(acc.begin(), acc.end(), d->accepted);
+  }
+  return (int32_t)m;
+}
+
+int32_t residual_norm(rb_ctx* c, const rb_residual_desc* d, uint32_t flags) {
+  if (!c) return fail(RB_ERR_BAD_HANDLE, "null context");
+  if (!d) return fail(RB_ERR_INVALID, "null descriptor");
+  if (int rc = row_dtype(d->dtype)) return rc;
+  if (int rc = row_dtype(d->x_dtype)) return rc;
+  if (d->n_rows == 0) return 0;
+  if (d->n_rows > (1u << 24)) return fail(RB_ERR_INVALID, "n_rows %u > 2^24", d->n_rows);
+  if (d->dim == 0 || d->dim > (uint32_t)kResidualMaxDim)
+    return fail(RB_ERR_UNSUPPORTED, "dim %u not in [1, %d]", d->dim, kResidualMaxDim);
+  if ((d->out == nullptr) != (d->pre_norm == nullptr)) return fail(RB_ERR_INVALID, "out and pre_norm go together");
+  if (!std::isfinite(d->scale) || !(d->eps >= 0.f) || !std::isfinite(d->eps))
+    return fail(RB_ERR_INVALID, "scale %g, eps %g", d->scale, d->eps);
+  RB_CUDA(cudaSetDevice(c->device));
+  const bool dev = flags & RB_PTR_DEVICE;
+  const size_t ey = d->dtype == RB_F16 ? 2 : 4, ex = d->x_dtype == RB_F16 ? 2 : 4, n = d->n_rows, w = d->dim;
+  Staged sy, sx, sg, sxo, so, s1, s2;
+  if (int rc = stage_rows(c, "y", d->y, d->ldy, n, w, ey, flags, sy)) return rc;
+  if (int rc = stage_rows(c, "x", d->x, d->ldx, n, w, ex, flags, sx)) return rc;
+  if (int rc = stage_rows(c, "x_out", d->x_out, d->ldxo, n, w, ex, flags, sxo)) return rc;
+  if (d->gate)
+    if (int rc = d->ldg ? stage_rows(c, "gate", d->gate, d->ldg, n, w, ey, flags, sg)
+                        : stage_rows(c, "gate", d->gate, w, 1, w, ey, flags, sg))
+      return rc;
+  if (d->out)
+    if (int rc = stage_rows(c, "out", d->out, d->ldo, n, w, ey, flags, so)) return rc;
+  if (d->post_norm)
+    if (int rc = stage_words(c, "post_norm", d->post_norm, w, flags, s1)) return rc;
+  if (d->pre_norm)
+    if (int rc = stage_words(c, "pre_norm", d->pre_norm, w, flags, s2)) return rc;
+  // each row's outputs are written after all its inputs have been read only where they are those inputs
+  struct Part {
+    const void* p;
+    uint64_t ld, w, rows;
+  };
+  const Part y{d->y, d->ldy * ey, w * ey, n}, x{d->x, d->ldx * ex, w * ex, n}, xo{d->x_out, d->ldxo * ex, w * ex, n},
+      o{d->out, d->ldo * ey, w * ey, n}, g{d->gate, (d->ldg ? d->ldg : w) * ey, w * ey, d->ldg ? n : 1},
+      p1{d->post_norm, w * 4, w * 4, 1}, p2{d->pre_norm, w * 4, w * 4, 1};
+  auto meet = [](const Part& a, const Part& b) {
+    if (a.rows == b.rows) return rows_meet(a.p, a.ld, a.w, b.p, b.ld, b.w, a.rows);
+    return rows_meet(a.p, 1, (a.rows - 1) * a.ld + a.w, b.p, 1, (b.rows - 1) * b.ld + b.w, 1);
+  };
+  const bool x_same = d->x_out == d->x && d->ldxo == d->ldx, y_same = d->out == d->y && d->ldo == d->ldy;
+  if ((!x_same && meet(xo, x)) || (!y_same && meet(o, y)) || meet(xo, y) || meet(xo, g) || meet(xo, p1) ||
+      meet(xo, p2) || meet(xo, o) || meet(o, x) || meet(o, g) || meet(o, p1) || meet(o, p2))
+    return fail(RB_ERR_INVALID, "x_out or out overlaps an input, or one another");
+  ResidualArgs a;
+  a.y = sy.dptr;
+  a.x = sx.dptr;
+  a.gate = sg.dptr;
+  a.x_out = const_cast<void*>(sxo.dptr);
+  a.out = const_cast<void*>(so.dptr);
+  a.ldy = (int64_t)d->ldy;
+  a.ldx = (int64_t)d->ldx;
+  a.ldg = (int64_t)d->ldg;
+  a.ldxo = (int64_t)d->ldxo;
+  a.ldo = (int64_t)d->ldo;
+  a.y16 = d->dtype == RB_F16;
+  a.x16 = d->x_dtype == RB_F16;
+  a.n_rows = (int)n;
+  a.dim = (int)w;
+  a.post = (const float*)s1.dptr;
+  a.pre = (const float*)s2.dptr;
+  a.scale = d->scale;
+  a.eps = d->eps;
+  RB_CUDA(residual_launch(a, c->num_sms, c->stream));
+  if (dev && (flags & RB_ASYNC)) return (int32_t)n;
+  if (!dev) {
+    RB_CUDA(cudaMemcpy2DAsync(d->x_out, d->ldxo * ex, a.x_out, d->ldxo * ex, w * ex, n, cudaMemcpyDeviceToHost, c->stream));
+    if (d->out)
+      RB_CUDA(cudaMemcpy2DAsync(d->out, d->ldo * ey, a.out, d->ldo * ey, w * ey, n, cudaMemcpyDeviceToHost, c->stream));
+  }
+  if (int rc = sync_ctx(c)) return rc;
+  return (int32_t)n;
+}
+
+AdapterSet* get_adapters(rb_ctx* c, int32_t set) {
+  if (!c) return nullptr;
+  auto it = c->adapters.find(set);
+  return it == c->adapters.end() ? nullptr : it->second.get();
+}
+
+int32_t adapters_create(rb_ctx* c, uint32_t n, uint32_t k, uint32_t n_slots, uint32_t max_rank, int32_t* set) {
+  if (!c || !set) return fail(RB_ERR_BAD_HANDLE, "null context/handle");
+  if (n == 0 || k == 0 || n > (uint32_t)kAdapterMaxDim || k > (uint32_t)kAdapterMaxDim)
+    return fail(RB_ERR_UNSUPPORTED, "projection [%u][%u]: sizes up to %d", n, k, kAdapterMaxDim);
+  if (n_slots == 0 || n_slots > (uint32_t)kAdapterMaxSlots)
+    return fail(RB_ERR_UNSUPPORTED, "n_slots %u not in [1, %d]", n_slots, kAdapterMaxSlots);
+  if (max_rank == 0 || max_rank > (uint32_t)kAdapterMaxRank)
+    return fail(RB_ERR_UNSUPPORTED, "max_rank %u not in [1, %d]", max_rank, kAdapterMaxRank);
+  if (c->next_adapters == INT32_MAX) return fail(RB_ERR_UNSUPPORTED, "no handle left");
+  RB_CUDA(cudaSetDevice(c->device));
+  auto S = std::make_unique<AdapterSet>();
+  S->n = (int)n;
+  S->k = (int)k;
+  S->kp = (int)(k + 7) / 8 * 8;
+  S->max_rank = (int)max_rank;
+  S->rp = (int)(max_rank + 7) / 8 * 8;
+  S->n_slots = (int)n_slots;
+  S->rank.assign(n_slots, 0);
+  const size_t per = (size_t)n_slots * S->rp * 2;
+  if (S->down.alloc(per * S->kp) != cudaSuccess || S->up.alloc(per * n) != cudaSuccess ||
+      S->meta.alloc((size_t)n_slots * sizeof(AdapterMeta)) != cudaSuccess) {
+    cudaGetLastError();
+    return fail(RB_ERR_OOM, "%u adapters of rank %u: %zu bytes", n_slots, max_rank, per * (S->kp + n));
+  }
+  RB_CUDA(cudaMemsetAsync(S->meta.p, 0, S->meta.n, c->stream));
+  c->adapters[c->next_adapters] = std::move(S);
+  *set = c->next_adapters++;
+  return RB_OK;
+}
+
+int32_t adapters_set(rb_ctx* c, int32_t set, uint32_t slot, int32_t dtype, uint32_t rank, const void* down,
+                     const void* up, float scale, uint32_t flags) {
+  AdapterSet* S = get_adapters(c, set);
+  if (!S) return fail(RB_ERR_BAD_HANDLE, "adapters %d", set);
+  if (int rc = row_dtype(dtype)) return rc;
+  if (slot >= (uint32_t)S->n_slots) return fail(RB_ERR_NOT_FOUND, "slot %u of %d", slot, S->n_slots);
+  if (rank == 0 || rank > (uint32_t)S->max_rank) return fail(RB_ERR_UNSUPPORTED, "rank %u not in [1, %d]", rank, S->max_rank);
+  if (!std::isfinite(scale)) return fail(RB_ERR_INVALID, "scale %g", scale);
+  RB_CUDA(cudaSetDevice(c->device));
+  const size_t esz = dtype == RB_F16 ? 2 : 4;
+  Staged sd, su;
+  if (int rc = stage_rows(c, "down", down, S->k, rank, S->k, esz, flags, sd)) return rc;
+  if (int rc = stage_rows(c, "up", up, rank, S->n, rank, esz, flags, su)) return rc;
+  AdapterSetArgs a;
+  a.down = S->down.as<uint16_t>() + (size_t)slot * S->rp * S->kp;
+  a.up = S->up.as<uint16_t>() + (size_t)slot * S->rp * S->n;
+  a.meta = S->meta.as<AdapterMeta>() + slot;
+  a.n = S->n;
+  a.k = S->k;
+  a.kp = S->kp;
+  a.rp = S->rp;
+  a.rank = (int)rank;
+  a.in16 = dtype == RB_F16;
+  a.scale = scale;
+  a.src_down = sd.dptr;
+  a.src_up = su.dptr;
+  RB_CUDA(adapters_set_launch(a, c->stream));
+  S->rank[slot] = (int)rank;
+  if (!((flags & RB_PTR_DEVICE) && (flags & RB_ASYNC)))
+    if (int rc = sync_ctx(c)) return rc;
+  return (int32_t)rank;
+}
+
+int32_t adapters_add(rb_ctx* c, int32_t set, const rb_adapters_desc* d, uint32_t flags) {
+  AdapterSet* S = get_adapters(c, set);
+  if (!S) return fail(RB_ERR_BAD_HANDLE, "adapters %d", set);
+  if (!d) return fail(RB_ERR_INVALID, "null descriptor");
+  if (int rc = row_dtype(d->dtype)) return rc;
+  if (d->n_rows == 0) return 0;
+  if (d->n_rows > (1u << 24)) return fail(RB_ERR_INVALID, "n_rows %u > 2^24", d->n_rows);
+  if (!d->slots) return fail(RB_ERR_INVALID, "slots NULL");
+  const bool dev = flags & RB_PTR_DEVICE;
+  if (!dev)
+    for (uint32_t r = 0; r < d->n_rows; ++r) {
+      const int s = d->slots[r];
+      if (s != -1 && (s < 0 || s >= S->n_slots || S->rank[s] == 0))
+        return fail(RB_ERR_NOT_FOUND, "row %u: no adapter in slot %d", r, s);
+    }
+  RB_CUDA(cudaSetDevice(c->device));
+  const size_t esz = d->dtype == RB_F16 ? 2 : 4, n = d->n_rows;
+  Staged ss, sx, sy, so;
+  if (int rc = stage_words(c, "slots", d->slots, n, flags, ss)) return rc;
+  if (int rc = stage_rows(c, "x", d->x, d->ldx, n, S->k, esz, flags, sx)) return rc;
+  if (int rc = stage_rows(c, "y", d->y, d->ldy, n, S->n, esz, flags, sy)) return rc;
+  const bool in_place = d->out == d->y && d->ldo == d->ldy;
+  if (!in_place || dev)
+    if (int rc = stage_rows(c, "out", d->out, d->ldo, n, S->n, esz, flags, so)) return rc;
+  if (rows_meet(d->out, d->ldo * esz, S->n * esz, d->x, d->ldx * esz, S->k * esz, n) ||
+      (!in_place && rows_meet(d->out, d->ldo * esz, S->n * esz, d->y, d->ldy * esz, S->n * esz, n)) ||
+      rows_meet(d->out, 1, ((n - 1) * d->ldo + S->n) * esz, d->slots, 1, n * 4, 1))
+    return fail(RB_ERR_INVALID, "out overlaps x, slots, or y without being y");
+  AdapterArgs a;
+  a.w.down = S->down.as<uint16_t>();
+  a.w.up = S->up.as<uint16_t>();
+  a.w.meta = S->meta.as<AdapterMeta>();
+  a.w.n = S->n;
+  a.w.k = S->k;
+  a.w.kp = S->kp;
+  a.w.rp = S->rp;
+  a.w.n_slots = S->n_slots;
+  a.x = sx.dptr;
+  a.y = sy.dptr;
+  a.out = const_cast<void*>(in_place ? sy.dptr : so.dptr);
+  a.ldx = (int64_t)d->ldx;
+  a.ldy = (int64_t)d->ldy;
+  a.ldo = (int64_t)d->ldo;
+  a.x16 = d->dtype == RB_F16;
+  a.n_rows = (int)n;
+  a.slots = (const int32_t*)ss.dptr;
+  a.err = c->err.as<uint32_t>();
+  RB_CUDA(adapters_launch(a, c->num_sms, c->stream));
+  if (!dev)
+    RB_CUDA(cudaMemcpy2DAsync(d->out, d->ldo * esz, a.out, d->ldo * esz, S->n * esz, n, cudaMemcpyDeviceToHost, c->stream));
+  if (!(dev && (flags & RB_ASYNC)))
+    if (int rc = sync_ctx(c)) return rc;
+  return (int32_t)n;
+}
+
 }  // namespace
 
 extern "C" {
@@ -2601,6 +2940,53 @@ int32_t rb_sample_filtered(rb_ctx* c, int32_t dtype, const void* logits, uint64_
   return guarded([&] {
     return sample_filtered(c, dtype, logits, ld, n_rows, vocab, params, prev, prev_off, uniforms, out, probs, flags);
   });
+}
+
+int32_t rb_filter_probs(rb_ctx* c, int32_t dtype, const void* logits, uint64_t ld, uint32_t n_rows, uint32_t vocab,
+                        const rb_sampling_filter* params, const uint32_t* prev, const uint32_t* prev_off, float* probs,
+                        uint64_t ldp, uint32_t flags) {
+  return guarded([&] {
+    return filter_probs(c, dtype, logits, ld, n_rows, vocab, params, prev, prev_off, probs, ldp, flags);
+  });
+}
+
+int32_t rb_verify_drafts(rb_ctx* c, const rb_verify_desc* d, uint32_t flags) {
+  return guarded([&] { return verify_drafts(c, d, flags); });
+}
+
+int32_t rb_residual_norm(rb_ctx* c, const rb_residual_desc* d, uint32_t flags) {
+  return guarded([&] { return residual_norm(c, d, flags); });
+}
+
+int32_t rb_adapters_create(rb_ctx* c, uint32_t n, uint32_t k, uint32_t n_slots, uint32_t max_rank, int32_t* set) {
+  return guarded([&] { return adapters_create(c, n, k, n_slots, max_rank, set); });
+}
+
+int32_t rb_adapters_destroy(rb_ctx* c, int32_t set) {
+  if (!get_adapters(c, set)) return fail(RB_ERR_BAD_HANDLE, "adapters %d", set);
+  cudaSetDevice(c->device);
+  cudaStreamSynchronize(c->stream);
+  c->adapters.erase(set);
+  return RB_OK;
+}
+
+int32_t rb_adapters_set(rb_ctx* c, int32_t set, uint32_t slot, int32_t dtype, uint32_t rank, const void* down,
+                        const void* up, float scale, uint32_t flags) {
+  return guarded([&] { return adapters_set(c, set, slot, dtype, rank, down, up, scale, flags); });
+}
+
+int32_t rb_adapters_clear(rb_ctx* c, int32_t set, uint32_t slot) {
+  AdapterSet* S = get_adapters(c, set);
+  if (!S) return fail(RB_ERR_BAD_HANDLE, "adapters %d", set);
+  if (slot >= (uint32_t)S->n_slots) return fail(RB_ERR_NOT_FOUND, "slot %u of %d", slot, S->n_slots);
+  RB_CUDA(cudaSetDevice(c->device));
+  RB_CUDA(adapters_clear_launch(S->meta.as<AdapterMeta>() + slot, c->stream));
+  S->rank[slot] = 0;
+  return RB_OK;
+}
+
+int32_t rb_adapters_add(rb_ctx* c, int32_t set, const rb_adapters_desc* d, uint32_t flags) {
+  return guarded([&] { return adapters_add(c, set, d, flags); });
 }
 
 }  // extern "C"

@@ -49,6 +49,7 @@ constexpr int kBinades = 48;      // 41 in use: binade b holds exponents 127 - b
 constexpr int kBins = 256;
 constexpr int kMaxCluster = 8;
 constexpr uint32_t kLeft = 0xfffffffeu;  // in place of a token: a row left to the second kernel
+constexpr uint32_t kLeftDist = 0x7fc0feedu;  // the same in place of a row's first probability: not a number
 constexpr int kShortWarp = 384;   // candidates a warp may find
 constexpr int kShortBins = 512;
 constexpr int kShortMax = 8192;   // candidates of a row
@@ -364,7 +365,29 @@ __device__ Cut short_cut(const ShortList& l, uint32_t c, u64 w, u64 want, int& t
   return r;
 }
 
+template <bool D>
+__device__ __forceinline__ void leave_row(const FilterArgs& a, int row) {
+  if (D) a.dist[row * a.ldd] = __uint_as_float(kLeftDist);
+  else a.tokens[row] = kLeft;
+}
+// Zeros over part `rank` of n of a row's distribution, by one CTA.
+__device__ void clear_dist(const FilterArgs& a, int row, int rank, int n) {
+  float* p = a.dist + row * a.ldd;
+  const int mis = (int)((reinterpret_cast<uintptr_t>(p) & 15) / 4);
+  const int vecs = (a.vocab + mis + 3) / 4, share = (vecs + n - 1) / n, end = min(vecs, (rank + 1) * share);
+  for (int v = rank * share + threadIdx.x; v < end; v += kFT) {
+    const int i = v * 4 - mis;
+    if (i >= 0 && i + 4 <= a.vocab) {
+      *reinterpret_cast<float4*>(p + i) = make_float4(0.f, 0.f, 0.f, 0.f);
+    } else {
+      for (int e = 0; e < 4; ++e)
+        if (i + e >= 0 && i + e < a.vocab) p[i + e] = 0.f;
+    }
+  }
+}
+
 // Thresholds and draw over the n candidates of `list`, by one CTA. False: more of one bin than its sums hold.
+template <bool D>
 __device__ bool short_finish(uint2* list, int n, const rb_sampling_filter& p, bool use_k, bool use_p, const FilterArgs& a,
                              int row, FilterShared& s) {
   const int tid = threadIdx.x;
@@ -406,6 +429,13 @@ __device__ bool short_finish(uint2* list, int n, const rb_sampling_filter& p, bo
     if (v.x >= cut.bits) sum += fix(__uint_as_float(v.x));
   });
   u64 at = block_scan(sum, s.red, total);
+  if (D) {  // the row has been cleared
+    const double inv = 1.0 / (double)total;
+    l.each([&](uint2 v) {
+      if (v.x && v.x >= cut.bits) a.dist[row * a.ldd + v.y] = (float)((double)fix(__uint_as_float(v.x)) * inv);
+    });
+    return true;
+  }
   const u64 target = draw_target(a.uniforms[row], total);
   if (target < at || target >= at + sum) return true;
   for (int e = 0; e < K; ++e) {
@@ -423,7 +453,7 @@ __device__ bool short_finish(uint2* list, int n, const rb_sampling_filter& p, bo
 
 // One CTA an SM, for the registers of four vectors in flight a thread: 96 rows of 151937
 // 50 us, with two vectors and two CTAs 65 us; 200 rows 93 and 114 (nothing in L2).
-template <class T, int N>
+template <class T, int N, bool D>
 __global__ void __launch_bounds__(kFT, 1) filter_short_kernel(const __grid_constant__ FilterArgs a) {
   constexpr int E = 16 / sizeof(T), U = 4;
   extern __shared__ uint2 list[];            // of the first CTA: all candidates
@@ -443,7 +473,7 @@ __global__ void __launch_bounds__(kFT, 1) filter_short_kernel(const __grid_const
   bool all_of = p.min_p >= kShortFloor;  // the list has all that is kept
   if (!(greedy || use_k || all_of) ||
       (a.prev_off && p.repetition_penalty != 1.0f && a.prev_off[row + 1] > a.prev_off[row])) {
-    if (cl.rank == 0 && tid == 0) a.tokens[row] = kLeft;
+    if (cl.rank == 0 && tid == 0) leave_row<D>(a, row);
     return;  // the whole cluster
   }
   if (tid == 0) kept = 0;
@@ -506,8 +536,9 @@ __global__ void __launch_bounds__(kFT, 1) filter_short_kernel(const __grid_const
     for (int r = 0; r < N; ++r) key = max(key, (uint32_t)all[r]);
   }
   top = __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
+  if (D && (top == -INFINITY || greedy)) clear_dist(a, row, cl.rank, N);
   if (top == -INFINITY) {
-    if (cl.rank == 0 && tid == 0) {
+    if (!D && cl.rank == 0 && tid == 0) {
       a.tokens[row] = 0xffffffffu;
       if (a.probs) a.probs[row] = 0.f;
     }
@@ -529,9 +560,14 @@ __global__ void __launch_bounds__(kFT, 1) filter_short_kernel(const __grid_const
 #pragma unroll
       for (int r = 0; r < N; ++r) at = min(at, (uint32_t)all[r]);
     }
+    if (D) cl.sync();  // the row has been cleared
     if (cl.rank == 0 && tid == 0) {
-      a.tokens[row] = at;
-      if (a.probs) a.probs[row] = 1.f;
+      if (D) {
+        a.dist[row * a.ldd + at] = 1.f;
+      } else {
+        a.tokens[row] = at;
+        if (a.probs) a.probs[row] = 1.f;
+      }
     }
     return;
   }
@@ -585,9 +621,10 @@ __global__ void __launch_bounds__(kFT, 1) filter_short_kernel(const __grid_const
     __syncthreads();  // s.red2 has been read
   }
   if (count > kShortMax) {  // the same in every thread of the cluster
-    if (cl.rank == 0 && tid == 0) a.tokens[row] = kLeft;
+    if (cl.rank == 0 && tid == 0) leave_row<D>(a, row);
     return;
   }
+  if (D) clear_dist(a, row, cl.rank, N);
   {
     uint2* first = N > 1 ? cl.g.map_shared_rank(list, 0) : list;
     uint32_t found = 0;
@@ -608,8 +645,8 @@ __global__ void __launch_bounds__(kFT, 1) filter_short_kernel(const __grid_const
   }
   cl.sync();
   if (cl.rank) return;
-  if ((!all_of && kept < p.top_k) || !short_finish(list, (int)count, p, use_k, use_p, a, row, s))
-    if (tid == 0) a.tokens[row] = kLeft;
+  if ((!all_of && kept < p.top_k) || !short_finish<D>(list, (int)count, p, use_k, use_p, a, row, s))
+    if (tid == 0) leave_row<D>(a, row);
 }
 
 // Two CTAs an SM (32 registers a thread) where their elements fit and keep a CTA busy
@@ -620,7 +657,7 @@ constexpr int two_ctas() {
   return NV >= 3 && NV * (16 / (int)sizeof(T)) <= 24 ? 2 : 1;
 }
 
-template <class T, int NV, int N>
+template <class T, int NV, int N, bool D>
 __global__ void __launch_bounds__(kFT, two_ctas<T, NV>()) filter_kernel(const __grid_constant__ FilterArgs a) {
   constexpr int E = 16 / sizeof(T), Q = E / 4, NQ = NV * Q;  // quads of a vector, of a thread
   extern __shared__ float4 quads[];
@@ -629,7 +666,7 @@ __global__ void __launch_bounds__(kFT, two_ctas<T, NV>()) filter_kernel(const __
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x / N;
   pdl_wait();
-  if (!a.all && a.tokens[row] != kLeft) return;  // the whole cluster
+  if (!a.all && (D ? __float_as_uint(a.dist[row * a.ldd]) != kLeftDist : a.tokens[row] != kLeft)) return;  // the whole cluster
   if (N > 1) cg::this_cluster().barrier_arrive();
   rb_sampling_filter p = a.params[row];
   p.min_p = fminf(p.min_p, 1.f);  // the first rank always stays
@@ -700,6 +737,38 @@ __global__ void __launch_bounds__(kFT, two_ctas<T, NV>()) filter_kernel(const __
   }
   const uint32_t mk = (uint32_t)(best >> 32);
   const float m = __uint_as_float((mk & 0x80000000u) ? mk & 0x7fffffffu : ~mk);
+  // a thread's elements as the row's distribution; `of` gives an element's probability. Every CTA has
+  // read the mark in the row's first place by now.
+  auto write_dist = [&](auto of) {
+    float* d = a.dist + row * a.ldd;
+#pragma unroll 1
+    for (int r = 0; r < NV; ++r) {
+      if (v0 + r * kFT + tid >= v1) break;
+#pragma unroll
+      for (int h = 0; h < Q; ++h) {
+        const int i = index(r) + 4 * h;
+        const float4 x = mine[(r * Q + h) * kFT];
+        const float4 y = make_float4(of(x.x, i), of(x.y, i + 1), of(x.z, i + 2), of(x.w, i + 3));
+        if (i >= 0 && i + 4 <= V && reinterpret_cast<uintptr_t>(d + i) % 16 == 0) {
+          __stcs(reinterpret_cast<float4*>(d + i), y);
+        } else {
+          const float z[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (i + e >= 0 && i + e < V) d[i + e] = z[e];
+        }
+      }
+    }
+  };
+  if (D && (m == -INFINITY || greedy)) {
+    if (m == -INFINITY) {
+      write_dist([](float, int) { return 0.f; });
+    } else {
+      const int at = (int)(0xffffffffu - (uint32_t)best);
+      write_dist([&](float, int i) { return i == at ? 1.f : 0.f; });
+    }
+    return;
+  }
   if (m == -INFINITY || greedy) {  // the same in every thread of the cluster
     if (cl.rank == 0 && tid == 0) {
       const bool none = m == -INFINITY;
@@ -807,6 +876,11 @@ __global__ void __launch_bounds__(kFT, two_ctas<T, NV>()) filter_kernel(const __
       total += all[r];
     }
   }
+  if (D) {
+    const double inv = 1.0 / (double)total;
+    write_dist([&](float x, int) { return x != 0.f ? (float)((double)fix(x) * inv) : 0.f; });
+    return;
+  }
   const u64 target = draw_target(a.uniforms[row], total);
   if (target < run || target >= run + mass) return;  // the whole CTA
   // exactly one CTA's, warp's and lane's kept weights reach past the target (target < total)
@@ -845,12 +919,12 @@ __global__ void __launch_bounds__(kFT, two_ctas<T, NV>()) filter_kernel(const __
   }
 }
 
-template <class T, int NV, int N>
-cudaError_t launch(const FilterArgs& a, cudaStream_t s) {
+template <class T, int NV, int N, bool D>
+cudaError_t launch_as(const FilterArgs& a, cudaStream_t s) {
   constexpr int smem = NV * kFT * (16 / (int)sizeof(T)) * 4;
   int dev = 0;
   cudaGetDevice(&dev);
-  if (cudaError_t e = ensure_smem_attr(filter_kernel<T, NV, N>, smem, dev)) return e;
+  if (cudaError_t e = ensure_smem_attr(filter_kernel<T, NV, N, D>, smem, dev)) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.n_rows * N));
   cfg.blockDim = dim3(kFT);
@@ -864,15 +938,19 @@ cudaError_t launch(const FilterArgs& a, cudaStream_t s) {
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, filter_kernel<T, NV, N>, a);
+  return cudaLaunchKernelEx(&cfg, filter_kernel<T, NV, N, D>, a);
+}
+template <class T, int NV, int N>
+cudaError_t launch(const FilterArgs& a, cudaStream_t s) {
+  return a.dist ? launch_as<T, NV, N, true>(a, s) : launch_as<T, NV, N, false>(a, s);
 }
 
-template <class T, int N>
-cudaError_t launch_short(const FilterArgs& a, cudaStream_t s) {
+template <class T, int N, bool D>
+cudaError_t launch_short_as(const FilterArgs& a, cudaStream_t s) {
   constexpr int smem = kShortMax * 8;
   int dev = 0;
   cudaGetDevice(&dev);
-  if (cudaError_t e = ensure_smem_attr(filter_short_kernel<T, N>, smem, dev)) return e;
+  if (cudaError_t e = ensure_smem_attr(filter_short_kernel<T, N, D>, smem, dev)) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.n_rows * N));
   cfg.blockDim = dim3(kFT);
@@ -884,7 +962,11 @@ cudaError_t launch_short(const FilterArgs& a, cudaStream_t s) {
   at.val.clusterDim.y = at.val.clusterDim.z = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, filter_short_kernel<T, N>, a);
+  return cudaLaunchKernelEx(&cfg, filter_short_kernel<T, N, D>, a);
+}
+template <class T, int N>
+cudaError_t launch_short(const FilterArgs& a, cudaStream_t s) {
+  return a.dist ? launch_short_as<T, N, true>(a, s) : launch_short_as<T, N, false>(a, s);
 }
 
 // CTAs a row: one for each SM, with a vector a thread at least. 1, 2, 3, 4, 6 and 8 CTAs a row,

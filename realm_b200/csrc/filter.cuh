@@ -21,6 +21,8 @@ struct FilterArgs {
   const float* uniforms = nullptr;
   uint32_t* tokens = nullptr;
   float* probs = nullptr;  // or null
+  float* dist = nullptr;   // not null: the rows' distributions go here instead of a draw
+  int64_t ldd = 0;
 };
 
 cudaError_t filter_launch(const FilterArgs& a, int num_sms, cudaStream_t s);
