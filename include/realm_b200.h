@@ -596,7 +596,8 @@ int32_t rb_residual_norm(rb_ctx* ctx, const rb_residual_desc* desc, uint32_t fla
  * reference adds the product of the factors to dequantised weights, one model a tenant
  * (crates/realm-runtime/src/lora.rs); here one call serves rows of any mix of adapters. A
  * set holds n_slots adapters of one projection, each of up to max_rank, in fp16:
- * n_slots * max_rank * (n + k) * 2 bytes, max_rank rounded up to a multiple of 8. */
+ * n_slots * max_rank * (n + k) * 2 bytes, max_rank rounded up to a multiple of 16 and k to
+ * one of 64. */
 int32_t rb_adapters_create(rb_ctx* ctx, uint32_t n, uint32_t k, uint32_t n_slots, uint32_t max_rank, int32_t* set);
 /* Waits for the context's stream, then frees the set. Its handle is not given out again. */
 int32_t rb_adapters_destroy(rb_ctx* ctx, int32_t set);

@@ -15,7 +15,8 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "librealm_b200.so")
 SOURCES = ["gemv.cu", "attention.cu", "engine.cu", "sample.cu", "scheduler.cpp", "gguf.cpp", "rows_plan.cpp",
-           "rows_append.cu", "rows_attn.cu", "rows_tile.cu", "filter.cu", "adapters.cu", "verify.cu", "residual.cu"]
+           "rows_append.cu", "rows_attn.cu", "rows_tile.cu", "filter.cu", "adapters.cu", "adapters_tile.cu", "verify.cu",
+           "residual.cu"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo",
          "-Xcompiler", "-fPIC"]

@@ -1,5 +1,6 @@
 // Low-rank adapters beside a shared projection: out_r = y_r + scale_a up_a (down_a x_r) for
-// the row's adapter a.
+// the row's adapter a. Here single tokens of many tenants; tiles of many rows are in
+// adapters_tile.cu.
 //
 // A cluster of CTAs has up to R rows that share an adapter. Its CTAs split k for
 // v = down x and then n for up v; in between each sends its part of v to all of them
@@ -25,7 +26,7 @@ namespace {
 
 constexpr int kT = 256, kWarps = kT / 32;
 constexpr int kBlock = 64;        // rows among which an item's rows are found
-constexpr int kGroup = 4;         // ranks a warp works on at a time
+constexpr int kGroup = 8;         // ranks a warp works on at a time: a line of weights
 constexpr int kTileK = 1536;      // elements of x in shared memory at a time
 constexpr int kMaxCluster = 8;
 static_assert(kWarps * kGroup <= kAdapterMaxRank && kTileK % 8 == 0, "");
@@ -47,24 +48,6 @@ __device__ __forceinline__ void unpack8(uint4 q, float (&f)[8]) {
     f[2 * i] = v.x;
     f[2 * i + 1] = v.y;
   }
-}
-
-// Sums of V values (a power of two up to 32) over the warp: lane l gets that of value l / (32 / V).
-template <int V>
-__device__ __forceinline__ float fold(float (&v)[V]) {
-  const int lane = threadIdx.x & 31;
-  int o = 16;
-#pragma unroll
-  for (int h = V / 2; h > 0; h >>= 1, o >>= 1) {
-    const bool up = lane & o;
-#pragma unroll
-    for (int i = 0; i < h; ++i) {
-      const float give = up ? v[i] : v[i + h], keep = up ? v[i + h] : v[i];
-      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
-    }
-  }
-  for (; o > 0; o >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
-  return v[0];
 }
 
 // The slot of a row, or -1 where it has no adapter.
@@ -150,7 +133,7 @@ __global__ void __launch_bounds__(kT) adapters_kernel(const __grid_constant__ Ad
   cluster.barrier_arrive();
   const int rank = a.w.meta[slot].rank;
   const float scale = a.w.meta[slot].scale;
-  const int groups = (rank + kGroup - 1) / kGroup;
+  const int groups = (rank + kGroup - 1) / kGroup, r16 = (rank + 15) / 16 * 16;
   // warps are split over groups of ranks, and with few of those over k
   const int ks = groups >= kWarps ? 1 : kWarps / groups, kpart = ks == 1 ? 0 : warp / groups;
   const int chunks = a.w.kp / 8, c0 = (int)((int64_t)chunks * c / C), c1 = (int)((int64_t)chunks * (c + 1) / C);
@@ -167,31 +150,30 @@ __global__ void __launch_bounds__(kT) adapters_kernel(const __grid_constant__ Ad
     if (kpart < ks) {
       const int b0 = (t1 - t0) * kpart / ks, b1 = (t1 - t0) * (kpart + 1) / ks;
       for (int g = ks == 1 ? warp : warp % groups; g < groups; g += ks == 1 ? kWarps : groups) {
-        float acc[kGroup * R];
+        float acc[R];
 #pragma unroll
-        for (int i = 0; i < kGroup * R; ++i) acc[i] = 0.f;
-        const uint16_t* w = down + (int64_t)(g * kGroup) * a.w.kp + k0;  // rows up to rp, a multiple of 8, exist
-        for (int b = b0 + lane; b < b1; b += 32) {
-          uint4 q[kGroup];
-#pragma unroll
-          for (int i = 0; i < kGroup; ++i) q[i] = __ldg(reinterpret_cast<const uint4*>(w + (int64_t)i * a.w.kp + b * 8));
+        for (int r = 0; r < R; ++r) acc[r] = 0.f;
+        // a lane has rank g * 8 + lane % 8 of every fourth block of 8 elements
+        const uint4* w = reinterpret_cast<const uint4*>(down) + (int64_t)t0 * r16 + g * kGroup + (lane & 7);
+#pragma unroll 4
+        for (int b = b0 + (lane >> 3); b < b1; b += 4) {
+          float f[8];
+          unpack8(__ldg(w + (int64_t)b * r16), f);
 #pragma unroll
           for (int r = 0; r < R; ++r) {
             const float4 lo = *reinterpret_cast<const float4*>(&xs[r][b * 8]),
                          hi = *reinterpret_cast<const float4*>(&xs[r][b * 8 + 4]);
             const float xv[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-            for (int i = 0; i < kGroup; ++i) {
-              float f[8];
-              unpack8(q[i], f);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) acc[i * R + r] = fmaf(f[e], xv[e], acc[i * R + r]);
-            }
+            for (int e = 0; e < 8; ++e) acc[r] = fmaf(f[e], xv[e], acc[r]);
           }
         }
-        const float sum = fold<kGroup * R>(acc);
-        constexpr int per = 32 / (kGroup * R);
-        if (lane % per == 0) part[kpart * nv + g * kGroup * R + lane / per] += sum;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], 8);
+          acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], 16);
+          if (lane < 8) part[kpart * nv + (g * kGroup + lane) * R + r] += acc[r];
+        }
       }
     }
   }
@@ -249,10 +231,12 @@ cudaError_t launch(const AdapterArgs& a, int cluster, cudaStream_t s) {
 template <class S>
 __global__ void adapters_set_kernel(const __grid_constant__ AdapterSetArgs a) {
   const S *sd = reinterpret_cast<const S*>(a.src_down), *su = reinterpret_cast<const S*>(a.src_up);
-  const int64_t nd = (int64_t)a.rp * a.kp, nu = (int64_t)a.rp * a.n;
+  const int r16 = (a.rank + 15) / 16 * 16;
+  const int64_t nd = (int64_t)r16 * a.kp, nu = (int64_t)r16 * a.n;
   const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, step = (int64_t)gridDim.x * blockDim.x;
   for (int64_t i = at; i < nd; i += step) {
-    const int r = (int)(i / a.kp), j = (int)(i % a.kp);
+    const int64_t v = i / 8;  // [k / 8][r16][8]
+    const int r = (int)(v % r16), j = (int)(v / r16) * 8 + (int)(i % 8);
     a.down[i] = r < a.rank && j < a.k ? __half_as_ushort(from_f<__half>(to_f(sd[(int64_t)r * a.k + j]))) : 0;
   }
   for (int64_t i = at; i < nu; i += step) {  // [rank / 8][n][8]
@@ -268,7 +252,7 @@ __global__ void adapters_clear_kernel(AdapterMeta* meta) { *meta = AdapterMeta{0
 }  // namespace
 
 cudaError_t adapters_set_launch(const AdapterSetArgs& a, cudaStream_t s) {
-  const int64_t most = (int64_t)a.rp * std::max(a.kp, a.n);
+  const int64_t most = (int64_t)(a.rank + 15) / 16 * 16 * std::max(a.kp, a.n);
   const int blocks = (int)std::min<int64_t>(1184, (most + 255) / 256);
   if (a.in16) adapters_set_kernel<__half><<<blocks, 256, 0, s>>>(a);
   else adapters_set_kernel<float><<<blocks, 256, 0, s>>>(a);
@@ -281,6 +265,7 @@ cudaError_t adapters_clear_launch(AdapterMeta* meta, cudaStream_t s) {
 }
 
 cudaError_t adapters_launch(const AdapterArgs& a, int num_sms, cudaStream_t s) {
+  if (a.n_rows > 64) return adapters_tile_launch(a, num_sms, s);
   const int cluster = 8;
   if (a.n_rows <= 16) return a.x16 ? launch<__half, 1>(a, cluster, s) : launch<float, 1>(a, cluster, s);
   return a.x16 ? launch<__half, 4>(a, cluster, s) : launch<float, 4>(a, cluster, s);

@@ -1,4 +1,4 @@
-// Low-rank adapters of many tenants beside one projection (adapters.cu).
+// Low-rank adapters of many tenants beside one projection (adapters.cu, adapters_tile.cu).
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -15,9 +15,11 @@ struct AdapterMeta {
 };
 
 // Adapters of one projection [n][k], in slots of equal size:
-//   down  [n_slots][rp][kp] fp16, zeros past the rank and past k
-//   up    [n_slots][rp / 8][n][8] fp16, zeros past the rank
-// rp, kp: max_rank and k rounded up to a multiple of 8.
+//   down  [n_slots][kp / 8][r16][8] fp16 (as much of rp * kp as the rank needs)
+//   up    [n_slots][rp / 8][n][8] fp16
+// with zeros past the rank and past k. r16, rp: the rank and max_rank rounded up to a multiple of 16;
+// kp: k to one of 64. Blocks of 8 rows x 16 bytes, as tensor-core operands lie, so that
+// they are copied as they are; eight elements a load for a thread.
 struct AdapterView {
   const uint16_t *down = nullptr, *up = nullptr;
   const AdapterMeta* meta = nullptr;
@@ -46,5 +48,7 @@ struct AdapterSetArgs {
 cudaError_t adapters_set_launch(const AdapterSetArgs& a, cudaStream_t s);
 cudaError_t adapters_clear_launch(AdapterMeta* meta, cudaStream_t s);
 cudaError_t adapters_launch(const AdapterArgs& a, int num_sms, cudaStream_t s);
+// many rows: tiles on the tensor cores
+cudaError_t adapters_tile_launch(const AdapterArgs& a, int num_sms, cudaStream_t s);
 
 }  // namespace rb

@@ -2671,9 +2671,9 @@ int32_t adapters_create(rb_ctx* c, uint32_t n, uint32_t k, uint32_t n_slots, uin
   auto S = std::make_unique<AdapterSet>();
   S->n = (int)n;
   S->k = (int)k;
-  S->kp = (int)(k + 7) / 8 * 8;
+  S->kp = (int)(k + 63) / 64 * 64;
   S->max_rank = (int)max_rank;
-  S->rp = (int)(max_rank + 7) / 8 * 8;
+  S->rp = (int)(max_rank + 15) / 16 * 16;
   S->n_slots = (int)n_slots;
   S->rank.assign(n_slots, 0);
   const size_t per = (size_t)n_slots * S->rp * 2;
