@@ -85,6 +85,16 @@ __device__ __forceinline__ void ld8(uint32_t ta, float* r) {
                : "r"(ta)
                : "memory");
 }
+// 16 (or 4) bytes to shared memory, the last 16 - n of them zero
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int n) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, int n) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void workers_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
@@ -97,8 +107,13 @@ struct Cfg {
   static constexpr int CE = 8 * E;                  // of a chunk: 128 bytes a row
   static constexpr int A = 128 * 128;               // bytes of a chunk's rows (one part)
   static constexpr int B = RP * 128;                // and of its weights
-  static constexpr int STAGE = (1 + F32) * A + B;
-  static constexpr int NS = F32 ? (RP == 64 ? 2 : 3) : (RP == 64 ? 4 : 5);
+  // fp32: the rows as they are (the tensor core reads their upper 19 bits), then the low parts and weights
+  // of two chunks, which threads make; fp16: rows and weights
+  static constexpr int STAGE = F32 ? A : A + B;
+  static constexpr int NS = F32 ? (RP == 64 ? 3 : 5) : (RP == 64 ? 4 : 6);
+  static constexpr int AHEAD = F32 && RP == 64 ? 2 : NS - 2;  // chunks on their way
+  static constexpr int LOW = F32 ? A + B : 0;
+  static constexpr int RING = NS * STAGE + 2 * LOW;
   static constexpr int CHAIN = F32 ? 256 / CE : 1024 / CE;  // chunks summed on the tensor core
   // after the chunks: v (hi, lo), two tiles of up, and the parts of v or the turned blocks
   static constexpr int V = RP * 256;                // bytes of v, one part: [RP / 8][128 rows][16]
@@ -107,53 +122,72 @@ struct Cfg {
   static constexpr int TURN = 8 * 32 * kStagePitch * 4;
   static constexpr int PARTS = RP * 128 * 4;
   static constexpr int MAIN0 = P_AT + (TURN > PARTS ? TURN : PARTS);
-  static constexpr int MAIN = MAIN0 > NS * STAGE ? MAIN0 : NS * STAGE;
+  static constexpr int MAIN = MAIN0 > RING ? MAIN0 : RING;
   static constexpr int CTAS = RP == 64 ? 2 : 1;
   static int smem(int n_slots) { return MAIN + 4 * n_slots; }
   // TMEM: 256 columns for each of up to two CTAs an SM, never a third
-  static_assert(CTAS * MAIN <= 226 * 1024 && 3 * MAIN > 228 * 1024, "");
+  static_assert(CTAS * MAIN <= 226 * 1024 && 3 * MAIN > 228 * 1024 && 2 * V == PARTS, "");
 };
 
 struct TileShared {
-  uint64_t full[5], empty[5], dfull[2], dfree[2], upfull[2], vready;
+  uint64_t full[6], empty[6], dfull[2], dfree[2], upfull[2], vready;
   uint32_t tmem;
   int n_tiles, scan[8], counts[8];
   int rows[128];
   float most[2][128];
 };
 
-// The rows of a tile: those of `slot` with ranks [r0, r0 + tile_rows) among its rows.
-__device__ int find_rows(const AdapterArgs& a, int slot, int r0, int tile_rows, TileShared& s) {
+// Slots of rows 4 i .. 4 i + 3; -1 past the last row.
+__device__ __forceinline__ int4 slots4(const AdapterArgs& a, int i, bool vec) {
+  const int r = 4 * i;
+  if (vec && r + 4 <= a.n_rows) return __ldg(reinterpret_cast<const int4*>(a.slots) + i);
+  int4 v = make_int4(-1, -1, -1, -1);
+  if (r < a.n_rows) v.x = a.slots[r];
+  if (r + 1 < a.n_rows) v.y = a.slots[r + 1];
+  if (r + 2 < a.n_rows) v.z = a.slots[r + 2];
+  if (r + 3 < a.n_rows) v.w = a.slots[r + 3];
+  return v;
+}
+
+// The rows of a tile: those of `slot` with ranks [r0, r0 + tile_rows) among its rows. Warp w has
+// the rows [w seg, (w + 1) seg), a lane four at a time.
+__device__ __noinline__ int find_rows(const AdapterArgs& a, int slot, int r0, int tile_rows, TileShared& s) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int seg = (a.n_rows + 8 * 128 - 1) / (8 * 128) * 128, b0 = warp * seg, b1 = min(a.n_rows, b0 + seg);
-  constexpr int kMost = kSpanRows / (8 * 32);
-  uint32_t mine = 0;  // bit i: row b0 + 32 i + lane
-  int count = 0;
-#pragma unroll
-  for (int i = 0; i < kMost; ++i) {
-    const int r = b0 + 32 * i + lane;
-    if (b0 + 32 * i < b1) {  // uniform
-      const bool in = r < b1 && a.slots[r] == slot;
-      mine |= (uint32_t)in << i;
-      count += __popc(__ballot_sync(0xffffffffu, in));
-    }
+  const int rounds = (a.n_rows + 8 * 128 - 1) / (8 * 128), i0 = warp * rounds * 32 + lane;
+  const bool vec = (reinterpret_cast<uintptr_t>(a.slots) & 15) == 0;
+  uint32_t mine = 0;  // bits 4 i .. 4 i + 3: the lane's rows of round i
+#pragma unroll 4
+  for (int i = 0; i < rounds; ++i) {
+    const int4 v = slots4(a, i0 + 32 * i, vec);
+    mine |= ((uint32_t)(v.x == slot) | (uint32_t)(v.y == slot) << 1 | (uint32_t)(v.z == slot) << 2 |
+             (uint32_t)(v.w == slot) << 3)
+            << (4 * i);
   }
+  const int count = __reduce_add_sync(0xffffffffu, __popc(mine));
   if (lane == 0) s.counts[warp] = count;
   workers_sync();
-  int at = 0, total = 0;
+  int at = -r0, total = 0;
 #pragma unroll
   for (int w = 0; w < 8; ++w) {
     if (w < warp) at += s.counts[w];
     total += s.counts[w];
   }
-  if (at < r0 + tile_rows && at + count > r0) {
-#pragma unroll 4
-    for (int i = 0; i < kMost; ++i) {
-      const bool in = mine >> i & 1;
-      const uint32_t b = __ballot_sync(0xffffffffu, in);
-      const int rank = at + __popc(b & ((1u << lane) - 1)) - r0;
-      if (in && rank >= 0 && rank < tile_rows) s.rows[rank] = b0 + 32 * i + lane;
-      at += __popc(b);
+  if (count && at < tile_rows && at + count > 0) {
+    for (int i = 0; i < rounds; ++i) {
+      const uint32_t m = mine >> (4 * i) & 15;
+      int incl = __popc(m);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+      }
+      int rank = at + incl - __popc(m);
+      for (int e = 0; e < 4; ++e)
+        if (m >> e & 1) {
+          if (rank >= 0 && rank < tile_rows) s.rows[rank] = 4 * (i0 + 32 * i) + e;
+          ++rank;
+        }
+      at += __shfl_sync(0xffffffffu, incl, 31);
     }
   }
   workers_sync();
@@ -177,15 +211,15 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
   }
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
-      mbar_init(&s.full[i], kWorkers);
+      mbar_init(&s.full[i], 8);  // warps
       mbar_init(&s.empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.dfull[i], 1);
-      mbar_init(&s.dfree[i], kWorkers);
+      mbar_init(&s.dfree[i], 8);
       mbar_init(&s.upfull[i], 1);
     }
-    mbar_init(&s.vready, kWorkers);
+    mbar_init(&s.vready, 8);
     fence_barrier_init();
   }
   for (int i = tid; i < a.w.n_slots; i += kTT) start[i] = 0;
@@ -204,15 +238,28 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
   const uint32_t tmem = s.tmem;
 
   // ---- tiles: rows of every slot, then the first tile of each ----
-  for (int b = 0; b < a.n_rows; b += kTT) {
-    const int v = b + tid < a.n_rows ? a.slots[b + tid] : -1;
-    const bool in = v >= 0 && v < a.w.n_slots;
-    // mostly rows of one slot follow one another
-    const int v0 = __shfl_sync(0xffffffffu, v, 0);
-    if (__all_sync(0xffffffffu, v == v0)) {
-      if (lane == 0 && in) atomicAdd(&start[v], 32);
-    } else if (in) {
-      atomicAdd(&start[v], 1);
+  {
+    const bool vec = (reinterpret_cast<uintptr_t>(a.slots) & 15) == 0;
+    auto count = [&](int v, int n) {
+      if (v >= 0 && v < a.w.n_slots) atomicAdd(&start[v], n);
+    };
+    const int quads = (a.n_rows + 3) / 4;
+#pragma unroll 4
+    for (int b = warp * 32; b < quads; b += kTT) {
+      const int4 v = b + lane < quads ? slots4(a, b + lane, vec) : make_int4(-1, -1, -1, -1);
+      const bool same = v.x == v.y && v.x == v.z && v.x == v.w;
+      const int lead = __shfl_sync(0xffffffffu, v.x, 0);
+      // mostly rows of one slot follow one another
+      if (__all_sync(0xffffffffu, same && v.x == lead)) {
+        if (lane == 0) count(v.x, 128);
+      } else if (same) {
+        count(v.x, 4);
+      } else {
+        count(v.x, 1);
+        count(v.y, 1);
+        count(v.z, 1);
+        count(v.w, 1);
+      }
     }
   }
   __syncthreads();
@@ -275,75 +322,88 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
       const T* xp[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        xp[j] = rg + 32 * j < cnt ? reinterpret_cast<const T*>(a.x) + s.rows[rg + 32 * j] * a.ldx : nullptr;
+        xp[j] = rg + 32 * j < cnt
+                    ? reinterpret_cast<const T*>(a.x) + s.rows[rg + 32 * j] * a.ldx + q0 * G::CE + piece * E
+                    : nullptr;
+      // where the piece goes; row & 7 is the same for all four, whose places are 4096 bytes apart
+      const uint32_t at = (uint32_t)rg * 128 + ((piece ^ (rg & 7)) << 4);
       constexpr int NB = RP * (F32 ? 4 : 8) / kWorkers;  // 16-byte pieces of weights a thread has of a chunk
       const int items = r16 * (F32 ? 4 : 8);
-      uint4 xa[2][4], wb[2][NB];
-      auto load = [&](int q, uint4 (&x)[4], uint4 (&w)[NB]) {
-        const int e0 = (q0 + q) * G::CE + piece * E;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          x[j] = make_uint4(0, 0, 0, 0);
-          if (!xp[j]) continue;
-          if (VX && e0 + E <= a.w.k) {
-            x[j] = __ldg(reinterpret_cast<const uint4*>(xp[j] + e0));
-          } else {
-            T t[E];
-#pragma unroll
-            for (int e = 0; e < E; ++e) t[e] = e0 + e < a.w.k ? xp[j][e0 + e] : T(0.f);
-            x[j] = *reinterpret_cast<uint4*>(t);
-          }
-        }
-        const uint4* wp = reinterpret_cast<const uint4*>(down) + (int64_t)(q0 + q) * (G::CE / 8) * r16;
-#pragma unroll
-        for (int i = 0; i < NB; ++i)
-          if (tid + i * kWorkers < items) w[i] = __ldg(wp + tid + i * kWorkers);
-      };
-      int bat[NB];  // where a piece of weights goes
+      const uint4* wp = reinterpret_cast<const uint4*>(down) + (int64_t)q0 * items + tid;
+      uint4 wb[NB];  // fp32: the next chunk's
+      uint32_t bat[NB];
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
         const int it = tid + i * kWorkers;
-        bat[i] = F32 ? (it / r16 * 2 * r16 + it % r16) * 16 : it * 16;
+        bat[i] = F32 ? (uint32_t)(it / r16 * 2 * r16 + it % r16) * 16 : (uint32_t)it * 16;
       }
-      auto store = [&](uint4 (&x)[4], uint4 (&w)[NB]) {
-        const int st = nc % NS;
-        if (nc >= NS) wait(&s.empty[st], nc / NS - 1, DEV_TIMEOUT_EMPTY);
-        uint8_t* base = smem + st * G::STAGE;
+      // chunk q of this CTA, the ch-th of all, is on its way
+      auto fetch = [&](int q, uint32_t ch) {
+        const uint32_t st = ch % NS;
+        if (ch >= NS) wait(&s.empty[st], ch / NS - 1, DEV_TIMEOUT_EMPTY);
+        const uint32_t base = sbase + st * G::STAGE + at;
+        const int left = a.w.k - (q0 + q) * G::CE - piece * E;  // elements up to the row's end
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int row = rg + 32 * j, at = row * 128 + ((piece ^ (row & 7)) << 4);
-          if (!xp[j]) continue;  // the products' rows stay apart
-          if constexpr (F32) {
-            const uint32_t v[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
-            uint32_t h[4], l[4];
+          if (!xp[j]) continue;  // rows of the products stay apart
+          const T* p = xp[j] + (int64_t)q * G::CE;
+          if constexpr (VX) {
+            const int n = min(max(left, 0), E) * (int)sizeof(T);
+            copy16(base + j * 4096, n ? p : xp[j], n);
+          } else if constexpr (F32) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) copy4(base + j * 4096 + e * 4, e < left ? p + e : xp[j], e < left ? 4 : 0);
+          } else {
+            uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              h[e] = v[e] & 0xffffe000u;
-              const float f = __uint_as_float(v[e]), g = __uint_as_float(h[e]);
-              l[e] = f == g ? 0u : (__float_as_uint(f - g) + 0x1000u) & 0xffffe000u;
+              const uint32_t lo = 2 * e < left ? __half_as_ushort(p[2 * e]) : 0u, hi = 2 * e + 1 < left ? __half_as_ushort(p[2 * e + 1]) : 0u;
+              w[e] = lo | hi << 16;
             }
-            *reinterpret_cast<uint4*>(base + at) = make_uint4(h[0], h[1], h[2], h[3]);
-            *reinterpret_cast<uint4*>(base + G::A + at) = make_uint4(l[0], l[1], l[2], l[3]);
-          } else {
-            *reinterpret_cast<uint4*>(base + at) = x[j];
+            *reinterpret_cast<uint4*>(smem + st * G::STAGE + at + j * 4096) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
-        uint8_t* wbase = base + (1 + F32) * G::A;
+        if constexpr (!F32)
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-          if (tid + i * kWorkers >= items) continue;
-          if constexpr (F32) {
-            const float2 f0 = __half22float2(u32_as_h2(w[i].x)), f1 = __half22float2(u32_as_h2(w[i].y)),
-                         f2 = __half22float2(u32_as_h2(w[i].z)), f3 = __half22float2(u32_as_h2(w[i].w));
-            *reinterpret_cast<float4*>(wbase + bat[i]) = make_float4(f0.x, f0.y, f1.x, f1.y);
-            *reinterpret_cast<float4*>(wbase + bat[i] + r16 * 16) = make_float4(f2.x, f2.y, f3.x, f3.y);
-          } else {
-            *reinterpret_cast<uint4*>(wbase + bat[i]) = w[i];
+          for (int i = 0; i < NB; ++i)
+            if (tid + i * kWorkers < items) copy16(sbase + st * G::STAGE + G::A + bat[i], wp + (int64_t)q * items + i * kWorkers, 16);
+      };
+      auto weights = [&](int q) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+          if (tid + i * kWorkers < items) wb[i] = __ldg(wp + (int64_t)q * items + i * kWorkers);
+      };
+      // the chunk is here: fp32 rows get their low part, and the products may begin
+      auto ready = [&](uint32_t ch) {
+        const uint32_t st = ch % NS;
+        if constexpr (F32) {
+          if (ch >= 2) wait(&s.empty[(ch - 2) % NS], (ch - 2) / NS, DEV_TIMEOUT_EMPTY);
+          uint8_t* low = smem + NS * G::STAGE + (ch & 1) * G::LOW;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (!xp[j]) continue;
+            const uint4 x = *reinterpret_cast<const uint4*>(smem + st * G::STAGE + at + j * 4096);
+            const uint32_t v[4] = {x.x, x.y, x.z, x.w};
+            uint32_t l[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float f = __uint_as_float(v[e]), g = __uint_as_float(v[e] & 0xffffe000u);
+              l[e] = f == g ? 0u : __float_as_uint(f - g) + 0x1000u;  // to the nearest; 0 for infinities
+            }
+            *reinterpret_cast<uint4*>(low + at + j * 4096) = make_uint4(l[0], l[1], l[2], l[3]);
+          }
+#pragma unroll
+          for (int i = 0; i < NB; ++i) {
+            if (tid + i * kWorkers >= items) continue;
+            const float2 f0 = __half22float2(u32_as_h2(wb[i].x)), f1 = __half22float2(u32_as_h2(wb[i].y)),
+                         f2 = __half22float2(u32_as_h2(wb[i].z)), f3 = __half22float2(u32_as_h2(wb[i].w));
+            *reinterpret_cast<float4*>(low + G::A + bat[i]) = make_float4(f0.x, f0.y, f1.x, f1.y);
+            *reinterpret_cast<float4*>(low + G::A + bat[i] + r16 * 16) = make_float4(f2.x, f2.y, f3.x, f3.y);
           }
         }
         proxy_fence();
-        mbar_arrive(&s.full[st]);
-        ++nc;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.full[st]);
       };
       const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane, hc = r16 / 2;
       const uint32_t tlane = tmem + ((uint32_t)(quarter * 32) << 16);
@@ -354,37 +414,40 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
         wait(&s.dfull[nd & 1], nd >> 1, DEV_TIMEOUT_DRAIN);
         tc_after();
 #pragma unroll
-        for (int h = 0; h < RP / 2; h += 32) {
-          float t[32];
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            if (h + u * 8 < hc) ld8(tlane + (nd & 1) * 128 + half * hc + h + u * 8, t + u * 8);
+        for (int h = 0; h < RP / 2; h += 16) {
+          float t[16];
+          if (h < hc) ld8(tlane + (nd & 1) * 128 + half * hc + h, t);
+          if (h + 8 < hc) ld8(tlane + (nd & 1) * 128 + half * hc + h + 8, t + 8);
           wait_ld();
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
-            if (h + u * 8 < hc)
-#pragma unroll
-              for (int e = 0; e < 8; ++e) v[h + u * 8 + e] += t[u * 8 + e];
+          for (int e = 0; e < 16; ++e)
+            if (h + (e & 8) < hc) v[h + e] += t[e];
         }
         tc_before();
-        mbar_arrive(&s.dfree[nd & 1]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.dfree[nd & 1]);
         ++nd;
       };
-      if (nq > 0) load(0, xa[0], wb[0]);
-      if (nq > 1) load(1, xa[1], wb[1]);
+      if (F32 && nq > 0) weights(0);
+#pragma unroll 1
+      for (int q = 0; q < G::AHEAD; ++q) {
+        if (q < nq) fetch(q, nc + q);
+        copies_commit();
+      }
       int drained = 0;
-      for (int q = 0; q < nq; q += 2) {
-        store(xa[0], wb[0]);
-        if (q + 2 < nq) load(q + 2, xa[0], wb[0]);
-        if (q + 1 < nq) {
-          store(xa[1], wb[1]);
-          if (q + 3 < nq) load(q + 3, xa[1], wb[1]);
-        }
-        if (q + 2 >= (drained + 1) * G::CHAIN + 2 && q + 2 < nq) {  // the next chain is under way
+#pragma unroll 1
+      for (int q = 0; q < nq; ++q) {
+        if (q + G::AHEAD < nq) fetch(q + G::AHEAD, nc + q + G::AHEAD);
+        copies_commit();
+        copies_wait<G::AHEAD>();
+        ready(nc + q);
+        if (F32 && q + 1 < nq) weights(q + 1);
+        if (q + 1 == (drained + 1) * G::CHAIN + 2 && q + 1 < nq) {  // the next chain is under way
           drain();
           ++drained;
         }
       }
+      nc += nq;
       while (drained * G::CHAIN < nq) {
         drain();
         ++drained;
@@ -396,15 +459,23 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
         if (j < hc) parts[(half * hc + j) * 128 + row] = v[j];
       cluster_arrive();
       cluster_wait();
-#pragma unroll
-      for (int j = 0; j < RP / 2; ++j) v[j] = 0.f;
-      for (int d = 0; d < C; ++d) {
-        const float* p = cg::this_cluster().map_shared_rank(parts, d);
-#pragma unroll
-        for (int j = 0; j < RP / 2; ++j)
-          if (j < hc) v[j] += p[(half * hc + j) * 128 + row];
+      // each CTA adds up some columns, and all get the sums, in place of the chunks
+      float* sums = reinterpret_cast<float*>(smem);
+      {
+        const int j0 = r16 * rank_c / C, j1 = r16 * (rank_c + 1) / C;
+#pragma unroll 2
+        for (int i = j0 * 128 + tid; i < j1 * 128; i += kWorkers) {
+          float t = 0.f;
+#pragma unroll 8
+          for (int d = 0; d < C; ++d) t += *cg::this_cluster().map_shared_rank(parts + i, d);
+#pragma unroll 8
+          for (int d = 0; d < C; ++d) *cg::this_cluster().map_shared_rank(sums + i, d) = t;
+        }
       }
       cluster_arrive();
+      cluster_wait();
+#pragma unroll
+      for (int j = 0; j < RP / 2; ++j) v[j] = j < hc ? sums[(half * hc + j) * 128 + row] : 0.f;
       float most = 0.f;
 #pragma unroll
       for (int j = 0; j < RP / 2; ++j)
@@ -433,12 +504,12 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
         *reinterpret_cast<uint4*>(smem + G::V + at) = make_uint4(l[0], l[1], l[2], l[3]);
       }
       proxy_fence();
-      mbar_arrive(&s.vready);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.vready);
       // ---- out = y + factor * D ----
       float* turn = reinterpret_cast<float*>(smem + G::P_AT) + warp * 32 * kStagePitch;
       const T* y = reinterpret_cast<const T*>(a.y);
       T* out = reinterpret_cast<T*>(a.out);
-      cluster_wait();  // the parts here have been read everywhere
       for (int t = 0; t < nt; ++t, ++nd) {
 #pragma unroll 1
         for (int b = 0; b < 2; ++b) {
@@ -479,7 +550,8 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
           wait_ld();
           if (b == 1) {
             tc_before();
-            mbar_arrive(&s.dfree[nd & 1]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s.dfree[nd & 1]);
           }
           __syncwarp();
 #pragma unroll
@@ -529,11 +601,11 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
         ok = __all_sync(0xffffffffu, ok);
         tc_after();
         if (ok) {
-          const uint32_t base = sbase + st * G::STAGE;
-          const uint64_t bd = desc_blocks(base + (1 + F32) * G::A, lbo);
+          const uint32_t base = sbase + st * G::STAGE, low = sbase + NS * G::STAGE + (nc & 1) * G::LOW;
+          const uint64_t bd = desc_blocks((F32 ? low : base) + G::A, lbo);
 #pragma unroll
           for (int part = F32; part >= 0; --part) {  // the low part first
-            const uint64_t ad = desc_rows(base + part * G::A);
+            const uint64_t ad = desc_rows(part ? low : base);
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks)
               mma<F32>(on, tmem + (nd & 1) * 128, ad + ks * 2, bd + (uint64_t)(ks * 2 * lbo >> 4), id1,
@@ -560,9 +632,10 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
       };
       int fetched = 0;
       for (; fetched < min(2, nt); ++fetched) fetch(fetched);
-      cluster_arrive();
-      cluster_wait();
-      cluster_arrive();
+      for (int i = 0; i < 2; ++i) {  // as above
+        cluster_arrive();
+        cluster_wait();
+      }
       wait(&s.vready, nv, DEV_TIMEOUT_SMEM);
       for (int t = 0; t < nt; ++t, ++nd) {
         const int b = (nu + t) & 1;
@@ -593,7 +666,6 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
         for (int b = 0; b < 2; ++b)
           if (fetched > 0) mbar_wait(&s.upfull[b], (nu + fetched - 1) >> 1 & 1, nullptr, 0);
       nu += nt;
-      cluster_wait();
     }
     ++nv;
   }
