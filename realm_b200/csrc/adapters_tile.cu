@@ -34,6 +34,8 @@ namespace rb {
 namespace {
 
 constexpr int kWarps = 4, kWorkers = kWarps * 32, kTT = kWorkers + 32;  // fetch and finish; a warp for the products
+constexpr uint32_t kNoSlot = 0xffff;
+static_assert(kAdapterMaxSlots < (int)kNoSlot, "");
 constexpr int kSpanRows = 8192;                     // rows of a launch
 constexpr int kCols = 64;                           // columns of out a product covers
 constexpr int kUps = 3;                             // bulk copies of weights in flight or use
@@ -129,6 +131,15 @@ __device__ __forceinline__ void workers_sync() { asm volatile("bar.sync 1, 128;"
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
+// mbar_wait without unrolling, which keeps these kernels' code small: a short call waits for it, a line at a time
+__device__ __forceinline__ bool wait_rolled(uint64_t* bar, uint32_t parity, uint32_t* err, uint32_t code) {
+#pragma unroll 1
+  for (uint32_t i = 0; i < kSpinLimit; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  report_error(err, code);
+  return false;
+}
+
 // T: type of the rows. RP: ranks up to 64 (two CTAs an SM) or 128.
 template <class T, int RP>
 struct Cfg {
@@ -138,7 +149,10 @@ struct Cfg {
   static constexpr int NS = RP == 64 ? 5 : 8;       // blocks of a warp's ring: 32 rows x 128 bytes
   static constexpr int RING = NS * 4096;
   static constexpr int B = RP * 128;                // bytes of a chunk's weights, and of a tile of up
-  static constexpr int W_AT = kWarps * RING, MAIN = W_AT + kUps * B;
+  // weights: places for bulk copies, before them (fp32 rows) two chunks of weights in fp32, in whose place up goes later
+  static constexpr int RAW = F32 ? B / 2 : B, RAW_AT = F32 ? 2 * B : 0;
+  static constexpr int W_AT = kWarps * RING, W = RAW_AT + kUps * RAW > kUps * B ? RAW_AT + kUps * RAW : kUps * B;
+  static constexpr int MAIN = W_AT + W;
   static constexpr int PARTS = RP * 128 * 4;        // of v in fp32, in place of the rings: the CTA's part, then the sum
   static constexpr int CHAIN = F32 ? 256 / CE : 1024 / CE;  // chunks summed on the tensor core
   static constexpr int CTAS = RP == 64 ? 2 : 1;
@@ -146,7 +160,7 @@ struct Cfg {
   // TMEM columns: two accumulators (of kCols later), then two chunks of x (v later)
   static constexpr int D = RP, A0 = 2 * RP, AW = F32 ? 64 : 32, COLS = RP == 64 ? 256 : 512;
   // never more CTAs an SM than have columns
-  static_assert(CTAS * MAIN <= 226 * 1024 && (CTAS + 1) * MAIN > 228 * 1024 && 2 * PARTS <= W_AT, "");
+  static_assert(CTAS * MAIN <= 226 * 1024 && (CTAS + 1) * MAIN > 228 * 1024 && 2 * PARTS <= W_AT && 2 * kSpanRows <= W_AT, "");
   static_assert(A0 + 2 * AW <= COLS && A0 + RP <= COLS && 2 * kCols <= A0 && 2 * kCols == 128, "");
 };
 
@@ -172,20 +186,42 @@ __device__ __forceinline__ int4 slots4(const AdapterArgs& a, int i, bool vec) {
   return v;
 }
 
-// The rows of a tile: those of `slot` with ranks [r0, r0 + tile_rows) among its rows. Warp w has a
-// share of the rows, a lane four at a time.
-__device__ __forceinline__ int find_rows(const AdapterArgs& a, int slot, int r0, int tile_rows, TileShared& s) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rounds = (a.n_rows + kWarps * 128 - 1) / (kWarps * 128), i0 = warp * rounds * 32 + lane;
-  static_assert(kSpanRows <= kWarps * 128 * 16, "");
+// The rows' slots into shared memory, kNoSlot where there is none, by `threads` threads; f(slot of four rows) for each four.
+template <class F>
+__device__ __forceinline__ void load_slots(const AdapterArgs& a, uint16_t* to, int threads, F f) {
   const bool vec = (reinterpret_cast<uintptr_t>(a.slots) & 15) == 0;
+  const int quads = (a.n_rows + 127) / 128 * 32;  // whole warps
+#pragma unroll 1
+  for (int b = threadIdx.x & ~31; b < quads; b += 4 * threads) {
+    int4 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = slots4(a, b + u * threads + (threadIdx.x & 31), vec);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (b + u * threads >= quads) break;
+      auto in = [&](int x) { return x >= 0 && x < a.w.n_slots ? (uint32_t)x : kNoSlot; };
+      const uint32_t lo = in(v[u].x) | in(v[u].y) << 16, hi = in(v[u].z) | in(v[u].w) << 16;
+      reinterpret_cast<uint2*>(to)[b + u * threads + (threadIdx.x & 31)] = make_uint2(lo, hi);
+      f(lo, hi);
+    }
+  }
+}
+
+// The rows of a tile: those of `slot` with ranks [r0, r0 + tile_rows) among its rows. Warp w looks through a
+// share of the rows, a lane through four at a time. Rank i of the tile goes to row i / 4 of warp i % 4, so
+// that a small tile keeps all warps busy.
+__device__ __forceinline__ int find_rows(const AdapterArgs& a, const uint16_t* slots, int slot, int r0, int tile_rows,
+                                         TileShared& s) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int all = (a.n_rows + 127) / 128, rounds = (all + kWarps - 1) / kWarps, first = warp * rounds;
+  static_assert(kSpanRows <= kWarps * 128 * 16, "");
   unsigned long long mine = 0;  // bits 4 i .. 4 i + 3: the lane's rows of round i
-#pragma unroll 4
-  for (int i = 0; i < rounds; ++i) {
-    const int4 v = slots4(a, i0 + 32 * i, vec);
-    mine |= (unsigned long long)((uint32_t)(v.x == slot) | (uint32_t)(v.y == slot) << 1 | (uint32_t)(v.z == slot) << 2 |
-                                 (uint32_t)(v.w == slot) << 3)
-            << (4 * i);
+  const uint32_t both = (uint32_t)slot * 0x10001u;
+  for (int i = 0; i < rounds && first + i < all; ++i) {
+    const uint2 v = reinterpret_cast<const uint2*>(slots)[(first + i) * 32 + lane];
+    const uint32_t x = v.x ^ both, y = v.y ^ both;
+    const uint32_t m = (uint32_t)!(x & 0xffff) | (uint32_t)!(x >> 16) << 1 | (uint32_t)!(y & 0xffff) << 2 | (uint32_t)!(y >> 16) << 3;
+    mine |= (unsigned long long)m << (4 * i);
   }
   const int count = __reduce_add_sync(0xffffffffu, __popcll(mine));
   if (lane == 0) s.counts[warp] = count;
@@ -197,22 +233,19 @@ __device__ __forceinline__ int find_rows(const AdapterArgs& a, int slot, int r0,
     total += s.counts[w];
   }
   if (count && at < tile_rows && at + count > 0) {
-    for (int i = 0; i < rounds; ++i) {
+    for (int i = 0; i < rounds && at < tile_rows; ++i) {
       const uint32_t m = (uint32_t)(mine >> (4 * i)) & 15;
-      int incl = __popc(m);
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += y;
-      }
-      int rank = at + incl - __popc(m);
+      const uint32_t b0 = __ballot_sync(0xffffffffu, m & 1), b1 = __ballot_sync(0xffffffffu, m & 2),
+                     b2 = __ballot_sync(0xffffffffu, m & 4), b3 = __ballot_sync(0xffffffffu, m & 8);
+      const uint32_t below = (1u << lane) - 1;
+      int rank = at + __popc(b0 & below) + __popc(b1 & below) + __popc(b2 & below) + __popc(b3 & below);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (m >> e & 1) {
-          if (rank >= 0 && rank < tile_rows) s.rows[rank] = 4 * (i0 + 32 * i) + e;
+          if (rank >= 0 && rank < tile_rows) s.rows[(rank & 3) * 32 + (rank >> 2)] = 4 * ((first + i) * 32 + lane) + e;
           ++rank;
         }
-      at += __shfl_sync(0xffffffffu, incl, 31);
+      at += __popc(b0) + __popc(b1) + __popc(b2) + __popc(b3);
     }
   }
   workers_sync();
@@ -259,30 +292,25 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
   const uint32_t tmem = s.tmem;
 
   // ---- tiles: rows of every slot, then the first tile of each ----
-  {
-    const bool vec = (reinterpret_cast<uintptr_t>(a.slots) & 15) == 0;
-    auto count = [&](int v, int n) {
-      if (v >= 0 && v < a.w.n_slots) atomicAdd(&start[v], n);
+  uint16_t* slots = reinterpret_cast<uint16_t*>(smem);  // while the rings are empty
+  load_slots(a, slots, kTT, [&](uint32_t x, uint32_t y) {
+    auto count = [&](uint32_t v, int n) {
+      if (v != kNoSlot) atomicAdd(&start[v], n);
     };
-    const int quads = (a.n_rows + 3) / 4;
-#pragma unroll 4
-    for (int b = warp * 32; b < quads; b += kTT) {
-      const int4 v = b + lane < quads ? slots4(a, b + lane, vec) : make_int4(-1, -1, -1, -1);
-      const bool same = v.x == v.y && v.x == v.z && v.x == v.w;
-      const int lead = __shfl_sync(0xffffffffu, v.x, 0);
-      // mostly rows of one slot follow one another
-      if (__all_sync(0xffffffffu, same && v.x == lead)) {
-        if (lane == 0) count(v.x, 128);
-      } else if (same) {
-        count(v.x, 4);
-      } else {
-        count(v.x, 1);
-        count(v.y, 1);
-        count(v.z, 1);
-        count(v.w, 1);
-      }
+    const bool same = x == y && x >> 16 == (x & 0xffff);
+    const uint32_t lead = __shfl_sync(0xffffffffu, x, 0);
+    // mostly rows of one slot follow one another
+    if (__all_sync(0xffffffffu, same && x == lead)) {
+      if (lane == 0) count(x & 0xffff, 128);
+    } else if (same) {
+      count(x & 0xffff, 4);
+    } else {
+      count(x & 0xffff, 1);
+      count(x >> 16, 1);
+      count(y & 0xffff, 1);
+      count(y >> 16, 1);
     }
-  }
+  });
   __syncthreads();
   if (warp < kWarps) {
     int base = 0;
@@ -315,7 +343,7 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
 
   bool ok = true;
   auto wait = [&](uint64_t* bar, uint32_t n, uint32_t code) {  // for the bar's n-th completion
-    if (ok) ok = mbar_wait(bar, n & 1, a.err, code);
+    if (ok) ok = wait_rolled(bar, n & 1, a.err, code);
     __syncwarp();
   };
   uint32_t nc = 0, nd = 0, no = 0, nv = 0, nw = 0;  // chunks, accumulators of v and out, tiles, copies of weights so far
@@ -338,7 +366,11 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
     const uint16_t* up = a.w.up + (int64_t)slot * a.w.rp * a.w.n;
 
     if (warp < kWarps) {
-      const int cnt = find_rows(a, slot, (tile - start[slot]) * tile_rows, tile_rows, s);
+      if (tile != cluster) {  // the rings have been in use
+        load_slots(a, slots, kWorkers, [](uint32_t, uint32_t) {});
+        workers_sync();
+      }
+      const int cnt = find_rows(a, slots, slot, (tile - start[slot]) * tile_rows, tile_rows, s);
       const int row = warp * 32 + lane;
       const uint32_t tlane = tmem + ((uint32_t)(warp * 32) << 16);
       // Blocks of the ring are 32 rows x 128 bytes, piece p of row r at r * 128 + (p ^ r & 7) * 16. A lane
@@ -349,41 +381,35 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
       const uint32_t put0 = top * 128 + ((piece ^ top) << 4), put1 = top * 128 + ((piece ^ top ^ 4) << 4);  // even, odd j
       // ---- fetch x and down ----
       const int first = q0 * G::CE + piece * E;
+      // the lane's rows that there are, the first ones of eight
+      const int mine = min(8, max(0, (cnt - warp + kWarps - 1) / kWarps - top + 3) / 4);
       const T* xp[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int r = warp * 32 + 4 * j + top;
-        xp[j] = r < cnt ? reinterpret_cast<const T*>(a.x) + s.rows[r] * a.ldx + first : nullptr;
-      }
+      for (int j = 0; j < 8; ++j)
+        xp[j] = reinterpret_cast<const T*>(a.x) + (j < mine ? s.rows[warp * 32 + 4 * j + top] : 0) * a.ldx + first;
+      uint32_t to = 0;  // the place in the ring that is filled next
       auto fetch = [&](int q) {
-        const uint32_t to = (uint32_t)(q % NS) * 4096;
         const int left = a.w.k - first - q * G::CE;  // elements up to the row's end
         if (VX && left >= E) {
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            if (xp[j]) copy16(ring_at + to + (j & 1 ? put1 : put0) + j * 512, xp[j] + q * G::CE);
+            if (j < mine) copy16(ring_at + to + (j & 1 ? put1 : put0) + j * 512, xp[j] + q * G::CE);
         } else {
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            if (xp[j]) copy_single(ring + to + (j & 1 ? put1 : put0) + j * 512, xp[j] + q * G::CE, left);
+            if (j < mine) copy_single(ring + to + (j & 1 ? put1 : put0) + j * 512, xp[j] + q * G::CE, left);
         }
       };
-      // fp32: a chunk's weights by 16-byte pieces, each of which becomes two of fp32
+      // where the pieces of weights that a thread has of a chunk go
       constexpr int NB = F32 ? RP * 4 / kWorkers : 1;
-      const int items = r16 * 4;
-      const uint4* wp = reinterpret_cast<const uint4*>(down) + (int64_t)q0 * items + tid;
-      uint4 wb[NB];  // the next chunk's
-      auto weights = [&](int q) {
-        if constexpr (F32) {
+      uint32_t bat[NB];
 #pragma unroll
-          for (int i = 0; i < NB; ++i)
-            if (tid + i * kWorkers < items) wb[i] = __ldg(wp + (int64_t)q * items + i * kWorkers);
-        }
-      };
+      for (int i = 0; i < NB; ++i) bat[i] = ((tid + i * kWorkers) / r16 * 2 * r16 + (tid + i * kWorkers) % r16) * 16;
       // chunk q is here: into the operands of the products
+      uint32_t at = 0;  // the place that is read next
       auto ready = [&](int q) {
         const uint32_t b = nc & 1, to = tlane + G::A0 + b * G::AW;
-        const uint8_t* from = ring + q % NS * 4096 + lane * 128;
+        const uint8_t* from = ring + at + lane * 128;
         if (nc >= 2) wait(&s.empty[b], nc / 2 - 1, DEV_TIMEOUT_EMPTY);
         tc_after();
 #pragma unroll
@@ -398,21 +424,25 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
           if constexpr (F32) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const float f = __uint_as_float(x[e]), g = __uint_as_float(x[e] & 0xffffe000u);
-              x[e] = f == g ? 0u : __float_as_uint(f - g) + 0x1000u;  // to the nearest; 0 for infinities
+              const float f = __uint_as_float(x[e]) - __uint_as_float(x[e] & 0xffffe000u);
+              x[e] = __float_as_uint(f) + 0x1000u;  // to the nearest
             }
             st16(to + 32 + h * 16, x);
           }
         }
-        if constexpr (F32) {
+        if constexpr (F32) {  // 16-byte pieces of weights, each of which becomes two of fp32
+          wait(&s.wfull[(nw + q) % kUps], (nw + q) / kUps, DEV_TIMEOUT_FULL);
+          const uint4* raw = reinterpret_cast<const uint4*>(smem + G::W_AT + G::RAW_AT + (nw + q) % kUps * G::RAW);
           uint8_t* wbase = smem + G::W_AT + b * G::B;
+          const int items = r16 * 4;
 #pragma unroll
           for (int i = 0; i < NB; ++i) {
             const int it = tid + i * kWorkers;
             if (it >= items) continue;
-            uint8_t* w = wbase + (it / r16 * 2 * r16 + it % r16) * 16;
-            const float2 f0 = __half22float2(u32_as_h2(wb[i].x)), f1 = __half22float2(u32_as_h2(wb[i].y)),
-                         f2 = __half22float2(u32_as_h2(wb[i].z)), f3 = __half22float2(u32_as_h2(wb[i].w));
+            const uint4 t = raw[it];
+            uint8_t* w = wbase + bat[i];
+            const float2 f0 = __half22float2(u32_as_h2(t.x)), f1 = __half22float2(u32_as_h2(t.y)),
+                         f2 = __half22float2(u32_as_h2(t.z)), f3 = __half22float2(u32_as_h2(t.w));
             *reinterpret_cast<float4*>(w) = make_float4(f0.x, f0.y, f1.x, f1.y);
             *reinterpret_cast<float4*>(w + r16 * 16) = make_float4(f2.x, f2.y, f3.x, f3.y);
           }
@@ -446,7 +476,6 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
         if (lane == 0) mbar_arrive(&s.dfree[nd & 1]);
         ++nd;
       };
-      if (nq > 0) weights(0);
       // one place for all fetches: the chunks NS - 1 ahead, before the first only those
       int drained = 0;
 #pragma unroll 1
@@ -457,9 +486,10 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
         }
         if (q + NS - 1 < nq) fetch(q + NS - 1);
         copies_commit();
+        to = to == (NS - 1) * 4096 ? 0 : to + 4096;
         if (q < 0) continue;
         ready(q);
-        if (q + 1 < nq) weights(q + 1);
+        at = at == (NS - 1) * 4096 ? 0 : at + 4096;
         if (q == (drained + 1) * G::CHAIN && q + 1 < nq) {  // the next chain is under way
           drain();
           ++drained;
@@ -481,16 +511,17 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
       cluster_wait();
       // each CTA adds up some columns, and all get the sums
       float* sums = reinterpret_cast<float*>(smem + G::PARTS);
-      {
-        const int j0 = r16 * rank_c / C, j1 = r16 * (rank_c + 1) / C;
-#pragma unroll 2
-        for (int i = j0 * 128 + tid; i < j1 * 128; i += kWorkers) {
-          float t = 0.f;
-#pragma unroll 8
-          for (int d = 0; d < C; ++d) t += *cg::this_cluster().map_shared_rank(parts + i, d);
-#pragma unroll 8
-          for (int d = 0; d < C; ++d) *cg::this_cluster().map_shared_rank(sums + i, d) = t;
-        }
+      for (int i = r16 * rank_c / C * 32 + tid; i < r16 * (rank_c + 1) / C * 32; i += kWorkers) {
+        float4 p[8], t = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int d = 0; d < 8; ++d)
+          if (d < C) p[d] = *cg::this_cluster().map_shared_rank(reinterpret_cast<float4*>(parts) + i, d);
+#pragma unroll
+        for (int d = 0; d < 8; ++d)
+          if (d < C) t = make_float4(t.x + p[d].x, t.y + p[d].y, t.z + p[d].z, t.w + p[d].w);
+#pragma unroll
+        for (int d = 0; d < 8; ++d)
+          if (d < C) *cg::this_cluster().map_shared_rank(reinterpret_cast<float4*>(sums) + i, d) = t;
       }
       cluster_arrive();
       cluster_wait();
@@ -510,20 +541,6 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
       const T* y = reinterpret_cast<const T*>(a.y);
       T* out = reinterpret_cast<T*>(a.out);
       const int blocks = nt * PER;
-      auto fetch_y = [&](int i) {
-        const uint32_t to = (uint32_t)(i % NS) * 4096;
-        const int col = n0 + i * BC + piece * E, left = n1 - col;
-        if (left <= 0) return;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int r = warp * 32 + 4 * j + top;
-          if (r >= cnt) continue;
-          const T* p = y + s.rows[r] * a.ldy + col;
-          const uint32_t at = to + (j & 1 ? put1 : put0) + j * 512;
-          if (VY && left >= E) copy16(ring_at + at, p);
-          else copy_single(ring + at, p, left);
-        }
-      };
       auto multiply_v = [&] {
 #pragma unroll
         for (int u = 0; u < RP / 8; ++u) {
@@ -535,7 +552,7 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
             const __half2 hh = __floats2half2_rn(x0, x1);
             const float2 hf = __half22float2(hh);
             h[e] = h2_as_u32(hh);
-            l[e] = h2_as_u32(__floats2half2_rn(x0 == hf.x ? 0.f : x0 - hf.x, x1 == hf.y ? 0.f : x1 - hf.y));
+            l[e] = h2_as_u32(__floats2half2_rn(x0 - hf.x, x1 - hf.y));
           }
           st4(tlane + G::A0 + u * 4, h);
           st4(tlane + G::A0 + RP / 2 + u * 4, l);
@@ -546,11 +563,33 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
         if (lane == 0) mbar_arrive(&s.vready);
       };
       multiply_v();
+      const T* yp[8];
+      T* op[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int r = j < mine ? s.rows[warp * 32 + 4 * j + top] : 0;
+        yp[j] = y + r * a.ldy + n0 + piece * E;
+        op[j] = out + r * a.ldo + n0 + piece * E;
+      }
+      to = at = 0;
+      auto fetch_y = [&](int i) {
+        const int left = n1 - n0 - i * BC - piece * E;
+        if (VY && left >= E) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (j < mine) copy16(ring_at + to + (j & 1 ? put1 : put0) + j * 512, yp[j] + i * BC);
+        } else if (left > 0) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (j < mine) copy_single(ring + to + (j & 1 ? put1 : put0) + j * 512, yp[j] + i * BC, left);
+        }
+      };
       // ---- out = y + factor * D ----
 #pragma unroll 1
       for (int i = 1 - NS; i < blocks; ++i) {
         if (i + NS - 1 < blocks) fetch_y(i + NS - 1);
         copies_commit();
+        to = to == (NS - 1) * 4096 ? 0 : to + 4096;
         if (i < 0) continue;
         const uint32_t tile_o = no + i / PER;
         if (i % PER == 0) {
@@ -559,7 +598,8 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
         }
         copies_wait<NS - 1>();
         __syncwarp();
-        uint8_t* block = ring + i % NS * 4096;
+        uint8_t* block = ring + at;
+        at = at == (NS - 1) * 4096 ? 0 : at + 4096;
         const uint32_t from = tlane + (tile_o & 1) * kCols + i % PER * BC;
 #pragma unroll
         for (int c = 0; c < BC; c += 16) {
@@ -592,30 +632,25 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
           }
         }
         __syncwarp();
-        const int col = n0 + i * BC + piece * E, left = n1 - col;
-        if (left > 0) {
+        const int left = n1 - n0 - i * BC - piece * E;
+        if (VY && left >= E) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (j < mine) *reinterpret_cast<uint4*>(op[j] + i * BC) = *reinterpret_cast<const uint4*>(block + (j & 1 ? put1 : put0) + j * 512);
+        } else if (left > 0) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const int r = warp * 32 + 4 * j + top;
-            if (r >= cnt) continue;
-            const uint4 t = *reinterpret_cast<const uint4*>(block + (j & 1 ? put1 : put0) + j * 512);
-            T* o = out + s.rows[r] * a.ldo + col;
-            if (VY && left >= E) {
-              *reinterpret_cast<uint4*>(o) = t;
-            } else {
-              const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+            if (j >= mine) continue;
+            const T* t = reinterpret_cast<const T*>(block + (j & 1 ? put1 : put0) + j * 512);
 #pragma unroll
-              for (int e = 0; e < E; ++e)
-                if (e < left) {
-                  if constexpr (F32) o[e] = __uint_as_float(w[e]);
-                  else o[e] = __ushort_as_half((unsigned short)(w[e / 2] >> 16 * (e & 1)));
-                }
-            }
+            for (int e = 0; e < E; ++e)
+              if (e < left) op[j][i * BC + e] = t[e];
           }
         }
         __syncwarp();  // before the block's place is filled again
       }
       no += nt;
+      nw += nq + nt;  // as the products' warp counts
       copies_wait<0>();
       workers_sync();  // before the next tile's rows
     } else {
@@ -623,17 +658,17 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
       const uint32_t lbo = (uint32_t)r16 * 16;
       const uint32_t id1 = idesc_of(F32, r16), id2 = idesc_of(0, kCols);
       // copies of weights take the places in turn
-      auto place = [&](uint32_t i) { return sbase + G::W_AT + i % kUps * G::B; };
       auto expect = [&](uint32_t i, int bytes) {
         if (lane == 0) mbar_arrive_expect_tx(&s.wfull[i % kUps], (uint32_t)bytes);
         __syncwarp();
       };
-      auto fetch_down = [&](int q) {  // fp16: a chunk's weights as they lie
+      auto fetch_down = [&](int q) {  // a chunk's weights as they lie
         const uint32_t i = nw + q;
         if (!ok) return;
-        expect(i, r16 * 128);
+        expect(i, r16 * G::CE * 2);
         if (lane == 0)
-          bulk_g2s(smem + G::W_AT + i % kUps * G::B, down + (int64_t)(q0 + q) * 64 * r16, (uint32_t)(r16 * 128), &s.wfull[i % kUps]);
+          bulk_g2s(smem + G::W_AT + G::RAW_AT + i % kUps * G::RAW, down + (int64_t)(q0 + q) * G::CE * r16,
+                   (uint32_t)(r16 * G::CE * 2), &s.wfull[i % kUps]);
       };
       auto fetch_up = [&](int t) {  // columns n0 + 64 t ...
         const uint32_t i = nw + t;
@@ -645,8 +680,7 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
                    (uint32_t)(rows * 16), &s.wfull[i % kUps]);
       };
       int fetched = 0;
-      if (!F32)
-        for (; fetched < min(kUps, nq); ++fetched) fetch_down(fetched);
+      for (; fetched < min(kUps, nq); ++fetched) fetch_down(fetched);
 #pragma unroll 1
       for (int q = 0; q < nq; ++q, ++nc) {
         const uint32_t b = nc & 1;
@@ -656,7 +690,7 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
         ok = __all_sync(0xffffffffu, ok);
         tc_after();
         if (ok) {
-          const uint64_t bd = desc_blocks(F32 ? sbase + G::W_AT + b * G::B : place(nw + q), lbo);
+          const uint64_t bd = desc_blocks(sbase + G::W_AT + (F32 ? b : (nw + q) % kUps) * G::B, lbo);
 #pragma unroll
           for (int part = F32; part >= 0; --part)  // the low part first
 #pragma unroll
@@ -669,8 +703,9 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
           if (ok) commit(on, &s.dfull[nd & 1]);
           ++nd;
         }
-        if (!F32 && q > 0 && fetched < nq) {  // into the place that the product before this one has read
-          wait(&s.empty[b ^ 1], (nc - 1) / 2, DEV_TIMEOUT_EMPTY);
+        // into the place that the threads have read, for the chunk at hand (fp32), or the product before this one
+        if ((F32 || q > 0) && fetched < nq) {
+          if (!F32) wait(&s.empty[b ^ 1], (nc - 1) / 2, DEV_TIMEOUT_EMPTY);
           ok = __all_sync(0xffffffffu, ok);
           fetch_down(fetched++);
         }
@@ -681,7 +716,7 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
             mbar_wait(&s.wfull[(nw + t) % kUps], (nw + t) / kUps & 1, nullptr, 0);
       };
       land();
-      if (!F32) nw += nq;
+      nw += nq;
       // the weights' places are free once the last accumulator is there
       if (nq > 0) wait(&s.dfull[(nd - 1) & 1], (nd - 1) >> 1, DEV_TIMEOUT_DRAIN);
       ok = __all_sync(0xffffffffu, ok);
@@ -699,7 +734,7 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
         ok = __all_sync(0xffffffffu, ok);
         tc_after();
         if (ok) {
-          const uint64_t bd = desc_blocks(place(nw + t), kCols * 16);
+          const uint64_t bd = desc_blocks(sbase + G::W_AT + (nw + t) % kUps * G::B, kCols * 16);
 #pragma unroll 1
           for (int part = 1; part >= 0; --part)
 #pragma unroll 1
@@ -743,11 +778,12 @@ cudaError_t launch(const AdapterArgs& a, int num_sms, cudaStream_t s) {
   const int smem = G::smem(a.w.n_slots);
   if (cudaError_t e = ensure_smem_attr(adapters_tile_kernel<T, RP, VX, VY>, G::smem(kAdapterMaxSlots), dev)) return e;
   const int ctas = num_sms * (2 * (smem + 3072) <= 228 * 1024 ? G::CTAS : 1);
-  // Small tiles while there are too few rows for all CTAs, then smaller clusters.
-  int tile_rows = 128;
-  while (tile_rows > 16 && (a.n_rows + tile_rows - 1) / tile_rows * 8 < ctas) tile_rows /= 2;
-  int cluster = 8;
-  while (cluster > 2 && (a.n_rows + tile_rows - 1) / tile_rows * cluster > ctas) cluster /= 2;
+  // Clusters of eight, and the smallest tiles whose CTAs all run at once: a CTA's steps over k and n, more than its
+  // rows, are what a call of few rows takes. Where even tiles of 128 rows are too many, smaller clusters.
+  auto tiles = [&](int rows) { return (a.n_rows + rows - 1) / rows; };
+  int tile_rows = 128, cluster = 8;
+  while (tile_rows > 16 && tiles(tile_rows / 2) * cluster <= ctas) tile_rows /= 2;
+  while (cluster > 4 && tiles(tile_rows) * cluster > ctas) cluster /= 2;
   const int most = a.n_rows / tile_rows + std::min(a.w.n_slots, a.n_rows);  // tiles
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(std::min(std::max(1, ctas / cluster), most) * cluster));
