@@ -56,12 +56,141 @@ __device__ __forceinline__ int slot_of(const AdapterArgs& a, int row) {
   return s >= 0 && s < a.w.n_slots && a.w.meta[s].rank > 0 ? s : -1;
 }
 
+template <int R>
+struct ItemShared {
+  __align__(16) float xs[R][kTileK];
+  float part[kAdapterMaxRank * R];                // [k part][rank][row]
+  float parts[kMaxCluster][kAdapterMaxRank * R];  // every CTA's v
+  __align__(16) float v[kAdapterMaxRank * R];     // [rank][row]
+};
+
+// Up to R rows of one slot, by a cluster.
+template <class T, int R, int RS>
+__device__ __forceinline__ void run_item(const AdapterArgs& a, ItemShared<RS>& sh, int slot, const int (&rows)[R], int nr) {
+  auto& xs = sh.xs;
+  float *part = sh.part, *v = sh.v;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = (int)cluster.num_blocks(), c = (int)cluster.block_rank();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const T* x = reinterpret_cast<const T*>(a.x);
+  const T* y = reinterpret_cast<const T*>(a.y);
+  T* out = reinterpret_cast<T*>(a.out);
+  // this CTA's columns of out
+  const int n0 = (int)((int64_t)a.w.n * c / C), n1 = (int)((int64_t)a.w.n * (c + 1) / C);
+  cluster.barrier_arrive();
+  const int rank = a.w.meta[slot].rank;
+  const float scale = a.w.meta[slot].scale;
+  const int groups = (rank + kGroup - 1) / kGroup, r16 = (rank + 15) / 16 * 16;
+  // warps are split over groups of ranks, and with few of those over k
+  const int ks = groups >= kWarps ? 1 : kWarps / groups, kpart = ks == 1 ? 0 : warp / groups;
+  const int chunks = a.w.kp / 8, c0 = (int)((int64_t)chunks * c / C), c1 = (int)((int64_t)chunks * (c + 1) / C);
+  const uint16_t* down = a.w.down + (int64_t)slot * a.w.rp * a.w.kp;
+  const uint16_t* up = a.w.up + (int64_t)slot * a.w.rp * a.w.n;
+  // what comes after v on its way to L2: a line of 128 bytes a thread
+  for (int i = tid, per = (n1 - n0 + 7) / 8; i < per * ((rank + 7) / 8); i += kT)
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(up + ((int64_t)(i / per) * a.w.n + n0 + i % per * 8) * 8));
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    for (int j = n0 + tid * 32; r < nr && j < n1; j += kT * 32)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(y + rows[r] * a.ldy + j));
+  const int nv = groups * kGroup * R;  // of a k part; ks > 1: at most kWarps groups in all
+  for (int i = tid; i < ks * nv; i += kT) part[i] = 0.f;
+  for (int t0 = c0; t0 < c1; t0 += kTileK / 8) {
+    const int t1 = min(c1, t0 + kTileK / 8), len = (t1 - t0) * 8, k0 = t0 * 8;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      for (int j = tid; j < len; j += kT) xs[r][j] = r < nr && k0 + j < a.w.k ? to_f(x[rows[r] * a.ldx + k0 + j]) : 0.f;
+    __syncthreads();
+    if (kpart < ks) {
+      const int b0 = (t1 - t0) * kpart / ks, b1 = (t1 - t0) * (kpart + 1) / ks;
+      for (int g = ks == 1 ? warp : warp % groups; g < groups; g += ks == 1 ? kWarps : groups) {
+        float acc[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) acc[r] = 0.f;
+        // a lane has rank g * 8 + lane % 8 of every fourth block of 8 elements
+        const uint4* w = reinterpret_cast<const uint4*>(down) + (int64_t)t0 * r16 + g * kGroup + (lane & 7);
+#pragma unroll 4
+        for (int b = b0 + (lane >> 3); b < b1; b += 4) {
+          float f[8];
+          unpack8(__ldg(w + (int64_t)b * r16), f);
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const float4 lo = *reinterpret_cast<const float4*>(&xs[r][b * 8]),
+                         hi = *reinterpret_cast<const float4*>(&xs[r][b * 8 + 4]);
+            const float xv[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[r] = fmaf(f[e], xv[e], acc[r]);
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], 8);
+          acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], 16);
+          if (lane < 8) part[kpart * nv + (g * kGroup + lane) * R + r] += acc[r];
+        }
+      }
+    }
+  }
+  __syncthreads();
+  cluster.barrier_wait();  // every CTA of the cluster runs before its shared memory is written
+  for (int i = tid; i < nv; i += kT) {
+    float s = 0.f;
+    for (int p = 0; p < ks; ++p) s += part[p * nv + i];
+    for (int d = 0; d < C; ++d) *cluster.map_shared_rank(&sh.parts[c][i], d) = s;
+  }
+  cluster.sync();
+  for (int i = tid; i < (rank + 7) / 8 * 8 * R; i += kT) {
+    float s = 0.f;
+    if (i < nv)
+      for (int d = 0; d < C; ++d) s += sh.parts[d][i];
+    v[i] = s * scale;
+  }
+  __syncthreads();
+  const int blocks8 = (rank + 7) / 8;
+  for (int j0 = n0 + tid; j0 < n1; j0 += 2 * kT) {  // two columns at a time, up to four blocks of each on their way
+    float acc[2][R];
+#pragma unroll
+    for (int c2 = 0; c2 < 2; ++c2)
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        acc[c2][r] = j0 + c2 * kT < n1 && r < nr ? to_f(y[rows[r] * a.ldy + j0 + c2 * kT]) : 0.f;
+#pragma unroll 1
+    for (int h0 = 0; h0 < blocks8; h0 += 4) {
+      uint4 q[2][4];
+#pragma unroll
+      for (int h = 0; h < 4; ++h)
+#pragma unroll
+        for (int c2 = 0; c2 < 2; ++c2) {
+          q[c2][h] = make_uint4(0, 0, 0, 0);
+          if (h0 + h < blocks8 && j0 + c2 * kT < n1)
+            q[c2][h] = __ldg(reinterpret_cast<const uint4*>(up + ((int64_t)(h0 + h) * a.w.n + j0 + c2 * kT) * 8));
+        }
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        if (h0 + h >= blocks8) continue;
+#pragma unroll
+        for (int c2 = 0; c2 < 2; ++c2) {
+          float f[8];
+          unpack8(q[c2][h], f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int r = 0; r < R; ++r) acc[c2][r] = fmaf(f[e], v[((h0 + h) * 8 + e) * R + r], acc[c2][r]);
+        }
+      }
+    }
+#pragma unroll
+    for (int c2 = 0; c2 < 2; ++c2)
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (r < nr && j0 + c2 * kT < n1) out[rows[r] * a.ldo + j0 + c2 * kT] = from_f<T>(acc[c2][r]);
+  }
+}
+
 template <class T, int R>
-__global__ void __launch_bounds__(kT) adapters_kernel(const __grid_constant__ AdapterArgs a) {
-  __shared__ __align__(16) float xs[R][kTileK];
-  __shared__ float part[kAdapterMaxRank * R];                        // [k part][rank][row]
-  __shared__ float parts[kMaxCluster][kAdapterMaxRank * R];          // every CTA's v
-  __shared__ __align__(16) float v[kAdapterMaxRank * R];             // [rank][row]
+__global__ void __launch_bounds__(kT, 4) adapters_kernel(const __grid_constant__ AdapterArgs a) {
+  __shared__ ItemShared<R> sh;
   __shared__ int s_slot[kBlock], s_rows[R], s_n, s_item;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), c = (int)cluster.block_rank();
@@ -120,94 +249,16 @@ __global__ void __launch_bounds__(kT) adapters_kernel(const __grid_constant__ Ad
 #pragma unroll
     for (int r = 0; r < R; ++r) rows[r] = s_rows[min(r, nr - 1)];
   }
-  const T* x = reinterpret_cast<const T*>(a.x);
-  const T* y = reinterpret_cast<const T*>(a.y);
-  T* out = reinterpret_cast<T*>(a.out);
-  // this CTA's columns of out
-  const int n0 = (int)((int64_t)a.w.n * c / C), n1 = (int)((int64_t)a.w.n * (c + 1) / C);
   if (slot < 0) {
     if (a.out != a.y)
-      for (int j = n0 + tid; j < n1; j += kT) out[rows[0] * a.ldo + j] = y[rows[0] * a.ldy + j];
+      for (int j = (int)((int64_t)a.w.n * c / C) + tid; j < (int)((int64_t)a.w.n * (c + 1) / C); j += kT) reinterpret_cast<T*>(a.out)[rows[0] * a.ldo + j] = reinterpret_cast<const T*>(a.y)[rows[0] * a.ldy + j];
     return;  // the whole cluster
   }
-  cluster.barrier_arrive();
-  const int rank = a.w.meta[slot].rank;
-  const float scale = a.w.meta[slot].scale;
-  const int groups = (rank + kGroup - 1) / kGroup, r16 = (rank + 15) / 16 * 16;
-  // warps are split over groups of ranks, and with few of those over k
-  const int ks = groups >= kWarps ? 1 : kWarps / groups, kpart = ks == 1 ? 0 : warp / groups;
-  const int chunks = a.w.kp / 8, c0 = (int)((int64_t)chunks * c / C), c1 = (int)((int64_t)chunks * (c + 1) / C);
-  const uint16_t* down = a.w.down + (int64_t)slot * a.w.rp * a.w.kp;
-  const int nv = groups * kGroup * R;  // of a k part; ks > 1: at most kWarps groups in all
-  for (int i = tid; i < ks * nv; i += kT) part[i] = 0.f;
-  for (int t0 = c0; t0 < c1; t0 += kTileK / 8) {
-    const int t1 = min(c1, t0 + kTileK / 8), len = (t1 - t0) * 8, k0 = t0 * 8;
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-      for (int j = tid; j < len; j += kT) xs[r][j] = r < nr && k0 + j < a.w.k ? to_f(x[rows[r] * a.ldx + k0 + j]) : 0.f;
-    __syncthreads();
-    if (kpart < ks) {
-      const int b0 = (t1 - t0) * kpart / ks, b1 = (t1 - t0) * (kpart + 1) / ks;
-      for (int g = ks == 1 ? warp : warp % groups; g < groups; g += ks == 1 ? kWarps : groups) {
-        float acc[R];
-#pragma unroll
-        for (int r = 0; r < R; ++r) acc[r] = 0.f;
-        // a lane has rank g * 8 + lane % 8 of every fourth block of 8 elements
-        const uint4* w = reinterpret_cast<const uint4*>(down) + (int64_t)t0 * r16 + g * kGroup + (lane & 7);
-#pragma unroll 4
-        for (int b = b0 + (lane >> 3); b < b1; b += 4) {
-          float f[8];
-          unpack8(__ldg(w + (int64_t)b * r16), f);
-#pragma unroll
-          for (int r = 0; r < R; ++r) {
-            const float4 lo = *reinterpret_cast<const float4*>(&xs[r][b * 8]),
-                         hi = *reinterpret_cast<const float4*>(&xs[r][b * 8 + 4]);
-            const float xv[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) acc[r] = fmaf(f[e], xv[e], acc[r]);
-          }
-        }
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], 8);
-          acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], 16);
-          if (lane < 8) part[kpart * nv + (g * kGroup + lane) * R + r] += acc[r];
-        }
-      }
-    }
-  }
-  __syncthreads();
-  cluster.barrier_wait();  // every CTA of the cluster runs before its shared memory is written
-  for (int i = tid; i < nv; i += kT) {
-    float s = 0.f;
-    for (int p = 0; p < ks; ++p) s += part[p * nv + i];
-    for (int d = 0; d < C; ++d) *cluster.map_shared_rank(&parts[c][i], d) = s;
-  }
-  cluster.sync();
-  for (int i = tid; i < (rank + 7) / 8 * 8 * R; i += kT) {
-    float s = 0.f;
-    if (i < nv)
-      for (int d = 0; d < C; ++d) s += parts[d][i];
-    v[i] = s;
-  }
-  __syncthreads();
-  const uint16_t* up = a.w.up + (int64_t)slot * a.w.rp * a.w.n;
-  for (int j = n0 + tid; j < n1; j += kT) {
-    float acc[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) acc[r] = 0.f;
-    for (int h = 0; h < (rank + 7) / 8; ++h) {
-      float f[8];
-      unpack8(__ldg(reinterpret_cast<const uint4*>(up + ((int64_t)h * a.w.n + j) * 8)), f);
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-#pragma unroll
-        for (int r = 0; r < R; ++r) acc[r] = fmaf(f[e], v[(h * 8 + e) * R + r], acc[r]);
-    }
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-      if (r < nr) out[rows[r] * a.ldo + j] = from_f<T>(fmaf(scale, acc[r], to_f(y[rows[r] * a.ldy + j])));
+  if (R > 1 && nr == 1) {
+    const int one[1] = {rows[0]};
+    run_item<T, 1, R>(a, sh, slot, one, 1);
+  } else {
+    run_item<T, R, R>(a, sh, slot, rows, nr);
   }
 }
 
@@ -265,7 +316,9 @@ cudaError_t adapters_clear_launch(AdapterMeta* meta, cudaStream_t s) {
 }
 
 cudaError_t adapters_launch(const AdapterArgs& a, int num_sms, cudaStream_t s) {
-  if (a.n_rows > 64) return adapters_tile_launch(a, num_sms, s);
+  // Rows of one adapter, k = n = 4096, fp32, rank 64: 256 rows 35 us here and 51 in tiles, 512 59 and 55, 1024 111 and
+  // 57; rank 16 fp16: 256 25 and 31, 512 41 and 33. Every row another's (rank 64): 256 rows 111 us and 578.
+  if (a.n_rows > 384) return adapters_tile_launch(a, num_sms, s);
   const int cluster = 8;
   if (a.n_rows <= 16) return a.x16 ? launch<__half, 1>(a, cluster, s) : launch<float, 1>(a, cluster, s);
   return a.x16 ? launch<__half, 4>(a, cluster, s) : launch<float, 4>(a, cluster, s);

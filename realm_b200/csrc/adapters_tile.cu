@@ -140,7 +140,7 @@ __device__ __forceinline__ bool wait_rolled(uint64_t* bar, uint32_t parity, uint
   return false;
 }
 
-// T: type of the rows. RP: ranks up to 64 (two CTAs an SM) or 128.
+// T: type of the rows. RP: ranks up to 64 (two CTAs an SM), or from 65 to 128.
 template <class T, int RP>
 struct Cfg {
   static constexpr int F32 = sizeof(T) == 4;
@@ -154,8 +154,8 @@ struct Cfg {
   static constexpr int W_AT = kWarps * RING, W = RAW_AT + kUps * RAW > kUps * B ? RAW_AT + kUps * RAW : kUps * B;
   static constexpr int MAIN = W_AT + W;
   static constexpr int PARTS = RP * 128 * 4;        // of v in fp32, in place of the rings: the CTA's part, then the sum
-  static constexpr int CHAIN = F32 ? 256 / CE : 1024 / CE;  // chunks summed on the tensor core
-  static constexpr int CTAS = RP == 64 ? 2 : 1;
+  static constexpr int CHAIN = F32 ? 128 / CE : 1024 / CE;  // chunks summed on the tensor core
+  static constexpr int CTAS = RP == 64 ? 2 : 1, ABOVE = RP == 64 ? 0 : 64;  // this kernel's ranks
   static int smem(int n_slots) { return MAIN + 4 * n_slots; }
   // TMEM columns: two accumulators (of kCols later), then two chunks of x (v later)
   static constexpr int D = RP, A0 = 2 * RP, AW = F32 ? 64 : 32, COLS = RP == 64 ? 256 : 512;
@@ -317,7 +317,8 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
     for (int b = 0; b < a.w.n_slots; b += kWorkers) {
       const int i = b + tid;
       int n = 0;
-      if (i < a.w.n_slots && a.w.meta[i].rank > 0) n = (start[i] + tile_rows - 1) / tile_rows;
+      const int rank = i < a.w.n_slots ? a.w.meta[i].rank : 0;
+      if (rank > G::ABOVE && rank <= RP) n = (start[i] + tile_rows - 1) / tile_rows;
       int incl = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -755,7 +756,7 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
     }
     ++nv;
   }
-  if (a.out != a.y && warp < kWarps)
+  if (RP == 64 && a.out != a.y && warp < kWarps)
     for (int r = blockIdx.x; r < a.n_rows; r += gridDim.x) {
       const int v = a.slots[r];
       if (v >= 0 && v < a.w.n_slots && a.w.meta[v].rank > 0) continue;
@@ -823,8 +824,10 @@ cudaError_t adapters_tile_launch(const AdapterArgs& a, int num_sms, cudaStream_t
     b.y = (const uint8_t*)a.y + r * a.ldy * esz;
     b.out = (uint8_t*)a.out + r * a.ldo * esz;
     cudaError_t e;
-    if (a.w.rp <= 64) e = a.x16 ? launch_rank<__half, 64>(b, num_sms, s) : launch_rank<float, 64>(b, num_sms, s);
-    else e = a.x16 ? launch_rank<__half, 128>(b, num_sms, s) : launch_rank<float, 128>(b, num_sms, s);
+    // Which ranks the rows' slots have is not known here (a captured call is replayed with others). Two launches where
+    // a set may have large ones: 4096 rows of ranks 8 to 128 (k = 11008) 233 us, in one launch for all ranks 278.
+    e = a.x16 ? launch_rank<__half, 64>(b, num_sms, s) : launch_rank<float, 64>(b, num_sms, s);
+    if (!e && a.w.rp > 64) e = a.x16 ? launch_rank<__half, 128>(b, num_sms, s) : launch_rank<float, 128>(b, num_sms, s);
     if (e) return e;
   }
   return cudaSuccess;
