@@ -15,8 +15,8 @@ import ctypes as C
 
 import numpy as np
 
-from . import _check, _lib, _sig
-from .rows import BAD_HANDLE, _call, _dtype, _is_tensor, _rows3, _space, _vec, _writable
+from . import PTR_DEVICE, _check, _lib, _sig
+from .rows import ASYNC, BAD_HANDLE, _SEEN, _call, _dtype, _is_tensor, _mat, _rows3, _vec, _writable
 
 _vp, _u32, _u64, _i32, _f = C.c_void_p, C.c_uint32, C.c_uint64, C.c_int32, C.c_float
 
@@ -77,25 +77,33 @@ class AdapterSet:
         slots: int32, -1 for rows without an adapter."""
         if out is None:
             out = y
-        dt, flags = _dtype((x, y, out), self.ctx)
         n_rows = x.shape[0]
+        d = self._desc
+        d.n_rows = n_rows
         if _is_tensor(x):
-            if _space((x, slots), self.ctx) != flags:
+            if not (_is_tensor(y) and _is_tensor(slots) and _is_tensor(out)):
+                raise ValueError("host arrays, or tensors on the context's device, wanted: not a mix")
+            t, dev, flags = x.dtype, self.ctx.device, PTR_DEVICE | ASYNC
+            d.dtype = _SEEN[t] if t in _SEEN else _dtype((x,), self.ctx)[0]
+            if slots.get_device() != dev:
                 raise ValueError("slots: a tensor on the context's device wanted")
+            d.slots = _vec(slots, "int32", n_rows, "slots")
+            d.x, d.ldx = _mat(x, n_rows, self.k, t, dev, "x")
+            d.y, d.ldy = _mat(y, n_rows, self.n, t, dev, "y")
+            d.out, d.ldo = (d.y, d.ldy) if out is y else _mat(out, n_rows, self.n, t, dev, "out")
         else:
+            d.dtype, flags = _dtype((x, y, out), self.ctx)
             if _is_tensor(slots):
                 raise ValueError("host arrays, or tensors on the context's device, wanted: not a mix")
             given, slots = np.asarray(slots), np.ascontiguousarray(slots, np.int32)
             if given.size and (given.dtype.kind not in "iu" or (given != slots).any()):
                 raise ValueError("slots: 32-bit integers wanted")
-        d = self._desc
-        d.dtype, d.n_rows = dt, n_rows
-        d.slots = _vec(slots, "int32", n_rows, "slots")
-        if n_rows:
-            d.x, d.ldx = _rows3(x, n_rows, 1, self.k, "x")
-            d.y, d.ldy = _rows3(y, n_rows, 1, self.n, "y")
-            d.out, d.ldo = (d.y, d.ldy) if out is y else _rows3(out, n_rows, 1, self.n, "out")
-            _writable(out, "out")
+            d.slots = _vec(slots, "int32", n_rows, "slots")
+            if n_rows:
+                d.x, d.ldx = _rows3(x, n_rows, 1, self.k, "x")
+                d.y, d.ldy = _rows3(y, n_rows, 1, self.n, "y")
+                d.out, d.ldo = (d.y, d.ldy) if out is y else _rows3(out, n_rows, 1, self.n, "out")
+                _writable(out, "out")
         _call(self.ctx, flags, _lib.rb_adapters_add, self.ctx.handle, self.handle, self._ref)
         return out
 

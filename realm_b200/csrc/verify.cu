@@ -23,7 +23,7 @@ namespace rb {
 
 namespace {
 
-constexpr int kVT = 512, kVW = kVT / 32;
+constexpr int kVT = 256, kVW = kVT / 32;
 constexpr int kVMaxCluster = 8;
 constexpr uint32_t kNone = 0xffffffffu;
 using u64 = unsigned long long;
@@ -132,11 +132,37 @@ __global__ void __launch_bounds__(kVT) verify_kernel(const __grid_constant__ Ver
 #pragma unroll 1
   for (int turn = 0; turn < 2; ++turn) {
     u64 s = 0;
-#pragma unroll 4
-    for (int v = v0 + lane; v < v1; v += 32) {
+    auto one = [&](int v) {
       u64 w[4];
       row.weights(v, w);
       s += (w[0] + w[1]) + (w[2] + w[3]);
+    };
+    if (row.skip == kNone && (!row.q || row.same)) {
+      // whole vectors, kDeep of each row on their way; then the row's ends
+      const int f0 = max(v0, row.mis > 0), f1 = min(v1, (a.vocab + row.mis) / 4);
+      constexpr int kDeep = 4;
+#pragma unroll 1
+      for (int b = f0 + lane; b < f1; b += 32 * kDeep) {
+        float4 x[kDeep], z[kDeep];
+#pragma unroll
+        for (int j = 0; j < kDeep; ++j) {
+          const int i = (b + 32 * j) * 4 - row.mis;
+          const bool in = b + 32 * j < f1;
+          x[j] = in ? __ldg(reinterpret_cast<const float4*>(row.p + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          z[j] = in && row.q ? __ldg(reinterpret_cast<const float4*>(row.q + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int j = 0; j < kDeep; ++j)
+          s += (weight(x[j].x, z[j].x) + weight(x[j].y, z[j].y)) + (weight(x[j].z, z[j].z) + weight(x[j].w, z[j].w));
+      }
+      if (lane == 0) {
+        if (row.mis > 0 && v0 == 0 && v1 > 0) one(0);
+        const int e = (a.vocab + row.mis) / 4;
+        if (e * 4 < a.vocab + row.mis && v0 <= e && e < v1 && !(row.mis > 0 && e == 0)) one(e);
+      }
+    } else {
+#pragma unroll 4
+      for (int v = v0 + lane; v < v1; v += 32) one(v);
     }
     s = warp_total(s);
     if (lane == 0) part[warp] = s;
@@ -218,7 +244,7 @@ cudaError_t launch(const VerifyArgs& a, cudaStream_t s) {
 }  // namespace
 
 cudaError_t verify_launch(const VerifyArgs& a, int num_sms, cudaStream_t s) {
-  const int n = std::min(2 * num_sms / a.n_requests, a.vocab / (4 * kVT));
+  const int n = std::min(4 * num_sms / a.n_requests, a.vocab / (4 * kVT));
   if (n >= 8) return launch<8>(a, s);
   if (n >= 4) return launch<4>(a, s);
   if (n >= 2) return launch<2>(a, s);

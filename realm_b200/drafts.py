@@ -15,8 +15,8 @@ import ctypes as C
 
 import numpy as np
 
-from . import _lib, _sig
-from .rows import _Filter, _call, _dtype, _is_tensor, _rows3, _space, _vec, _writable
+from . import PTR_DEVICE, _lib, _sig
+from .rows import ASYNC, _Filter, _call, _dtype, _is_tensor, _mat, _rows3, _space, _vec, _writable
 from .sampling import _prev_arrays
 
 _vp, _u32, _u64, _i32 = C.c_void_p, C.c_uint32, C.c_uint64, C.c_int32
@@ -85,32 +85,36 @@ def verify_drafts(ctx, probs, drafts, uniforms, offsets, draft_probs=None, token
     m = len(offsets) - 1
     if m < 0:
         raise ValueError("offsets: one more than requests wanted")
-    dev = _is_tensor(probs)
-    if dev:
+    d = _VerifyDesc(n_requests=m, n_rows=n, vocab=v)
+    if _is_tensor(probs):
         import torch
+        dev, flags, f32 = ctx.device, PTR_DEVICE | ASYNC, torch.float32
         if tokens is None:
             tokens = torch.full((n,), -1, dtype=torch.int32, device=probs.device)
         if accepted is None:
             accepted = torch.empty(m, dtype=torch.int32, device=probs.device)
+        _space([probs, drafts, uniforms, offsets, draft_probs, tokens, accepted], ctx)
+        d.probs, d.ldp = _mat(probs, n, v, f32, dev, "probs")
+        if draft_probs is not None:
+            d.draft_probs, d.ldq = _mat(draft_probs, n, v, f32, dev, "draft_probs")
     else:
         drafts, offsets = (np.ascontiguousarray(a, np.int32) if not _is_tensor(a) else a for a in (drafts, offsets))
         uniforms = uniforms if _is_tensor(uniforms) else np.ascontiguousarray(uniforms, np.float32)
         tokens = np.full(n, -1, np.int32) if tokens is None else tokens
         accepted = np.empty(m, np.int32) if accepted is None else accepted
-    flags = _space([probs, drafts, uniforms, offsets, draft_probs, tokens, accepted], ctx)
-    if _dtype([probs] if draft_probs is None else [probs, draft_probs], ctx)[0] != 0:
-        raise ValueError(f"probs: float32 wanted, got {probs.dtype}")
-    if draft_probs is not None and _matrix(draft_probs, "draft_probs") != (n, v):
-        raise ValueError(f"draft_probs: [{n}][{v}] wanted, got {tuple(draft_probs.shape)}")
-    d = _VerifyDesc(n_requests=m, n_rows=n, vocab=v)
+        flags = _space([probs, drafts, uniforms, offsets, draft_probs, tokens, accepted], ctx)
+        if _dtype([probs] if draft_probs is None else [probs, draft_probs], ctx)[0] != 0:
+            raise ValueError(f"probs: float32 wanted, got {probs.dtype}")
+        if draft_probs is not None and _matrix(draft_probs, "draft_probs") != (n, v):
+            raise ValueError(f"draft_probs: [{n}][{v}] wanted, got {tuple(draft_probs.shape)}")
+        if n:
+            d.probs, d.ldp = _rows3(probs, n, 1, v, "probs")
+            if draft_probs is not None:
+                d.draft_probs, d.ldq = _rows3(draft_probs, n, 1, v, "draft_probs")
     d.offsets = _vec(offsets, "int32", m + 1, "offsets")
     d.drafts = _vec(drafts, "int32", n, "drafts")
     d.uniforms = _vec(uniforms, "float32", n, "uniforms")
     d.tokens = _vec(_writable(tokens, "tokens"), "int32", n, "tokens")
     d.accepted = _vec(_writable(accepted, "accepted"), "int32", m, "accepted")
-    if n:
-        d.probs, d.ldp = _rows3(probs, n, 1, v, "probs")
-        if draft_probs is not None:
-            d.draft_probs, d.ldq = _rows3(draft_probs, n, 1, v, "draft_probs")
     _call(ctx, flags, _lib.rb_verify_drafts, ctx.handle, C.byref(d))
     return tokens, accepted

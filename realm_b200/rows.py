@@ -113,6 +113,18 @@ def _rows3(a, n, heads, hd, name):
     return ptr, ld
 
 
+def _mat(a, n, width, dtype, device, name):
+    """(pointer, elements between rows) of a tensor [n][width] of `dtype` on `device` (its index)."""
+    st = a.stride()
+    if a.shape == (n, width) and (st[1] == 1 or width == 1) and a.dtype is dtype and a.get_device() == device:
+        if n == 1:
+            return a.data_ptr(), width
+        if st[0] >= width:
+            return a.data_ptr(), st[0]
+    raise ValueError(f"{name}: [{n}][{width}] of {dtype} on the context's device wanted, rows contiguous, got "
+                     f"{tuple(a.shape)} / {tuple(st)} of {a.dtype} on {a.device}")
+
+
 _DTYPES = {"torch.float32": F32, "torch.float16": F16, "float32": F32, "float16": F16}
 _SEEN = {}  # dtype objects met so far
 
