@@ -95,9 +95,10 @@ class AdapterSet:
             d.dtype, flags = _dtype((x, y, out), self.ctx)
             if _is_tensor(slots):
                 raise ValueError("host arrays, or tensors on the context's device, wanted: not a mix")
-            given, slots = np.asarray(slots), np.ascontiguousarray(slots, np.int32)
-            if given.size and (given.dtype.kind not in "iu" or (given != slots).any()):
+            given = np.asarray(slots)
+            if given.size and (given.dtype.kind not in "iu" or given.min() < -2 ** 31 or given.max() >= 2 ** 31):
                 raise ValueError("slots: 32-bit integers wanted")
+            slots = np.ascontiguousarray(given, np.int32)
             d.slots = _vec(slots, "int32", n_rows, "slots")
             if n_rows:
                 d.x, d.ldx = _rows3(x, n_rows, 1, self.k, "x")
