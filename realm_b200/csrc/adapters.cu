@@ -28,7 +28,7 @@ constexpr int kT = 256, kWarps = kT / 32;
 constexpr int kBlock = 64;        // rows among which an item's rows are found
 constexpr int kGroup = 8;         // ranks a warp works on at a time: a line of weights
 constexpr int kTileK = 1536;      // elements of x in shared memory at a time
-constexpr int kMaxCluster = 8;
+constexpr int kMaxCluster = 16;  // above 8: not portable, but every B200 has it
 static_assert(kWarps * kGroup <= kAdapterMaxRank && kTileK % 8 == 0, "");
 
 __device__ __forceinline__ float to_f(float v) { return v; }
@@ -59,14 +59,13 @@ __device__ __forceinline__ int slot_of(const AdapterArgs& a, int row) {
 template <int R>
 struct ItemShared {
   __align__(16) float xs[R][kTileK];
-  float part[kAdapterMaxRank * R];                // [k part][rank][row]
-  float parts[kMaxCluster][kAdapterMaxRank * R];  // every CTA's v
-  __align__(16) float v[kAdapterMaxRank * R];     // [rank][row]
+  float part[kAdapterMaxRank * R];             // [k part][rank][row]
+  __align__(16) float v[kAdapterMaxRank * R];  // [rank][row]
 };
 
 // Up to R rows of one slot, by a cluster.
 template <class T, int R, int RS>
-__device__ __forceinline__ void run_item(const AdapterArgs& a, ItemShared<RS>& sh, int slot, const int (&rows)[R], int nr) {
+__device__ __forceinline__ void run_item(const AdapterArgs& a, ItemShared<RS>& sh, float* parts, int slot, const int (&rows)[R], int nr) {
   auto& xs = sh.xs;
   float *part = sh.part, *v = sh.v;
   cg::cluster_group cluster = cg::this_cluster();
@@ -93,6 +92,7 @@ __device__ __forceinline__ void run_item(const AdapterArgs& a, ItemShared<RS>& s
   for (int r = 0; r < R; ++r)
     for (int j = n0 + tid * 32; r < nr && j < n1; j += kT * 32)
       asm volatile("prefetch.global.L2 [%0];" ::"l"(y + rows[r] * a.ldy + j));
+  const int stride = a.w.rp * R;       // between the CTAs' parts
   const int nv = groups * kGroup * R;  // of a k part; ks > 1: at most kWarps groups in all
   for (int i = tid; i < ks * nv; i += kT) part[i] = 0.f;
   for (int t0 = c0; t0 < c1; t0 += kTileK / 8) {
@@ -137,13 +137,13 @@ __device__ __forceinline__ void run_item(const AdapterArgs& a, ItemShared<RS>& s
   for (int i = tid; i < nv; i += kT) {
     float s = 0.f;
     for (int p = 0; p < ks; ++p) s += part[p * nv + i];
-    for (int d = 0; d < C; ++d) *cluster.map_shared_rank(&sh.parts[c][i], d) = s;
+    for (int d = 0; d < C; ++d) *cluster.map_shared_rank(parts + c * stride + i, d) = s;
   }
   cluster.sync();
   for (int i = tid; i < (rank + 7) / 8 * 8 * R; i += kT) {
     float s = 0.f;
     if (i < nv)
-      for (int d = 0; d < C; ++d) s += sh.parts[d][i];
+      for (int d = 0; d < C; ++d) s += parts[d * stride + i];
     v[i] = s * scale;
   }
   __syncthreads();
@@ -191,6 +191,7 @@ __device__ __forceinline__ void run_item(const AdapterArgs& a, ItemShared<RS>& s
 template <class T, int R>
 __global__ void __launch_bounds__(kT, 4) adapters_kernel(const __grid_constant__ AdapterArgs a) {
   __shared__ ItemShared<R> sh;
+  extern __shared__ float parts[];  // [CTA of the cluster][rank][row] of v
   __shared__ int s_slot[kBlock], s_rows[R], s_n, s_item;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), c = (int)cluster.block_rank();
@@ -256,17 +257,25 @@ __global__ void __launch_bounds__(kT, 4) adapters_kernel(const __grid_constant__
   }
   if (R > 1 && nr == 1) {
     const int one[1] = {rows[0]};
-    run_item<T, 1, R>(a, sh, slot, one, 1);
+    run_item<T, 1, R>(a, sh, parts, slot, one, 1);
   } else {
-    run_item<T, R, R>(a, sh, slot, rows, nr);
+    run_item<T, R, R>(a, sh, parts, slot, rows, nr);
   }
 }
 
 template <class T, int R>
 cudaError_t launch(const AdapterArgs& a, int cluster, cudaStream_t s) {
+  if (cluster > 8) {
+    if (cudaError_t e = cudaFuncSetAttribute(adapters_kernel<T, R>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) return e;
+  }
+  const int smem = cluster * a.w.rp * R * 4;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (cudaError_t e = ensure_smem_attr(adapters_kernel<T, R>, kMaxCluster * kAdapterMaxRank * R * 4, dev)) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a.n_rows * cluster);
   cfg.blockDim = dim3(kT);
+  cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = s;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -319,7 +328,9 @@ cudaError_t adapters_launch(const AdapterArgs& a, int num_sms, cudaStream_t s) {
   // Rows of one adapter, k = n = 4096, fp32, rank 64: 256 rows 35 us here and 51 in tiles, 512 59 and 55, 1024 111 and
   // 57; rank 16 fp16: 256 25 and 31, 512 41 and 33. Every row another's (rank 64): 256 rows 111 us and 578.
   if (a.n_rows > 384) return adapters_tile_launch(a, num_sms, s);
-  const int cluster = 8;
+  // Sixteen CTAs a row where there are few: one row 11.5 us and 15.6 with eight (rank 64, k = n = 4096), 17.6 and 28 at k =
+  // 11008; 64 rows of 64 adapters 39 and 29. (Nothing in L2, as above; the times include about 3 us of launch.)
+  const int cluster = a.n_rows <= 16 ? 16 : 8;
   if (a.n_rows <= 16) return a.x16 ? launch<__half, 1>(a, cluster, s) : launch<float, 1>(a, cluster, s);
   return a.x16 ? launch<__half, 4>(a, cluster, s) : launch<float, 4>(a, cluster, s);
 }

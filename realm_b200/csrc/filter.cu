@@ -779,6 +779,7 @@ __global__ void __launch_bounds__(kFT, two_ctas<T, NV>()) filter_kernel(const __
   }
   const bool use_k = p.top_k > 0 && p.top_k < (uint32_t)V, use_p = p.top_p > 0.f && p.top_p < 1.f;
   const bool hist = use_k || use_p;
+  u64 kept_sum = 0;  // D: of what the cuts keep
   change<NQ>(mine, [&](float x) {
     const float w = x == m ? 1.f : expf(x - m);
     int b;
@@ -812,7 +813,7 @@ __global__ void __launch_bounds__(kFT, two_ctas<T, NV>()) filter_kernel(const __
       bc = (uint32_t)cl.gather(&s.cnt[turn][tid]);
       bw = (cl.gather(&s.lo[turn][tid]) + (cl.gather(&s.hi[turn][tid]) << 10)) << shift_of(tid);
     }
-    u64 total = 0;
+    u64 total = 0;  // of what is kept
     if (use_k) {
       cut = radix_cut<true, NQ, N>(mine, bc, bw, p.top_k, cl, total);
     } else {
@@ -827,10 +828,13 @@ __global__ void __launch_bounds__(kFT, two_ctas<T, NV>()) filter_kernel(const __
     if (use_p) {
       u64 want = (u64)((double)total * (double)p.top_p);
       if (want < 1) want = 1;
+      const u64 first = total;
       const Cut c = radix_cut<false, NQ, N>(mine, bc, bw, want, cl, total);
       // never below the first cut; at the same weight, the fewer ties
       if (c.bits > cut.bits || (c.bits == cut.bits && c.ties < cut.ties)) cut = c;
+      else total = first;
     }
+    if (D) kept_sum = total;
     // kept: bits above the cut, and its ties with the lowest indices
     change<NQ>(mine, [&](float x) { return __float_as_uint(x) < cut.bits ? 0.f : x; });
     if (cut.ties < cut.equal) {  // the same in every thread of the cluster
@@ -851,6 +855,17 @@ __global__ void __launch_bounds__(kFT, two_ctas<T, NV>()) filter_kernel(const __
         change<Q>(mine + r * Q * kFT, [&](float x) { return __float_as_uint(x) == cut.bits && rank++ >= cut.ties ? 0.f : x; });
       }
     }
+  }
+  if (D && hist) {
+    // W = w 2^40 unless its last bits lie below the fixed point; the quotient from two fp32 products, the rounding
+    // of the first in the second (2^-45 of it)
+    const double inv = 1.0 / (double)kept_sum, scaled = inv * 0x1p40;
+    const float s0 = (float)scaled, s1 = (float)(scaled - (double)s0);
+    write_dist([&](float x, int) {
+      const float y = x * s0;
+      return x >= 0x1p-17f ? y + fmaf(x, s1, fmaf(x, s0, -y)) : x != 0.f ? (float)((double)fix(x) * inv) : 0.f;
+    });
+    return;
   }
   // the draw: rounds of vectors, then warps, then lanes are in the order of the indices
   for (int r = 0; r < NV; ++r) {

@@ -177,7 +177,7 @@ cudaError_t launch(const ResidualArgs& a, int threads, int rows, cudaStream_t s)
 template <class TY, class TX, bool VEC>
 cudaError_t launch_chunks(const ResidualArgs& a, int num_sms, cudaStream_t s) {
   const int chunks = (a.dim + kE - 1) / kE;
-  const int nc = chunks <= 512 ? 1 : chunks <= 1024 ? 2 : 4, most = chunks <= 2048 ? 512 : 1024;
+  const int nc = chunks <= 256 ? 1 : chunks <= 1024 ? 2 : 4, most = chunks <= 2048 ? 512 : 1024;
   const int threads = std::min(most, ((chunks + nc - 1) / nc + 31) / 32 * 32);
   const int rows = threads == 32 ? 4 : 1;
   if (nc == 1) return launch<TY, TX, 1, VEC, 512>(a, threads, rows, s);
