@@ -325,9 +325,10 @@ cudaError_t adapters_clear_launch(AdapterMeta* meta, cudaStream_t s) {
 }
 
 cudaError_t adapters_launch(const AdapterArgs& a, int num_sms, cudaStream_t s) {
-  // Rows of one adapter, k = n = 4096, fp32, rank 64: 256 rows 35 us here and 51 in tiles, 512 59 and 55, 1024 111 and
-  // 57; rank 16 fp16: 256 25 and 31, 512 41 and 33. Every row another's (rank 64): 256 rows 111 us and 578.
-  if (a.n_rows > 384) return adapters_tile_launch(a, num_sms, s);
+  // One launch for rows of any slots, whose number is not known here. Rows of one adapter, k = n = 4096, fp32, rank 64: 256
+  // rows 33 us here and 51 in tiles, 384 47 and 53, 512 59 and 55, 1024 111 and 57; every row another's: 256 rows 82 and
+  // 612, 1024 373 and 605. So up to 384 rows here, and up to 1024 where there are slots for rows mostly apart.
+  if (a.n_rows > 1024 || (a.n_rows > 384 && a.n_rows > 4 * a.w.n_slots)) return adapters_tile_launch(a, num_sms, s);
   // Sixteen CTAs a row where there are few: one row 11.5 us and 15.6 with eight (rank 64, k = n = 4096), 17.6 and 28 at k =
   // 11008; 64 rows of 64 adapters 39 and 29. (Nothing in L2, as above; the times include about 3 us of launch.)
   const int cluster = a.n_rows <= 16 ? 16 : 8;

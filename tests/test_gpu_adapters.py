@@ -113,13 +113,13 @@ def test_many_slots_and_spans(ctx, rows):
     """More slots than rows have, all rows of one, every row of another, and calls of more than 8192 rows."""
     import torch
     rng = np.random.default_rng(rows)
-    k, n, slots_n = 128, 64, 300
+    k, n, slots_n = 128, 64, 300  # (500 rows go one by one then)
     x, y, down, up, scales = make(rng, rows, k, n, [4] * slots_n, torch.float32, [1.0] * slots_n)
     with load(ctx, n, k, down, up, scales) as s:
         for slots in (np.full(rows, 299), np.arange(rows) % slots_n, np.full(rows, -1), np.arange(rows) // 130 % 7):
             slots = slots.astype(np.int32)
             out = s.add(x.cuda(), torch.from_numpy(slots).cuda(), y.cuda())
-            check(out, x, y, down, up, scales, slots, rows > 384)
+            check(out, x, y, down, up, scales, slots, rows > 1024)
 
 
 @pytest.mark.parametrize("rows", [9, 50, 401])
