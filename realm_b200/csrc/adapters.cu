@@ -10,10 +10,17 @@
 //
 // The rows of an adapter find one another in the kernel: cluster i of a block of kBlock
 // rows takes the block's i-th item, an item being the next R rows of one slot, counted from the
-// block's first row; clusters past the last item have nothing to do.
+// block's first row; clusters past the last item have nothing to do. A lone row takes a quarter of the work of four.
+//
+// Bound by latency: the slots, an adapter's rank, x and down, the exchange, up, one after the other; up and
+// y are on their way to L2 from the start. Nothing in L2, about 3 us of launch within: one row of rank 16 (k = n =
+// 4096, 0.3 MB) 9.5 us, rank 64 11.5, rank 128 16; 64 rows of 64 adapters of rank 64 (67 MB) 29 us, 2.3 TB/s; 48
+// rows of 31 adapters of rank 8 to 64, n = 11008 (32 MB), 26 us. With up read four blocks of two columns at a time
+// instead of one by one 64 rows went from 35 to 29 us.
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "adapters.cuh"
 #include "common.cuh"
@@ -265,13 +272,17 @@ __global__ void __launch_bounds__(kT, 4) adapters_kernel(const __grid_constant__
 
 template <class T, int R>
 cudaError_t launch(const AdapterArgs& a, int cluster, cudaStream_t s) {
-  if (cluster > 8) {
-    if (cudaError_t e = cudaFuncSetAttribute(adapters_kernel<T, R>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) return e;
-  }
   const int smem = cluster * a.w.rp * R * 4;
   int dev = 0;
   cudaGetDevice(&dev);
   if (cudaError_t e = ensure_smem_attr(adapters_kernel<T, R>, kMaxCluster * kAdapterMaxRank * R * 4, dev)) return e;
+  if (cluster > 8) {
+    static std::atomic<uint64_t> allowed{0};  // by device
+    if (!(allowed.load() >> (dev & 63) & 1)) {
+      if (cudaError_t e = cudaFuncSetAttribute(adapters_kernel<T, R>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) return e;
+      allowed |= 1ull << (dev & 63);
+    }
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a.n_rows * cluster);
   cfg.blockDim = dim3(kT);
@@ -326,8 +337,8 @@ cudaError_t adapters_clear_launch(AdapterMeta* meta, cudaStream_t s) {
 
 cudaError_t adapters_launch(const AdapterArgs& a, int num_sms, cudaStream_t s) {
   // One launch for rows of any slots, whose number is not known here. Rows of one adapter, k = n = 4096, fp32, rank 64: 256
-  // rows 33 us here and 51 in tiles, 384 47 and 53, 512 59 and 55, 1024 111 and 57; every row another's: 256 rows 82 and
-  // 612, 1024 373 and 605. So up to 384 rows here, and up to 1024 where there are slots for rows mostly apart.
+  // rows 33 us here and 51 in tiles, 384 47 and 53, 512 54 and 55, 1024 100 and 57; every row another's: 256 rows 82 and
+  // 612, 1024 258 and 593. So up to 384 rows here, and up to 1024 where there are slots for rows mostly apart.
   if (a.n_rows > 1024 || (a.n_rows > 384 && a.n_rows > 4 * a.w.n_slots)) return adapters_tile_launch(a, num_sms, s);
   // Sixteen CTAs a row where there are few: one row 11.5 us and 15.6 with eight (rank 64, k = n = 4096), 17.6 and 28 at k =
   // 11008; 64 rows of 64 adapters 39 and 29. (Nothing in L2, as above; the times include about 3 us of launch.)

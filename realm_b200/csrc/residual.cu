@@ -7,6 +7,10 @@
 // elements, T chunks apart: 16 or 32 bytes a load, coalesced. Rows off 16 bytes (odd
 // widths) take single elements T apart instead: as many bytes in flight, all lines still
 // used whole.
+//
+// Bound by memory: 8192 x 4096, fp16 on an fp32 stream with a shared gate 75 us (403 MB, 5.4 TB/s, 83 % of a copy's
+// rate); with one chunk of 512 threads 79 us, four of 128 80 us, one with registers cut for a third CTA 82. One row of 4096
+// is the call: 9 us, of which the kernel about 3.
 #include <algorithm>
 
 #include "common.cuh"
