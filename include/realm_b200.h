@@ -619,9 +619,9 @@ typedef struct rb_adapters_desc {
   uint64_t ldx, ldy, ldo;
 } rb_adapters_desc;
 /* Rows in any order; those without an adapter are copied as they are, whatever their x
- * holds. All sums are fp32, x and down x in fp32 (x of RB_F32 in 22 bits where a call's
- * rows are many), the result is rounded once. out must not overlap x, nor y unless it is y.
- * Returns n_rows. */
+ * holds. All sums are fp32; where a call's rows are many, an RB_F32 x has 22 bits, and down x 22
+ * bits of its row's largest element (an infinite one makes the row's sums NaN). The result is
+ * rounded once. out must not overlap x, nor y unless it is y. Returns n_rows. */
 int32_t rb_adapters_add(rb_ctx* ctx, int32_t set, const rb_adapters_desc* desc, uint32_t flags);
 
 /* The counter-based uniform draw in [0, 1) (a multiple of 2^-23) of (seed, counter):

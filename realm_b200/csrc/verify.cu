@@ -8,17 +8,18 @@
 // running sum exceeds floor(u sum F).
 //
 // One cluster a request. Each CTA finds row j by itself (a few gathered values), each warp sums
-// its contiguous share of the row, the cluster adds up, and the one warp in whose
-// share the target falls goes over it once more: the row is read once.
+// its contiguous share of the row and remembers the sum of each batch of 512 elements, the cluster adds up, and the one
+// warp in whose share the target falls goes over its batch once more: the row is read once.
 //
 // Bound by latency: offsets, drafts, their probabilities, the row, the exchange, the share again, one after the other.
-// 64 requests of 1 to 9 rows of 151937 30 us (63 MB read: 2.1 TB/s, the sums' loop four vectors of each row
-// deep; one by one 37 us); one request of 7 rows of 32000 the call itself, 9.5 us.
+// 64 requests of 1 to 9 rows of 151937 25 us (63 MB read: 2.5 TB/s; 30 us when the share was gone over vector by vector,
+// 37 when the sums were too); one request of 7 rows of 32000 the call itself, 9 us.
 #include <cooperative_groups.h>
 
 #include <algorithm>
 
 #include "common.cuh"
+#include "filter.cuh"
 #include "verify.cuh"
 
 namespace cg = cooperative_groups;
@@ -29,6 +30,8 @@ namespace {
 
 constexpr int kVT = 256, kVW = kVT / 32;
 constexpr int kVMaxCluster = 8;
+constexpr int kDeep = 4, kBatch = 32 * kDeep;                     // vectors of 4 elements a lane, a warp takes at a time
+constexpr int kBatches = (kFilterMaxVocab / 4 / kVW + kBatch) / kBatch + 1;  // of a warp's share, at most
 constexpr uint32_t kNone = 0xffffffffu;
 using u64 = unsigned long long;
 
@@ -88,9 +91,16 @@ struct DrawRow {
   }
 };
 
+__device__ __forceinline__ u64 vector(const DrawRow& row, int v) {
+  u64 w[4];
+  row.weights(v, w);
+  return (w[0] + w[1]) + (w[2] + w[3]);
+}
+
 template <int N>
 __global__ void __launch_bounds__(kVT) verify_kernel(const __grid_constant__ VerifyArgs a) {
   __shared__ u64 part[kVW];
+  __shared__ u64 batch[kVW][kBatches];
   __shared__ u64 sums[2][kVMaxCluster];
   __shared__ uint32_t first;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -135,40 +145,33 @@ __global__ void __launch_bounds__(kVT) verify_kernel(const __grid_constant__ Ver
   u64 total = 0, before = 0;
 #pragma unroll 1
   for (int turn = 0; turn < 2; ++turn) {
+    // whole vectors, a batch of kDeep of each row a lane on their way; what lies at the row's ends, or unlike in
+    // p and q, by elements
+    const bool alike = row.skip == kNone && (!row.q || row.same);
+    const int f0 = row.mis > 0, f1 = (a.vocab + row.mis) / 4;
     u64 s = 0;
-    auto one = [&](int v) {
-      u64 w[4];
-      row.weights(v, w);
-      s += (w[0] + w[1]) + (w[2] + w[3]);
-    };
-    if (row.skip == kNone && (!row.q || row.same)) {
-      // whole vectors, kDeep of each row on their way; then the row's ends
-      const int f0 = max(v0, row.mis > 0), f1 = min(v1, (a.vocab + row.mis) / 4);
-      constexpr int kDeep = 4;
 #pragma unroll 1
-      for (int b = f0 + lane; b < f1; b += 32 * kDeep) {
-        float4 x[kDeep], z[kDeep];
+    for (int k = 0; v0 + k * kBatch < v1; ++k) {
+      const int b = v0 + k * kBatch + lane;
+      u64 here = 0;
+      float4 x[kDeep], z[kDeep];
 #pragma unroll
-        for (int j = 0; j < kDeep; ++j) {
-          const int i = (b + 32 * j) * 4 - row.mis;
-          const bool in = b + 32 * j < f1;
-          x[j] = in ? __ldg(reinterpret_cast<const float4*>(row.p + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
-          z[j] = in && row.q ? __ldg(reinterpret_cast<const float4*>(row.q + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
+      for (int j = 0; j < kDeep; ++j) {
+        const int v = b + 32 * j, i = v * 4 - row.mis;
+        const bool whole = alike && v < v1 && v >= f0 && v < f1;
+        x[j] = whole ? __ldg(reinterpret_cast<const float4*>(row.p + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        z[j] = whole && row.q ? __ldg(reinterpret_cast<const float4*>(row.q + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
 #pragma unroll
-        for (int j = 0; j < kDeep; ++j)
-          s += (weight(x[j].x, z[j].x) + weight(x[j].y, z[j].y)) + (weight(x[j].z, z[j].z) + weight(x[j].w, z[j].w));
-      }
-      if (lane == 0) {
-        if (row.mis > 0 && v0 == 0 && v1 > 0) one(0);
-        const int e = (a.vocab + row.mis) / 4;
-        if (e * 4 < a.vocab + row.mis && v0 <= e && e < v1 && !(row.mis > 0 && e == 0)) one(e);
-      }
-    } else {
-#pragma unroll 4
-      for (int v = v0 + lane; v < v1; v += 32) one(v);
+      for (int j = 0; j < kDeep; ++j)
+        here += (weight(x[j].x, z[j].x) + weight(x[j].y, z[j].y)) + (weight(x[j].z, z[j].z) + weight(x[j].w, z[j].w));
+#pragma unroll 1
+      for (int v = b; v < v1 && v < b + kBatch; v += 32)
+        if (!(alike && v >= f0 && v < f1)) here += vector(row, v);
+      here = warp_total(here);
+      if (lane == 0) batch[warp][k] = here;
+      s += here;
     }
-    s = warp_total(s);
     if (lane == 0) part[warp] = s;
     __syncthreads();
     u64 mine = 0;
@@ -204,21 +207,39 @@ __global__ void __launch_bounds__(kVT) verify_kernel(const __grid_constant__ Ver
   // the share that holds the target: exactly one warp's, as target < total
   if (total && before <= target && target < before + part[warp]) {
     u64 sum = before;
-    for (int b = v0; b < v1; b += 32) {
-      u64 w[4] = {0, 0, 0, 0};
-      if (b + lane < v1) row.weights(b + lane, w);
-      const u64 here = (w[0] + w[1]) + (w[2] + w[3]), incl = warp_incl(here);
-      u64 run = sum + incl - here;
-      if (run <= target && target < run + here) {
-        int i = (b + lane) * 4 - row.mis;
+    int k = 0;  // the batch of the share that holds it
+    for (int n = (v1 - v0 + kBatch - 1) / kBatch; k < n; k += 32) {
+      const u64 here = k + lane < n ? batch[warp][k + lane] : 0, incl = warp_incl(here);
+      const uint32_t past = __ballot_sync(0xffffffffu, target < sum + incl);
+      if (past) {
+        const int l = __ffs(past) - 1;
+        sum += __shfl_sync(0xffffffffu, incl - here, l);
+        k += l;
+        break;
+      }
+      sum += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    u64 here[kDeep];
+#pragma unroll
+    for (int j = 0; j < kDeep; ++j) {
+      const int v = v0 + k * kBatch + 32 * j + lane;
+      here[j] = v < v1 ? vector(row, v) : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < kDeep; ++j) {
+      const u64 incl = warp_incl(here[j]);
+      u64 run = sum + incl - here[j];
+      if (run <= target && target < run + here[j]) {
+        const int v = v0 + k * kBatch + 32 * j + lane;
+        u64 w[4];
+        row.weights(v, w);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          if (run <= target && target < run + w[e]) a.tokens[at] = (uint32_t)(i + e);
+          if (run <= target && target < run + w[e]) a.tokens[at] = (uint32_t)(v * 4 - row.mis + e);
           run += w[e];
         }
       }
       sum += __shfl_sync(0xffffffffu, incl, 31);
-      if (target < sum) break;
     }
   }
   if (rank) return;
