@@ -564,7 +564,8 @@ typedef struct rb_verify_desc {
  * to the request's last row; accepted the number of the accepted. A p without a positive
  * value draws 0xffffffff; unless RB_ASYNC, the call then returns RB_ERR_INVALID ("Failed to create
  * weighted index"). A request without rows gets accepted = 0, one whose offsets fall or pass
- * n_rows -1 (device memory; on the host that is refused). Returns n_requests. */
+ * n_rows -1 (device memory; on the host that is refused); the others are verified, though where they
+ * share rows after a fall, those rows' tokens are left open. Returns n_requests. */
 int32_t rb_verify_drafts(rb_ctx* ctx, const rb_verify_desc* desc, uint32_t flags);
 
 /* ---- norms around a block ----

@@ -11,6 +11,10 @@
 // its contiguous share of the row and remembers the sum of each batch of 512 elements, the cluster adds up, and the one
 // warp in whose share the target falls goes over its batch once more: the row is read once.
 //
+// Rows of device memory may be those of two requests (offsets that fell between them), and tokens may be drafts: then one
+// request writes drafts that another reads. What is drawn there is left open, but CTAs that meet different drafts take
+// the same turns: a CTA's threads share one reading of the refused draft, and whether there is a second turn goes with the sums.
+//
 // Bound by latency: offsets, drafts, their probabilities, the row, the exchange, the share again, one after the other.
 // 64 requests of 1 to 9 rows of 151937 25 us (63 MB read: 2.5 TB/s; 30 us when the share was gone over vector by vector,
 // 37 when the sums were too); one request of 7 rows of 32000 the call itself, 9 us.
@@ -102,7 +106,7 @@ __global__ void __launch_bounds__(kVT) verify_kernel(const __grid_constant__ Ver
   __shared__ u64 part[kVW];
   __shared__ u64 batch[kVW][kBatches];
   __shared__ u64 sums[2][kVMaxCluster];
-  __shared__ uint32_t first;
+  __shared__ uint32_t first, refused_draft;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = N > 1 ? (int)cg::this_cluster().block_rank() : 0, req = blockIdx.x / N;
   pdl_launch_dependents();
@@ -132,10 +136,14 @@ __global__ void __launch_bounds__(kVT) verify_kernel(const __grid_constant__ Ver
   }
   const uint32_t at = first;
   const bool inner = at < r1 - 1;
+  if (!a.draft_probs) {
+    if (tid == 0) refused_draft = inner ? a.drafts[at] : kNone;
+    __syncthreads();
+  }
   DrawRow row;
   row.p = a.probs + (int64_t)at * a.ldp;
   row.q = inner && a.draft_probs ? a.draft_probs + (int64_t)at * a.ldq : nullptr;
-  row.skip = inner && !a.draft_probs ? a.drafts[at] : kNone;
+  row.skip = a.draft_probs ? kNone : refused_draft;
   row.vocab = a.vocab;
   row.mis = (int)((reinterpret_cast<uintptr_t>(row.p) & 15) / 4);
   row.same = ((reinterpret_cast<uintptr_t>(row.p) ^ reinterpret_cast<uintptr_t>(row.q)) & 15) == 0;
@@ -181,21 +189,26 @@ __global__ void __launch_bounds__(kVT) verify_kernel(const __grid_constant__ Ver
       if (w < warp) before += part[w];
       mine += part[w];
     }
+    bool less = row.q || row.skip != kNone;  // something was taken off p
     if (N > 1) {
-      if (tid < N) *cg::this_cluster().map_shared_rank(&sums[turn][rank], tid) = mine;
+      constexpr u64 kLess = 1ull << 63;  // above all sums
+      if (tid < N) *cg::this_cluster().map_shared_rank(&sums[turn][rank], tid) = mine | (less ? kLess : 0);
       cg::this_cluster().sync();
       total = 0;
+      less = false;
 #pragma unroll
       for (int c = 0; c < N; ++c) {
-        if (c < rank) before += sums[turn][c];
-        total += sums[turn][c];
+        const u64 s = sums[turn][c];
+        if (c < rank) before += s & ~kLess;
+        total += s & ~kLess;
+        less |= s >= kLess;
       }
     } else {
       __syncthreads();  // part has been read
       total = mine;
     }
     // p nowhere above q (the same in every thread of the cluster): from p
-    if (total || (!row.q && row.skip == kNone)) break;
+    if (total || !less) break;
     row.q = nullptr;
     row.skip = kNone;
   }
