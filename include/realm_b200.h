@@ -603,8 +603,9 @@ int32_t rb_adapters_create(rb_ctx* ctx, uint32_t n, uint32_t k, uint32_t n_slots
 /* Waits for the context's stream, then frees the set. Its handle is not given out again. */
 int32_t rb_adapters_destroy(rb_ctx* ctx, int32_t set);
 /* Puts an adapter in a slot, in place of what it held: down [rank][k], up [n][rank], both of
- * dtype RB_F32 (rounded to fp16) or RB_F16. Ordered on the stream: rows of earlier calls
- * have the slot's old adapter. Returns rank. */
+ * dtype RB_F32 or RB_F16. RB_F32 factors are rounded to fp16 behind a power of two each, which brings the
+ * largest element to [2^14, 2^15) (2^126 at most): none overflows, and elements keep 11 bits down to 2^-28 of the
+ * largest. Ordered on the stream: rows of earlier calls have the slot's old adapter. Returns rank. */
 int32_t rb_adapters_set(rb_ctx* ctx, int32_t set, uint32_t slot, int32_t dtype, uint32_t rank, const void* down,
                         const void* up, float scale, uint32_t flags);
 /* Empties a slot (RB_ERR_NOT_FOUND beyond n_slots). */

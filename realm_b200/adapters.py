@@ -56,7 +56,7 @@ class AdapterSet:
 
     def set(self, slot: int, down, up, scale: float = 1.0):
         """Puts an adapter in `slot`: down [rank][k], up [n][rank], contiguous, float16 or float32 (rounded to
-        float16), numpy arrays or CUDA tensors. Calls made before it keep the old one."""
+        float16 behind a power of two), numpy arrays or CUDA tensors. Calls made before it keep the old one."""
         dt, flags = _dtype((down, up), self.ctx)
         rank = down.shape[0] if len(down.shape) == 2 else -1
         name = str(down.dtype).replace("torch.", "")

@@ -86,6 +86,7 @@ __device__ __forceinline__ void run_item(const AdapterArgs& a, ItemShared<RS>& s
   cluster.barrier_arrive();
   const int rank = a.w.meta[slot].rank;
   const float scale = a.w.meta[slot].scale;
+  const int exp = a.w.meta[slot].exp;
   const int groups = (rank + kGroup - 1) / kGroup, r16 = (rank + 15) / 16 * 16;
   // warps are split over groups of ranks, and with few of those over k
   const int ks = groups >= kWarps ? 1 : kWarps / groups, kpart = ks == 1 ? 0 : warp / groups;
@@ -151,7 +152,7 @@ __device__ __forceinline__ void run_item(const AdapterArgs& a, ItemShared<RS>& s
     float s = 0.f;
     if (i < nv)
       for (int d = 0; d < C; ++d) s += parts[d * stride + i];
-    v[i] = s * scale;
+    v[i] = scalbnf(s * scale, exp);
   }
   __syncthreads();
   const int blocks8 = (rank + 7) / 8;
@@ -305,32 +306,59 @@ cudaError_t launch(const AdapterArgs& a, int cluster, cudaStream_t s) {
   return cudaLaunchKernelEx(&cfg, adapters_kernel<T, R>, a);
 }
 
+// The largest finite elements of fp32 factors, as bits (which order like the values), into a.most[0] and [1].
+__global__ void adapters_most_kernel(const __grid_constant__ AdapterSetArgs a) {
+  const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, step = (int64_t)gridDim.x * blockDim.x;
+#pragma unroll
+  for (int f = 0; f < 2; ++f) {
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(f ? a.src_up : a.src_down);
+    uint32_t most = 0;
+    for (int64_t i = at; i < (int64_t)a.rank * (f ? a.n : a.k); i += step) {
+      const uint32_t x = p[i] & 0x7fffffffu;
+      if (x < 0x7f800000u) most = max(most, x);
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    if ((threadIdx.x & 31) == 0) atomicMax(a.most + f, most);
+  }
+}
+
+// The power of two that brings a factor's largest element to [2^14, 2^15): 2^126 at most, behind which the
+// smallest numbers of fp32 are still multiples of fp16's.
+__device__ __forceinline__ int lift_of(uint32_t most) {
+  return most ? min(14 - ilogbf(__uint_as_float(most)), 126) : 0;
+}
+
 template <class S>
 __global__ void adapters_set_kernel(const __grid_constant__ AdapterSetArgs a) {
   const S *sd = reinterpret_cast<const S*>(a.src_down), *su = reinterpret_cast<const S*>(a.src_up);
   const int r16 = (a.rank + 15) / 16 * 16;
+  const int lift_d = a.most ? lift_of(a.most[0]) : 0, lift_u = a.most ? lift_of(a.most[1]) : 0;
   const int64_t nd = (int64_t)r16 * a.kp, nu = (int64_t)r16 * a.n;
   const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, step = (int64_t)gridDim.x * blockDim.x;
   for (int64_t i = at; i < nd; i += step) {
     const int64_t v = i / 8;  // [k / 8][r16][8]
     const int r = (int)(v % r16), j = (int)(v / r16) * 8 + (int)(i % 8);
-    a.down[i] = r < a.rank && j < a.k ? __half_as_ushort(from_f<__half>(to_f(sd[(int64_t)r * a.k + j]))) : 0;
+    a.down[i] = r < a.rank && j < a.k ? __half_as_ushort(from_f<__half>(scalbnf(to_f(sd[(int64_t)r * a.k + j]), lift_d))) : 0;
   }
   for (int64_t i = at; i < nu; i += step) {  // [rank / 8][n][8]
     const int64_t v = i / 8;
     const int r = (int)(v / a.n) * 8 + (int)(i % 8), j = (int)(v % a.n);
-    a.up[i] = r < a.rank ? __half_as_ushort(from_f<__half>(to_f(su[(int64_t)j * a.rank + r]))) : 0;
+    a.up[i] = r < a.rank ? __half_as_ushort(from_f<__half>(scalbnf(to_f(su[(int64_t)j * a.rank + r]), lift_u))) : 0;
   }
-  if (at == 0) *a.meta = AdapterMeta{a.rank, a.scale};
+  if (at == 0) *a.meta = AdapterMeta{a.rank, a.scale, -lift_d - lift_u};
 }
 
-__global__ void adapters_clear_kernel(AdapterMeta* meta) { *meta = AdapterMeta{0, 0.f}; }
+__global__ void adapters_clear_kernel(AdapterMeta* meta) { *meta = AdapterMeta{0, 0.f, 0}; }
 
 }  // namespace
 
 cudaError_t adapters_set_launch(const AdapterSetArgs& a, cudaStream_t s) {
   const int64_t most = (int64_t)(a.rank + 15) / 16 * 16 * std::max(a.kp, a.n);
   const int blocks = (int)std::min<int64_t>(1184, (most + 255) / 256);
+  if (a.most) {
+    if (cudaError_t e = cudaMemsetAsync(a.most, 0, 8, s)) return e;
+    adapters_most_kernel<<<blocks, 256, 0, s>>>(a);
+  }
   if (a.in16) adapters_set_kernel<__half><<<blocks, 256, 0, s>>>(a);
   else adapters_set_kernel<float><<<blocks, 256, 0, s>>>(a);
   return cudaGetLastError();

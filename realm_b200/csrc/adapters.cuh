@@ -12,12 +12,15 @@ constexpr int kAdapterMaxDim = 1 << 20;  // of k and n
 struct AdapterMeta {
   int32_t rank;  // 0: the slot is empty
   float scale;
+  int32_t exp;   // down and up are held behind powers of two; their products are 2^exp of what is held
 };
 
 // Adapters of one projection [n][k], in slots of equal size:
 //   down  [n_slots][kp / 8][r16][8] fp16 (as much of rp * kp as the rank needs)
 //   up    [n_slots][rp / 8][n][8] fp16
-// with zeros past the rank and past k. r16, rp: the rank and max_rank rounded up to a multiple of 16;
+// with zeros past the rank and past k. Factors given in fp32 are multiplied by a power of two that
+// brings their largest element to [2^14, 2^15), so that none is infinite and small ones keep their 11 bits
+// (AdapterMeta::exp); those given in fp16 lie as they are. r16, rp: the rank and max_rank rounded up to a multiple of 16;
 // kp: k to one of 64. Blocks of 8 rows x 16 bytes, as tensor-core operands lie, so that
 // they are copied as they are; eight elements a load for a thread.
 struct AdapterView {
@@ -40,6 +43,7 @@ struct AdapterArgs {
 struct AdapterSetArgs {
   uint16_t *down = nullptr, *up = nullptr;  // of the slot
   AdapterMeta* meta = nullptr;              // of the slot
+  uint32_t* most = nullptr;                 // of the slot, fp32 factors: the largest element of down, of up
   int32_t n = 0, k = 0, kp = 0, rp = 0, rank = 0, in16 = 0;
   float scale = 0.f;
   const void *src_down = nullptr, *src_up = nullptr;  // [rank][k], [n][rank]

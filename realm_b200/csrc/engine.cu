@@ -294,7 +294,7 @@ struct RowSet {
 // The adapters of one projection (rb_adapters_create).
 struct AdapterSet {
   int n = 0, k = 0, kp = 0, max_rank = 0, rp = 0, n_slots = 0;
-  DevBuf down, up, meta;
+  DevBuf down, up, meta, most;
   std::vector<int> rank;  // by slot; 0: empty
 };
 
@@ -2678,7 +2678,7 @@ int32_t adapters_create(rb_ctx* c, uint32_t n, uint32_t k, uint32_t n_slots, uin
   S->rank.assign(n_slots, 0);
   const size_t per = (size_t)n_slots * S->rp * 2;
   if (S->down.alloc(per * S->kp) != cudaSuccess || S->up.alloc(per * n) != cudaSuccess ||
-      S->meta.alloc((size_t)n_slots * sizeof(AdapterMeta)) != cudaSuccess) {
+      S->meta.alloc((size_t)n_slots * sizeof(AdapterMeta)) != cudaSuccess || S->most.alloc((size_t)n_slots * 8) != cudaSuccess) {
     cudaGetLastError();
     return fail(RB_ERR_OOM, "%u adapters of rank %u: %zu bytes", n_slots, max_rank, per * (S->kp + n));
   }
@@ -2705,6 +2705,7 @@ int32_t adapters_set(rb_ctx* c, int32_t set, uint32_t slot, int32_t dtype, uint3
   a.down = S->down.as<uint16_t>() + (size_t)slot * S->rp * S->kp;
   a.up = S->up.as<uint16_t>() + (size_t)slot * S->rp * S->n;
   a.meta = S->meta.as<AdapterMeta>() + slot;
+  if (dtype == RB_F32) a.most = S->most.as<uint32_t>() + 2 * slot;
   a.n = S->n;
   a.k = S->k;
   a.kp = S->kp;
