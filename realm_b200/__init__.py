@@ -31,7 +31,7 @@ LIB_PATH = os.path.join(_HERE, "librealm_b200.so")
 F32, F16, Q8_0, Q4_K, Q6_K = 0, 1, 8, 12, 14
 BLOCK_BYTES = {Q4_K: 144, Q6_K: 210, Q8_0: 34, F32: 4, F16: 2}
 BLOCK_ELEMS = {Q4_K: 256, Q6_K: 256, Q8_0: 32, F32: 1, F16: 1}
-PTR_HOST, PTR_DEVICE = 0, 1
+PTR_HOST, PTR_DEVICE, ASYNC = 0, 1, 2
 
 W_TOKEN_EMBD, W_OUTPUT_NORM, W_OUTPUT = 0, 1, 2
 W_ATTN_NORM, W_Q, W_K, W_V, W_O, W_FFN_NORM, W_GATE, W_UP, W_DOWN = range(10, 19)
@@ -335,7 +335,8 @@ class Weight:
         self.handle = h.value
 
     def matmul(self, x, batch_size: int, out=None, adapters: Optional["AdapterSet"] = None, slots=None):
-        """x W^T; with `adapters` and every row's slot, what its adapter adds is in it (AdapterSet.add)."""
+        """x W^T; with `adapters` and every row's slot, what its adapter adds is in it (AdapterSet.add). Then CUDA tensors
+        are not waited for, and a refused call leaves `out` as it was."""
         x = _f32(x)
         if adapters is not None and (adapters.n, adapters.k, adapters.ctx) != (self.n, self.k, self.ctx):
             raise ValueError(f"adapters of a [{adapters.n}][{adapters.k}] projection of their context, weight [{self.n}][{self.k}]")
@@ -343,11 +344,24 @@ class Weight:
             raise ValueError("adapters and slots go together")
         if out is None:
             out = np.empty((batch_size, self.n), np.float32)
-        _check(_lib.rb_weight_matmul(self.ctx.handle, self.handle, _ptr(x), _ptr(out), batch_size,
-                                     _flags(self.ctx, x, out)))
-        if adapters is not None:
-            adapters.add(x.reshape(batch_size, self.k), slots, out.reshape(batch_size, self.n))
+        if adapters is None:
+            self._product(x, out, batch_size, _flags(self.ctx, x, out))
+            return out
+        flags = _flags(self.ctx, x, out)
+        if flags == PTR_DEVICE:
+            flags |= ASYNC
+            if not str(x.dtype) == str(out.dtype) == "torch.float32":
+                raise ValueError(f"float32 x and out wanted, got {x.dtype} and {out.dtype}")
+        for a, width, name in ((x, self.k, "x"), (out, self.n, "out")):
+            _ptr(a)  # contiguous
+            if (a.numel() if _is_dev(a) else a.size) != batch_size * width:
+                raise ValueError(f"{name}: [{batch_size}][{width}] wanted, got {tuple(a.shape)}")
+        adapters.add(x.reshape(batch_size, self.k), slots, out.reshape(batch_size, self.n),
+                     _product=lambda: self._product(x, out, batch_size, flags))
         return out
+
+    def _product(self, x, out, batch_size, flags):
+        _check(_lib.rb_weight_matmul(self.ctx.handle, self.handle, _ptr(x), _ptr(out), batch_size, flags))
 
     def matmul_noalloc(self, x, out, batch_size: int):
         """rb_weight_matmul_noalloc: x [batch][k] and out [batch][n] are CUDA

@@ -31,6 +31,7 @@ _sig("rb_adapters_destroy", [_vp, _i32])
 _sig("rb_adapters_set", [_vp, _i32, _u32, _i32, _u32, _vp, _vp, _f, _u32])
 _sig("rb_adapters_clear", [_vp, _i32, _u32])
 _sig("rb_adapters_add", [_vp, _i32, C.POINTER(_AdaptersDesc), _u32])
+_sig("rb_adapters_check", [_vp, _i32, C.POINTER(_AdaptersDesc), _u32])
 
 
 def _size(v, name, most=0xffffffff):
@@ -70,7 +71,7 @@ class AdapterSet:
         """Empties a slot; ordered like set()."""
         _check(_lib.rb_adapters_clear(self.ctx.handle, self.handle, _size(slot, "slot")))
 
-    def add(self, x, slots, y, out=None):
+    def add(self, x, slots, y, out=None, _product=None):
         """y with scale up (down x) of every row's adapter added (rb_adapters_add), in place, or in `out`; returns it.
 
         x [rows][k], y and out [rows][n]: float32 or float16, numpy arrays or CUDA tensors; rows may lie apart.
@@ -105,6 +106,9 @@ class AdapterSet:
                 d.y, d.ldy = _rows3(y, n_rows, 1, self.n, "y")
                 d.out, d.ldo = (d.y, d.ldy) if out is y else _rows3(out, n_rows, 1, self.n, "out")
                 _writable(out, "out")
+        if _product is not None:  # Weight.matmul: writes y once nothing is refused
+            _check(_lib.rb_adapters_check(self.ctx.handle, self.handle, self._ref, flags))
+            _product()
         _call(self.ctx, flags, _lib.rb_adapters_add, self.ctx.handle, self.handle, self._ref)
         return out
 

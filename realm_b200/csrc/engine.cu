@@ -2722,34 +2722,48 @@ int32_t adapters_set(rb_ctx* c, int32_t set, uint32_t slot, int32_t dtype, uint3
   return (int32_t)rank;
 }
 
-int32_t adapters_add(rb_ctx* c, int32_t set, const rb_adapters_desc* d, uint32_t flags) {
-  AdapterSet* S = get_adapters(c, set);
+// What adapters_add refuses. Nothing is copied.
+int adapters_check(rb_ctx* c, const AdapterSet* S, int32_t set, const rb_adapters_desc* d, uint32_t flags) {
   if (!S) return fail(RB_ERR_BAD_HANDLE, "adapters %d", set);
   if (!d) return fail(RB_ERR_INVALID, "null descriptor");
   if (int rc = row_dtype(d->dtype)) return rc;
-  if (d->n_rows == 0) return 0;
+  if (d->n_rows == 0) return RB_OK;
   if (d->n_rows > (1u << 24)) return fail(RB_ERR_INVALID, "n_rows %u > 2^24", d->n_rows);
   if (!d->slots) return fail(RB_ERR_INVALID, "slots NULL");
-  const bool dev = flags & RB_PTR_DEVICE;
-  if (!dev)
+  if (!(flags & RB_PTR_DEVICE))
     for (uint32_t r = 0; r < d->n_rows; ++r) {
       const int s = d->slots[r];
       if (s != -1 && (s < 0 || s >= S->n_slots || S->rank[s] == 0))
         return fail(RB_ERR_NOT_FOUND, "row %u: no adapter in slot %d", r, s);
     }
+  const size_t esz = d->dtype == RB_F16 ? 2 : 4, n = d->n_rows;
+  Staged as;  // of device memory: checked, no more
+  if (flags & RB_PTR_DEVICE)
+    if (int rc = stage_words(c, "slots", d->slots, n, flags, as)) return rc;
+  if (int rc = stage_rows(c, "x", d->x, d->ldx, n, S->k, esz, RB_PTR_DEVICE, as)) return rc;
+  if (int rc = stage_rows(c, "y", d->y, d->ldy, n, S->n, esz, RB_PTR_DEVICE, as)) return rc;
+  if (int rc = stage_rows(c, "out", d->out, d->ldo, n, S->n, esz, RB_PTR_DEVICE, as)) return rc;
+  const bool in_place = d->out == d->y && d->ldo == d->ldy;
+  if (rows_meet(d->out, d->ldo * esz, S->n * esz, d->x, d->ldx * esz, S->k * esz, n) ||
+      (!in_place && rows_meet(d->out, d->ldo * esz, S->n * esz, d->y, d->ldy * esz, S->n * esz, n)) ||
+      rows_meet(d->out, 1, ((n - 1) * d->ldo + S->n) * esz, d->slots, 1, n * 4, 1))
+    return fail(RB_ERR_INVALID, "out overlaps x, slots, or y without being y");
+  return RB_OK;
+}
+
+int32_t adapters_add(rb_ctx* c, int32_t set, const rb_adapters_desc* d, uint32_t flags) {
+  AdapterSet* S = get_adapters(c, set);
+  if (int rc = adapters_check(c, S, set, d, flags)) return rc;
+  if (d->n_rows == 0) return 0;
   RB_CUDA(cudaSetDevice(c->device));
+  const bool dev = flags & RB_PTR_DEVICE, in_place = d->out == d->y && d->ldo == d->ldy;
   const size_t esz = d->dtype == RB_F16 ? 2 : 4, n = d->n_rows;
   Staged ss, sx, sy, so;
   if (int rc = stage_words(c, "slots", d->slots, n, flags, ss)) return rc;
   if (int rc = stage_rows(c, "x", d->x, d->ldx, n, S->k, esz, flags, sx)) return rc;
   if (int rc = stage_rows(c, "y", d->y, d->ldy, n, S->n, esz, flags, sy)) return rc;
-  const bool in_place = d->out == d->y && d->ldo == d->ldy;
-  if (!in_place || dev)
+  if (!in_place)
     if (int rc = stage_rows(c, "out", d->out, d->ldo, n, S->n, esz, flags, so)) return rc;
-  if (rows_meet(d->out, d->ldo * esz, S->n * esz, d->x, d->ldx * esz, S->k * esz, n) ||
-      (!in_place && rows_meet(d->out, d->ldo * esz, S->n * esz, d->y, d->ldy * esz, S->n * esz, n)) ||
-      rows_meet(d->out, 1, ((n - 1) * d->ldo + S->n) * esz, d->slots, 1, n * 4, 1))
-    return fail(RB_ERR_INVALID, "out overlaps x, slots, or y without being y");
   AdapterArgs a;
   a.w.down = S->down.as<uint16_t>();
   a.w.up = S->up.as<uint16_t>();
@@ -2984,6 +2998,10 @@ int32_t rb_adapters_clear(rb_ctx* c, int32_t set, uint32_t slot) {
   RB_CUDA(adapters_clear_launch(S->meta.as<AdapterMeta>() + slot, c->stream));
   S->rank[slot] = 0;
   return RB_OK;
+}
+
+int32_t rb_adapters_check(rb_ctx* c, int32_t set, const rb_adapters_desc* d, uint32_t flags) {
+  return guarded([&] { return adapters_check(c, get_adapters(c, set), set, d, flags); });
 }
 
 int32_t rb_adapters_add(rb_ctx* c, int32_t set, const rb_adapters_desc* d, uint32_t flags) {
