@@ -12,11 +12,13 @@ serves rows of any mix of adapters.
 from __future__ import annotations
 
 import ctypes as C
+import sys
 
 import numpy as np
 
 from . import PTR_DEVICE, _check, _lib, _sig
-from .rows import ASYNC, BAD_HANDLE, _SEEN, _call, _dtype, _is_tensor, _mat, _rows3, _vec, _writable
+from .rows import (ASYNC, BAD_HANDLE, _SEEN, _Order, _call, _current_stream, _dtype, _is_tensor, _mat, _rows3, _vec,
+                   _writable)
 
 _vp, _u32, _u64, _i32, _f = C.c_void_p, C.c_uint32, C.c_uint64, C.c_int32, C.c_float
 
@@ -38,6 +40,19 @@ def _size(v, name, most=0xffffffff):
     if int(v) != v or not 0 <= v <= most:
         raise ValueError(f"{name}: an integer of at least 0 wanted")
     return int(v)
+
+
+def _change(ctx, flags, fn, *args):
+    """_call, for what changes a slot: ordered with torch's current stream also without tensors, since captured calls
+    that read the slot are replayed there."""
+    torch = sys.modules.get("torch")
+    if flags & PTR_DEVICE or torch is None or not torch.cuda.is_initialized() or \
+            _current_stream(ctx.device) == ctx._stream_id:
+        return _call(ctx, flags, fn, *args)
+    order = _Order(ctx)
+    rc = fn(*args, flags)
+    order.done()
+    _check(rc)
 
 
 class AdapterSet:
@@ -64,12 +79,12 @@ class AdapterSet:
         if tuple(down.shape) != (rank, self.k) or tuple(up.shape) != (self.n, rank):
             raise ValueError(f"down [rank][{self.k}] and up [{self.n}][rank] wanted, got {tuple(down.shape)} and "
                              f"{tuple(up.shape)}")
-        _call(self.ctx, flags, _lib.rb_adapters_set, self.ctx.handle, self.handle, _size(slot, "slot"), dt, rank,
+        _change(self.ctx, flags, _lib.rb_adapters_set, self.ctx.handle, self.handle, _size(slot, "slot"), dt, rank,
               _vec(down, name, rank * self.k, "down"), _vec(up, name, rank * self.n, "up"), scale)
 
     def clear(self, slot: int):
         """Empties a slot; ordered like set()."""
-        _check(_lib.rb_adapters_clear(self.ctx.handle, self.handle, _size(slot, "slot")))
+        _change(self.ctx, 0, lambda *a: _lib.rb_adapters_clear(*a[:3]), self.ctx.handle, self.handle, _size(slot, "slot"))
 
     def add(self, x, slots, y, out=None, _product=None):
         """y with scale up (down x) of every row's adapter added (rb_adapters_add), in place, or in `out`; returns it.
