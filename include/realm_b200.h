@@ -532,7 +532,7 @@ int32_t rb_sample_filtered(rb_ctx* ctx, int32_t dtype, const void* logits, uint6
 /* The distribution that rb_sample_filtered draws from: probs [n_rows][ldp] (fp32), each
  * kept token's share of the kept weight, rounded once, and 0 for the others. A row that
  * has no finite or +infinite logit is 0 throughout. Arguments as rb_sample_filtered;
- * probs must not overlap logits. Returns n_rows. */
+ * probs must not overlap logits, params or what the history is in. Returns n_rows. */
 int32_t rb_filter_probs(rb_ctx* ctx, int32_t dtype, const void* logits, uint64_t ld, uint32_t n_rows, uint32_t vocab,
                         const rb_sampling_filter* params, const uint32_t* prev_tokens, const uint32_t* prev_offsets,
                         float* probs, uint64_t ldp, uint32_t flags);

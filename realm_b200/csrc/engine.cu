@@ -2488,6 +2488,11 @@ int32_t filter_probs(rb_ctx* c, int32_t dtype, const void* logits, uint64_t ld, 
   const size_t esz = dtype == RB_F16 ? 2 : 4;
   if (rows_meet(logits, ld * esz, vocab * esz, probs, ldp * 4, (uint64_t)vocab * 4, n_rows))
     return fail(RB_ERR_INVALID, "probs overlaps logits");
+  // a row's CTAs read its filter while another row's write probabilities
+  const uint64_t all = ((uint64_t)(n_rows - 1) * ldp + vocab) * 4, np = (uint64_t)n_rows * sizeof(rb_sampling_filter);
+  if (rows_meet(probs, all, all, params, np, np, 1) ||
+      (prev_off && rows_meet(probs, all, all, prev_off, ((uint64_t)n_rows + 1) * 4, ((uint64_t)n_rows + 1) * 4, 1)))
+    return fail(RB_ERR_INVALID, "probs overlaps params or prev_offsets");
   Staged sp;  // host: a buffer of the same shape, whose gaps between rows go back as they came
   if (int rc = stage_rows(c, "probs", probs, ldp, n_rows, vocab, 4, flags, sp)) return rc;
   a.dist = (float*)const_cast<void*>(sp.dptr);
