@@ -625,6 +625,9 @@ typedef struct rb_adapters_desc {
  * bits of its row's largest element (an infinite one makes the row's sums NaN). The result is
  * rounded once. out must not overlap x, nor y unless it is y. Returns n_rows. */
 int32_t rb_adapters_add(rb_ctx* ctx, int32_t set, const rb_adapters_desc* desc, uint32_t flags);
+/* Test hook: the set's calls of few rows take clusters of 8 CTAs, as on a part of a GPU, instead of the 16 that they
+ * take where the GPU has them. Returns the number before. */
+int32_t rb_test_adapters_portable(rb_ctx* ctx, int32_t set);
 /* What rb_adapters_add refuses, with the same error, and nothing else: for a caller that writes y first, by
  * rb_weight_matmul say, and wants to know before. 0 where the call would run. */
 int32_t rb_adapters_check(rb_ctx* ctx, int32_t set, const rb_adapters_desc* desc, uint32_t flags);

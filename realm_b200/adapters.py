@@ -33,6 +33,7 @@ _sig("rb_adapters_destroy", [_vp, _i32])
 _sig("rb_adapters_set", [_vp, _i32, _u32, _i32, _u32, _vp, _vp, _f, _u32])
 _sig("rb_adapters_clear", [_vp, _i32, _u32])
 _sig("rb_adapters_add", [_vp, _i32, C.POINTER(_AdaptersDesc), _u32])
+_sig("rb_test_adapters_portable", [_vp, _i32])
 _sig("rb_adapters_check", [_vp, _i32, C.POINTER(_AdaptersDesc), _u32])
 
 

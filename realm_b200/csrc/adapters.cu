@@ -20,7 +20,6 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
-#include <atomic>
 
 #include "adapters.cuh"
 #include "common.cuh"
@@ -35,7 +34,7 @@ constexpr int kT = 256, kWarps = kT / 32;
 constexpr int kBlock = 64;        // rows among which an item's rows are found
 constexpr int kGroup = 8;         // ranks a warp works on at a time: a line of weights
 constexpr int kTileK = 1536;      // elements of x in shared memory at a time
-constexpr int kMaxCluster = 16;  // above 8: not portable, but every B200 has it
+constexpr int kMaxCluster = 16;  // where the GPU has it (adapters_max_cluster)
 static_assert(kWarps * kGroup <= kAdapterMaxRank && kTileK % 8 == 0, "");
 
 __device__ __forceinline__ float to_f(float v) { return v; }
@@ -283,13 +282,6 @@ cudaError_t launch(const AdapterArgs& a, int cluster, cudaStream_t s) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (cudaError_t e = ensure_smem_attr(adapters_kernel<T, R>, kMaxCluster * kAdapterMaxRank * R * 4, dev)) return e;
-  if (cluster > 8) {
-    static std::atomic<uint64_t> allowed{0};  // by device
-    if (!(allowed.load() >> (dev & 63) & 1)) {
-      if (cudaError_t e = cudaFuncSetAttribute(adapters_kernel<T, R>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) return e;
-      allowed |= 1ull << (dev & 63);
-    }
-  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a.n_rows * cluster);
   cfg.blockDim = dim3(kT);
@@ -364,6 +356,29 @@ cudaError_t adapters_set_launch(const AdapterSetArgs& a, cudaStream_t s) {
   return cudaGetLastError();
 }
 
+int adapters_max_cluster() {
+  // more than eight CTAs are not portable: asked for by the kernels that may have them, and had where so many SMs lie
+  // together, which a part of a GPU may not have
+  auto fits = [](auto kernel) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return false;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(kMaxCluster);
+    cfg.blockDim = dim3(kT);
+    cfg.dynamicSmemBytes = kMaxCluster * kAdapterMaxRank * 4;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = kMaxCluster;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    int n = 0;
+    return cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess && n > 0;
+  };
+  const bool all = fits(adapters_kernel<float, 1>) && fits(adapters_kernel<__half, 1>);
+  cudaGetLastError();
+  return all ? kMaxCluster : 8;
+}
+
 cudaError_t adapters_clear_launch(AdapterMeta* meta, cudaStream_t s) {
   adapters_clear_kernel<<<1, 1, 0, s>>>(meta);
   return cudaGetLastError();
@@ -376,7 +391,7 @@ cudaError_t adapters_launch(const AdapterArgs& a, int num_sms, cudaStream_t s) {
   if (a.n_rows > 1024 || (a.n_rows > 384 && a.n_rows > 4 * a.w.n_slots)) return adapters_tile_launch(a, num_sms, s);
   // Sixteen CTAs a row where there are few: one row 11.5 us and 15.6 with eight (rank 64, k = n = 4096), 17.6 and 28 at k =
   // 11008; 64 rows of 64 adapters 39 and 29. (Nothing in L2, as above; the times include about 3 us of launch.)
-  const int cluster = a.n_rows <= 16 ? 16 : 8;
+  const int cluster = a.n_rows <= 16 ? a.max_cluster : 8;
   if (a.n_rows <= 16) return a.x16 ? launch<__half, 1>(a, cluster, s) : launch<float, 1>(a, cluster, s);
   return a.x16 ? launch<__half, 4>(a, cluster, s) : launch<float, 4>(a, cluster, s);
 }

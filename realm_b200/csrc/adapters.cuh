@@ -38,6 +38,7 @@ struct AdapterArgs {
   int32_t n_rows = 0;
   const int32_t* slots = nullptr;
   uint32_t* err = nullptr;
+  int32_t max_cluster = 8;  // adapters_max_cluster()
 };
 
 struct AdapterSetArgs {
@@ -49,6 +50,8 @@ struct AdapterSetArgs {
   const void *src_down = nullptr, *src_up = nullptr;  // [rank][k], [n][rank]
 };
 
+// CTAs that a cluster may have on the current device: 16, or 8 where so many do not fit. Not while a stream is captured.
+int adapters_max_cluster();
 cudaError_t adapters_set_launch(const AdapterSetArgs& a, cudaStream_t s);
 cudaError_t adapters_clear_launch(AdapterMeta* meta, cudaStream_t s);
 cudaError_t adapters_launch(const AdapterArgs& a, int num_sms, cudaStream_t s);

@@ -293,7 +293,7 @@ struct RowSet {
 
 // The adapters of one projection (rb_adapters_create).
 struct AdapterSet {
-  int n = 0, k = 0, kp = 0, max_rank = 0, rp = 0, n_slots = 0;
+  int n = 0, k = 0, kp = 0, max_rank = 0, rp = 0, n_slots = 0, max_cluster = 8;
   DevBuf down, up, meta, most;
   std::vector<int> rank;  // by slot; 0: empty
 };
@@ -2680,6 +2680,7 @@ int32_t adapters_create(rb_ctx* c, uint32_t n, uint32_t k, uint32_t n_slots, uin
   S->max_rank = (int)max_rank;
   S->rp = (int)(max_rank + 15) / 16 * 16;
   S->n_slots = (int)n_slots;
+  S->max_cluster = adapters_max_cluster();
   S->rank.assign(n_slots, 0);
   const size_t per = (size_t)n_slots * S->rp * 2;
   if (S->down.alloc(per * S->kp) != cudaSuccess || S->up.alloc(per * n) != cudaSuccess ||
@@ -2788,6 +2789,7 @@ int32_t adapters_add(rb_ctx* c, int32_t set, const rb_adapters_desc* d, uint32_t
   a.n_rows = (int)n;
   a.slots = (const int32_t*)ss.dptr;
   a.err = c->err.as<uint32_t>();
+  a.max_cluster = S->max_cluster;
   RB_CUDA(adapters_launch(a, c->num_sms, c->stream));
   if (!dev)
     RB_CUDA(cudaMemcpy2DAsync(d->out, d->ldo * esz, a.out, d->ldo * esz, S->n * esz, n, cudaMemcpyDeviceToHost, c->stream));
@@ -3003,6 +3005,14 @@ int32_t rb_adapters_clear(rb_ctx* c, int32_t set, uint32_t slot) {
   RB_CUDA(adapters_clear_launch(S->meta.as<AdapterMeta>() + slot, c->stream));
   S->rank[slot] = 0;
   return RB_OK;
+}
+
+int32_t rb_test_adapters_portable(rb_ctx* c, int32_t set) {
+  AdapterSet* S = get_adapters(c, set);
+  if (!S) return fail(RB_ERR_BAD_HANDLE, "adapters %d", set);
+  const int had = S->max_cluster;
+  S->max_cluster = 8;
+  return had;
 }
 
 int32_t rb_adapters_check(rb_ctx* c, int32_t set, const rb_adapters_desc* d, uint32_t flags) {
