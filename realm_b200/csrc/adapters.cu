@@ -205,7 +205,7 @@ template <class T, int R>
 __global__ void __launch_bounds__(kT, 4) adapters_kernel(const __grid_constant__ AdapterArgs a) {
   __shared__ ItemShared<R> sh;
   extern __shared__ float parts[];  // [CTA of the cluster][rank][row] of v
-  __shared__ int s_slot[kBlock], s_rows[R], s_n, s_item;
+  __shared__ int s_slot[kBlock], s_rows[R], s_n;
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), c = (int)cluster.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(kT, 4) adapters_kernel(const __grid_constant__
   } else {
     const int b0 = id / kBlock * kBlock, nb = min(kBlock, a.n_rows - b0);
     if (tid < nb) s_slot[tid] = slot_of(a, b0 + tid);
-    if (tid == 0) s_n = s_item = 0;
+    if (tid == 0) s_n = 0;
     __syncthreads();
     if (warp == 0) {
       // rows b0 + lane and b0 + 32 + lane: which of its slot's rows is it; a row without an adapter is one by itself

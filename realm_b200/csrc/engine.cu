@@ -318,6 +318,7 @@ struct Ctx {
   int next_plan = 0;
   std::map<int, std::unique_ptr<AdapterSet>> adapters;  // the same
   int next_adapters = 0;
+  int adapter_cluster = 0;  // adapters_max_cluster(), once asked for
   // RowAttnArgs::hold. Made with the first fp16 pool of a caller's, or the first plan with tile units over a
   // model's: a model's decode steps take 0.5 % longer when it lies between the memory of the model.
   DevBuf tile_hold, tile_busy;
@@ -2646,7 +2647,7 @@ int32_t residual_norm(rb_ctx* c, const rb_residual_desc* d, uint32_t flags) {
   a.pre = (const float*)s2.dptr;
   a.scale = d->scale;
   a.eps = d->eps;
-  RB_CUDA(residual_launch(a, c->num_sms, c->stream));
+  RB_CUDA(residual_launch(a, c->stream));
   if (dev && (flags & RB_ASYNC)) return (int32_t)n;
   if (!dev) {
     RB_CUDA(cudaMemcpy2DAsync(d->x_out, d->ldxo * ex, a.x_out, d->ldxo * ex, w * ex, n, cudaMemcpyDeviceToHost, c->stream));
@@ -2680,7 +2681,8 @@ int32_t adapters_create(rb_ctx* c, uint32_t n, uint32_t k, uint32_t n_slots, uin
   S->max_rank = (int)max_rank;
   S->rp = (int)(max_rank + 15) / 16 * 16;
   S->n_slots = (int)n_slots;
-  S->max_cluster = adapters_max_cluster();
+  if (!c->adapter_cluster) c->adapter_cluster = adapters_max_cluster();
+  S->max_cluster = c->adapter_cluster;
   S->rank.assign(n_slots, 0);
   const size_t per = (size_t)n_slots * S->rp * 2;
   if (S->down.alloc(per * S->kp) != cudaSuccess || S->up.alloc(per * n) != cudaSuccess ||

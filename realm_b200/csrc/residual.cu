@@ -179,7 +179,7 @@ cudaError_t launch(const ResidualArgs& a, int threads, int rows, cudaStream_t s)
 }
 
 template <class TY, class TX, bool VEC>
-cudaError_t launch_chunks(const ResidualArgs& a, int num_sms, cudaStream_t s) {
+cudaError_t launch_chunks(const ResidualArgs& a, cudaStream_t s) {
   const int chunks = (a.dim + kE - 1) / kE;
   const int nc = chunks <= 256 ? 1 : chunks <= 1024 ? 2 : 4, most = chunks <= 2048 ? 512 : 1024;
   const int threads = std::min(most, ((chunks + nc - 1) / nc + 31) / 32 * 32);
@@ -191,21 +191,21 @@ cudaError_t launch_chunks(const ResidualArgs& a, int num_sms, cudaStream_t s) {
 }
 
 template <class TY, class TX>
-cudaError_t launch_type(const ResidualArgs& a, int num_sms, cudaStream_t s) {
+cudaError_t launch_type(const ResidualArgs& a, cudaStream_t s) {
   auto on16 = [&](const void* p, int64_t ld, int esz) {
     return !p || ((uintptr_t)p % 16 == 0 && (a.n_rows == 1 || ld * esz % 16 == 0));
   };
   const int ey = sizeof(TY), ex = sizeof(TX);
   const bool vec = a.dim % kE == 0 && on16(a.y, a.ldy, ey) && on16(a.gate, a.ldg, ey) && on16(a.out, a.ldo, ey) &&
                    on16(a.x, a.ldx, ex) && on16(a.x_out, a.ldxo, ex) && on16(a.post, 0, 4) && on16(a.pre, 0, 4);
-  return vec ? launch_chunks<TY, TX, true>(a, num_sms, s) : launch_chunks<TY, TX, false>(a, num_sms, s);
+  return vec ? launch_chunks<TY, TX, true>(a, s) : launch_chunks<TY, TX, false>(a, s);
 }
 
 }  // namespace
 
-cudaError_t residual_launch(const ResidualArgs& a, int num_sms, cudaStream_t s) {
-  if (a.y16) return a.x16 ? launch_type<__half, __half>(a, num_sms, s) : launch_type<__half, float>(a, num_sms, s);
-  return a.x16 ? launch_type<float, __half>(a, num_sms, s) : launch_type<float, float>(a, num_sms, s);
+cudaError_t residual_launch(const ResidualArgs& a, cudaStream_t s) {
+  if (a.y16) return a.x16 ? launch_type<__half, __half>(a, s) : launch_type<__half, float>(a, s);
+  return a.x16 ? launch_type<float, __half>(a, s) : launch_type<float, float>(a, s);
 }
 
 }  // namespace rb

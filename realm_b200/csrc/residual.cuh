@@ -17,6 +17,6 @@ struct ResidualArgs {
   float scale = 1.f, eps = 0.f;
 };
 
-cudaError_t residual_launch(const ResidualArgs& a, int num_sms, cudaStream_t s);
+cudaError_t residual_launch(const ResidualArgs& a, cudaStream_t s);
 
 }  // namespace rb
