@@ -559,10 +559,10 @@ typedef struct rb_verify_desc {
  * drawn from the positive part of p - q (without draft_probs from p without d), after the
  * last from p. Weights of the draw are p - q in fixed point with 44 fractional bits, so it
  * depends on no order: the first index whose running sum exceeds uniform * total
- * (uniforms past either end draw the last and the first). Where p - q has no positive part
- * the draw is from p. tokens gets the accepted tokens, then the drawn one, then 0xffffffff up
- * to the request's last row; accepted the number of the accepted. A p without a positive
- * value draws 0xffffffff; unless RB_ASYNC, the call then returns RB_ERR_INVALID ("Failed to create
+ * (uniforms past either end draw the last and the first). Where p - q is nowhere 2^-44 or
+ * more the draw is from p. tokens gets the accepted tokens, then the drawn one, then 0xffffffff up
+ * to the request's last row; accepted the number of the accepted. A p without a value
+ * of 2^-44 or more draws 0xffffffff; unless RB_ASYNC, the call then returns RB_ERR_INVALID ("Failed to create
  * weighted index"). A request without rows gets accepted = 0, one whose offsets fall or pass
  * n_rows -1 (device memory; on the host that is refused); the others are verified, though where they
  * share rows after a fall, those rows' tokens are left open. Returns n_requests. */
@@ -621,9 +621,10 @@ typedef struct rb_adapters_desc {
   uint64_t ldx, ldy, ldo;
 } rb_adapters_desc;
 /* Rows in any order; those without an adapter are copied as they are, whatever their x
- * holds. All sums are fp32; where a call's rows are many, an RB_F32 x has 22 bits, and down x 22
- * bits of its row's largest element (an infinite one makes the row's sums NaN). The result is
- * rounded once. out must not overlap x, nor y unless it is y. Returns n_rows. */
+ * holds. All sums are fp32. Calls of more than 1024 rows, and of more than 384 and more than 4 n_slots, run in
+ * tiles on the tensor cores: there an RB_F32 x has 22 bits, and down x 22 bits of its row's largest element (an
+ * infinite one makes the row's sums NaN). So a row's last bits depend on how many rows a call has and on how
+ * many slots its set was made with, never on what the other rows hold. The result is rounded once. out must not overlap x, nor y unless it is y. Returns n_rows. */
 int32_t rb_adapters_add(rb_ctx* ctx, int32_t set, const rb_adapters_desc* desc, uint32_t flags);
 /* Test hook: the set's calls of few rows take clusters of 8 CTAs, as on a part of a GPU, instead of the 16 that they
  * take where the GPU has them. Returns the number before. */

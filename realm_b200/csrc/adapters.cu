@@ -15,7 +15,7 @@
 // Bound by latency: the slots, an adapter's rank, x and down, the exchange, up, one after the other; up and
 // y are on their way to L2 from the start. Nothing in L2, about 3 us of launch within: one row of rank 16 (k = n =
 // 4096, 0.3 MB) 9.5 us, rank 64 11.5, rank 128 16; 64 rows of 64 adapters of rank 64 (67 MB) 29 us, 2.3 TB/s; 48
-// rows of 31 adapters of rank 8 to 64, n = 11008 (32 MB), 26 us. With up read four blocks of two columns at a time
+// rows of 31 adapters of rank 8 to 64, n = 11008 (32 MB), 25.7 us. With up read four blocks of two columns at a time
 // instead of one by one 64 rows went from 35 to 29 us.
 #include <cooperative_groups.h>
 
@@ -387,7 +387,9 @@ cudaError_t adapters_clear_launch(AdapterMeta* meta, cudaStream_t s) {
 cudaError_t adapters_launch(const AdapterArgs& a, int num_sms, cudaStream_t s) {
   // One launch for rows of any slots, whose number is not known here. Rows of one adapter, k = n = 4096, fp32, rank 64: 256
   // rows 33 us here and 51 in tiles, 384 47 and 53, 512 54 and 55, 1024 100 and 57; every row another's: 256 rows 82 and
-  // 612, 1024 258 and 593. So up to 384 rows here, and up to 1024 where there are slots for rows mostly apart.
+  // 612, 1024 258 and 593. So up to 384 rows here, and up to 1024 where there are slots for rows mostly apart. It is the
+  // set's slots that count, not those that its rows have, which are not known here: 1024 rows of one adapter take 52 us
+  // with a set of 8 slots and 98 with one of 256.
   if (a.n_rows > 1024 || (a.n_rows > 384 && a.n_rows > 4 * a.w.n_slots)) return adapters_tile_launch(a, num_sms, s);
   // Sixteen CTAs a row where there are few: one row 11.5 us and 15.6 with eight (rank 64, k = n = 4096), 17.6 and 28 at k =
   // 11008; 64 rows of 64 adapters 39 and 29. (Nothing in L2, as above; the times include about 3 us of launch.)

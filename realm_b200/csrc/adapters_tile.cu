@@ -14,7 +14,7 @@
 //     row's thread adds its part there, and whole lines go out.
 //
 // The tensor core cuts a running sum off (towards 0) after every instruction, so fp32 rows sum at
-// most 256 elements of k there; the sums of these chains are added in registers, with rounding.
+// most 128 elements of k there; the sums of these chains are added in registers, with rounding.
 //
 // x and y are read and out is written once, which is most of the bytes. 8192 rows, rank 64, k = n = 4096, fp16 72 us
 // (2.9 TB/s, floor 32 us), fp32 111 us (floor 62); 1024 rows 39 and 55 us. Bound by the workers' instructions
