@@ -345,7 +345,8 @@ class Weight:
         if out is None:
             out = np.empty((batch_size, self.n), np.float32)
         if adapters is None:
-            self._product(x, out, batch_size, _flags(self.ctx, x, out))
+            _check(_lib.rb_weight_matmul(self.ctx.handle, self.handle, _ptr(x), _ptr(out), batch_size,
+                                         _flags(self.ctx, x, out)))
             return out
         flags = _flags(self.ctx, x, out)
         if flags == PTR_DEVICE:
