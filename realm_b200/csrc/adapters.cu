@@ -15,7 +15,7 @@
 // Bound by latency: the slots, an adapter's rank, x and down, the exchange, up, one after the other; up and
 // y are on their way to L2 from the start. Nothing in L2, about 3 us of launch within: one row of rank 16 (k = n =
 // 4096, 0.3 MB) 9.5 us, rank 64 11.5, rank 128 16; 64 rows of 64 adapters of rank 64 (67 MB) 29 us, 2.3 TB/s; 48
-// rows of 31 adapters of rank 8 to 64, n = 11008 (32 MB), 25.7 us. With up read four blocks of two columns at a time
+// rows of 31 adapters of rank 8 to 64, n = 11008 (32 MB), 25.8 us. With up read four blocks of two columns at a time
 // instead of one by one 64 rows went from 35 to 29 us.
 #include <cooperative_groups.h>
 
@@ -83,9 +83,8 @@ __device__ __forceinline__ void run_item(const AdapterArgs& a, ItemShared<RS>& s
   // this CTA's columns of out
   const int n0 = (int)((int64_t)a.w.n * c / C), n1 = (int)((int64_t)a.w.n * (c + 1) / C);
   cluster.barrier_arrive();
-  const int rank = a.w.meta[slot].rank;
-  const float scale = a.w.meta[slot].scale;
-  const int exp = a.w.meta[slot].exp;
+  const AdapterMeta meta = a.w.meta[slot];
+  const int rank = meta.rank;
   const int groups = (rank + kGroup - 1) / kGroup, r16 = (rank + 15) / 16 * 16;
   // warps are split over groups of ranks, and with few of those over k
   const int ks = groups >= kWarps ? 1 : kWarps / groups, kpart = ks == 1 ? 0 : warp / groups;
@@ -151,7 +150,7 @@ __device__ __forceinline__ void run_item(const AdapterArgs& a, ItemShared<RS>& s
     float s = 0.f;
     if (i < nv)
       for (int d = 0; d < C; ++d) s += parts[d * stride + i];
-    v[i] = scalbnf(s * scale, exp);
+    v[i] = s * meta.scale * meta.f1 * meta.f2;
   }
   __syncthreads();
   const int blocks8 = (rank + 7) / 8;
@@ -337,10 +336,13 @@ __global__ void adapters_set_kernel(const __grid_constant__ AdapterSetArgs a) {
     const int r = (int)(v / a.n) * 8 + (int)(i % 8), j = (int)(v % a.n);
     a.up[i] = r < a.rank ? __half_as_ushort(from_f<__half>(scalbnf(to_f(su[(int64_t)j * a.rank + r]), lift_u))) : 0;
   }
-  if (at == 0) *a.meta = AdapterMeta{a.rank, a.scale, -lift_d - lift_u};
+  if (at == 0) {
+    const int e = -lift_d - lift_u;  // in -252 .. 226
+    *a.meta = AdapterMeta{a.rank, a.scale, scalbnf(1.f, e / 2), scalbnf(1.f, e - e / 2)};
+  }
 }
 
-__global__ void adapters_clear_kernel(AdapterMeta* meta) { *meta = AdapterMeta{0, 0.f, 0}; }
+__global__ void adapters_clear_kernel(AdapterMeta* meta) { *meta = AdapterMeta{0, 0.f, 1.f, 1.f}; }
 
 }  // namespace
 

@@ -9,10 +9,10 @@ constexpr int kAdapterMaxRank = 128;
 constexpr int kAdapterMaxSlots = 4096;
 constexpr int kAdapterMaxDim = 1 << 20;  // of k and n
 
-struct AdapterMeta {
+struct __align__(16) AdapterMeta {  // one load
   int32_t rank;  // 0: the slot is empty
   float scale;
-  int32_t exp;   // down and up are held behind powers of two; their products are 2^exp of what is held
+  float f1, f2;  // down and up are held behind powers of two: their products are f1 f2 of what is held, two powers of one side of 1
 };
 
 // Adapters of one projection [n][k], in slots of equal size:
@@ -20,7 +20,7 @@ struct AdapterMeta {
 //   up    [n_slots][rp / 8][n][8] fp16
 // with zeros past the rank and past k. Factors given in fp32 are multiplied by a power of two that
 // brings their largest element to [2^14, 2^15), so that none is infinite and small ones keep their 11 bits
-// (AdapterMeta::exp); those given in fp16 lie as they are. r16, rp: the rank and max_rank rounded up to a multiple of 16;
+// (AdapterMeta); those given in fp16 lie as they are. r16, rp: the rank and max_rank rounded up to a multiple of 16;
 // kp: k to one of 64. Blocks of 8 rows x 16 bytes, as tensor-core operands lie, so that
 // they are copied as they are; eight elements a load for a thread.
 struct AdapterView {

@@ -542,7 +542,8 @@ __global__ void __launch_bounds__(kTT, Cfg<T, RP>::CTAS) adapters_tile_kernel(co
       // 2^(13 - exponent of the row's largest), and its inverse; no row is lifted by more than 2^110
       const int ex = max(30, (int)(__float_as_uint(most) >> 23));
       const float lift = __uint_as_float((uint32_t)(127 + 13 - min(ex - 127, 126)) << 23);
-      const float factor = scalbnf(a.w.meta[slot].scale, min(ex - 127, 126) - 13 + a.w.meta[slot].exp);
+      const AdapterMeta meta = a.w.meta[slot];
+      const float factor = meta.scale * __uint_as_float((uint32_t)(127 - 13 + min(ex - 127, 126)) << 23) * meta.f1 * meta.f2;
       // ---- y, a block at a time ----
       constexpr int BC = 8 * E, PER = kCols / BC;  // columns of a block, blocks of a tile
       const T* y = reinterpret_cast<const T*>(a.y);
