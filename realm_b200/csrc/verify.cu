@@ -16,7 +16,7 @@
 // the same turns: a CTA's threads share one reading of the refused draft, and whether there is a second turn goes with the sums.
 //
 // Bound by latency: offsets, drafts, their probabilities, the row, the exchange, the share again, one after the other.
-// 64 requests of 1 to 9 rows of 151937 25 us (63 MB read: 2.5 TB/s; 30 us when the share was gone over vector by vector,
+// 64 requests of 1 to 9 rows of 151937 22.5 us (63 MB read: 2.8 TB/s; 30 us when the share was gone over vector by vector,
 // 37 when the sums were too); one request of 7 rows of 32000 the call itself, 9 us. Rows of which a looked-up draft is
 // taken out, and p and q that lie unlike, go vector by vector, one on its way a lane: the same requests looked up 35 us.
 #include <cooperative_groups.h>
