@@ -605,7 +605,8 @@ int32_t rb_adapters_destroy(rb_ctx* ctx, int32_t set);
 /* Puts an adapter in a slot, in place of what it held: down [rank][k], up [n][rank], both of
  * dtype RB_F32 or RB_F16. RB_F32 factors are rounded to fp16 behind a power of two each, which brings the
  * largest element to [2^14, 2^15) (2^126 at most): none overflows, and elements keep 11 bits down to 2^-28 of the
- * largest. Ordered on the stream: rows of earlier calls have the slot's old adapter. Returns rank. */
+ * largest. Sums of down x are of what is held: in fp32 they reach up to |x| of 1e34 / k. Ordered on the stream: rows of
+ * earlier calls have the slot's old adapter. Returns rank. */
 int32_t rb_adapters_set(rb_ctx* ctx, int32_t set, uint32_t slot, int32_t dtype, uint32_t rank, const void* down,
                         const void* up, float scale, uint32_t flags);
 /* Empties a slot (RB_ERR_NOT_FOUND beyond n_slots). */
@@ -624,7 +625,8 @@ typedef struct rb_adapters_desc {
  * holds. All sums are fp32. Calls of more than 1024 rows, and of more than 384 and more than 4 n_slots, run in
  * tiles on the tensor cores: there an RB_F32 x has 22 bits, and down x 22 bits of its row's largest element (an
  * infinite one makes the row's sums NaN). So a row's last bits depend on how many rows a call has and on how
- * many slots its set was made with, never on what the other rows hold. The result is rounded once. out must not overlap x, nor y unless it is y. Returns n_rows. */
+ * many slots its set was made with, never on what the other rows hold. The result is rounded once. out must not
+ * overlap x, nor y unless it is y. Returns n_rows. */
 int32_t rb_adapters_add(rb_ctx* ctx, int32_t set, const rb_adapters_desc* desc, uint32_t flags);
 /* Test hook: the set's calls of few rows take clusters of 8 CTAs, as on a part of a GPU, instead of the 16 that they
  * take where the GPU has them. Returns the number before. */
